@@ -302,6 +302,41 @@ typedef struct unok_draft_layer_args {
 int64_t unok_draft_layer_scratch(const unok_draft_layer_args* args);
 int unok_draft_layer(const unok_draft_layer_args* args, void* stream);
 
+/* ---- Trees of drafted tokens over the KV cache ------------------------------------------------- */
+
+/* Attention of a tree of T <= 256 drafted tokens per sequence. Node t's parent parents[b * ldp + t] (ldp 0: one
+ * tree for every sequence) is an earlier node, or -1 for a root; below -1 the node is padding. A node attends to
+ * cache rows [0, lengths[b]), its ancestors and itself, node a being cache row lengths[b] + a (rows at or past
+ * max_len do not exist; a parent that is no earlier node, or is padding, ends the chain): O = softmax(scale Q K^T) V, zeros for
+ * padding. Q and O [B T, nq D] with row strides ldq / ldo, q head h reading K/V head h / (nq / nk); K and V row
+ * (b, head, j) at b * batch + head * head stride + j * row stride. dtype 0 / 1, D 64 or 128, every operand and stride a multiple of 16
+ * bytes. workspace: unok_tree_attn_workspace() bytes, 16-byte aligned (0: none is read). */
+int64_t unok_tree_attn_workspace(int B, int T, int nq, int nk, int D, int max_len);
+int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
+                   int64_t k_batch, int64_t k_head, int64_t k_row, const void* v, int64_t v_batch, int64_t v_head,
+                   int64_t v_row, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp,
+                   float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream);
+/* Depth of every node of B trees (parents [B, T] dense): its number of ancestors; 0 for roots and padding. */
+int unok_tree_depths(int B, int T, const int32_t* parents, int32_t* depths, void* stream);
+/* As unok_decode_prep for the nodes of a tree: node t's q and k are rotated to position lengths[b] + depth[b, t], its
+ * K and V go to cache rows lengths[b] + t, and its queries to q [B * T, nq * D]. */
+int unok_tree_prep(int B, int T, int nq, int nk, int D, const void* qkv, int64_t ld, const void* wq, const void* wk,
+                   const int64_t* lengths, const int32_t* depth, const float* inv_freq, float eps, void* kc, void* vc,
+                   int max_len, void* q, void* stream);
+/* The accepted path of a tree: in each of ntensors cache tensors [B, nk, max_len] rows of row_bytes (a multiple of 16, at most 512),
+ * row lengths[b] + nodes[b, i] goes to row lengths[b] + i for i < counts[b]; every row is read before any is
+ * written. nodes [B, P], P <= 256; entries outside [0, max_len - lengths[b]) are skipped. `caches` is a host array
+ * of device pointers. */
+int unok_cache_keep(int ntensors, void* const* caches, int row_bytes, int B, int nk, int max_len, int P,
+                    const int64_t* lengths, const int64_t* nodes, const int64_t* counts, void* stream);
+/* Copies sequences between cache slots: for each of npairs (source slot, destination slot) pairs and every tensor, rows
+ * [0, src_lengths[source]) (no more than either cache holds), and dst_lengths[destination] (null: left alone) becomes that number.
+ * src and dst are host arrays of ntensors device pointers, pairs a host array. No slot is written twice; source and
+ * destination tensors are disjoint, or the same, and then no slot is both read and written. */
+int unok_cache_copy(int ntensors, const void* const* src, void* const* dst, int row_bytes, int nk, int src_batch, int src_max,
+                    int dst_batch, int dst_max, const int64_t* src_lengths, int64_t* dst_lengths, int npairs,
+                    const int* pairs, void* stream);
+
 /* ---- Block-diffusion batch preparation ----------------------------------------------------- */
 
 /* Noising, [noisy | clean] concatenation, stream maps and interval tables of one batch.
@@ -362,6 +397,24 @@ int unok_lmhead_ce_grad(int R, int V, int K, const void* H, int64_t ldh, const v
 /* First-index argmax over vocab chunks: the "clean_argmax" CE target (training/losses.py:38-56). */
 int unok_row_argmax_update(int dtype, int R, int Vc, const void* z, int64_t ldz, int c0,
                            float* best_val, int64_t* best_idx, int first, void* stream);
+/* The k <= 256 largest values of each row of z [R, V] in descending order (equal values: the lower column first; NaN above
+ * every number), their columns, and the row's log-sum-exp. values [R, k] and lse [R] fp32, cols [R, k]. workspace:
+ * unok_row_topk_workspace() bytes, 8-byte aligned (0: none is read). */
+int64_t unok_row_topk_workspace(int R, int V, int k);
+int unok_row_topk(int dtype, int R, int V, int k, const void* z, int64_t ldz, float* values, int64_t* cols, float* lse,
+                  void* workspace, int64_t ws_bytes, void* stream);
+/* Distillation from a teacher's top logits t [R, k <= 256] at columns idx [R, k]: with p = softmax(t / tau) over a row's
+ * entries (t = -inf or a column outside [0, V): no entry) and q = softmax(z / tau) over the row's V columns,
+ * row_loss[r] = sum_i p_i (log p_i - log q_idx_i), 0 in a row without entries; row_stat [R, 2] (max and sum of q's
+ * exponentials) is what the backward reads. workspace: unok_distill_workspace() bytes, 8-byte aligned. */
+int64_t unok_distill_workspace(int R, int V);
+int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
+                     float* row_stat, float* row_loss, void* workspace, int64_t ws_bytes, void* stream);
+/* grad [R, V] = gscale[0] inv_n[0] tau (q - p), rows without entries 0: the gradient of tau^2 inv_n sum row_loss.
+ * grad may be z itself. */
+int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
+                     const float* row_stat, const float* gscale, const float* inv_n, void* grad, int64_t ldg, void* stream);
+
 /* Total variation / reverse KL over full-vocabulary logits (training/losses.py:59-183). */
 int unok_softmax_stats(int dtype, int R, int V, const void* z, int64_t ldz, float* mx, float* se,
                        void* stream);

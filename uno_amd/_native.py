@@ -18,7 +18,7 @@ _EINVAL, _EALIGN, _EUNSUPPORTED = -1, -2, -3
 
 _i, _i64, _p, _f = C.c_int, C.c_int64, C.c_void_p, C.c_float
 _u64 = C.c_uint64
-_ip = C.POINTER(C.c_int)
+_ip, _pp = C.POINTER(C.c_int), C.POINTER(C.c_void_p)
 
 
 class DraftLayerArgs(C.Structure):
@@ -69,6 +69,13 @@ SIGNATURES: dict[str, tuple] = {
     "unok_draft_layer_scratch": (_i64, [C.POINTER(DraftLayerArgs)]),
     "unok_draft_layer": (_i, [C.POINTER(DraftLayerArgs), _p]),
     "unok_decode_prep": (_i, [_i, _i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _f, _p, _p, _i, _p, _p]),
+    "unok_tree_attn_workspace": (_i64, [_i, _i, _i, _i, _i, _i]),
+    "unok_tree_attn": (_i, [_i, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _i64,
+                            _f, _p, _i64, _p, _i64, _p]),
+    "unok_tree_depths": (_i, [_i, _i, _p, _p, _p]),
+    "unok_tree_prep": (_i, [_i, _i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _p, _f, _p, _p, _i, _p, _p]),
+    "unok_cache_keep": (_i, [_i, _pp, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
+    "unok_cache_copy": (_i, [_i, _pp, _pp, _i, _i, _i, _i, _i, _i, _p, _p, _i, _ip, _p]),
     "unok_attn_bwd": (_i, [_i, _i, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64,
                            _p, _p, _p, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _f, _p]),
     "unok_attn_bwd_qknorm": (_i, [_i, _i, _i, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64,
@@ -89,6 +96,11 @@ SIGNATURES: dict[str, tuple] = {
     "unok_tv_bwd": (_i, [_i, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "unok_kl_fwd": (_i, [_i, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p]),
     "unok_kl_bwd": (_i, [_i, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "unok_row_topk_workspace": (_i64, [_i, _i, _i]),
+    "unok_row_topk": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _i64, _p]),
+    "unok_distill_workspace": (_i64, [_i, _i]),
+    "unok_distill_fwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _p, _p, _i64, _p]),
+    "unok_distill_bwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _p, _p, _p, _i64, _p]),
     "unok_sum_scaled": (_i, [_i64, _p, _p, _p, _p]),
     "unok_grad_clip_coef": (_i, [_i64, _p, _p, _i, _f, _p, _p]),
     "unok_adamw_step": (_i, [_i64, _p, _p, _p, _p, _p, _f, _f, _f, _f, _f, _i, _i, _p, _i64, _f, _p]),
@@ -156,6 +168,10 @@ def dtype_code(dt: torch.dtype) -> int:
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def ptr_array(tensors) -> C.Array:
+    return (C.c_void_p * max(1, len(tensors)))(*[t.data_ptr() for t in tensors])
 
 
 def int_array(values) -> C.Array:

@@ -37,10 +37,11 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found; the uno_amd kernel library cannot be built")
 
 
-# Per-file additions. attention.hip: MFMA accumulators in VGPRs, so the softmax and the
+# Per-file additions. The attention kernels: MFMA accumulators in VGPRs, so the softmax and the
 # accumulator rescale run on them directly instead of shuttling through AGPRs.
 FILE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

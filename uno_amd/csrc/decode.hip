@@ -463,13 +463,15 @@ bool rows_needs_ws(int epilogue, int R, int splits) { return splits > 1 || epilo
 //   combine  the S partial rows of each query merged by their log-sum-exp weights and written to
 //            the attention output [B * L, nq * D] at (b * L + t, head h).
 // ---------------------------------------------------------------------------------------
-template <int D>
+// TREE: node t's position is lengths[b] + depth[b, t], and the queries stay rows [B * L, nq * D] in qd.
+template <int D, bool TREE>
 __global__ __launch_bounds__(256) void decode_prep_kernel(const bf16_t* __restrict__ qkv, int64_t ld,
                                                           const bf16_t* __restrict__ wq, const bf16_t* __restrict__ wk,
                                                           const int64_t* __restrict__ lengths,
                                                           const float* __restrict__ inv_freq, float eps,
                                                           bf16_t* __restrict__ kc, bf16_t* __restrict__ vc,
-                                                          int max_len, bf16_t* __restrict__ qd, int B, int L, int nq,
+                                                          int max_len, bf16_t* __restrict__ qd,
+                                                          const int32_t* __restrict__ depth, int B, int L, int nq,
                                                           int nk) {
   constexpr int LPH = D / 8, HALF = D / 2;          // lanes per head row, 8 elements per lane
   const int lane = threadIdx.x & 63;
@@ -479,6 +481,7 @@ __global__ __launch_bounds__(256) void decode_prep_kernel(const bf16_t* __restri
   const int64_t heads = (int64_t)M * nh;
   const int pad = 128 - rep * L;
   if (item >= heads) {
+    if (TREE) return;
     // zero padding rows of the decode query layout
     const int64_t z = item - heads;
     if (z >= (int64_t)B * nk * pad) return;
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(256) void decode_prep_kernel(const bf16_t* __restri
         x[2 * i + 1] = x[2 * i + 1] * r * w1;
       }
     }
-    const float p = (float)(len + t);
+    const float p = (float)(len + (TREE ? depth[m] : t));
     const int j0 = c0 % HALF;
     const float sgn = c0 < HALF ? -1.f : 1.f;
     float out[8];
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(256) void decode_prep_kernel(const bf16_t* __restri
     for (int e = 0; e < 8; ++e) x[e] = out[e];
     if (isq) {
       const int kv = hd / rep, rr = hd % rep;
-      dst = qd + ((int64_t)(b * nk + kv) * 128 + rr * L + t) * D;
+      dst = qd + (TREE ? (int64_t)m * nq + hd : (int64_t)(b * nk + kv) * 128 + rr * L + t) * D;
     } else {
       if (len + t >= max_len) return;
       dst = kc + ((int64_t)(b * nk + hd - nq) * max_len + len + t) * D;
@@ -741,14 +744,40 @@ UNOK_EXPORT int unok_decode_prep(int B, int L, int nq, int nk, int D, const void
   const int64_t blocks = ((heads + pads) * lph + 255) / 256;
   hipStream_t st = (hipStream_t)stream;
   if (D == 128)
-    hipLaunchKernelGGL((decode_prep_kernel<128>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
+    hipLaunchKernelGGL((decode_prep_kernel<128, false>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
                        (const bf16_t*)wq, (const bf16_t*)wk, lengths, inv_freq, eps, (bf16_t*)kc, (bf16_t*)vc, max_len,
-                       (bf16_t*)qd, B, L, nq, nk);
+                       (bf16_t*)qd, (const int32_t*)nullptr, B, L, nq, nk);
   else
-    hipLaunchKernelGGL((decode_prep_kernel<64>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
+    hipLaunchKernelGGL((decode_prep_kernel<64, false>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
                        (const bf16_t*)wq, (const bf16_t*)wk, lengths, inv_freq, eps, (bf16_t*)kc, (bf16_t*)vc, max_len,
-                       (bf16_t*)qd, B, L, nq, nk);
+                       (bf16_t*)qd, (const int32_t*)nullptr, B, L, nq, nk);
   return unok::check_launch("decode_prep");
+}
+
+// The same for the nodes of a tree: positions lengths[b] + depth[b, t], queries into q [B * T, nq * D].
+UNOK_EXPORT int unok_tree_prep(int B, int T, int nq, int nk, int D, const void* qkv, int64_t ld, const void* wq, const void* wk,
+                               const int64_t* lengths, const int32_t* depth, const float* inv_freq, float eps, void* kc, void* vc,
+                               int max_len, void* q, void* stream) {
+  UNOK_REQUIRE(B >= 0 && T >= 0 && nq > 0 && nk > 0 && nq % nk == 0, UNOK_EINVAL, "tree_prep: B=%d T=%d nq=%d nk=%d", B, T,
+               nq, nk);
+  if (B == 0 || T == 0) return 0;
+  UNOK_REQUIRE(D == 64 || D == 128, UNOK_EINVAL, "tree_prep: head dim %d not in {64,128}", D);
+  UNOK_REQUIRE(qkv && lengths && depth && inv_freq && kc && vc && q, UNOK_EINVAL, "tree_prep: null operand");
+  UNOK_REQUIRE(ld % 8 == 0 && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)kc & 15) == 0 && ((uintptr_t)vc & 15) == 0 &&
+                   ((uintptr_t)q & 15) == 0 && ((uintptr_t)wq & 15) == 0 && ((uintptr_t)wk & 15) == 0,
+               UNOK_EALIGN, "tree_prep: rows must be 16-byte aligned");
+  const int64_t blocks = ((int64_t)B * T * (nq + 2 * nk) * (D / 8) + 255) / 256;
+  UNOK_REQUIRE(blocks < (1ll << 31) && (int64_t)B * T < (1ll << 31), UNOK_EINVAL, "tree_prep: grid too large");
+  hipStream_t st = (hipStream_t)stream;
+  if (D == 128)
+    hipLaunchKernelGGL((decode_prep_kernel<128, true>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
+                       (const bf16_t*)wq, (const bf16_t*)wk, lengths, inv_freq, eps, (bf16_t*)kc, (bf16_t*)vc, max_len,
+                       (bf16_t*)q, depth, B, T, nq, nk);
+  else
+    hipLaunchKernelGGL((decode_prep_kernel<64, true>), dim3((unsigned)blocks), dim3(256), 0, st, (const bf16_t*)qkv, ld,
+                       (const bf16_t*)wq, (const bf16_t*)wk, lengths, inv_freq, eps, (bf16_t*)kc, (bf16_t*)vc, max_len,
+                       (bf16_t*)q, depth, B, T, nq, nk);
+  return unok::check_launch("tree_prep");
 }
 
 // Merge of the S partial rows of split-key attention (see attn_split_combine_kernel). bf16.

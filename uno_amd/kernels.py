@@ -581,6 +581,166 @@ def decode_maps(lengths, B: int, L: int, nq: int, nk: int, max_len: int, S: int)
     return ivs, dst
 
 
+# ------------------------------------------------------------------------------------------
+# Trees of drafted tokens over the KV cache
+# ------------------------------------------------------------------------------------------
+def _same_device(what: str, *tensors: torch.Tensor) -> None:
+    """The operands lie on the current device, whose current stream the kernels are enqueued on."""
+    dev = torch.cuda.current_device() if tensors and tensors[0].is_cuda else None
+    for t in tensors:
+        if not t.is_cuda or t.device.index != dev:
+            raise RuntimeError(f"{what}: operands must be on the current device, got {t.device}")
+
+
+def _int64_vector(what: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int64 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be contiguous int64 [{n}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_caches(what: str, caches: Sequence[torch.Tensor]) -> torch.Tensor:
+    """Cache tensors of one shape [B, nk, max_len, D], dtype and device, contiguous; returns the first."""
+    if not caches:
+        raise RuntimeError(f"{what}: no cache tensors")
+    c = caches[0]
+    shape, dtype, device = c.shape, c.dtype, c.device
+    if c.dim() != 4:
+        raise RuntimeError(f"{what}: caches must be [B, nk, max_len, D], got {tuple(shape)}")
+    for t in caches:
+        if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise RuntimeError(f"{what}: caches must be contiguous {dtype} {tuple(shape)} on {device}, got {t.dtype} "
+                               f"{tuple(t.shape)} on {t.device}")
+    return c
+
+
+def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
+              scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens over a KV cache; returns [B*T, nq*D].
+
+    q [B*T, nq*D]: row b*T + t is node t of sequence b. k, v [B, nk, max_len, D] (any strides but the last): rows
+    [0, lengths[b]) are committed, row lengths[b] + t holds node t (rows at or past max_len do not exist).
+    lengths int64 [B]. parents int32 [B, T], or [T] for one tree of all sequences: the index of an earlier node,
+    -1 for a root, below -1 for padding, whose output rows are 0; a parent that is no earlier node, or is padding,
+    ends the chain. A node sees the committed rows, its ancestors and itself; what else the cache holds does not
+    matter. T <= 256, D 64 or 128, fp32 or bf16."""
+    _rowmajor(q, "q")
+    if k.dim() != 4 or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError(f"tree_attn: k and v must be [B, nk, max_len, D] in the dtype of q, got {tuple(k.shape)} "
+                           f"{tuple(v.shape)}")
+    B, nk, max_len, D = k.shape
+    if D > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
+        raise RuntimeError("tree_attn: k and v must have unit stride along their last dimension")
+    _int64_vector("tree_attn", "lengths", lengths, B)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or (parents.dim() == 2 and parents.shape[0] != B) \
+            or (parents.shape[-1] > 1 and parents.stride(-1) != 1):
+        raise RuntimeError(f"tree_attn: parents must be int32 [{B}, T] or [T], got {parents.dtype} {tuple(parents.shape)}")
+    T = parents.shape[-1]
+    ldp = parents.stride(0) if parents.dim() == 2 and B > 1 else 0
+    nq = q.shape[1] // D if D else 0
+    if q.shape[0] != B * T or nk == 0 or nq == 0 or nq % nk or nq * D != q.shape[1]:
+        raise RuntimeError(f"tree_attn: q must be [{B} * {T}, nq * {D}] with nq a multiple of {nk}, got {tuple(q.shape)}")
+    if out is None:
+        out = torch.empty((B * T, nq * D), device=q.device, dtype=q.dtype)
+    _rowmajor(out, "out")
+    if out.shape != (B * T, nq * D) or out.dtype != q.dtype:
+        raise RuntimeError("tree_attn: out must have the shape and dtype of q")
+    _same_device("tree_attn", q, k, v, lengths, parents, out)
+    ks, vs = ([t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)] for t in (k, v))
+    nbytes = N.lib().unok_tree_attn_workspace(B, T, nq, nk, D, max_len)
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    N.call("unok_tree_attn", N.dtype_code(q.dtype), B, T, nq, nk, D, N.ptr(q), _ld(q), N.ptr(k), *ks, N.ptr(v), *vs, max_len,
+           N.ptr(lengths), N.ptr(parents), ldp, float(D ** -0.5 if scale is None else scale), N.ptr(out), _ld(out), N.ptr(ws),
+           max(nbytes, 0), N.stream())
+    return out
+
+
+def tree_depths(parents: torch.Tensor) -> torch.Tensor:
+    """Depth [B, T] int32 of every node of the trees ``parents`` (int32 [B, T], as tree_attn reads them): roots and
+    padding 0."""
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
+        raise RuntimeError("tree_depths: contiguous int32 parents [B, T] required")
+    _same_device("tree_depths", parents)
+    out = torch.empty_like(parents)
+    N.call("unok_tree_depths", *parents.shape, N.ptr(parents), N.ptr(out), N.stream())
+    return out
+
+
+def tree_prep(qkv, wq, wk, lengths, depths, inv_freq, eps: float, kc, vc, B: int, T: int, nq: int, nk: int, D: int):
+    """q/k norm + RoPE of a tree's qkv rows [B*T, (nq+2nk)*D] at positions lengths + depths, its K/V rows into the
+    caches kc / vc [B, nk, max_len, D] at rows lengths + t; returns the queries [B*T, nq*D]."""
+    _rowmajor(qkv, "qkv")
+    if qkv.dtype != torch.bfloat16 or qkv.shape != (B * T, (nq + 2 * nk) * D):
+        raise RuntimeError("tree_prep: bf16 qkv [B*T, (nq+2nk)*D] required")
+    _int64_vector("tree_prep", "lengths", lengths, B)
+    if depths.dtype != torch.int32 or depths.shape != (B, T) or not depths.is_contiguous():
+        raise RuntimeError("tree_prep: contiguous int32 depths [B, T] required")
+    if _check_caches("tree_prep", (kc, vc)).shape[:2] != (B, nk) or kc.shape[3] != D or kc.dtype != qkv.dtype:
+        raise RuntimeError("tree_prep: bf16 caches [B, nk, max_len, D] required")
+    for w in (wq, wk):
+        if w is not None and (w.numel() != D or w.dtype != qkv.dtype or not w.is_contiguous()):
+            raise RuntimeError("tree_prep: norm weights must be [D] in the dtype of qkv")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+        raise RuntimeError("tree_prep: fp32 inv_freq [D/2] required")
+    q = torch.empty((B * T, nq * D), device=qkv.device, dtype=qkv.dtype)
+    _same_device("tree_prep", qkv, lengths, depths, inv_freq, kc)
+    N.call("unok_tree_prep", B, T, nq, nk, D, N.ptr(qkv), _ld(qkv), N.ptr(wq), N.ptr(wk), N.ptr(lengths), N.ptr(depths),
+           N.ptr(inv_freq), float(eps), N.ptr(kc), N.ptr(vc), kc.shape[2], N.ptr(q), N.stream())
+    return q
+
+
+def cache_keep(caches: Sequence[torch.Tensor], lengths: torch.Tensor, nodes: torch.Tensor, counts: torch.Tensor) -> None:
+    """Keeps the accepted nodes of drafted trees: in every cache tensor ([B, nk, max_len, D], contiguous, K and V of
+    all layers) row lengths[b] + nodes[b, i] moves to row lengths[b] + i for i < counts[b]. Every row is read before
+    any is written. nodes int64 [B, P], P <= 256; entries whose row does not exist are skipped. The lengths
+    stay as they are."""
+    c = _check_caches("cache_keep", caches)
+    B, nk, max_len, D = c.shape
+    _int64_vector("cache_keep", "lengths", lengths, B)
+    _int64_vector("cache_keep", "counts", counts, B)
+    if nodes.dtype != torch.int64 or nodes.dim() != 2 or nodes.shape[0] != B or not nodes.is_contiguous():
+        raise RuntimeError(f"cache_keep: nodes must be contiguous int64 [{B}, P], got {nodes.dtype} {tuple(nodes.shape)}")
+    _same_device("cache_keep", c, lengths, nodes, counts)
+    N.call("unok_cache_keep", len(caches), N.ptr_array(caches), D * c.element_size(), B, nk, max_len, nodes.shape[1],
+           N.ptr(lengths), N.ptr(nodes), N.ptr(counts), N.stream())
+
+
+def cache_copy(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], src_lengths: torch.Tensor,
+               dst_lengths: torch.Tensor, pairs: Sequence[tuple[int, int]]) -> None:
+    """Copies sequences between cache slots: for every (source slot, destination slot) of ``pairs`` and every tensor
+    ([batch, nk, max_len, D], contiguous; the batch and max_len of src and dst may differ) the source's committed
+    rows, as many as both caches hold, and dst_lengths[destination] becomes their number. src and dst may be the same
+    tensors: then no slot is both read and written. No slot is written twice."""
+    s, d = _check_caches("cache_copy", src), _check_caches("cache_copy", dst)
+    if len(src) != len(dst) or s.shape[1] != d.shape[1] or s.shape[3] != d.shape[3] or s.dtype != d.dtype:
+        raise RuntimeError(f"cache_copy: {len(src)} caches {s.dtype} {tuple(s.shape)} do not match {len(dst)} {d.dtype} "
+                           f"{tuple(d.shape)}")
+    _int64_vector("cache_copy", "source lengths", src_lengths, s.shape[0])
+    _int64_vector("cache_copy", "destination lengths", dst_lengths, d.shape[0])
+    _same_device("cache_copy", s, d, src_lengths, dst_lengths)
+    flat = [int(i) for pair in pairs for i in pair]
+    if len(flat) != 2 * len(pairs):
+        raise RuntimeError("cache_copy: pairs must be (source slot, destination slot)")
+    N.call("unok_cache_copy", len(src), N.ptr_array(src), N.ptr_array(dst), s.shape[3] * s.element_size(), s.shape[1],
+           s.shape[0], s.shape[2], d.shape[0], d.shape[2], N.ptr(src_lengths), N.ptr(dst_lengths), len(pairs),
+           N.int_array(flat), N.stream())
+
+
+def row_top_k(z: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The k <= 256 largest values of each row of z [R, V] (fp32 or bf16) in descending order: (values [R, k] fp32,
+    columns [R, k] int64, log-sum-exp [R] fp32 of the whole row). Equal values: the lower column first; NaN counts as
+    larger than every number."""
+    _rowmajor(z, "z")
+    R, V = z.shape
+    _same_device("row_top_k", z)
+    values = torch.empty((R, k), device=z.device, dtype=torch.float32)
+    cols = torch.empty((R, k), device=z.device, dtype=torch.int64)
+    lse = torch.empty(R, device=z.device, dtype=torch.float32)
+    nbytes = N.lib().unok_row_topk_workspace(R, V, k)
+    ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes > 0 else None
+    N.call("unok_row_topk", N.dtype_code(z.dtype), R, V, k, N.ptr(z), _ld(z), N.ptr(values), N.ptr(cols), N.ptr(lse),
+           N.ptr(ws), nbytes, N.stream())
+    return values, cols, lse
+
+
 def attn_bwd_qknorm(q, k1, v1, iv, o, lse, do, Hq, Hkv, D, k2, v2, pre, rstd, wq, wk, pos, cos_tab, sin_tab, dqkv,
                     scale=None):
     """Noisy-stream backward with the q/k RMSNorm + RoPE backward in the dQ / dK epilogues (bf16): writes

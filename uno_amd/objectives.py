@@ -11,6 +11,8 @@
   (training/losses.py:38-56, target source "clean_argmax").
 * ``distribution_losses``: reverse KL and total variation (training/losses.py:59-183) over
   bf16 logits of the supervised rows, fp32 per-row statistics, with hand-written backward.
+* ``top_k_distillation_loss``: forward KL from a teacher of which only the top logits are kept
+  (``teacher_top_k``), over the student's logits.
 """
 from __future__ import annotations
 
@@ -24,6 +26,8 @@ DEFAULT_CE_CHUNK = 32768
 # The bf16 CE keeps the LM-head logits of its rows (fp32) from the forward for the backward when
 # they take at most this many bytes; beyond it the backward recomputes them inside its GEMM.
 CE_STORED_LOGITS_MAX_BYTES = 6 << 30
+# Rows of teacher logits that teacher_top_k holds at a time (2.5 GB in bf16 at 151936 columns).
+TOP_K_ROWS = 8192
 
 
 def lm_head_logits(lm_head, x: torch.Tensor) -> torch.Tensor:
@@ -173,6 +177,102 @@ def logits_argmax(z: torch.Tensor) -> torch.Tensor:
         N.call("unok_row_argmax_update", N.dtype_code(z.dtype), R, V, N.ptr(z), z.stride(0) if R > 1 else V, 0,
                N.ptr(best_val), N.ptr(best_idx), 1, N.stream())
     return best_idx
+
+
+@torch.no_grad()
+def teacher_top_k(lm_head, h_rows: torch.Tensor, k: int, rows: int = TOP_K_ROWS):
+    """The top k logits of a teacher's hidden rows: (values [R, k] fp32, vocabulary indices [R, k], log-sum-exp [R]),
+    ``rows`` rows of logits at a time (K.row_top_k)."""
+    h_rows = h_rows.contiguous()
+    parts = [K.row_top_k(K.gemm_nt(h_rows[r:r + rows], lm_head.weight), k) for r in range(0, h_rows.shape[0], rows)]
+    if not parts:
+        f32 = dict(device=h_rows.device, dtype=torch.float32)
+        return torch.empty((0, k), **f32), torch.empty((0, k), device=h_rows.device, dtype=torch.int64), torch.empty(0, **f32)
+    return parts[0] if len(parts) == 1 else tuple(torch.cat(p) for p in zip(*parts))
+
+
+def _distill_operands(z: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, temperature: float) -> None:
+    if z.dim() != 2 or values.shape != indices.shape or values.dim() != 2 or values.shape[0] != z.shape[0]:
+        raise RuntimeError(f"top-k distillation: teacher values and indices [rows, k] must match the student's rows, got "
+                           f"{tuple(values.shape)} {tuple(indices.shape)} for {tuple(z.shape)}")
+    if indices.dtype != torch.int64:
+        raise RuntimeError("top-k distillation: teacher indices must be int64")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError("top-k distillation: the temperature must be positive and finite")
+    for t in (values, indices):
+        if t.device != z.device:
+            raise RuntimeError(f"top-k distillation: teacher on {t.device}, student on {z.device}")
+
+
+def _distill_fwd(z, values, indices, inv_n, temperature):
+    """(loss, row statistics for _distill_bwd) over [R, V] logits with unit column stride."""
+    R, V = z.shape
+    f32 = dict(device=z.device, dtype=torch.float32)
+    stat, rows, loss = torch.empty((R, 2), **f32), torch.empty(R, **f32), torch.empty((), **f32)
+    nbytes = N.lib().unok_distill_workspace(R, V)
+    ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8)
+    N.call("unok_distill_fwd", N.dtype_code(z.dtype), R, V, values.shape[1], N.ptr(z), z.stride(0), N.ptr(values),
+           N.ptr(indices), temperature, N.ptr(stat), N.ptr(rows), N.ptr(ws), nbytes, N.stream())
+    N.call("unok_sum_scaled", R, N.ptr(rows), N.ptr(inv_n), N.ptr(loss), N.stream())
+    return loss * (temperature * temperature) if temperature != 1.0 else loss, stat
+
+
+def _distill_bwd(z, values, indices, stat, g, inv_n, temperature, grad):
+    g = g.reshape(1).float().contiguous()
+    N.call("unok_distill_bwd", N.dtype_code(z.dtype), *z.shape, values.shape[1], N.ptr(z), z.stride(0), N.ptr(values),
+           N.ptr(indices), temperature, N.ptr(stat), N.ptr(g), N.ptr(inv_n), N.ptr(grad), grad.stride(0), N.stream())
+    return grad
+
+
+class TopKDistillation(torch.autograd.Function):
+    """Distillation from a teacher's top logits over the LM head: logits from h_s (differentiable), gradient formed in
+    their place. See top_k_distillation_loss."""
+
+    @staticmethod
+    def forward(ctx, h_s, values, indices, w_lm, w_lm_t, inv_n, temperature):
+        z = K.gemm_nt(h_s.contiguous(), w_lm)
+        loss, stat = _distill_fwd(z, values, indices, inv_n, temperature)
+        ctx.save = (z, values, indices, stat, inv_n, w_lm_t, temperature)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        z, values, indices, stat, inv_n, w_lm_t, temperature = ctx.save
+        ctx.save = None
+        _distill_bwd(z, values, indices, stat, g, inv_n, temperature, z)
+        return K.gemm_nt(z, w_lm_t), None, None, None, None, None, None
+
+
+def top_k_distillation_loss(lm_head, h_s: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, inv_n: torch.Tensor,
+                            temperature: float = 1.0) -> torch.Tensor:
+    """tau^2 inv_n sum over rows of KL(p || q): p = softmax(values / tau) over a row's teacher entries ([R, k] logits and
+    their vocabulary indices, k <= 256, as teacher_top_k returns them), q = softmax of the student's logits / tau over the
+    whole vocabulary. Entries of value -inf, or with an index outside the vocabulary, do not count; a row without
+    entries contributes nothing, to the loss and to the gradient. The teacher is not differentiated."""
+    _distill_operands(h_s, values, indices, temperature)
+    if h_s.shape[0] == 0:
+        return h_s.sum() * 0.0
+    return TopKDistillation.apply(h_s, values.detach().float().contiguous(), indices.contiguous(), lm_head.weight,
+                                  lm_head.weight_t, inv_n, float(temperature))
+
+
+class LogitsTopKDistillation(torch.autograd.Function):
+    """The same over given logits (the losses.py call surface); gradient w.r.t. the student's."""
+
+    @staticmethod
+    def forward(ctx, z, values, indices, inv_n, temperature):
+        if z.stride(1) != 1 and z.shape[1] > 1:
+            z = z.contiguous()
+        loss, stat = _distill_fwd(z, values, indices, inv_n, temperature)
+        ctx.save_for_backward(z, values, indices, stat, inv_n)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        z, values, indices, stat, inv_n = ctx.saved_tensors
+        grad = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        return _distill_bwd(z, values, indices, stat, g, inv_n, ctx.temperature, grad), None, None, None, None
 
 
 class DistributionLoss(torch.autograd.Function):

@@ -9,7 +9,8 @@ from __future__ import annotations
 import torch
 
 from ..layers import GatherRows
-from ..objectives import LogitsDistributionLoss, lm_head_logits, logits_argmax
+from ..objectives import (LogitsDistributionLoss, LogitsTopKDistillation, _distill_operands, lm_head_logits,
+                          logits_argmax)
 from .constants import IGNORE_INDEX
 
 
@@ -87,5 +88,24 @@ def token_normalized_total_variation(student_logits, teacher_logits, num_tokens:
     return LogitsDistributionLoss.apply(s, teacher_logits.detach().reshape(-1, V), _inv_n(s, num_tokens), "tv")
 
 
+def token_normalized_top_k_distillation(student_logits, teacher_values, teacher_indices, num_tokens: int,
+                                        temperature: float = 1.0) -> torch.Tensor:
+    """temperature^2 times KL(teacher || student) summed over rows, divided by max(num_tokens, 1), from the teacher's top
+    logits alone: teacher_values / teacher_indices [..., k] (k <= 256, uno_amd.objectives.teacher_top_k or
+    uno_amd.kernels.row_top_k), the teacher's distribution being their softmax and the student's that of all its logits,
+    both at ``temperature``. Entries of value -inf or with an index outside the vocabulary do not count; rows
+    without entries contribute nothing."""
+    V = student_logits.size(-1)
+    s = student_logits.reshape(-1, V)
+    values = teacher_values.detach().reshape(-1, teacher_values.shape[-1])
+    indices = teacher_indices.reshape(-1, teacher_indices.shape[-1])
+    _distill_operands(s, values, indices, temperature)
+    if not s.size(0):
+        return s.sum() * 0.0
+    return LogitsTopKDistillation.apply(s, values.float().contiguous(), indices.contiguous(), _inv_n(s, num_tokens),
+                                        float(temperature))
+
+
 __all__ = ["shift_labels_for_next_token", "project_hidden_states", "resolve_ce_targets",
-           "token_normalized_reverse_kl", "token_normalized_total_variation", "lm_head_logits"]
+           "token_normalized_reverse_kl", "token_normalized_total_variation", "token_normalized_top_k_distillation",
+           "lm_head_logits"]
