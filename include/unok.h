@@ -311,7 +311,7 @@ int unok_draft_layer(const unok_draft_layer_args* args, void* stream);
  * padding. Q and O [B T, nq D] with row strides ldq / ldo, q head h reading K/V head h / (nq / nk); K and V row
  * (b, head, j) at b * batch + head * head stride + j * row stride. dtype 0 / 1, D 64 or 128, every operand and stride a multiple of 16
  * bytes. workspace: unok_tree_attn_workspace() bytes, 16-byte aligned (0: none is read). */
-int64_t unok_tree_attn_workspace(int B, int T, int nq, int nk, int D, int max_len);
+int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len);
 int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
                    int64_t k_batch, int64_t k_head, int64_t k_row, const void* v, int64_t v_batch, int64_t v_head,
                    int64_t v_row, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp,

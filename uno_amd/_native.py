@@ -69,7 +69,7 @@ SIGNATURES: dict[str, tuple] = {
     "unok_draft_layer_scratch": (_i64, [C.POINTER(DraftLayerArgs)]),
     "unok_draft_layer": (_i, [C.POINTER(DraftLayerArgs), _p]),
     "unok_decode_prep": (_i, [_i, _i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _f, _p, _p, _i, _p, _p]),
-    "unok_tree_attn_workspace": (_i64, [_i, _i, _i, _i, _i, _i]),
+    "unok_tree_attn_workspace": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
     "unok_tree_attn": (_i, [_i, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _i64,
                             _f, _p, _i64, _p, _i64, _p]),
     "unok_tree_depths": (_i, [_i, _i, _p, _p, _p]),

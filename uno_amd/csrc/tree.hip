@@ -17,6 +17,7 @@
 // within fp32 and bf16 range), so that most tiles pass without a reduction across lanes. Scores,
 // statistics and outputs are fp32; the weights of bf16 products are rounded to bf16, as their V is.
 #include "common.h"
+#include "lds_tile.h"
 #include "../../include/unok.h"
 
 #include <type_traits>
@@ -24,7 +25,6 @@
 namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int TREE_MAX = 256, TREE_WORDS = TREE_MAX / 32;
 
@@ -34,17 +34,69 @@ struct TreeAttn {
   int64_t kb, kh, kr, vb, vh, vr;
   const int64_t* lengths;
   const int32_t* parents; int64_t ldp;               // row stride 0: one tree for all sequences
-  int B, T, nq, nk, max_len, S, rt;
+  int B, T, nq, nk, max_len, rt, target;             // rt: row tiles per (sequence, K/V head)
   void* o; int64_t ldo;
-  float *po, *pm;                                    // S > 1: partial outputs [pair][S][rep T][D] and (max, sum) pairs
+  float *po, *pm;                                    // partial outputs [range][nk][rep T][D], (max, sum) pairs
   float scale_log2;
 };
 
-// Keys [lo, hi) of range s of S ranges over `end` keys: ranges are whole steps of four waves' tiles of KT keys, at
-// least two steps long, so a short sequence leaves the later ranges empty.
-__device__ __forceinline__ int tree_step(int end, int S, int kt) {
-  const int step = 4 * kt, steps = (end + step - 1) / step, per = (steps + S - 1) / S;
-  return (per < 2 ? 2 : per) * step;
+// How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
+// together. A range is c blocks of TB keys, c the least from 4 on for which all ranges together make about
+// `target` workgroups; a sequence's ranges are evened out, and numbered after those of the sequences before it.
+constexpr int TB = 64;
+
+struct Range { int b, n, end, first, count, lo, hi; };   // sequence, its lengths, its ranges, this range's keys
+
+__device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
+  const int64_t len = a.lengths[b];
+  n = (int)(len < 0 ? 0 : len < a.max_len ? len : a.max_len);
+  return n + a.T < a.max_len ? n + a.T : a.max_len;
+}
+
+// Finds range `id` (by_range), or the ranges of sequence `id`. Every wave of the workgroup does it for itself.
+template <bool BY_RANGE> __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int n, blocks = 0;
+    if (b0 + lane < a.B) blocks = (tree_end(a, b0 + lane, n) + TB - 1) / TB;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) blocks += __shfl_xor(blocks, o, 64);
+    total += blocks;
+  }
+  const int64_t wgs = total * a.nk * a.rt;
+  const int c = (int)max((wgs + a.target - 1) / a.target, (int64_t)4);
+  Range r{-1, 0, 0, 0, 0, 0, 0};
+  int first = 0;
+  for (int b0 = 0; b0 < a.B && r.b < 0; b0 += 64) {
+    int n = 0, end = 0, count = 0;
+    if (b0 + lane < a.B) {
+      end = tree_end(a, b0 + lane, n);
+      count = ((end + TB - 1) / TB + c - 1) / c;
+    }
+    int upto = count;                                // ranges of the sequences up to this lane's
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
+    }
+    const uint64_t hit = BY_RANGE ? __ballot(id < first + upto) : __ballot(b0 + lane == id);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      r.b = b0 + l;
+      r.n = __shfl(n, l, 64);
+      r.end = __shfl(end, l, 64);
+      r.count = __shfl(count, l, 64);
+      r.first = first + __shfl(upto, l, 64) - r.count;
+    }
+    first += __shfl(upto, 63, 64);
+  }
+  if (BY_RANGE && r.b >= 0) {
+    const int blocks = (r.end + TB - 1) / TB, per = (blocks + r.count - 1) / r.count;
+    r.lo = (id - r.first) * per * TB;
+    r.hi = min(r.lo + per * TB, r.end);
+  }
+  return r;
 }
 
 // Each node's ancestors (itself among them) as bits, by pointer doubling: thread t holds node t's set and how far
@@ -241,16 +293,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   __shared__ int next[TREE_MAX];
 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-  const int pairs = a.B * a.nk, rep = a.nq / a.nk, T = a.T, NR = rep * T;
-  const int lin = xcd_remap(blockIdx.x, pairs * a.S * a.rt);
-  const int tile = lin % a.rt, pair = lin / a.rt % pairs, split = lin / (a.rt * pairs);
-  const int b = pair / a.nk, h = pair % a.nk;
-  const int64_t len = a.lengths[b];
-  const int n = (int)(len < 0 ? 0 : len < a.max_len ? len : a.max_len);
-  const int end = n + T < a.max_len ? n + T : a.max_len;
-  const int per = tree_step(end, a.S, KT);
-  const int lo = split * per, hi = lo + per < end ? lo + per : end;
-  if (lo >= end) return;
+  const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
+  const int lin = xcd_remap(blockIdx.x, gridDim.x);
+  const int tile = lin % a.rt, h = lin / a.rt % a.nk, id = lin / (a.rt * a.nk);
+  const Range range = tree_range<true>(a, id);
+  if (range.b < 0 || range.lo >= range.hi) return;
+  const int b = range.b, n = range.n, end = range.end, lo = range.lo, hi = range.hi;
 
   if (hi > n) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
   const int W = (T + 31) / 32;
@@ -413,7 +461,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
         *(f32x4_t*)(dst + Ops::dim(c, e, g)) = f32x4_t{o[i][c][e] * f, o[i][c + 1][e] * f, o[i][c + 2][e] * f, o[i][c + 3][e] * f};
   }
   __syncthreads();
-  const bool whole = per >= end;                         // this range is the only one
+  const bool whole = range.count == 1;
   for (int it = threadIdx.x; it < ROWS * (D / 4); it += 256) {
     const int rl = it / (D / 4), d = it % (D / 4) * 4, r = tile * ROWS + rl;
     if (r >= NR) continue;
@@ -436,36 +484,312 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
       if constexpr (sizeof(E) == 2) *(u32x2_t*)dst = u32x2_t{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
       else *(f32x4_t*)dst = x;
     } else {
-      const int64_t at = ((int64_t)pair * a.S + split) * NR + r;
+      const int64_t at = ((int64_t)id * a.nk + h) * NR + r;
       *(f32x4_t*)(a.po + at * D + d) = x;
       if (d == 0) { a.pm[2 * at] = top; a.pm[2 * at + 1] = sum; }
     }
   }
 }
 
-// The ranges of each query row merged: one thread per four dims. Sequences short enough for one range were written by
-// the kernel above.
+// bf16, more than 32 query rows: K and V tiles of 64 keys in LDS (two stages, filled by direct-to-LDS loads one tile
+// ahead), 32x32x16 MFMAs, 32 rows per wave. RG = 4: the four waves take four row groups and all keys; RG = 2: two row groups
+// and one half of every tile's keys each, merged at the end. S^T = K Q^T puts a query in a lane's column; P^T goes to the
+// P V product from the accumulators, V's columns come by LDS transpose loads (see lds_tile.h).
+template <int D, int RG>
+__global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a) {
+  constexpr int NKS = D / 16, NDT = D / 32, NKK = RG / 2, ROWS = 32 * RG, TILE = TB * D;
+  constexpr int STAGE = 2 * TILE;                       // a stage: the K tile, then the V tile
+  extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+  __shared__ uint32_t anc[TREE_MAX * TREE_WORDS];
+  __shared__ int next[TREE_MAX];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, lq = lane & 31;
+  const int wid = __builtin_amdgcn_readfirstlane(w);
+  const int rep = a.nq / a.nk, T = a.T, NR = rep * T, W = (T + 31) / 32;
+  const int lin = xcd_remap(blockIdx.x, gridDim.x);
+  const int tile0 = lin % a.rt, h = lin / a.rt % a.nk, id = lin / (a.rt * a.nk);
+  const Range range = tree_range<true>(a, id);
+  if (range.b < 0 || range.lo >= range.hi) return;
+  const int b = range.b, n = range.n, lo = range.lo, hi = range.hi;
+  const bf16_t* kbase = (const bf16_t*)a.k + b * a.kb + h * a.kh;
+  const bf16_t* vbase = (const bf16_t*)a.v + b * a.vb + h * a.vh;
+  const uint32_t ko = dma_lane_off<D>(a.kr, 0, wid, lane), vo = dma_lane_off<D>(a.vr, 0, wid, lane);
+  auto fetch = [&](int key, int stage) {               // rows at or past hi read as zeros
+    dma_tile<D>(kbase, a.kr, ko, key, hi, smem + stage * STAGE, wid);
+    dma_tile<D>(vbase, a.vr, vo, key, hi, smem + stage * STAGE + TILE, wid);
+  };
+  fetch(lo, 0);
+  if (hi > n) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
+
+  // this lane's query (rows past the pair's last repeat it; their results are dropped)
+  const int row = tile0 * ROWS + (wid % RG) * 32 + lq, rc = row < NR ? row : NR - 1, node = rc % T;
+  const int half = RG == 2 ? wid / 2 : 0;
+  bf16x8_t q[NKS];
+  {
+    const bf16_t* qp = (const bf16_t*)a.q + ((int64_t)b * T + node) * a.ldq + ((int64_t)h * rep + rc / T) * D;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) q[ks] = *(const bf16x8_t*)(qp + ks * 16 + g * 8);
+  }
+  float m = -INFINITY, l = 0.f;
+  f32x16_t o[NDT];
+#pragma unroll
+  for (int t = 0; t < NDT; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[t][j] = 0.f;
+
+  int koff[NKS];
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) koff[ks] = lq * D + (((ks * 2 + g) ^ kswz<D>(lq)) << 3) + half * 32 * D;
+  uint2 vaddr[NDT];
+  const uint32_t vbase0 = lds_addr(smem + TILE) + half * 32 * D * 2;
+#pragma unroll
+  for (int t = 0; t < NDT; ++t) {
+    const int2 off = tr_frag_off<D>(t, lane);
+    vaddr[t] = make_uint2(vbase0 + 2 * off.x, vbase0 + 2 * off.y);
+  }
+
+  // One tile: of committed rows, which every query sees, in stage ST; or (MASKED) with tree rows, in stage `stage`.
+  auto tile = [&](const int key, const int stage, auto stc, auto maskc) {
+    constexpr bool MASKED = decltype(maskc)::value;
+    constexpr int ST = decltype(stc)::value;
+    const int at = MASKED ? stage * STAGE : ST * STAGE;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                                    // the tile is in LDS; every wave is done with the one before
+    bool odd = false;
+    if constexpr (MASKED) {
+      // An infinity or NaN in a V row that some queries do not see: 0 in the product, added afterwards where seen.
+      uint32_t* vt = (uint32_t*)(smem + at + TILE);
+      for (int i = tid; i < TILE / 2; i += 256) odd |= (vt[i] & 0x7f80u) == 0x7f80u || (vt[i] & 0x7f800000u) == 0x7f800000u;
+      odd = __syncthreads_or(odd);
+      if (odd) {
+        for (int i = tid; i < TILE / 2; i += 256) {
+          uint32_t u = vt[i];
+          if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+          if ((u & 0x7f800000u) == 0x7f800000u) u &= 0x0000ffffu;
+          vt[i] = u;
+        }
+        __syncthreads();
+      }
+    }
+    const int ahead = MASKED ? stage ^ 1 : ST ^ 1;
+    if (key + TB < hi && !odd) fetch(key + TB, ahead);
+    const bf16_t* Kc = smem + at;
+    f32x16_t s[NKK];
+    {
+      bf16x8_t kf[NKK][NKS];
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) kf[kk][ks] = *(const bf16x8_t*)(Kc + kk * 32 * D + koff[ks]);
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[kk][j] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s[kk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk][ks], q[ks], s[kk], 0, 0, 0);
+      }
+    }
+    // V operands of the 16-key steps of half kk
+    u32x2_t vlo[NKK][2][NDT], vhi[NKK][2][NDT];
+    auto issue_v = [&](int kk) {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int t = 0; t < NDT; ++t) {
+          const uint32_t dyn = MASKED ? stage * STAGE * 2 : 0;
+          tr_issue_p<D, MASKED ? 0 : ST * STAGE * 2>(make_uint2(vaddr[t].x + dyn, vaddr[t].y + dyn), kk * 2 + hh, vlo[kk][hh][t],
+                                                     vhi[kk][hh][t]);
+        }
+    };
+    issue_v(0);
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = key + (half + kk) * 32 + 8 * (j >> 2) + 4 * g + (j & 3), t = r - n;
+          if (t >= 0 && (r >= hi || !(anc[node * W + t / 32] >> (t % 32) & 1))) s[kk][j] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, s[kk][j]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale_log2;
+    const bool grow = top > m + 8.f;
+    if (__ballot(grow)) {
+      // (for the queries that need it alone: a row's result does not depend on the rows beside it)
+      const float to = grow ? top : m, f = !grow ? 1.f : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < NDT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.f : -m;
+    bf16x8_t p[NKK][2];
+    auto weights = [&](int kk) {
+      float e[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(fmaf(s[kk][j], a.scale_log2, ref));
+        l += e[j];
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+        p[kk][hh] = __builtin_bit_cast(bf16x8_t, u32x4_t{pack2_bf16(e[8 * hh], e[8 * hh + 1]), pack2_bf16(e[8 * hh + 2], e[8 * hh + 3]),
+                                                         pack2_bf16(e[8 * hh + 4], e[8 * hh + 5]), pack2_bf16(e[8 * hh + 6], e[8 * hh + 7])});
+      if (MASKED && odd) {
+        // this half's weights (-1: not seen) through the free stage, its V rows from memory
+        float* ws = (float*)(smem + ahead * STAGE) + wid * 1024;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          ws[(8 * (j >> 2) + 4 * g + (j & 3)) * 32 + lq] = s[kk][j] == -INFINITY ? -1.f : e[j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int j = 0; j < 32; ++j) {
+          const int r = key + (half + kk) * 32 + j;
+          if (r >= hi) break;
+          const float x = ws[j * 32 + lq];          // (a NaN weight is seen)
+          const bf16_t* vr = vbase + (int64_t)r * a.vr + 4 * g;
+#pragma unroll
+          for (int t = 0; t < NDT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float y = bf16_to_f32(vr[32 * t + 8 * (i >> 2) + (i & 3)]);
+              if (!(x < 0.f) && !(fabsf(y) < INFINITY)) o[t][i] += x * y;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    };
+    auto pv = [&](int kk) {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int t = 0; t < NDT; ++t)
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_join(vlo[kk][hh][t], vhi[kk][hh][t]), p[kk][hh], o[t], 0, 0, 0);
+    };
+    weights(0);
+    tr_wait_all<NDT>(vlo[0], vhi[0]);
+    if constexpr (NKK == 2) {
+      issue_v(1);
+      pv(0);
+      weights(1);
+      tr_wait_all<NDT>(vlo[1], vhi[1]);
+      pv(1);
+    } else {
+      pv(0);
+    }
+    if (odd && key + TB < hi) {
+      __syncthreads();                                  // every wave has read its weights from the stage ahead
+      fetch(key + TB, ahead);
+    }
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  const int full = min(hi, n / TB * TB);                // (ranges begin at whole tiles)
+  int key = lo;
+#pragma unroll 1
+  for (; key + TB < full; key += 2 * TB) {
+    tile(key, 0, I0{}, std::false_type{});
+    tile(key + TB, 0, I1{}, std::false_type{});
+  }
+  int stage = 0;
+  if (key < full) {
+    tile(key, 0, I0{}, std::false_type{});
+    key += TB;
+    stage = 1;
+  }
+#pragma unroll 1
+  for (; key < hi; key += TB, stage ^= 1) tile(key, stage, I0{}, std::true_type{});
+  l += __shfl_xor(l, 32, 64);
+
+  if constexpr (RG == 2) {
+    // the second half's waves hand their outputs over, relative to the common maximum
+    float* mo = (float*)smem;                            // [2][NDT 16][64]
+    float* ml = mo + 2 * NDT * 16 * 64;                  // [4][64]
+    __syncthreads();
+    if (g == 0) { ml[wid * 64 + lq] = m; ml[wid * 64 + 32 + lq] = l; }
+    __syncthreads();
+    const float m2 = ml[(wid ^ 2) * 64 + lq], l2 = ml[(wid ^ 2) * 64 + 32 + lq], top = fmaxf(m, m2);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - top);
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        o[t][j] *= f;
+        if (wid >= 2) mo[((wid & 1) * NDT * 16 + t * 16 + j) * 64 + lane] = o[t][j];
+      }
+    l = wid < 2 ? l * f + l2 * f2 : l2 * f2 + l * f;
+    m = top;
+    __syncthreads();
+    if (wid >= 2) return;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[t][j] += mo[(wid * NDT * 16 + t * 16 + j) * 64 + lane];
+  }
+  if (row >= NR) return;
+  if (range.count == 1) {
+    const bool none = l == 0.f || a.parents[b * a.ldp + node] < -1;
+    bf16_t* dst = (bf16_t*)a.o + ((int64_t)b * T + node) * a.ldo + ((int64_t)h * rep + row / T) * D + 4 * g;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : o[t][4 * j + e] / l;
+        *(u32x2_t*)(dst + 32 * t + 8 * j) = u32x2_t{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
+      }
+  } else {
+    const int64_t at = ((int64_t)id * a.nk + h) * NR + row;
+    float* dst = a.po + at * D + 4 * g;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(f32x4_t*)(dst + 32 * t + 8 * j) = f32x4_t{o[t][4 * j], o[t][4 * j + 1], o[t][4 * j + 2], o[t][4 * j + 3]};
+    if (g == 0) { a.pm[2 * at] = m; a.pm[2 * at + 1] = l; }
+  }
+}
+
+// The ranges of each query row merged: one thread per four dims, grid (.., sequences). Sequences of one range were
+// written by the kernels above.
 template <typename E, int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a, int kt) {
-  const int rep = a.nq / a.nk, NR = rep * a.T;
-  const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = it / (D / 4);
-  const int d = (int)(it % (D / 4)) * 4;
-  if (row >= (int64_t)a.B * a.nk * NR) return;
-  const int pair = (int)(row / NR), r = (int)(row % NR), b = pair / a.nk, h = pair % a.nk, t = r % a.T;
-  const int64_t len = a.lengths[b];
-  const int n = (int)(len < 0 ? 0 : len < a.max_len ? len : a.max_len);
-  const int end = n + a.T < a.max_len ? n + a.T : a.max_len;
-  const int per = tree_step(end, a.S, kt), ranges = (end + per - 1) / per;
-  if (ranges == 1) return;
+__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
+  const int b = blockIdx.y, rep = a.nq / a.nk, NR = rep * a.T;
+  const Range range = tree_range<false>(a, b);
+  if (range.count <= 1) return;
+  const int it = blockIdx.x * 256 + threadIdx.x, row = it / (D / 4), d = it % (D / 4) * 4;
+  if (row >= a.nk * NR) return;
+  const int h = row / NR, r = row % NR, t = r % a.T;
+  const int64_t at0 = (int64_t)range.first * a.nk * NR + row, step = (int64_t)a.nk * NR;
+  // four ranges' rows in flight at a time; the ranges are few, so their maxima are read twice
   float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < ranges; ++s) top = fmaxf(top, a.pm[2 * (((int64_t)pair * a.S + s) * NR + r)]);
+  for (int s = 0; s < range.count; ++s) top = fmaxf(top, a.pm[2 * (at0 + s * step)]);
   f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ranges; ++s) {
-    const int64_t at = ((int64_t)pair * a.S + s) * NR + r;
-    const float ms = a.pm[2 * at], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - top);
-    sum += a.pm[2 * at + 1] * f;
-    x += *(const f32x4_t*)(a.po + at * D + d) * f;
+  for (int s0 = 0; s0 < range.count; s0 += 4) {
+    f32x4_t v[4];
+    float ms[4], ls[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = at0 + min(s0 + i, range.count - 1) * step;
+      v[i] = *(const f32x4_t*)(a.po + at * D + d);
+      ms[i] = s0 + i < range.count ? a.pm[2 * at] : -INFINITY;
+      ls[i] = a.pm[2 * at + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (ms[i] == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(ms[i] - top);
+      sum += ls[i] * f;
+      x += v[i] * f;
+    }
   }
   const bool none = sum == 0.f || a.parents[b * a.ldp + t] < -1;
 #pragma unroll
@@ -487,14 +811,16 @@ __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restr
   depths[(int64_t)blockIdx.x * T + t] = n > 0 ? n - 1 : 0;
 }
 
-int tree_qt(int NR) { return NR <= 16 ? 1 : NR <= 32 ? 2 : 4; }
+struct TreePlan { int rows, rt, target; int64_t ranges; };   // rows per row tile; most ranges of all sequences
 
-int tree_splits(int B, int T, int nq, int nk, int max_len) {
-  const int NR = nq / nk * T, rows = 16 * tree_qt(NR);
-  const int64_t wgs = (int64_t)B * nk * ((NR + rows - 1) / rows);
-  const int64_t want = (512 + wgs - 1) / wgs, most = (max_len + 255) / 256;
-  const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int max_len) {
+  const int NR = nq / nk * T;
+  TreePlan p;
+  p.rows = NR <= 16 ? 16 : NR <= 32 ? 32 : dtype == UNOK_F32 || NR <= 64 ? 64 : 128;
+  p.rt = (NR + p.rows - 1) / p.rows;
+  p.target = 512;
+  p.ranges = max_len + T <= 4 * TB ? B : B + p.target / ((int64_t)nk * p.rt);
+  return p;
 }
 
 int tree_sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
@@ -509,11 +835,11 @@ int tree_sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
 
 }  // namespace
 
-UNOK_EXPORT int64_t unok_tree_attn_workspace(int B, int T, int nq, int nk, int D, int max_len) {
+UNOK_EXPORT int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   if (tree_sizes_ok(B, T, nq, nk, D, max_len)) return -1;
   if (B == 0 || T == 0) return 0;
-  const int64_t S = tree_splits(B, T, nq, nk, max_len);
-  return S == 1 ? 0 : S * B * nq * T * (D + 2) * (int64_t)sizeof(float);
+  const TreePlan p = tree_plan(dtype, B, T, nq, nk, max_len);
+  return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float);
 }
 
 UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
@@ -525,49 +851,61 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn: bad dtype %d", dtype);
   if (B == 0 || T == 0) return 0;
   UNOK_REQUIRE(q && k && v && lengths && parents && o, UNOK_EINVAL, "tree_attn: null operand");
+  UNOK_REQUIRE(k_row >= D && v_row >= D && k_row < (1 << 23) && v_row < (1 << 23), UNOK_EINVAL,
+               "tree_attn: row strides %lld and %lld must lie in [D, 2^23)", (long long)k_row, (long long)v_row);
   UNOK_REQUIRE(ldp == 0 || ldp >= T, UNOK_EINVAL, "tree_attn: parents' row stride %lld for %d nodes", (long long)ldp, T);
   const int per16 = dtype == UNOK_BF16 ? 8 : 4;
   int64_t bits = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15;
   for (int64_t s : {ldq, k_batch, k_head, k_row, v_batch, v_head, v_row, ldo}) bits |= s % per16;
   UNOK_REQUIRE(bits == 0, UNOK_EALIGN, "tree_attn: operands and their strides must be multiples of 16 bytes");
-  const int64_t need = unok_tree_attn_workspace(B, T, nq, nk, D, max_len);
+  const int64_t need = unok_tree_attn_workspace(dtype, B, T, nq, nk, D, max_len);
   UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0), UNOK_EINVAL,
                "tree_attn: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)need, (long long)ws_bytes);
-  const int NR = nq / nk * T, qt = tree_qt(NR);
+  const TreePlan plan = tree_plan(dtype, B, T, nq, nk, max_len);
   TreeAttn a{};
   a.q = q; a.ldq = ldq; a.k = k; a.v = v;
   a.kb = k_batch; a.kh = k_head; a.kr = k_row; a.vb = v_batch; a.vh = v_head; a.vr = v_row;
   a.lengths = lengths; a.parents = parents; a.ldp = ldp;
   a.B = B; a.T = T; a.nq = nq; a.nk = nk; a.max_len = max_len;
-  a.S = tree_splits(B, T, nq, nk, max_len);
-  a.rt = (NR + 16 * qt - 1) / (16 * qt);
+  a.rt = plan.rt;
+  a.target = plan.target;
   a.o = o; a.ldo = ldo;
   a.po = (float*)workspace;
-  a.pm = a.po + (int64_t)a.S * B * nq * T * D;
+  a.pm = a.po + plan.ranges * nq * T * D;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t nb = (int64_t)B * nk * a.S * a.rt;
-  UNOK_REQUIRE(nb < (1ll << 31), UNOK_EINVAL, "tree_attn: grid too large");
+  const int64_t nb = plan.ranges * nk * plan.rt;
+  UNOK_REQUIRE(nb < (1ll << 31) && B < 65536, UNOK_EINVAL, "tree_attn: grid too large");
   hipStream_t st = (hipStream_t)stream;
-  auto go = [&](auto e, auto d, auto t) {
+  const dim3 grid((unsigned)nb), block(256);
+  auto run = [&](auto e, auto d) {
     using E = decltype(e);
-    constexpr int DD = decltype(d)::value, QT = decltype(t)::value;
-    constexpr size_t lds = 4ull * 16 * QT * (DD + 4) * sizeof(float);
-    UNOK_SET_LDS_ONCE((tree_attn_kernel<E, DD, QT>), lds);
-    hipLaunchKernelGGL((tree_attn_kernel<E, DD, QT>), dim3((unsigned)nb), dim3(256), lds, st, a);
-    if (a.S > 1) {
-      const int64_t items = (int64_t)B * nq * T * (DD / 4);
-      hipLaunchKernelGGL((tree_combine_kernel<E, DD>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a,
-                         TileOps<E, DD>::KT);
+    constexpr int DD = decltype(d)::value;
+    auto registers = [&](auto t) {
+      constexpr int QT = decltype(t)::value;
+      constexpr size_t lds = 4ull * 16 * QT * (DD + 4) * sizeof(float);
+      UNOK_SET_LDS_ONCE((tree_attn_kernel<E, DD, QT>), lds);
+      hipLaunchKernelGGL((tree_attn_kernel<E, DD, QT>), grid, block, lds, st, a);
+    };
+    if (plan.rows == 16) registers(std::integral_constant<int, 1>{});
+    else if (plan.rows == 32) registers(std::integral_constant<int, 2>{});
+    else if constexpr (sizeof(E) == 4) registers(std::integral_constant<int, 4>{});
+    else {
+      auto tiles = [&](auto g) {
+        constexpr int RG = decltype(g)::value;
+        constexpr size_t lds = 4ull * TB * DD * sizeof(bf16_t);
+        UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<DD, RG>), lds);
+        hipLaunchKernelGGL((tree_attn_lds_kernel<DD, RG>), grid, block, lds, st, a);
+      };
+      if (plan.rows == 64) tiles(std::integral_constant<int, 2>{});
+      else tiles(std::integral_constant<int, 4>{});
     }
-  };
-  auto by_rows = [&](auto e, auto d) {
-    if (qt == 1) go(e, d, std::integral_constant<int, 1>{});
-    else if (qt == 2) go(e, d, std::integral_constant<int, 2>{});
-    else go(e, d, std::integral_constant<int, 4>{});
+    if (plan.ranges > B)
+      hipLaunchKernelGGL((tree_combine_kernel<E, DD>), dim3((unsigned)(((int64_t)nq * T * (DD / 4) + 255) / 256), (unsigned)B),
+                         block, 0, st, a);
   };
   auto by_dim = [&](auto e) {
-    if (D == 128) by_rows(e, std::integral_constant<int, 128>{});
-    else by_rows(e, std::integral_constant<int, 64>{});
+    if (D == 128) run(e, std::integral_constant<int, 128>{});
+    else run(e, std::integral_constant<int, 64>{});
   };
   if (dtype == UNOK_BF16) by_dim(bf16_t{});
   else by_dim(float{});

@@ -644,8 +644,8 @@ def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.
     if out.shape != (B * T, nq * D) or out.dtype != q.dtype:
         raise RuntimeError("tree_attn: out must have the shape and dtype of q")
     _same_device("tree_attn", q, k, v, lengths, parents, out)
-    ks, vs = ([t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)] for t in (k, v))
-    nbytes = N.lib().unok_tree_attn_workspace(B, T, nq, nk, D, max_len)
+    ks, vs = ((*t.stride()[:2], t.stride(2) if max_len > 1 else D) for t in (k, v))
+    nbytes = N.lib().unok_tree_attn_workspace(N.dtype_code(q.dtype), B, T, nq, nk, D, max_len)
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
     N.call("unok_tree_attn", N.dtype_code(q.dtype), B, T, nq, nk, D, N.ptr(q), _ld(q), N.ptr(k), *ks, N.ptr(v), *vs, max_len,
            N.ptr(lengths), N.ptr(parents), ldp, float(D ** -0.5 if scale is None else scale), N.ptr(out), _ld(out), N.ptr(ws),
