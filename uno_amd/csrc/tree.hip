@@ -36,6 +36,7 @@ struct TreeAttn {
   const int32_t* parents; int64_t ldp;               // row stride 0: one tree for all sequences
   int B, T, nq, nk, max_len, rt, target;             // rt: row tiles per (sequence, K/V head)
   void* o; int64_t ldo;
+  int2* table;                                       // each sequence's (first range, ranges); null: never more than one
   float *po, *pm;                                    // partial outputs [range][nk][rep T][D], (max, sum) pairs
   float scale_log2;
 };
@@ -53,8 +54,24 @@ __device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
   return n + a.T < a.max_len ? n + a.T : a.max_len;
 }
 
-// Finds range `id` (by_range), or the ranges of sequence `id`. Every wave of the workgroup does it for itself.
-template <bool BY_RANGE> __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
+// A workgroup's row tile, K/V head and range. Workgroups go round the 8 XCDs: eight in a row take different (range,
+// head) pairs, and the row tiles of a pair follow on the same XCD, where they share its L2. (With neighbouring pairs on
+// one XCD instead, streams that are whole cache slots apart meet in the same memory channels: 8 sequences of
+// 4096 rows 46 us, this way 37; 16384 rows 141 and 117.)
+__device__ __forceinline__ void tree_place(const TreeAttn& a, int& tile, int& h, int& id) {
+  const int x = blockIdx.x, unit = x / (8 * a.rt) * 8 + x % 8;
+  tile = x / 8 % a.rt;
+  h = unit % a.nk;
+  id = unit / a.nk;
+}
+
+// Notes a sequence's ranges for the kernel that merges them.
+__device__ __forceinline__ void tree_note(const TreeAttn& a, const Range& r, int id, int h, int tile) {
+  if (a.table && id == r.first && h == 0 && tile == 0 && threadIdx.x == 0) a.table[r.b] = make_int2(r.first, r.count);
+}
+
+// Finds range `id`. Every wave of the workgroup does it for itself.
+__device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
   const int lane = threadIdx.x & 63;
   int64_t total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -80,7 +97,7 @@ template <bool BY_RANGE> __device__ __forceinline__ Range tree_range(const TreeA
       const int x = __shfl_up(upto, o, 64);
       upto += lane >= o ? x : 0;
     }
-    const uint64_t hit = BY_RANGE ? __ballot(id < first + upto) : __ballot(b0 + lane == id);
+    const uint64_t hit = __ballot(id < first + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       r.b = b0 + l;
@@ -91,7 +108,7 @@ template <bool BY_RANGE> __device__ __forceinline__ Range tree_range(const TreeA
     }
     first += __shfl(upto, 63, 64);
   }
-  if (BY_RANGE && r.b >= 0) {
+  if (r.b >= 0) {
     const int blocks = (r.end + TB - 1) / TB, per = (blocks + r.count - 1) / r.count;
     r.lo = (id - r.first) * per * TB;
     r.hi = min(r.lo + per * TB, r.end);
@@ -294,11 +311,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
 
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
-  const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = lin % a.rt, h = lin / a.rt % a.nk, id = lin / (a.rt * a.nk);
-  const Range range = tree_range<true>(a, id);
+  int tile, h, id;
+  tree_place(a, tile, h, id);
+  const Range range = tree_range(a, id);
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, end = range.end, lo = range.lo, hi = range.hi;
+  tree_note(a, range, id, h, tile);
 
   if (hi > n) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
   const int W = (T + 31) / 32;
@@ -491,6 +509,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   }
 }
 
+// max over lanes l and l ^ 32
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // bf16, more than 32 query rows: K and V tiles of 64 keys in LDS (two stages, filled by direct-to-LDS loads one tile
 // ahead), 32x32x16 MFMAs, 32 rows per wave. RG = 4: the four waves take four row groups and all keys; RG = 2: two row groups
 // and one half of every tile's keys each, merged at the end. S^T = K Q^T puts a query in a lane's column; P^T goes to the
@@ -506,11 +530,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, lq = lane & 31;
   const int wid = __builtin_amdgcn_readfirstlane(w);
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T, W = (T + 31) / 32;
-  const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile0 = lin % a.rt, h = lin / a.rt % a.nk, id = lin / (a.rt * a.nk);
-  const Range range = tree_range<true>(a, id);
+  int tile0, h, id;
+  tree_place(a, tile0, h, id);
+  const Range range = tree_range(a, id);
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, lo = range.lo, hi = range.hi;
+  tree_note(a, range, id, h, tile0);
   const bf16_t* kbase = (const bf16_t*)a.k + b * a.kb + h * a.kh;
   const bf16_t* vbase = (const bf16_t*)a.v + b * a.vb + h * a.vh;
   const uint32_t ko = dma_lane_off<D>(a.kr, 0, wid, lane), vo = dma_lane_off<D>(a.vr, 0, wid, lane);
@@ -588,6 +613,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) s[kk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk][ks], q[ks], s[kk], 0, 0, 0);
       }
+      // every K fragment is read before the first product
+#pragma unroll
+      for (int i = 0; i < NKK * NKS; ++i) __builtin_amdgcn_sched_group_barrier(SG_DS_READ, 1, 0);
+#pragma unroll
+      for (int i = 0; i < NKK * NKS; ++i) __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
     // V operands of the 16-key steps of half kk
     u32x2_t vlo[NKK][2][NDT], vhi[NKK][2][NDT];
@@ -596,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
         for (int t = 0; t < NDT; ++t) {
-          const uint32_t dyn = MASKED ? stage * STAGE * 2 : 0;
+          const uint32_t dyn = MASKED ? at * 2 : 0;
           tr_issue_p<D, MASKED ? 0 : ST * STAGE * 2>(make_uint2(vaddr[t].x + dyn, vaddr[t].y + dyn), kk * 2 + hh, vlo[kk][hh][t],
                                                      vhi[kk][hh][t]);
         }
@@ -616,7 +647,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
     for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, s[kk][j]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale_log2;
+    top = half_max(top) * a.scale_log2;
     const bool grow = top > m + 8.f;
     if (__ballot(grow)) {
       // (for the queries that need it alone: a row's result does not depend on the rows beside it)
@@ -676,8 +707,16 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
     tr_wait_all<NDT>(vlo[0], vhi[0]);
     if constexpr (NKK == 2) {
       issue_v(1);
+      // the first half's products run while the VALU forms the second half's weights
       pv(0);
       weights(1);
+      if constexpr (!MASKED) {
+#pragma unroll
+        for (int i = 0; i < 2 * NDT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(SG_VALU, 56 / (2 * NDT), 0);
+        }
+      }
       tr_wait_all<NDT>(vlo[1], vhi[1]);
       pv(1);
     } else {
@@ -691,13 +730,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   const int full = min(hi, n / TB * TB);                // (ranges begin at whole tiles)
-  int key = lo;
+  int key = lo, stage = 0;
 #pragma unroll 1
   for (; key + TB < full; key += 2 * TB) {
     tile(key, 0, I0{}, std::false_type{});
     tile(key + TB, 0, I1{}, std::false_type{});
   }
-  int stage = 0;
   if (key < full) {
     tile(key, 0, I0{}, std::false_type{});
     key += TB;
@@ -763,24 +801,24 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
 template <typename E, int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
   const int b = blockIdx.y, rep = a.nq / a.nk, NR = rep * a.T;
-  const Range range = tree_range<false>(a, b);
-  if (range.count <= 1) return;
+  const int2 range = a.table[b];                       // first, count
+  if (range.y <= 1) return;
   const int it = blockIdx.x * 256 + threadIdx.x, row = it / (D / 4), d = it % (D / 4) * 4;
   if (row >= a.nk * NR) return;
   const int h = row / NR, r = row % NR, t = r % a.T;
-  const int64_t at0 = (int64_t)range.first * a.nk * NR + row, step = (int64_t)a.nk * NR;
+  const int64_t at0 = (int64_t)range.x * a.nk * NR + row, step = (int64_t)a.nk * NR;
   // four ranges' rows in flight at a time; the ranges are few, so their maxima are read twice
   float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < range.count; ++s) top = fmaxf(top, a.pm[2 * (at0 + s * step)]);
+  for (int s = 0; s < range.y; ++s) top = fmaxf(top, a.pm[2 * (at0 + s * step)]);
   f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < range.count; s0 += 4) {
+  for (int s0 = 0; s0 < range.y; s0 += 4) {
     f32x4_t v[4];
     float ms[4], ls[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t at = at0 + min(s0 + i, range.count - 1) * step;
+      const int64_t at = at0 + min(s0 + i, range.y - 1) * step;
       v[i] = *(const f32x4_t*)(a.po + at * D + d);
-      ms[i] = s0 + i < range.count ? a.pm[2 * at] : -INFINITY;
+      ms[i] = s0 + i < range.y ? a.pm[2 * at] : -INFINITY;
       ls[i] = a.pm[2 * at + 1];
     }
 #pragma unroll
@@ -839,7 +877,7 @@ UNOK_EXPORT int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, in
   if (tree_sizes_ok(B, T, nq, nk, D, max_len)) return -1;
   if (B == 0 || T == 0) return 0;
   const TreePlan p = tree_plan(dtype, B, T, nq, nk, max_len);
-  return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float);
+  return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
 }
 
 UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
@@ -872,8 +910,9 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   a.o = o; a.ldo = ldo;
   a.po = (float*)workspace;
   a.pm = a.po + plan.ranges * nq * T * D;
+  a.table = plan.ranges > B ? (int2*)(a.pm + plan.ranges * nq * T * 2) : nullptr;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t nb = plan.ranges * nk * plan.rt;
+  const int64_t nb = (plan.ranges * nk + 7) / 8 * 8 * plan.rt;
   UNOK_REQUIRE(nb < (1ll << 31) && B < 65536, UNOK_EINVAL, "tree_attn: grid too large");
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)nb), block(256);
