@@ -34,7 +34,7 @@ struct TreeAttn {
   int64_t kb, kh, kr, vb, vh, vr;
   const int64_t* lengths;
   const int32_t* parents; int64_t ldp;               // row stride 0: one tree for all sequences
-  int B, T, nq, nk, max_len, rt, target;             // rt: row tiles per (sequence, K/V head)
+  int B, T, nq, nk, max_len, rt, share;              // row tiles per (sequence, K/V head); ranges to make of all keys
   void* o; int64_t ldo;
   int2* table;                                       // each sequence's (first range, ranges); null: never more than one
   float *po, *pm;                                    // partial outputs [range][nk][rep T][D], (max, sum) pairs
@@ -42,9 +42,9 @@ struct TreeAttn {
 };
 
 // How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
-// together. A range is c blocks of TB keys, c the least from 4 on for which all ranges together make about
-// `target` workgroups; a sequence's ranges are evened out, and numbered after those of the sequences before it.
-constexpr int TB = 64;
+// together. A range is at most c blocks of TB keys, c the least from TREE_LEAST on for which all sequences' keys make about
+// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it.
+constexpr int TB = 128, TREE_LEAST = 2;
 
 struct Range { int b, n, end, first, count, lo, hi; };   // sequence, its lengths, its ranges, this range's keys
 
@@ -70,46 +70,54 @@ __device__ __forceinline__ void tree_note(const TreeAttn& a, const Range& r, int
   if (a.table && id == r.first && h == 0 && tile == 0 && threadIdx.x == 0) a.table[r.b] = make_int2(r.first, r.count);
 }
 
+// Sum over lanes 0 .. l in lane l, by data-parallel moves within the wave.
+__device__ __forceinline__ int wave_scan(int v) {
+#define TREE_ADD(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
+  TREE_ADD(0x111, 0xf);                                  // row_shr 1, 2, 4, 8
+  TREE_ADD(0x112, 0xf);
+  TREE_ADD(0x114, 0xf);
+  TREE_ADD(0x118, 0xf);
+  TREE_ADD(0x142, 0xa);                                  // row_bcast 15 into rows 1 and 3
+  TREE_ADD(0x143, 0xc);                                  // row_bcast 31 into rows 2 and 3
+#undef TREE_ADD
+  return v;
+}
+
 // Finds range `id`. Every wave of the workgroup does it for itself.
 __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
+  int total = 0, n = 0, end = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int n, blocks = 0;
-    if (b0 + lane < a.B) blocks = (tree_end(a, b0 + lane, n) + TB - 1) / TB;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) blocks += __shfl_xor(blocks, o, 64);
-    total += blocks;
+    end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
+    total += __builtin_amdgcn_readlane(wave_scan((end + TB - 1) / TB), 63);
   }
-  const int64_t wgs = total * a.nk * a.rt;
-  const int c = (int)max((wgs + a.target - 1) / a.target, (int64_t)4);
+  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), TREE_LEAST);
+  // sequences end inside ranges: larger ones until no more than `share` are left (one round of workgroups)
+  if (a.B <= 64)
+    for (int i = 0; i < 12; ++i) {
+      const int count = (int)((uint32_t)((end + TB - 1) / TB + c - 1) / (uint32_t)c);
+      if (__builtin_amdgcn_readlane(wave_scan(count), 63) <= max(a.share, a.B)) break;
+      c += (c + 15) / 16;
+    }
   Range r{-1, 0, 0, 0, 0, 0, 0};
   int first = 0;
   for (int b0 = 0; b0 < a.B && r.b < 0; b0 += 64) {
-    int n = 0, end = 0, count = 0;
-    if (b0 + lane < a.B) {
-      end = tree_end(a, b0 + lane, n);
-      count = ((end + TB - 1) / TB + c - 1) / c;
-    }
-    int upto = count;                                // ranges of the sequences up to this lane's
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      upto += lane >= o ? x : 0;
-    }
+    if (a.B > 64) end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
+    const int count = (int)((uint32_t)((end + TB - 1) / TB + c - 1) / (uint32_t)c);
+    const int upto = wave_scan(count);                   // ranges of the sequences up to this lane's
     const uint64_t hit = __ballot(id < first + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       r.b = b0 + l;
-      r.n = __shfl(n, l, 64);
-      r.end = __shfl(end, l, 64);
-      r.count = __shfl(count, l, 64);
-      r.first = first + __shfl(upto, l, 64) - r.count;
+      r.n = __builtin_amdgcn_readlane(n, l);
+      r.end = __builtin_amdgcn_readlane(end, l);
+      r.count = __builtin_amdgcn_readlane(count, l);
+      r.first = first + __builtin_amdgcn_readlane(upto, l) - r.count;
     }
-    first += __shfl(upto, 63, 64);
+    first += __builtin_amdgcn_readlane(upto, 63);
   }
   if (r.b >= 0) {
-    const int blocks = (r.end + TB - 1) / TB, per = (blocks + r.count - 1) / r.count;
+    const int blocks = (r.end + TB - 1) / TB, per = (int)((uint32_t)(blocks + r.count - 1) / (uint32_t)r.count);
     r.lo = (id - r.first) * per * TB;
     r.hi = min(r.lo + per * TB, r.end);
   }
@@ -129,7 +137,13 @@ __device__ __forceinline__ void tree_ancestors(const int32_t* parents, int T, ui
   if (t < T) {
     p = parents[t];
     real = p >= -1;
-    if (p >= t || p < 0 || parents[p] < -1) p = -1;
+    next[t] = p;
+  }
+  __syncthreads();
+  const bool cut = t < T && (p >= t || p < 0 || next[p] < -1);
+  __syncthreads();
+  if (t < T) {
+    if (cut) p = -1;
 #pragma unroll
     for (int i = 0; i < TREE_WORDS; ++i) w[i] = real && t / 32 == i ? 1u << (t % 32) : 0u;
     for (int i = 0; i < W; ++i) anc[t * W + i] = real && t / 32 == i ? 1u << (t % 32) : 0u;
@@ -154,6 +168,13 @@ __device__ __forceinline__ void tree_ancestors(const int32_t* parents, int T, ui
     }
     __syncthreads();
   }
+}
+
+// Whether node t is among the ancestors of `node` (t outside the tree: some bit or other; no branch, so that it can stand in a
+// select).
+__device__ __forceinline__ bool tree_sees(const uint32_t* anc, int node, int W, int t) {
+  const int i = min(max(t >> 5, 0), W - 1);
+  return anc[node * W + i] >> (t & 31) & 1;
 }
 
 template <typename T, int D> struct TileOps;
@@ -306,6 +327,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   constexpr int KT = Ops::KT, NS = Ops::NS, NDT = Ops::NDT, NP = 4 * NS, ROWS = 16 * QT, LDO = D + 4;
   extern __shared__ __attribute__((aligned(16))) float merge_o[];     // [4][ROWS][LDO]
   __shared__ float merge_ml[4][ROWS][2];
+  __shared__ bool merge_pad[ROWS];
   __shared__ uint32_t anc[TREE_MAX * TREE_WORDS];
   __shared__ int next[TREE_MAX];
 
@@ -329,6 +351,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
     const int r = tile * ROWS + 16 * i + m, rc = r < NR ? r : NR - 1;
     node[i] = rc % T;
     Ops::load_q(q[i], (const E*)a.q + ((int64_t)b * T + node[i]) * a.ldq + ((int64_t)h * rep + rc / T) * D, g);
+    if (threadIdx.x < 16) merge_pad[16 * i + m] = a.parents[b * a.ldp + node[i]] < -1;
   }
 
   const E* kbase = (const E*)a.k + b * a.kb + h * a.kh;
@@ -420,7 +443,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const int r = key + Ops::slot_key(j, g), t = r - n;
-        if (t >= 0 && (r >= hi || !(anc[node[i] * W + t / 32] >> (t % 32) & 1))) p[i][j] = -INFINITY;
+        p[i][j] = r < hi && (t < 0 | tree_sees(anc, node[i], W, t)) ? p[i][j] : -INFINITY;
       }
     weights(p);
     const bool odd = __ballot(Ops::odd(v)) != 0;
@@ -447,7 +470,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
             if (!__ballot(!(fabsf(x) < INFINITY))) continue;
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
-              const bool seen = t < 0 || (anc[node[i] * W + t / 32] >> (t % 32) & 1);
+              const bool seen = t < 0 | tree_sees(anc, node[i], W, t);
               if (seen && !(fabsf(x) < INFINITY)) o[i][c][e] += ps[(16 * i + m) * (KT + 1) + j] * x;
             }
           }
@@ -495,7 +518,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
     }
     if (whole) {
       const int t = r % T;
-      const bool none = sum == 0.f || a.parents[b * a.ldp + t] < -1;
+      const bool none = sum == 0.f || merge_pad[rl];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / sum;
       E* dst = (E*)a.o + ((int64_t)b * T + t) * a.ldo + ((int64_t)h * rep + r / T) * D + d;
@@ -520,8 +543,12 @@ __device__ __forceinline__ float half_max(float v) {
 // and one half of every tile's keys each, merged at the end. S^T = K Q^T puts a query in a lane's column; P^T goes to the
 // P V product from the accumulators, V's columns come by LDS transpose loads (see lds_tile.h).
 template <int D, int RG>
-__global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a) {
-  constexpr int NKS = D / 16, NDT = D / 32, NKK = RG / 2, ROWS = 32 * RG, TILE = TB * D;
+__global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(const TreeAttn a) {
+  constexpr int NKS = D / 16, NDT = D / 32, ROWS = 32 * RG, NW = RG == 2 ? 4 : 8;
+  constexpr int KG = NW / RG, NKK = RG == 2 ? 1 : 2;    // key groups; a wave's 32-key parts of a tile
+  constexpr int TK = 32 * NKK * KG, TILE = TK * D;      // keys of a tile
+  constexpr int NST = RG == 8 ? 4 : 2;                  // stages
+  constexpr int LPT = TK * D * 2 * 2 / (1024 * NW);     // direct-to-LDS loads per wave and tile
   constexpr int STAGE = 2 * TILE;                       // a stage: the K tile, then the V tile
   extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
   __shared__ uint32_t anc[TREE_MAX * TREE_WORDS];
@@ -538,17 +565,23 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
   tree_note(a, range, id, h, tile0);
   const bf16_t* kbase = (const bf16_t*)a.k + b * a.kb + h * a.kh;
   const bf16_t* vbase = (const bf16_t*)a.v + b * a.vb + h * a.vh;
-  const uint32_t ko = dma_lane_off<D>(a.kr, 0, wid, lane), vo = dma_lane_off<D>(a.vr, 0, wid, lane);
+  const uint32_t ko = dma_lane_off<D, NW>(a.kr, 0, wid, lane), vo = dma_lane_off<D, NW>(a.vr, 0, wid, lane);
   auto fetch = [&](int key, int stage) {               // rows at or past hi read as zeros
-    dma_tile<D>(kbase, a.kr, ko, key, hi, smem + stage * STAGE, wid);
-    dma_tile<D>(vbase, a.vr, vo, key, hi, smem + stage * STAGE + TILE, wid);
+#pragma unroll
+    for (int i = 0; i < TK / 64; ++i) {
+      dma_tile<D, NW>(kbase, a.kr, ko, key + 64 * i, hi, smem + stage * STAGE + 64 * i * D, wid);
+      dma_tile<D, NW>(vbase, a.vr, vo, key + 64 * i, hi, smem + stage * STAGE + TILE + 64 * i * D, wid);
+    }
   };
-  fetch(lo, 0);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (lo + i * TK < hi) fetch(lo + i * TK, i);
   if (hi > n) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
 
   // this lane's query (rows past the pair's last repeat it; their results are dropped)
   const int row = tile0 * ROWS + (wid % RG) * 32 + lq, rc = row < NR ? row : NR - 1, node = rc % T;
-  const int half = RG == 2 ? wid / 2 : 0;
+  const int part = wid / RG * NKK;                       // this wave's first 32-key part of a tile
+  const bool pad = a.parents[b * a.ldp + node] < -1;
   bf16x8_t q[NKS];
   {
     const bf16_t* qp = (const bf16_t*)a.q + ((int64_t)b * T + node) * a.ldq + ((int64_t)h * rep + rc / T) * D;
@@ -564,9 +597,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
 
   int koff[NKS];
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) koff[ks] = lq * D + (((ks * 2 + g) ^ kswz<D>(lq)) << 3) + half * 32 * D;
+  for (int ks = 0; ks < NKS; ++ks) koff[ks] = lq * D + (((ks * 2 + g) ^ kswz<D>(lq)) << 3) + part * 32 * D;
   uint2 vaddr[NDT];
-  const uint32_t vbase0 = lds_addr(smem + TILE) + half * 32 * D * 2;
+  const uint32_t vbase0 = lds_addr(smem + TILE) + part * 32 * D * 2;
 #pragma unroll
   for (int t = 0; t < NDT; ++t) {
     const int2 off = tr_frag_off<D>(t, lane);
@@ -577,17 +610,21 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
   auto tile = [&](const int key, const int stage, auto stc, auto maskc) {
     constexpr bool MASKED = decltype(maskc)::value;
     constexpr int ST = decltype(stc)::value;
-    const int at = MASKED ? stage * STAGE : ST * STAGE;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                                    // the tile is in LDS; every wave is done with the one before
+    constexpr bool DYN = MASKED || NST > 2;             // the stage is no constant
+    const int at = DYN ? stage * STAGE : ST * STAGE;
+    // the tile is in LDS (the NST - 2 after it may still be on their way), and every wave is done with the one
+    // before, whose stage the next load overwrites
+    if (NST > 2 && key + (NST - 2) * TK < hi) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((NST - 2) * LPT) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     bool odd = false;
     if constexpr (MASKED) {
       // An infinity or NaN in a V row that some queries do not see: 0 in the product, added afterwards where seen.
       uint32_t* vt = (uint32_t*)(smem + at + TILE);
-      for (int i = tid; i < TILE / 2; i += 256) odd |= (vt[i] & 0x7f80u) == 0x7f80u || (vt[i] & 0x7f800000u) == 0x7f800000u;
+      for (int i = tid; i < TILE / 2; i += 64 * NW) odd |= (vt[i] & 0x7f80u) == 0x7f80u || (vt[i] & 0x7f800000u) == 0x7f800000u;
       odd = __syncthreads_or(odd);
       if (odd) {
-        for (int i = tid; i < TILE / 2; i += 256) {
+        for (int i = tid; i < TILE / 2; i += 64 * NW) {
           uint32_t u = vt[i];
           if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
           if ((u & 0x7f800000u) == 0x7f800000u) u &= 0x0000ffffu;
@@ -596,8 +633,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
         __syncthreads();
       }
     }
-    const int ahead = MASKED ? stage ^ 1 : ST ^ 1;
-    if (key + TB < hi && !odd) fetch(key + TB, ahead);
+    const int ahead = DYN ? (stage + NST - 1) % NST : ST ^ 1, next_key = key + (NST - 1) * TK;
+    if (next_key < hi && !odd) fetch(next_key, ahead);
     const bf16_t* Kc = smem + at;
     f32x16_t s[NKK];
     {
@@ -627,8 +664,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
         for (int t = 0; t < NDT; ++t) {
-          const uint32_t dyn = MASKED ? at * 2 : 0;
-          tr_issue_p<D, MASKED ? 0 : ST * STAGE * 2>(make_uint2(vaddr[t].x + dyn, vaddr[t].y + dyn), kk * 2 + hh, vlo[kk][hh][t],
+          const uint32_t dyn = at * 2;
+          tr_issue_p<D>(make_uint2(vaddr[t].x + dyn, vaddr[t].y + dyn), kk * 2 + hh, vlo[kk][hh][t],
                                                      vhi[kk][hh][t]);
         }
     };
@@ -638,8 +675,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
       for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const int r = key + (half + kk) * 32 + 8 * (j >> 2) + 4 * g + (j & 3), t = r - n;
-          if (t >= 0 && (r >= hi || !(anc[node * W + t / 32] >> (t % 32) & 1))) s[kk][j] = -INFINITY;
+          const int r = key + (part + kk) * 32 + 8 * (j >> 2) + 4 * g + (j & 3), t = r - n;
+          s[kk][j] = r < hi && (t < 0 | tree_sees(anc, node, W, t)) ? s[kk][j] : -INFINITY;
         }
     }
     float top = s[0][0];
@@ -681,7 +718,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
         for (int j = 0; j < 32; ++j) {
-          const int r = key + (half + kk) * 32 + j;
+          const int r = key + (part + kk) * 32 + j;
           if (r >= hi) break;
           const float x = ws[j * 32 + lq];          // (a NaN weight is seen)
           const bf16_t* vr = vbase + (int64_t)r * a.vr + 4 * g;
@@ -722,58 +759,72 @@ __global__ __launch_bounds__(256, 2) void tree_attn_lds_kernel(const TreeAttn a)
     } else {
       pv(0);
     }
-    if (odd && key + TB < hi) {
+    if (odd && next_key < hi) {
       __syncthreads();                                  // every wave has read its weights from the stage ahead
-      fetch(key + TB, ahead);
+      fetch(next_key, ahead);
     }
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
-  const int full = min(hi, n / TB * TB);                // (ranges begin at whole tiles)
+  const int full = lo + max(min(hi, n) - lo, 0) / TK * TK;
   int key = lo, stage = 0;
+  if constexpr (NST == 2) {
 #pragma unroll 1
-  for (; key + TB < full; key += 2 * TB) {
-    tile(key, 0, I0{}, std::false_type{});
-    tile(key + TB, 0, I1{}, std::false_type{});
-  }
-  if (key < full) {
-    tile(key, 0, I0{}, std::false_type{});
-    key += TB;
-    stage = 1;
+    for (; key + TK < full; key += 2 * TK) {
+      tile(key, 0, I0{}, std::false_type{});
+      tile(key + TK, 1, I1{}, std::false_type{});
+    }
+    if (key < full) {
+      tile(key, 0, I0{}, std::false_type{});
+      key += TK;
+      stage = 1;
+    }
+  } else {
+#pragma unroll 1
+    for (; key < full; key += TK, stage = (stage + 1) % NST) tile(key, stage, I0{}, std::false_type{});
   }
 #pragma unroll 1
-  for (; key < hi; key += TB, stage ^= 1) tile(key, stage, I0{}, std::true_type{});
+  for (; key < hi; key += TK, stage = (stage + 1) % NST) tile(key, stage, I0{}, std::true_type{});
   l += __shfl_xor(l, 32, 64);
 
-  if constexpr (RG == 2) {
-    // the second half's waves hand their outputs over, relative to the common maximum
-    float* mo = (float*)smem;                            // [2][NDT 16][64]
-    float* ml = mo + 2 * NDT * 16 * 64;                  // [4][64]
+  if constexpr (KG > 1) {
+    // the other key groups' waves hand their outputs over, relative to the common maximum
+    float* mo = (float*)smem;                            // [KG - 1][RG][NDT 16][64]
+    float* ml = mo + (KG - 1) * RG * NDT * 16 * 64;      // [NW][64]
+    const int rg = wid % RG;
     __syncthreads();
     if (g == 0) { ml[wid * 64 + lq] = m; ml[wid * 64 + 32 + lq] = l; }
     __syncthreads();
-    const float m2 = ml[(wid ^ 2) * 64 + lq], l2 = ml[(wid ^ 2) * 64 + 32 + lq], top = fmaxf(m, m2);
+    float top = ml[rg * 64 + lq];
+#pragma unroll
+    for (int i = 1; i < KG; ++i) top = fmaxf(top, ml[(i * RG + rg) * 64 + lq]);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      const float mi = ml[(i * RG + rg) * 64 + lq];
+      l += mi == -INFINITY ? 0.f : ml[(i * RG + rg) * 64 + 32 + lq] * __builtin_amdgcn_exp2f(mi - top);
+    }
     const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - top);
+    m = top;
 #pragma unroll
     for (int t = 0; t < NDT; ++t)
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         o[t][j] *= f;
-        if (wid >= 2) mo[((wid & 1) * NDT * 16 + t * 16 + j) * 64 + lane] = o[t][j];
+        if (wid >= RG) mo[((wid - RG) * NDT * 16 + t * 16 + j) * 64 + lane] = o[t][j];
       }
-    l = wid < 2 ? l * f + l2 * f2 : l2 * f2 + l * f;
-    m = top;
     __syncthreads();
-    if (wid >= 2) return;
+    if (wid >= RG) return;
 #pragma unroll
-    for (int t = 0; t < NDT; ++t)
+    for (int i = 0; i < KG - 1; ++i)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[t][j] += mo[(wid * NDT * 16 + t * 16 + j) * 64 + lane];
+      for (int t = 0; t < NDT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] += mo[((i * RG + wid) * NDT * 16 + t * 16 + j) * 64 + lane];
   }
   if (row >= NR) return;
   if (range.count == 1) {
-    const bool none = l == 0.f || a.parents[b * a.ldp + node] < -1;
+    const bool none = l == 0.f || pad;
     bf16_t* dst = (bf16_t*)a.o + ((int64_t)b * T + node) * a.ldo + ((int64_t)h * rep + row / T) * D + 4 * g;
 #pragma unroll
     for (int t = 0; t < NDT; ++t)
@@ -849,15 +900,16 @@ __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restr
   depths[(int64_t)blockIdx.x * T + t] = n > 0 ? n - 1 : 0;
 }
 
-struct TreePlan { int rows, rt, target; int64_t ranges; };   // rows per row tile; most ranges of all sequences
+struct TreePlan { int rows, rt, share; int64_t ranges; };   // rows per row tile; most ranges of all sequences
 
-TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int max_len) {
+TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   const int NR = nq / nk * T;
   TreePlan p;
-  p.rows = NR <= 16 ? 16 : NR <= 32 ? 32 : dtype == UNOK_F32 || NR <= 64 ? 64 : 128;
+  p.rows = NR <= 16 ? 16 : dtype == UNOK_F32 ? 32 : NR <= 64 ? 64 : NR <= 128 || D == 64 ? 128 : 256;
   p.rt = (NR + p.rows - 1) / p.rows;
-  p.target = 512;
-  p.ranges = max_len + T <= 4 * TB ? B : B + p.target / ((int64_t)nk * p.rt);
+  const int64_t share = (p.rows > 64 ? 256 : 512) / ((int64_t)nk * p.rt);   // one round of the workgroups that fit
+  p.share = share > 1 ? (int)share : 1;
+  p.ranges = max_len <= TREE_LEAST * TB ? B : B + p.share;
   return p;
 }
 
@@ -876,7 +928,7 @@ int tree_sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
 UNOK_EXPORT int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   if (tree_sizes_ok(B, T, nq, nk, D, max_len)) return -1;
   if (B == 0 || T == 0) return 0;
-  const TreePlan p = tree_plan(dtype, B, T, nq, nk, max_len);
+  const TreePlan p = tree_plan(dtype, B, T, nq, nk, D, max_len);
   return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
 }
 
@@ -899,14 +951,14 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   const int64_t need = unok_tree_attn_workspace(dtype, B, T, nq, nk, D, max_len);
   UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0), UNOK_EINVAL,
                "tree_attn: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)need, (long long)ws_bytes);
-  const TreePlan plan = tree_plan(dtype, B, T, nq, nk, max_len);
+  const TreePlan plan = tree_plan(dtype, B, T, nq, nk, D, max_len);
   TreeAttn a{};
   a.q = q; a.ldq = ldq; a.k = k; a.v = v;
   a.kb = k_batch; a.kh = k_head; a.kr = k_row; a.vb = v_batch; a.vh = v_head; a.vr = v_row;
   a.lengths = lengths; a.parents = parents; a.ldp = ldp;
   a.B = B; a.T = T; a.nq = nq; a.nk = nk; a.max_len = max_len;
   a.rt = plan.rt;
-  a.target = plan.target;
+  a.share = plan.share;
   a.o = o; a.ldo = ldo;
   a.po = (float*)workspace;
   a.pm = a.po + plan.ranges * nq * T * D;
@@ -925,18 +977,20 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
       UNOK_SET_LDS_ONCE((tree_attn_kernel<E, DD, QT>), lds);
       hipLaunchKernelGGL((tree_attn_kernel<E, DD, QT>), grid, block, lds, st, a);
     };
-    if (plan.rows == 16) registers(std::integral_constant<int, 1>{});
-    else if (plan.rows == 32) registers(std::integral_constant<int, 2>{});
-    else if constexpr (sizeof(E) == 4) registers(std::integral_constant<int, 4>{});
-    else {
+    if (plan.rows == 16) {
+      registers(std::integral_constant<int, 1>{});
+    } else if constexpr (sizeof(E) == 4) {
+      registers(std::integral_constant<int, 2>{});
+    } else {
       auto tiles = [&](auto g) {
         constexpr int RG = decltype(g)::value;
-        constexpr size_t lds = 4ull * TB * DD * sizeof(bf16_t);
+        constexpr size_t lds = (RG == 2 ? 128ull : 256ull) * 2 * DD * sizeof(bf16_t);   // all stages' keys
         UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<DD, RG>), lds);
-        hipLaunchKernelGGL((tree_attn_lds_kernel<DD, RG>), grid, block, lds, st, a);
+        hipLaunchKernelGGL((tree_attn_lds_kernel<DD, RG>), grid, dim3(RG == 2 ? 256 : 512), lds, st, a);
       };
       if (plan.rows == 64) tiles(std::integral_constant<int, 2>{});
-      else tiles(std::integral_constant<int, 4>{});
+      else if (plan.rows == 128) tiles(std::integral_constant<int, 4>{});
+      else if constexpr (DD == 128) tiles(std::integral_constant<int, 8>{});
     }
     if (plan.ranges > B)
       hipLaunchKernelGGL((tree_combine_kernel<E, DD>), dim3((unsigned)(((int64_t)nq * T * (DD / 4) + 255) / 256), (unsigned)B),
