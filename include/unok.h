@@ -405,15 +405,17 @@ int unok_row_topk(int dtype, int R, int V, int k, const void* z, int64_t ldz, fl
                   void* workspace, int64_t ws_bytes, void* stream);
 /* Distillation from a teacher's top logits t [R, k <= 256] at columns idx [R, k]: with p = softmax(t / tau) over a row's
  * entries (t = -inf or a column outside [0, V): no entry) and q = softmax(z / tau) over the row's V columns,
- * row_loss[r] = sum_i p_i (log p_i - log q_idx_i), 0 in a row without entries; row_stat [R, 2] (max and sum of q's
- * exponentials) is what the backward reads. workspace: unok_distill_workspace() bytes, 8-byte aligned. */
+ * loss[0] = scale inv_n[0] sum over rows with entries of sum_i p_i (log p_i - log q_idx_i) (inv_n null: 1); row_stat [R, 2] is
+ * what the backward reads. workspace: unok_distill_workspace() bytes, 8-byte aligned. */
 int64_t unok_distill_workspace(int R, int V);
 int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
-                     float* row_stat, float* row_loss, void* workspace, int64_t ws_bytes, void* stream);
-/* grad [R, V] = gscale[0] inv_n[0] tau (q - p), rows without entries 0: the gradient of tau^2 inv_n sum row_loss.
- * grad may be z itself. */
+                     const float* inv_n, float scale, float* row_stat, float* loss, void* workspace, int64_t ws_bytes,
+                     void* stream);
+/* grad [R, V] = gscale[0] inv_n[0] scale (q - p), rows without entries 0 (for the gradient, the forward's scale over
+ * tau). grad may be z itself. */
 int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
-                     const float* row_stat, const float* gscale, const float* inv_n, void* grad, int64_t ldg, void* stream);
+                     const float* row_stat, const float* gscale, const float* inv_n, float scale, void* grad, int64_t ldg,
+                     void* stream);
 
 /* Total variation / reverse KL over full-vocabulary logits (training/losses.py:59-183). */
 int unok_softmax_stats(int dtype, int R, int V, const void* z, int64_t ldz, float* mx, float* se,

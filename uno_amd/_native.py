@@ -99,8 +99,8 @@ SIGNATURES: dict[str, tuple] = {
     "unok_row_topk_workspace": (_i64, [_i, _i, _i]),
     "unok_row_topk": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _i64, _p]),
     "unok_distill_workspace": (_i64, [_i, _i]),
-    "unok_distill_fwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _p, _p, _i64, _p]),
-    "unok_distill_bwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _p, _p, _p, _i64, _p]),
+    "unok_distill_fwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _f, _p, _p, _p, _i64, _p]),
+    "unok_distill_bwd": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _f, _p, _p, _p, _f, _p, _i64, _p]),
     "unok_sum_scaled": (_i, [_i64, _p, _p, _p, _p]),
     "unok_grad_clip_coef": (_i, [_i64, _p, _p, _i, _f, _p, _p]),
     "unok_adamw_step": (_i, [_i64, _p, _p, _p, _p, _p, _f, _f, _f, _f, _f, _i, _i, _p, _i64, _f, _p]),
@@ -167,7 +167,7 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr_array(tensors) -> C.Array:

@@ -52,11 +52,50 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// Maximum over the wave, by data-parallel moves; the same value in every lane.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#define TK_MAX_STEP(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+  TK_MAX_STEP(0x111, 0xf);                               // row_shr 1, 2, 4, 8
+  TK_MAX_STEP(0x112, 0xf);
+  TK_MAX_STEP(0x114, 0xf);
+  TK_MAX_STEP(0x118, 0xf);
+  TK_MAX_STEP(0x142, 0xa);                               // row_bcast 15 into rows 1 and 3
+  TK_MAX_STEP(0x143, 0xc);                               // row_bcast 31 into rows 2 and 3
+#undef TK_MAX_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// The greatest t with at least k of the wave's N x 64 values v >= t, where `on` (0: a value that does not count, which no t
+// may reach); 0 if fewer than k count. SH low bits of t are not looked for: they are those of every value.
+template <int N, int SH>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[N], int used, int k) {
+  uint32_t top = 0, low = 0;                             // low: ~ of the least value that counts
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    top = max(top, v[j]);
+    low = max(low, v[j] == 0 ? 0u : ~v[j]);
+  }
+  uint32_t hi = wave_umax(top) >> SH, lo = (~wave_umax(low)) >> SH;
+  if (hi == 0) return 0;
+  // invariant: at least k values >= lo, or lo is the least value
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < used) n += __popcll(__ballot((v[j] >> SH) >= mid));
+    if (n >= k) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo << SH;
+}
+
 // Candidates of one wave: (value key, ~column) pairs in CAP entries of LDS, of which the wave's k largest are
 // always among the first `cnt`. Nothing with a value key <= `floor` can still enter the k largest.
 constexpr int TK_CAP = 512, TK_KEEP = 384, TK_MAX = 256;
 
-struct Candidates {
+// SH: value keys differ in their upper 32 - SH bits only (bf16: 16).
+template <int SH> struct Candidates {
   uint64_t* buf;
   int lane, k, cnt;
   uint32_t floor, next_floor;
@@ -77,10 +116,11 @@ struct Candidates {
   __device__ __forceinline__ void step_end() { floor = next_floor > floor ? next_floor : floor; }
 
   // Keeps the entries whose value is among the k largest, ties included; with `exact`, or when ties leave more than
-  // TK_KEEP, the k largest entries and no more. The k-th largest is found bit by bit with ballots.
+  // TK_KEEP, the k largest entries and no more.
   __device__ __forceinline__ void cut(bool exact) {
     if (cnt <= k) return;
     constexpr int NE = TK_CAP / 64;
+    const int used = (cnt + 63) / 64;
     uint32_t hi[NE], lo[NE];
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -90,34 +130,32 @@ struct Candidates {
       hi[j] = (uint32_t)(e >> 32);
       lo[j] = (uint32_t)e;
     }
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t c = t | (1u << bit);
-      int n = 0;
+    uint32_t t = kth_largest<NE, SH>(hi, used, k);
+    if (SH > 0) {                                        // the low bits: ones for negative values (and NaN), zeros for others
+      uint32_t low = 0;
 #pragma unroll
-      for (int j = 0; j < NE; ++j) n += __popcll(__ballot(hi[j] >= c));
-      if (n >= k) t = c;
+      for (int j = 0; j < NE; ++j) low = max(low, (hi[j] >> SH) == (t >> SH) ? hi[j] : 0u);
+      t = wave_umax(low);
     }
     int above = 0, tied = 0;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
+      if (j >= used) continue;
       above += __popcll(__ballot(hi[j] > t));
       tied += __popcll(__ballot(hi[j] == t));
     }
     uint32_t u = 0;                                    // least ~column of the kept ties
     if (above + tied > k && (exact || above + tied > TK_KEEP)) {
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = u | (1u << bit);
-        int n = 0;
+      uint32_t tie[NE];
 #pragma unroll
-        for (int j = 0; j < NE; ++j) n += __popcll(__ballot(hi[j] == t && lo[j] >= c));
-        if (n >= k - above) u = c;
-      }
+      for (int j = 0; j < NE; ++j) tie[j] = hi[j] == t ? lo[j] : 0u;
+      u = kth_largest<NE, 0>(tie, used, k - above);
     }
     __builtin_amdgcn_wave_barrier();
     int at = 0;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
+      if (j >= used) continue;
       const bool keep = hi[j] > t || (hi[j] == t && lo[j] >= u);
       const uint64_t mask = __ballot(keep);
       if (keep) buf[at + lanes_below(mask)] = ((uint64_t)hi[j] << 32) | lo[j];
@@ -138,18 +176,20 @@ __device__ __forceinline__ float floor_value(uint32_t floor) {
 
 // Merges the waves' candidates of a row: every wave leaves its at most k largest, and an entry's rank is the number
 // of larger entries.
-template <typename F>
-__device__ __forceinline__ void rank_entries(uint64_t* all, int* wave_cnt, Candidates& c, int k, int wid, F emit) {
+template <int SH, typename F>
+__device__ __forceinline__ void rank_entries(uint64_t* all, int* wave_cnt, Candidates<SH>& c, int k, int wid, F emit) {
   c.cut(true);
   if (c.lane == 0) wave_cnt[wid] = c.cnt;
   __syncthreads();
-  for (int i = threadIdx.x; i < 4 * k; i += 256) {
-    const int w = i / k, j = i % k;
-    if (j >= wave_cnt[w]) continue;
-    const uint64_t e = all[w * TK_CAP + j];
+  const int n0 = wave_cnt[0], n1 = n0 + wave_cnt[1], n2 = n1 + wave_cnt[2], n3 = n2 + wave_cnt[3];
+  for (int i = threadIdx.x; i < n3; i += 256) {
+    const int w = (i >= n0) + (i >= n1) + (i >= n2);
+    const uint64_t e = all[w * TK_CAP + i - (w == 0 ? 0 : w == 1 ? n0 : w == 2 ? n1 : n2)];
     int rank = 0;
+#pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int n = wave_cnt[v];
+#pragma unroll 8
       for (int q = 0; q < n; ++q) rank += all[v * TK_CAP + q] > e;
     }
     if (rank < k) emit(rank, e);
@@ -172,13 +212,18 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
   __shared__ uint64_t buf[4 * TK_CAP];
   __shared__ float red[32];
   __shared__ int wave_cnt[4];
+  __shared__ uint32_t bound_[4];                         // per wave: a value key that k of its elements reach
+  volatile uint32_t* bound = bound_;
+  if (threadIdx.x < 4) bound[threadIdx.x] = 0;
+  __syncthreads();
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
   const int c0 = part * width, n = min(width, V - c0);
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const T* p = z + row * ldz + c0;
   const Span<T> sp(p, n);
-  Candidates cand(buf + wid * TK_CAP, lane, k);
+  constexpr int SH = sizeof(T) == 2 ? 16 : 0;
+  Candidates<SH> cand(buf + wid * TK_CAP, lane, k);
   float m = -INFINITY, s = 0.f;
 
   constexpr uint32_t NOTHING = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
@@ -216,19 +261,24 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
 #pragma unroll
       for (int e = 0; e < N; ++e) s += fast_expf(v[e] - ref);
     }
+    // what the other waves have found by now spares this one candidates (whenever it is seen: the k largest are
+    // the same)
+    const uint32_t others = max(max(bound[0], bound[1]), max(bound[2], bound[3]));
+    if (others > 0 && others - 1 > cand.floor) cand.floor = others - 1;
     if (fresh) {
       fresh = false;
-      uint32_t t = 0, key[U];
+      uint32_t key[U];
+      int cnt = 0;
 #pragma unroll
-      for (int i = 0; i < U; ++i) key[i] = q0 + i * 64 + lane < sp.nv ? value_key(gm[i]) : 0u;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = t | (1u << bit);
-        int cnt = 0;
-#pragma unroll
-        for (int i = 0; i < U; ++i) cnt += __popcll(__ballot(key[i] >= c));
-        if (cnt >= k) t = c;
+      for (int i = 0; i < U; ++i) {
+        key[i] = q0 + i * 64 + lane < sp.nv ? value_key(gm[i]) : 0u;
+        cnt += __popcll(__ballot(key[i] != 0));
       }
-      if (t > 0 && t - 1 > cand.floor) cand.floor = t - 1;
+      if (cnt >= k) {
+        const uint32_t t = kth_largest<U, SH>(key, U, k);  // (its low bits zero: a bound all the same)
+        if (t > 0 && t - 1 > cand.floor) cand.floor = t - 1;
+        if (lane == 0) bound[wid] = t;
+      }
     }
     // bit 8 i + e (fp32: 4 i + e): element e of vector i may enter. (A lane that has met a NaN, which fmaxf
     // drops, looks into every vector from then on.)
@@ -254,6 +304,7 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
       may &= may - 1;
     }
     cand.step_end();
+    if (lane == 0 && cand.next_floor > bound[wid]) bound[wid] = cand.next_floor;
   }
   if (wid == 3) single(sp.tail(), n - sp.tail());
 
@@ -288,7 +339,7 @@ __global__ __launch_bounds__(256) void topk_merge_kernel(const uint64_t* __restr
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const uint64_t* src = ws_key + row * parts * k;
   const int n = parts * k;
-  Candidates cand(buf + wid * TK_CAP, lane, k);
+  Candidates<0> cand(buf + wid * TK_CAP, lane, k);
   for (int i = wid * 64; i < n; i += 256) {
     const uint64_t e = i + lane < n ? src[i + lane] : 0;
     cand.push(e != 0, (uint32_t)(e >> 32), ~(uint32_t)e);
@@ -325,42 +376,8 @@ int topk_parts(int R, int V) {
 // ---------------------------------------------------------------------------------------
 constexpr int DK_MAX = 256;
 
-// (max, sum of e^(x - max)) of x = z / tau over a part of a row; one workgroup per (row, part). Bound by HBM.
-template <typename T>
-__global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict__ z, int64_t ldz, int V, int parts,
-                                                            int width, float inv_tau, float2* __restrict__ stat) {
-  constexpr int N = VN<T>;
-  __shared__ float red[32];
-  const int64_t row = blockIdx.x / parts;
-  const int c0 = (int)(blockIdx.x % parts) * width, n = min(width, V - c0);
-  const T* p = z + row * ldz + c0;
-  const Span<T> sp(p, n);
-  float m = -INFINITY, s = 0.f;
-  const u32x4_t* pv = (const u32x4_t*)(p + sp.head);
-  for (int q = threadIdx.x; q < sp.nv; q += 256) {
-    float v[N];
-    unpack16<T>(pv[q], v);
-    float g = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < N; ++e) { v[e] *= inv_tau; g = fmaxf(g, v[e]); }
-    if (g > m) { s *= fast_expf(m - g); m = g; }
-    const float ref = m == -INFINITY ? 0.f : m;        // -inf then adds 0, and a NaN is seen
-#pragma unroll
-    for (int e = 0; e < N; ++e) s += fast_expf(v[e] - ref);
-  }
-  auto single = [&](float v) {
-    if (v > m) { s *= fast_expf(m - v); m = v; }
-    s += fast_expf(v - (m == -INFINITY ? 0.f : m));
-  };
-  for (int j = threadIdx.x; j < sp.head; j += 256) single(Elem<T>::load(p + j) * inv_tau);
-  for (int j = sp.tail() + threadIdx.x; j < n; j += 256) single(Elem<T>::load(p + j) * inv_tau);
-  const float mb = block_max(m, red);
-  s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
-  if (threadIdx.x == 0) stat[blockIdx.x] = make_float2(mb, s);
-}
-
-// The entries of a row as a wave sees them, entry lane + 64 i in step i: columns (-1: does not count) and
-// probabilities; returns whether there is any.
+// The entries of a row as a wave sees them, entry lane + 64 i in step i: columns (-1: does not count) and the
+// logarithms of their probabilities; returns whether there is any.
 template <typename F>
 __device__ __forceinline__ bool teacher_row(const float* __restrict__ t, const int64_t* __restrict__ idx, int k, int V,
                                             float inv_tau, int lane, F use) {
@@ -392,7 +409,63 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ t, const i
   return true;
 }
 
-// Per row: (max, sum of e^(z / tau - max)) from its parts, and sum_i p_i (log p_i - log q_i). One wave per row.
+// sum_i p_i (log p_i - log q_i) of a row, in one wave, from the row's (max, sum of e^(z / tau - max)).
+template <typename T>
+__device__ __forceinline__ float distill_row(const T* __restrict__ z, const float* __restrict__ t,
+                                             const int64_t* __restrict__ idx, int k, int V, float inv_tau, int lane, float m,
+                                             float s) {
+  const float l = logf(s);
+  float acc = 0.f;
+  teacher_row(t, idx, k, V, inv_tau, lane, [&](int, int col, float logp) {
+    if (col < 0) return;
+    const float pr = expf(logp);
+    if (!(pr == 0.f)) acc += pr * (logp - (Elem<T>::load(z + col) * inv_tau - m) + l);
+  });
+  return wave_sum(acc);
+}
+
+// (max, sum of e^(x - max)) of x = z / tau over a part of a row; one workgroup per (row, part). A row in one part also gets
+// its loss. Bound by HBM.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict__ z, int64_t ldz, int V, int parts,
+                                                            int width, int k, const float* __restrict__ t,
+                                                            const int64_t* __restrict__ idx, float inv_tau,
+                                                            float2* __restrict__ stat, float* __restrict__ row_loss) {
+  constexpr int N = VN<T>;
+  __shared__ float red[32];
+  const int64_t row = blockIdx.x / parts;
+  const int c0 = (int)(blockIdx.x % parts) * width, n = min(width, V - c0);
+  const T* p = z + row * ldz + c0;
+  const Span<T> sp(p, n);
+  float m = -INFINITY, s = 0.f;
+  const u32x4_t* pv = (const u32x4_t*)(p + sp.head);
+  for (int q = threadIdx.x; q < sp.nv; q += 256) {
+    float v[N];
+    unpack16<T>(pv[q], v);
+    float g = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) { v[e] *= inv_tau; g = fmaxf(g, v[e]); }
+    if (g > m) { s *= fast_expf(m - g); m = g; }
+    const float ref = m == -INFINITY ? 0.f : m;        // -inf then adds 0, and a NaN is seen
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += fast_expf(v[e] - ref);
+  }
+  auto single = [&](float v) {
+    if (v > m) { s *= fast_expf(m - v); m = v; }
+    s += fast_expf(v - (m == -INFINITY ? 0.f : m));
+  };
+  for (int j = threadIdx.x; j < sp.head; j += 256) single(Elem<T>::load(p + j) * inv_tau);
+  for (int j = sp.tail() + threadIdx.x; j < n; j += 256) single(Elem<T>::load(p + j) * inv_tau);
+  const float mb = block_max(m, red);
+  s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
+  if (threadIdx.x == 0) stat[blockIdx.x] = make_float2(mb, s);
+  if (parts == 1 && threadIdx.x < 64) {
+    const float loss = distill_row(p, t + row * k, idx + row * k, k, V, inv_tau, threadIdx.x, mb, s);
+    if (threadIdx.x == 0) row_loss[row] = loss;
+  }
+}
+
+// The same for rows in several parts. One wave per row.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_rows_kernel(const T* __restrict__ z, int64_t ldz, int R, int V, int parts,
                                                            int k, const float2* __restrict__ stat,
@@ -410,25 +483,29 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(const T* __restrict__
     s += st.x == -INFINITY ? st.y : st.y * fast_expf(st.x - m);
   }
   s = wave_sum(s);
-  const float l = logf(s);
-  float acc = 0.f;
-  teacher_row(t + row * k, idx + row * k, k, V, inv_tau, lane, [&](int, int col, float logp) {
-    if (col < 0) return;
-    const float pr = expf(logp);
-    if (!(pr == 0.f)) acc += pr * (logp - (Elem<T>::load(z + row * ldz + col) * inv_tau - m) + l);
-  });
-  acc = wave_sum(acc);
-  if (lane == 0) { row_stat[row] = make_float2(m, s); row_loss[row] = acc; }
+  const float loss = distill_row(z + row * ldz, t + row * k, idx + row * k, k, V, inv_tau, lane, m, s);
+  if (lane == 0) { row_stat[row] = make_float2(m, s); row_loss[row] = loss; }
 }
 
-// grad = g tau inv_n (q - p) of a part of a row; grad may be z itself. The entries' columns are written after the
+// loss = scale inv_n sum of the rows' losses, in a fixed order (one workgroup).
+__global__ __launch_bounds__(1024) void distill_sum_kernel(int R, const float* __restrict__ row_loss,
+                                                           const float* __restrict__ inv_n, float scale, float* loss) {
+  __shared__ float red[32];
+  float acc = 0.f;
+  for (int r = threadIdx.x; r < R; r += 1024) acc += row_loss[r];
+  acc = block_sum(acc, red);
+  if (threadIdx.x == 0) loss[0] = acc * scale * (inv_n ? inv_n[0] : 1.f);
+}
+
+// grad = g inv_n scale (q - p) of a part of a row; grad may be z itself. The entries' columns are written after the
 // barrier, once more, from the logits read before it: entries that name the same column each write the sum of
 // all their probabilities.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ldz, int V, int parts, int width, int k,
                                                           const float2* __restrict__ row_stat, const float* __restrict__ t,
-                                                          const int64_t* __restrict__ idx, float tau, float inv_tau,
+                                                          const int64_t* __restrict__ idx, float inv_tau,
                                                           const float* __restrict__ gscale, const float* __restrict__ inv_n,
+                                                          float scale,
                                                           T* grad, int64_t ldg) {
   constexpr int N = VN<T>;
   __shared__ int cols[DK_MAX];
@@ -453,7 +530,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
     return;
   }
   const float2 rs = row_stat[row];
-  const float c = gscale[0] * inv_n[0] * tau, m = rs.x, cq = c / rs.y;
+  const float c = gscale[0] * scale * (inv_n ? inv_n[0] : 1.f), m = rs.x, cq = c / rs.y;
   // the entry of this thread in this part: its logit, and the sum of the probabilities at its column
   const int col = threadIdx.x < (unsigned)k ? cols[threadIdx.x] - c0 : -1;
   const bool mine = col >= 0 && col < n;
@@ -544,49 +621,56 @@ UNOK_EXPORT int unok_row_topk(int dtype, int R, int V, int k, const void* z, int
 
 UNOK_EXPORT int64_t unok_distill_workspace(int R, int V) {
   if (R <= 0 || V <= 0) return 0;
-  return (int64_t)R * distill_parts(R, V) * 8;
+  const int64_t parts = distill_parts(R, V);
+  return (int64_t)R * ((parts > 1 ? parts * 8 : 0) + 4);
 }
 
 UNOK_EXPORT int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx,
-                                 float tau, float* row_stat, float* row_loss, void* workspace, int64_t ws_bytes, void* stream) {
+                                 float tau, const float* inv_n, float scale, float* row_stat, float* loss, void* workspace,
+                                 int64_t ws_bytes, void* stream) {
   int rc = distill_check("distill_fwd", dtype, R, V, k, ldz, tau);
-  if (rc || R == 0) return rc;
-  UNOK_REQUIRE(z && t && idx && row_stat && row_loss, UNOK_EINVAL, "distill_fwd: null operand");
+  if (rc) return rc;
+  UNOK_REQUIRE(loss && (R == 0 || (z && t && idx && row_stat)), UNOK_EINVAL, "distill_fwd: null operand");
   const int64_t need = unok_distill_workspace(R, V);
-  UNOK_REQUIRE(workspace && ws_bytes >= need && ((uintptr_t)workspace & 7) == 0, UNOK_EINVAL,
+  UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 7) == 0), UNOK_EINVAL,
                "distill_fwd: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)need, (long long)ws_bytes);
-  int parts, width;
-  distill_split(R, V, parts, width);
+  int parts = 1, width = V;
+  if (R > 0) distill_split(R, V, parts, width);
   UNOK_REQUIRE((int64_t)R * parts < (1ll << 31), UNOK_EINVAL, "distill_fwd: R=%d", R);
-  float2* stat = (float2*)workspace;
+  float2* stat = parts > 1 ? (float2*)workspace : (float2*)row_stat;
+  float* row_loss = (float*)workspace + (parts > 1 ? 2ll * R * parts : 0);
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto* zt) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(zt)>>;
-    hipLaunchKernelGGL(distill_stats_kernel<T>, dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V, parts, width,
-                       1.f / tau, stat);
-    hipLaunchKernelGGL(distill_rows_kernel<T>, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, st, zt, ldz, R, V, parts, k, stat, t,
-                       idx, 1.f / tau, (float2*)row_stat, row_loss);
+    hipLaunchKernelGGL(distill_stats_kernel<T>, dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V, parts, width, k, t,
+                       idx, 1.f / tau, stat, row_loss);
+    if (parts > 1)
+      hipLaunchKernelGGL(distill_rows_kernel<T>, dim3((unsigned)((R + 3) / 4)), dim3(256), 0, st, zt, ldz, R, V, parts, k, stat,
+                         t, idx, 1.f / tau, (float2*)row_stat, row_loss);
   };
-  if (dtype == UNOK_BF16) go((const bf16_t*)z);
-  else go((const float*)z);
+  if (R > 0) {
+    if (dtype == UNOK_BF16) go((const bf16_t*)z);
+    else go((const float*)z);
+  }
+  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, st, R, row_loss, inv_n, scale, loss);
   return unok::check_launch("distill_fwd");
 }
 
 UNOK_EXPORT int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx,
-                                 float tau, const float* row_stat, const float* gscale, const float* inv_n, void* grad, int64_t ldg,
-                                 void* stream) {
+                                 float tau, const float* row_stat, const float* gscale, const float* inv_n, float scale,
+                                 void* grad, int64_t ldg, void* stream) {
   int rc = distill_check("distill_bwd", dtype, R, V, k, ldz, tau);
   if (rc || R == 0) return rc;
   UNOK_REQUIRE(R <= 1 || ldg >= V, UNOK_EINVAL, "distill_bwd: ldg=%lld", (long long)ldg);
-  UNOK_REQUIRE(z && t && idx && row_stat && gscale && inv_n && grad, UNOK_EINVAL, "distill_bwd: null operand");
+  UNOK_REQUIRE(z && t && idx && row_stat && gscale && grad, UNOK_EINVAL, "distill_bwd: null operand");
   int parts, width;
   distill_split(R, V, parts, width);
   UNOK_REQUIRE((int64_t)R * parts < (1ll << 31), UNOK_EINVAL, "distill_bwd: R=%d", R);
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto* zt, auto* gt) {
     using T = std::remove_pointer_t<decltype(gt)>;
-    hipLaunchKernelGGL(distill_bwd_kernel<T>, dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V, parts, width, k, (const float2*)row_stat, t,
-                       idx, tau, 1.f / tau, gscale, inv_n, gt, ldg);
+    hipLaunchKernelGGL(distill_bwd_kernel<T>, dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V, parts, width, k,
+                       (const float2*)row_stat, t, idx, 1.f / tau, gscale, inv_n, scale, gt, ldg);
   };
   if (dtype == UNOK_BF16) go((const bf16_t*)z, (bf16_t*)grad);
   else go((const float*)z, (float*)grad);

@@ -204,23 +204,23 @@ def _distill_operands(z: torch.Tensor, values: torch.Tensor, indices: torch.Tens
             raise RuntimeError(f"top-k distillation: teacher on {t.device}, student on {z.device}")
 
 
-def _distill_fwd(z, values, indices, inv_n, temperature):
-    """(loss, row statistics for _distill_bwd) over [R, V] logits with unit column stride."""
+def _distill_fwd(z, values, indices, inv_n, scale, temperature):
+    """(loss, row statistics for _distill_bwd) over [R, V] logits with unit column stride; inv_n None: 1."""
     R, V = z.shape
     f32 = dict(device=z.device, dtype=torch.float32)
-    stat, rows, loss = torch.empty((R, 2), **f32), torch.empty(R, **f32), torch.empty((), **f32)
     nbytes = N.lib().unok_distill_workspace(R, V)
-    ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8)
+    stat, loss, ws = torch.empty((R, 2), **f32), torch.empty((), **f32), torch.empty(nbytes // 4, **f32)
     N.call("unok_distill_fwd", N.dtype_code(z.dtype), R, V, values.shape[1], N.ptr(z), z.stride(0), N.ptr(values),
-           N.ptr(indices), temperature, N.ptr(stat), N.ptr(rows), N.ptr(ws), nbytes, N.stream())
-    N.call("unok_sum_scaled", R, N.ptr(rows), N.ptr(inv_n), N.ptr(loss), N.stream())
-    return loss * (temperature * temperature) if temperature != 1.0 else loss, stat
+           N.ptr(indices), temperature, N.ptr(inv_n), scale * temperature * temperature, N.ptr(stat), N.ptr(loss), N.ptr(ws),
+           nbytes, N.stream())
+    return loss, stat
 
 
-def _distill_bwd(z, values, indices, stat, g, inv_n, temperature, grad):
-    g = g.reshape(1).float().contiguous()
+def _distill_bwd(z, values, indices, stat, g, inv_n, scale, temperature, grad):
+    g = g.float()
     N.call("unok_distill_bwd", N.dtype_code(z.dtype), *z.shape, values.shape[1], N.ptr(z), z.stride(0), N.ptr(values),
-           N.ptr(indices), temperature, N.ptr(stat), N.ptr(g), N.ptr(inv_n), N.ptr(grad), grad.stride(0), N.stream())
+           N.ptr(indices), temperature, N.ptr(stat), N.ptr(g), N.ptr(inv_n), scale * temperature, N.ptr(grad), grad.stride(0),
+           N.stream())
     return grad
 
 
@@ -231,7 +231,7 @@ class TopKDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h_s, values, indices, w_lm, w_lm_t, inv_n, temperature):
         z = K.gemm_nt(h_s.contiguous(), w_lm)
-        loss, stat = _distill_fwd(z, values, indices, inv_n, temperature)
+        loss, stat = _distill_fwd(z, values, indices, inv_n, 1.0, temperature)
         ctx.save = (z, values, indices, stat, inv_n, w_lm_t, temperature)
         return loss
 
@@ -239,7 +239,7 @@ class TopKDistillation(torch.autograd.Function):
     def backward(ctx, g):
         z, values, indices, stat, inv_n, w_lm_t, temperature = ctx.save
         ctx.save = None
-        _distill_bwd(z, values, indices, stat, g, inv_n, temperature, z)
+        _distill_bwd(z, values, indices, stat, g, inv_n, 1.0, temperature, z)
         return K.gemm_nt(z, w_lm_t), None, None, None, None, None, None
 
 
@@ -257,22 +257,22 @@ def top_k_distillation_loss(lm_head, h_s: torch.Tensor, values: torch.Tensor, in
 
 
 class LogitsTopKDistillation(torch.autograd.Function):
-    """The same over given logits (the losses.py call surface); gradient w.r.t. the student's."""
+    """The same over given logits (the losses.py call surface), scaled by a number; gradient w.r.t. the student's."""
 
     @staticmethod
-    def forward(ctx, z, values, indices, inv_n, temperature):
+    def forward(ctx, z, values, indices, scale, temperature):
         if z.stride(1) != 1 and z.shape[1] > 1:
             z = z.contiguous()
-        loss, stat = _distill_fwd(z, values, indices, inv_n, temperature)
-        ctx.save_for_backward(z, values, indices, stat, inv_n)
-        ctx.temperature = temperature
+        loss, stat = _distill_fwd(z, values, indices, None, scale, temperature)
+        ctx.save_for_backward(z, values, indices, stat)
+        ctx.scale, ctx.temperature = scale, temperature
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        z, values, indices, stat, inv_n = ctx.saved_tensors
+        z, values, indices, stat = ctx.saved_tensors
         grad = torch.empty(z.shape, device=z.device, dtype=z.dtype)
-        return _distill_bwd(z, values, indices, stat, g, inv_n, ctx.temperature, grad), None, None, None, None
+        return _distill_bwd(z, values, indices, stat, g, None, ctx.scale, ctx.temperature, grad), None, None, None, None
 
 
 class DistributionLoss(torch.autograd.Function):

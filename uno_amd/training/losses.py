@@ -102,7 +102,7 @@ def token_normalized_top_k_distillation(student_logits, teacher_values, teacher_
     _distill_operands(s, values, indices, temperature)
     if not s.size(0):
         return s.sum() * 0.0
-    return LogitsTopKDistillation.apply(s, values.float().contiguous(), indices.contiguous(), _inv_n(s, num_tokens),
+    return LogitsTopKDistillation.apply(s, values.float().contiguous(), indices.contiguous(), 1.0 / max(num_tokens, 1),
                                         float(temperature))
 
 
