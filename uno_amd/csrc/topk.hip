@@ -90,47 +90,61 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[N], int used
   return lo << SH;
 }
 
-// Candidates of one wave: (value key, ~column) pairs in CAP entries of LDS, of which the wave's k largest are
-// always among the first `cnt`. Nothing with a value key <= `floor` can still enter the k largest.
+// Candidates of one wave of a row's four: (value key, ~column) pairs in TK_CAP entries of LDS, of which the wave's k
+// largest are always among the first `cnt` unless they are known not to be among the row's. Nothing with a value
+// key <= `floor` can still enter. SH: value keys differ in their upper 32 - SH bits only (bf16: 16).
+//
+// The waves share what they know: `whole`, a key that k of the wave's elements reach, and `quarter`, one that a quarter
+// of k reach. k elements of the row reach the greatest `whole`, and the least `quarter`, which for rows without an order is
+// close to the row's k-th largest value so far. (Whenever a wave sees them: the k largest are the same.)
 constexpr int TK_CAP = 512, TK_KEEP = 384, TK_MAX = 256;
 
-// SH: value keys differ in their upper 32 - SH bits only (bf16: 16).
-template <int SH> struct Candidates {
-  uint64_t* buf;
-  int lane, k, cnt;
-  uint32_t floor, next_floor;
+struct Shared { uint32_t whole[4], quarter[4]; };
 
-  __device__ __forceinline__ Candidates(uint64_t* b, int l, int kk) : buf(b), lane(l), k(kk), cnt(0), floor(0), next_floor(0) {}
+#define TK_LDS __attribute__((address_space(3)))
+typedef TK_LDS uint64_t* LdsKeys;
+typedef TK_LDS Shared* LdsShared;
 
-  // Appends the lanes' candidates with `on`; drops what cannot be among the k largest when the room ends.
-  __device__ __forceinline__ void push(bool on, uint32_t key, uint32_t col) {
-    on = on && key > floor;
-    const uint64_t mask = __ballot(on);
-    if (mask == 0) return;
-    if (on) buf[cnt + lanes_below(mask)] = ((uint64_t)key << 32) | (uint32_t)~col;
-    cnt += __popcll(mask);
-    if (cnt > TK_CAP - 64) cut(false);
-  }
+__device__ __forceinline__ uint32_t tk_read(const TK_LDS uint32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
 
-  // Between two steps all candidates lie left of what follows, so of equal values only the old ones count.
-  __device__ __forceinline__ void step_end() { floor = next_floor > floor ? next_floor : floor; }
-
-  // Keeps the entries whose value is among the k largest, ties included; with `exact`, or when ties leave more than
-  // TK_KEEP, the k largest entries and no more.
-  __device__ __forceinline__ void cut(bool exact) {
-    if (cnt <= k) return;
-    constexpr int NE = TK_CAP / 64;
-    const int used = (cnt + 63) / 64;
-    uint32_t hi[NE], lo[NE];
-    __builtin_amdgcn_wave_barrier();
+// A key that k elements of the row reach (0: none known).
+__device__ __forceinline__ uint32_t known(LdsShared s) {
+  uint32_t w = 0, q = 0xffffffffu;
 #pragma unroll
-    for (int j = 0; j < NE; ++j) {
-      const int i = j * 64 + lane;
-      const uint64_t e = i < cnt ? buf[i] : 0;
-      hi[j] = (uint32_t)(e >> 32);
-      lo[j] = (uint32_t)e;
-    }
-    uint32_t t = kth_largest<NE, SH>(hi, used, k);
+  for (int i = 0; i < 4; ++i) {
+    w = max(w, tk_read(&s->whole[i]));
+    q = min(q, tk_read(&s->quarter[i]));
+  }
+  return max(w, q);
+}
+
+struct Cut { int cnt; uint32_t floor, next_floor; };
+
+// Looks for higher keys among a wave's cnt entries and drops those below them: keeps the entries whose value is among the k
+// largest, ties included; with `exact`, or when ties leave more than TK_KEEP, the k largest entries and no more. Not
+// inlined: it is rare, and four copies would not fit the instruction cache beside the walk.
+template <int SH>
+__device__ __attribute__((noinline)) Cut cut_candidates(LdsKeys buf, LdsShared shared, int wid, int k, int cnt, uint32_t floor,
+                                                        uint32_t next_floor, bool exact) {
+  constexpr int NE = TK_CAP / 64;
+  const int lane = threadIdx.x & 63, quarter = (k + 3) / 4;
+  cnt = __builtin_amdgcn_readfirstlane(cnt);
+  k = __builtin_amdgcn_readfirstlane(k);
+  const int used = (cnt + 63) / 64;
+  uint32_t hi[NE], lo[NE];
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    const int i = j * 64 + lane;
+    const uint64_t e = i < cnt ? buf[i] : 0;
+    hi[j] = (uint32_t)(e >> 32);
+    lo[j] = (uint32_t)e;
+  }
+  uint32_t t = 0, u = 0;                                 // the k-th largest key; the least ~column of its kept ties
+  if (cnt > k) {
+    t = kth_largest<NE, SH>(hi, used, k);
     if (SH > 0) {                                        // the low bits: ones for negative values (and NaN), zeros for others
       uint32_t low = 0;
 #pragma unroll
@@ -144,27 +158,71 @@ template <int SH> struct Candidates {
       above += __popcll(__ballot(hi[j] > t));
       tied += __popcll(__ballot(hi[j] == t));
     }
-    uint32_t u = 0;                                    // least ~column of the kept ties
     if (above + tied > k && (exact || above + tied > TK_KEEP)) {
       uint32_t tie[NE];
 #pragma unroll
       for (int j = 0; j < NE; ++j) tie[j] = hi[j] == t ? lo[j] : 0u;
       u = kth_largest<NE, 0>(tie, used, k - above);
     }
-    __builtin_amdgcn_wave_barrier();
-    int at = 0;
-#pragma unroll
-    for (int j = 0; j < NE; ++j) {
-      if (j >= used) continue;
-      const bool keep = hi[j] > t || (hi[j] == t && lo[j] >= u);
-      const uint64_t mask = __ballot(keep);
-      if (keep) buf[at + lanes_below(mask)] = ((uint64_t)hi[j] << 32) | lo[j];
-      at += __popcll(mask);
-    }
-    __builtin_amdgcn_wave_barrier();
-    cnt = at;
     floor = t - 1 > floor ? t - 1 : floor;
-    next_floor = t;
+    next_floor = t > next_floor ? t : next_floor;
+  }
+  if (cnt >= quarter) {
+    const uint32_t q = kth_largest<NE, SH>(hi, used, quarter);
+    if (lane == 0) {                                     // (both only ever grow; no other wave writes them)
+      if (next_floor > tk_read(&shared->whole[wid]))
+        __hip_atomic_store(&shared->whole[wid], next_floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (q > tk_read(&shared->quarter[wid]))
+        __hip_atomic_store(&shared->quarter[wid], q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  }
+  const uint32_t least = known(shared);
+  __builtin_amdgcn_wave_barrier();
+  int at = 0;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    if (j >= used) continue;
+    const bool keep = hi[j] >= least && hi[j] != 0 && (hi[j] > t || (hi[j] == t && lo[j] >= u));
+    const uint64_t mask = __ballot(keep);
+    if (keep) buf[at + lanes_below(mask)] = ((uint64_t)hi[j] << 32) | lo[j];
+    at += __popcll(mask);
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (least > 0 && least - 1 > floor) floor = least - 1;
+  return Cut{at, floor, next_floor};
+}
+
+template <int SH> struct Candidates {
+  LdsKeys buf;
+  LdsShared shared;
+  int wid, k, cnt, next;                                 // next: the count at which to look for higher keys
+  uint32_t floor, next_floor;
+
+  __device__ __forceinline__ Candidates(uint64_t* b, Shared* s, int w, int kk)
+      : buf((LdsKeys)(b + w * TK_CAP)), shared((LdsShared)s), wid(w), k(kk), cnt(0), next((kk + 3) / 4), floor(0), next_floor(0) {}
+
+  // Appends the lanes' candidates with `on`; the caller sees to it that there is room for 64.
+  __device__ __forceinline__ void push(bool on, uint32_t key, uint32_t col) {
+    on = on && key > floor;
+    const uint64_t mask = __ballot(on);
+    if (on) buf[cnt + lanes_below(mask)] = ((uint64_t)key << 32) | (uint32_t)~col;
+    cnt += __popcll(mask);
+  }
+  __device__ __forceinline__ bool full() const { return cnt > TK_CAP - 64; }
+
+  // Between two steps all candidates lie left of what follows, so of equal values only the old ones count.
+  __device__ __forceinline__ void step_end() { floor = next_floor > floor ? next_floor : floor; }
+
+  __device__ __forceinline__ void learn() {
+    const uint32_t t = known(shared);
+    if (t > 0 && t - 1 > floor) floor = t - 1;
+  }
+  __device__ __forceinline__ void cut(bool exact) {
+    const Cut c = cut_candidates<SH>(buf, shared, wid, k, cnt, floor, next_floor, exact);
+    cnt = __builtin_amdgcn_readfirstlane(c.cnt);
+    floor = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.floor);
+    next_floor = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.next_floor);
+    next = cnt + (k + 3) / 4;
   }
 };
 
@@ -174,26 +232,54 @@ __device__ __forceinline__ float floor_value(uint32_t floor) {
   return key_value(floor);
 }
 
-// Merges the waves' candidates of a row: every wave leaves its at most k largest, and an entry's rank is the number
-// of larger entries.
-template <int SH, typename F>
-__device__ __forceinline__ void rank_entries(uint64_t* all, int* wave_cnt, Candidates<SH>& c, int k, int wid, F emit) {
-  c.cut(true);
-  if (c.lane == 0) wave_cnt[wid] = c.cnt;
-  __syncthreads();
-  const int n0 = wave_cnt[0], n1 = n0 + wave_cnt[1], n2 = n1 + wave_cnt[2], n3 = n2 + wave_cnt[3];
-  for (int i = threadIdx.x; i < n3; i += 256) {
-    const int w = (i >= n0) + (i >= n1) + (i >= n2);
-    const uint64_t e = all[w * TK_CAP + i - (w == 0 ? 0 : w == 1 ? n0 : w == 2 ? n1 : n2)];
+// Ranks n distinct entries in LDS: an entry's rank is the number of larger ones.
+template <typename F> __device__ __forceinline__ void rank_entries(LdsKeys all, int n, int k, F emit) {
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const uint64_t e = all[i];
     int rank = 0;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int n = wave_cnt[v];
 #pragma unroll 8
-      for (int q = 0; q < n; ++q) rank += all[v * TK_CAP + q] > e;
-    }
+    for (int q = 0; q < n; ++q) rank += all[q] > e;
     if (rank < k) emit(rank, e);
   }
+}
+
+// Merges the waves' candidates of a row into the k largest in order. If the waves hold many, each first drops what the
+// others' keys rule out.
+template <int SH, typename F>
+__device__ __forceinline__ void merge_waves(uint64_t* all, int* wave_cnt, Candidates<SH>& c, int k, F emit) {
+  const int lane = threadIdx.x & 63;
+  int first[4], n = 0;
+  auto counts = [&] {
+    if (lane == 0) wave_cnt[c.wid] = c.cnt;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      first[w] = n;
+      n += wave_cnt[w];
+    }
+  };
+  counts();
+  if (n > 256) {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {                        // the second time with what every wave found in the first
+      if (c.cnt > 0) c.cut(i > 0);
+      __syncthreads();
+    }
+    counts();
+  }
+  // dense: every entry is read before any is written
+  uint64_t e[TK_CAP / 64];
+#pragma unroll
+  for (int j = 0; j < TK_CAP / 64; ++j) e[j] = j * 64 + lane < c.cnt ? c.buf[j * 64 + lane] : 0;
+  __syncthreads();
+  LdsKeys dense = (LdsKeys)all;
+  const int at = c.wid == 0 ? first[0] : c.wid == 1 ? first[1] : c.wid == 2 ? first[2] : first[3];
+#pragma unroll
+  for (int j = 0; j < TK_CAP / 64; ++j)
+    if (j * 64 + lane < c.cnt) dense[at + j * 64 + lane] = e[j];
+  __syncthreads();
+  rank_entries(dense, n, k, emit);
 }
 
 // The k largest of a row's columns [c0, c0 + width) and the part's softmax statistics, one workgroup per (row, part).
@@ -212,9 +298,8 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
   __shared__ uint64_t buf[4 * TK_CAP];
   __shared__ float red[32];
   __shared__ int wave_cnt[4];
-  __shared__ uint32_t bound_[4];                         // per wave: a value key that k of its elements reach
-  volatile uint32_t* bound = bound_;
-  if (threadIdx.x < 4) bound[threadIdx.x] = 0;
+  __shared__ Shared shared;
+  if (threadIdx.x < 4) shared.whole[threadIdx.x] = shared.quarter[threadIdx.x] = 0;
   __syncthreads();
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
@@ -223,7 +308,7 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
   const T* p = z + row * ldz + c0;
   const Span<T> sp(p, n);
   constexpr int SH = sizeof(T) == 2 ? 16 : 0;
-  Candidates<SH> cand(buf + wid * TK_CAP, lane, k);
+  Candidates<SH> cand(buf, &shared, wid, k);
   float m = -INFINITY, s = 0.f;
 
   constexpr uint32_t NOTHING = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
@@ -232,6 +317,7 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
     for (int i = 0; i < cnt; i += 64) {
       const bool in = i + lane < cnt;
       const float v = in ? Elem<T>::load(p + first + i + lane) : -INFINITY;
+      if (cand.full()) cand.cut(false);
       cand.push(in, value_key(v), (uint32_t)(c0 + first + i + lane));
       if (v > m) { s *= fast_expf(m - v); m = v; }
       s += fast_expf(v - (m == -INFINITY ? 0.f : m));
@@ -248,7 +334,7 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
       const int q = q0 + i * 64 + lane;
       raw[i] = q < sp.nv ? pv[q] : u32x4_t{NOTHING, NOTHING, NOTHING, NOTHING};
     }
-    float gm[U];
+    float gm[U], sm = -INFINITY;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       float v[N];
@@ -256,16 +342,21 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
       gm[i] = v[0];
 #pragma unroll
       for (int e = 1; e < N; ++e) gm[i] = fmaxf(gm[i], v[e]);
-      if (gm[i] > m) { s *= fast_expf(m - gm[i]); m = gm[i]; }
-      const float ref = m == -INFINITY ? 0.f : m;      // -inf then adds 0, and a NaN is seen
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += fast_expf(v[e] - ref);
+      sm = fmaxf(sm, gm[i]);
     }
-    // what the other waves have found by now spares this one candidates (whenever it is seen: the k largest are
-    // the same)
-    const uint32_t others = max(max(bound[0], bound[1]), max(bound[2], bound[3]));
-    if (others > 0 && others - 1 > cand.floor) cand.floor = others - 1;
+    if (sm > m) { s *= fast_expf(m - sm); m = sm; }
+    const float ref = m == -INFINITY ? 0.f : m;          // -inf then adds 0, and a NaN is seen
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float v[N];
+      unpack16<T>(raw[i], v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) part[e % 4] += fast_expf(v[e] - ref);
+    }
+    s += (part[0] + part[1]) + (part[2] + part[3]);
     if (fresh) {
+      // the first step's 256 largest-of-a-vector: each is one element
       fresh = false;
       uint32_t key[U];
       int cnt = 0;
@@ -274,44 +365,60 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
         key[i] = q0 + i * 64 + lane < sp.nv ? value_key(gm[i]) : 0u;
         cnt += __popcll(__ballot(key[i] != 0));
       }
-      if (cnt >= k) {
-        const uint32_t t = kth_largest<U, SH>(key, U, k);  // (its low bits zero: a bound all the same)
-        if (t > 0 && t - 1 > cand.floor) cand.floor = t - 1;
-        if (lane == 0) bound[wid] = t;
+      // (the keys' low bits come as zeros: bounds all the same)
+      if (cnt >= (k + 3) / 4) {
+        const uint32_t whole = cnt >= k ? kth_largest<U, SH>(key, U, k) : 0u, quarter = kth_largest<U, SH>(key, U, (k + 3) / 4);
+        if (lane == 0) {
+          __hip_atomic_store(&shared.whole[wid], whole, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          __hip_atomic_store(&shared.quarter[wid], quarter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
       }
     }
-    // bit 8 i + e (fp32: 4 i + e): element e of vector i may enter. (A lane that has met a NaN, which fmaxf
-    // drops, looks into every vector from then on.)
+    cand.learn();
+    // bit e of may[i]: element e of vector i may enter. (A lane that has met a NaN, which fmaxf drops, looks into
+    // every vector from then on.)
     const float least = floor_value(cand.floor);
-    uint32_t may = 0;
+    uint32_t may[U];
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const bool look = q0 + i * 64 + lane < sp.nv && (!(gm[i] < least) || s != s);
+      may[i] = 0;
       if (__ballot(look) == 0) continue;
+      any = true;
       float v[N];
       unpack16<T>(raw[i], v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) may |= look && !(v[e] < least) ? 1u << (i * N + e) : 0u;
+      for (int e = 0; e < N; ++e) may[i] |= look && !(v[e] < least) ? 1u << e : 0u;
     }
-    while (__ballot(may != 0)) {
-      const int at = may ? __builtin_ctz(may) : 0;
-      uint32_t w = raw[0][0];
-      const int word = at * (int)sizeof(T) / 4;
+    while (any) {
+      any = false;
 #pragma unroll
-      for (int i = 0; i < 4 * U; ++i) w = word == i ? raw[i / 4][i % 4] : w;
-      if constexpr (sizeof(T) == 2) w = at & 1 ? w & 0xffff0000u : w << 16;
-      cand.push(may != 0, value_key(__uint_as_float(w)), (uint32_t)(c0 + sp.head + (q0 + (at / N) * 64 + lane) * N + at % N));
-      may &= may - 1;
+      for (int i = 0; i < U; ++i) {
+        while (!cand.full() && __ballot(may[i] != 0)) {
+          const bool on = may[i] != 0;
+          const int e = on ? __builtin_ctz(may[i]) : 0;
+          may[i] &= may[i] - 1;                          // (0 stays 0)
+          const int word = e * (int)sizeof(T) / 4;
+          const uint32_t w01 = word & 1 ? raw[i][1] : raw[i][0], w23 = word & 1 ? raw[i][3] : raw[i][2];
+          uint32_t w = word & 2 ? w23 : w01;
+          if constexpr (sizeof(T) == 2) w = e & 1 ? w & 0xffff0000u : w << 16;
+          cand.push(on, value_key(__uint_as_float(w)),
+                    (uint32_t)(c0 + sp.head + (q0 + i * 64 + lane) * N + e));
+        }
+        any |= __ballot(may[i] != 0) != 0;
+      }
+      // (higher keys cost less than the candidates under them)
+      if (any || cand.cnt >= cand.next) cand.cut(false);
     }
     cand.step_end();
-    if (lane == 0 && cand.next_floor > bound[wid]) bound[wid] = cand.next_floor;
   }
   if (wid == 3) single(sp.tail(), n - sp.tail());
 
   const float mb = block_max(m, red);
   s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
   if (parts == 1) {
-    rank_entries(buf, wave_cnt, cand, k, wid, [&](int rank, uint64_t e) {
+    merge_waves(buf, wave_cnt, cand, k, [&](int rank, uint64_t e) {
       const float v = key_value((uint32_t)(e >> 32));
       values[row * k + rank] = v;
       cols[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)e;
@@ -323,47 +430,78 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
     if (threadIdx.x == 0) ws_stat[row * parts + part] = make_float2(mb, s);
     for (int i = threadIdx.x; i < k; i += 256)
       if (i >= n) o[i] = 0;
-    rank_entries(buf, wave_cnt, cand, k, wid, [&](int rank, uint64_t e) { o[rank] = e; });
+    merge_waves(buf, wave_cnt, cand, k, [&](int rank, uint64_t e) { o[rank] = e; });
   }
 }
 
-// The parts' entries and statistics of a row, merged; one workgroup per row.
+// The parts' entries (sorted, at most TK_MERGE together) and statistics of a row, merged; one workgroup per row. k elements reach
+// the greatest of the parts' last entries, and the least of their ceil(k / parts)-th ones: what lies below is dropped, and the
+// rest ranked. Bound by latency.
+constexpr int TK_MERGE = 1024;
+
 __global__ __launch_bounds__(256) void topk_merge_kernel(const uint64_t* __restrict__ ws_key,
                                                          const float2* __restrict__ ws_stat, int k, int parts,
                                                          float* __restrict__ values, int64_t* __restrict__ cols,
                                                          float* __restrict__ lse) {
-  __shared__ uint64_t buf[4 * TK_CAP];
-  __shared__ float red[32];
-  __shared__ int wave_cnt[4];
+  __shared__ uint64_t buf[TK_MERGE];
+  __shared__ uint64_t red[8];
+  __shared__ float fred[32];
+  __shared__ int count;
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const uint64_t* src = ws_key + row * parts * k;
-  const int n = parts * k;
-  Candidates<0> cand(buf + wid * TK_CAP, lane, k);
-  for (int i = wid * 64; i < n; i += 256) {
-    const uint64_t e = i + lane < n ? src[i + lane] : 0;
-    cand.push(e != 0, (uint32_t)(e >> 32), ~(uint32_t)e);
+  const int n = parts * k, nth = (k + parts - 1) / parts - 1;
+  uint64_t e[TK_MERGE / 256];
+#pragma unroll
+  for (int i = 0; i < TK_MERGE / 256; ++i) {
+    const int at = i * 256 + (int)threadIdx.x;
+    e[i] = at < n ? src[at] : 0;
   }
+  uint64_t most = 0, least = ~0ull;
   float m = -INFINITY, s = 0.f;
   for (int i = threadIdx.x; i < parts; i += 256) {
+    most = max(most, src[(int64_t)i * k + k - 1]);
+    least = min(least, src[(int64_t)i * k + nth]);
     const float2 st = ws_stat[row * parts + i];
     if (st.x > m) { s = s * fast_expf(m - st.x) + st.y; m = st.x; }
-    else if (st.x > -INFINITY) s += st.y * fast_expf(st.x - m);
+    else s += st.x == -INFINITY ? st.y : st.y * fast_expf(st.x - m);
   }
-  const float mb = block_max(m, red);
-  s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
-  rank_entries(buf, wave_cnt, cand, k, wid, [&](int rank, uint64_t e) {
-    const float v = key_value((uint32_t)(e >> 32));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    most = max(most, (uint64_t)__shfl_xor((unsigned long long)most, o, 64));
+    least = min(least, (uint64_t)__shfl_xor((unsigned long long)least, o, 64));
+  }
+  if (lane == 0) { red[wid] = most; red[4 + wid] = least; }
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  most = max(max(red[0], red[1]), max(red[2], red[3]));
+  least = min(min(red[4], red[5]), min(red[6], red[7]));
+  most = max(most, least);
+#pragma unroll
+  for (int i = 0; i < TK_MERGE / 256; ++i) {
+    const bool on = e[i] != 0 && e[i] >= most;
+    const uint64_t mask = __ballot(on);
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&count, __popcll(mask));
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (on) buf[at + lanes_below(mask)] = e[i];          // (in any order: the entries' ranks decide)
+  }
+  const float mb = block_max(m, fred);
+  s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), fred);
+  rank_entries((LdsKeys)buf, count, k, [&](int rank, uint64_t x) {
+    const float v = key_value((uint32_t)(x >> 32));
     values[row * k + rank] = v;
-    cols[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)e;
+    cols[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)x;
     if (rank == 0) lse[row] = v - v == 0.f ? mb + logf(s) : v;
   });
 }
 
-// Parts of a row: with fewer rows than fill the chip (two workgroups per CU), as many as do, of at least 4096 columns.
-int topk_parts(int R, int V) {
-  const int want = (512 + R - 1) / (R > 0 ? R : 1), most = V / 4096;
-  const int p = want < most ? want : most;
+// Parts of a row: with fewer rows than fill the chip (two workgroups per CU), as many as do, of at least 4096 columns, whose
+// entries the merge holds.
+int topk_parts(int R, int V, int k) {
+  const int want = (512 + R - 1) / (R > 0 ? R : 1), most = V / 4096, room = TK_MERGE / k;
+  int p = want < most ? want : most;
+  p = p < room ? p : room;
   return p < 1 ? 1 : p;
 }
 
@@ -586,7 +724,7 @@ int distill_check(const char* what, int dtype, int R, int V, int k, int64_t ldz,
 
 UNOK_EXPORT int64_t unok_row_topk_workspace(int R, int V, int k) {
   if (R <= 0 || V <= 0 || k <= 0) return 0;
-  const int64_t parts = topk_parts(R, V);
+  const int64_t parts = topk_parts(R, V, k);
   return parts == 1 ? 0 : R * parts * (8ll * k + 8);
 }
 
@@ -597,7 +735,7 @@ UNOK_EXPORT int unok_row_topk(int dtype, int R, int V, int k, const void* z, int
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "row_topk: bad dtype %d", dtype);
   if (R == 0) return 0;
   UNOK_REQUIRE(z && values && cols && lse, UNOK_EINVAL, "row_topk: null operand");
-  const int parts = topk_parts(R, V);
+  const int parts = topk_parts(R, V, k);
   const int64_t need = unok_row_topk_workspace(R, V, k);
   UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 7) == 0), UNOK_EINVAL,
                "row_topk: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)need, (long long)ws_bytes);
