@@ -89,6 +89,18 @@ def test_row_top_k_orders(dev, dtype, V, k):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [5, 3001, 70001])
+def test_row_top_k_far_from_zero(dev, dtype, V):
+    """Values whose product with log2 e is coarse, or no float."""
+    g = torch.Generator(device=dev).manual_seed(V)
+    r = torch.randn(V, device=dev, generator=g)
+    step = torch.randint(0, 4, (V,), device=dev, generator=g).float()
+    rows = [1e5 + r, -1e5 + r, 1048576.0 + step, -1048570.0 - step, 1e7 + step, -1e7 - step, 3e38 + 0 * r, -3e38 + 0 * r,
+            torch.where(step == 0, 2e38, -2e38), torch.where(step == 0, 1e7, r), torch.where(step == 0, -1e7, -3e38)]
+    _check_top(torch.stack(rows).to(dtype), min(V, 9), K.row_top_k(torch.stack(rows).to(dtype), min(V, 9)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("offset,stride", [(0, 1009), (1, 1010), (3, 1024), (7, 1111)])
 def test_row_top_k_strides(dev, dtype, offset, stride):
     """Rows at every alignment; what lies between the rows is not read as a value."""

@@ -123,12 +123,11 @@ __device__ __forceinline__ uint32_t known(LdsShared s) {
 struct Cut { int cnt; uint32_t floor, next_floor; };
 
 // Looks for higher keys among a wave's cnt entries and drops those below them: keeps the entries whose value is among the k
-// largest, ties included; with `exact`, or when ties leave more than TK_KEEP, the k largest entries and no more. Not
-// inlined: it is rare, and four copies would not fit the instruction cache beside the walk.
-template <int SH>
+// largest, ties included; with `exact`, or when ties leave more than TK_KEEP, the k largest entries and no more. Takes
+// up to 64 NE entries. Not inlined: it is rare, and four copies would not fit the instruction cache beside the walk.
+template <int SH, int NE>
 __device__ __attribute__((noinline)) Cut cut_candidates(LdsKeys buf, LdsShared shared, int wid, int k, int cnt, uint32_t floor,
                                                         uint32_t next_floor, bool exact) {
-  constexpr int NE = TK_CAP / 64;
   const int lane = threadIdx.x & 63, quarter = (k + 3) / 4;
   cnt = __builtin_amdgcn_readfirstlane(cnt);
   k = __builtin_amdgcn_readfirstlane(k);
@@ -218,7 +217,8 @@ template <int SH> struct Candidates {
     if (t > 0 && t - 1 > floor) floor = t - 1;
   }
   __device__ __forceinline__ void cut(bool exact) {
-    const Cut c = cut_candidates<SH>(buf, shared, wid, k, cnt, floor, next_floor, exact);
+    const Cut c = cnt <= 128 ? cut_candidates<SH, 2>(buf, shared, wid, k, cnt, floor, next_floor, exact)
+                             : cut_candidates<SH, TK_CAP / 64>(buf, shared, wid, k, cnt, floor, next_floor, exact);
     cnt = __builtin_amdgcn_readfirstlane(c.cnt);
     floor = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.floor);
     next_floor = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.next_floor);
@@ -282,15 +282,38 @@ __device__ __forceinline__ void merge_waves(uint64_t* all, int* wave_cnt, Candid
   rank_entries(dense, n, k, emit);
 }
 
+// The sum of e^(z - m) over a lane's elements of a row's part, as row_topk_kernel hands them out.
+constexpr float TK_FAR = 1048576.f, LOG2E = 1.4426950408889634f;
+template <typename T>
+__device__ __attribute__((noinline)) float far_sum(const T* p, int n, Span<T> sp, int wid, int lane, float m) {
+  const float ref = m == -INFINITY ? 0.f : m;
+  const u32x4_t* pv = (const u32x4_t*)(p + sp.head);
+  float s = 0.f;
+  if (wid == 0)
+    for (int i = lane; i < sp.head; i += 64) s += fast_expf(Elem<T>::load(p + i) - ref);
+#pragma unroll 1
+  for (int q = wid * 256 + lane; q < sp.nv; q += (q & 192) == 192 ? 1024 - 192 : 64) {   // four vectors of each step
+    float v[VN<T>];
+    unpack16<T>(pv[q], v);
+#pragma unroll
+    for (int e = 0; e < VN<T>; ++e) s += fast_expf(v[e] - ref);
+  }
+  if (wid == 3)
+    for (int i = sp.tail() + lane; i < n; i += 64) s += fast_expf(Elem<T>::load(p + i) - ref);
+  return s;
+}
+
 // The k largest of a row's columns [c0, c0 + width) and the part's softmax statistics, one workgroup per (row, part).
 // parts == 1 writes values, columns and log-sum-exp; otherwise the part's sorted entries (missing ones 0) and
 // (max, sum of e^(z - max)) go to the workspace for topk_merge_kernel.
 //
 // One pass: a wave takes every fourth step of 4 x 64 16-byte loads. A group of 16 bytes is looked into only
 // if its largest value can pass the wave's floor; the first step sets the floor to the k-th largest of its
-// 256 groups' maxima (each is one element, so k elements reach it).
+// 256 groups' maxima (each is one element, so k elements reach it). Bound by its vector instructions: unpacking, comparing,
+// the exponential (4096 x 151936 bf16, k = 64: 290 us, 4.3 TB/s; with a subtraction and a product before the exponential 325;
+// six waves a SIMD: with five 310, held to seven or eight 333 and 493 for spilled registers).
 template <typename T>
-__global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, int64_t ldz, int V, int k, int parts,
+__global__ __launch_bounds__(256, 6) void row_topk_kernel(const T* __restrict__ z, int64_t ldz, int V, int k, int parts,
                                                        int width, float* __restrict__ values, int64_t* __restrict__ cols,
                                                        float* __restrict__ lse, uint64_t* __restrict__ ws_key,
                                                        float2* __restrict__ ws_stat) {
@@ -309,7 +332,16 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
   const Span<T> sp(p, n);
   constexpr int SH = sizeof(T) == 2 ? 16 : 0;
   Candidates<SH> cand(buf, &shared, wid, k);
-  float m = -INFINITY, s = 0.f;
+  // s: the lane's sum of 2^(z log2 e - shift) with shift = m log2 e as rounded, one fused multiply-add an element. What the
+  // rounding of shift left out is put right at the end.
+  float m = -INFINITY, s = 0.f, shift = 0.f;
+  auto raise = [&](float to) {
+    const float before = shift;
+    m = to;
+    shift = m == -INFINITY ? 0.f : m * LOG2E;            // -inf then adds 0, and a NaN is seen
+    if (s != 0.f) s *= __builtin_amdgcn_exp2f(before - shift);
+  };
+  auto power = [&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -shift)); };
 
   constexpr uint32_t NOTHING = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // -inf
   // elements outside the vectors: the head by wave 0 before its steps, the tail by wave 3 after its steps
@@ -319,8 +351,8 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
       const float v = in ? Elem<T>::load(p + first + i + lane) : -INFINITY;
       if (cand.full()) cand.cut(false);
       cand.push(in, value_key(v), (uint32_t)(c0 + first + i + lane));
-      if (v > m) { s *= fast_expf(m - v); m = v; }
-      s += fast_expf(v - (m == -INFINITY ? 0.f : m));
+      if (v > m) raise(v);
+      s += power(v);
       cand.step_end();
     }
   };
@@ -344,15 +376,14 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
       for (int e = 1; e < N; ++e) gm[i] = fmaxf(gm[i], v[e]);
       sm = fmaxf(sm, gm[i]);
     }
-    if (sm > m) { s *= fast_expf(m - sm); m = sm; }
-    const float ref = m == -INFINITY ? 0.f : m;          // -inf then adds 0, and a NaN is seen
+    if (sm > m) raise(sm);
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       float v[N];
       unpack16<T>(raw[i], v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) part[e % 4] += fast_expf(v[e] - ref);
+      for (int e = 0; e < N; ++e) part[e % 4] += power(v[e]);
     }
     s += (part[0] + part[1]) + (part[2] + part[3]);
     if (fresh) {
@@ -415,6 +446,10 @@ __global__ __launch_bounds__(256) void row_topk_kernel(const T* __restrict__ z, 
   }
   if (wid == 3) single(sp.tail(), n - sp.tail());
 
+  // The rounding left m log2 e - shift out of every exponent, at most 2^-25 |shift|. Far from 0 that is more than a
+  // factor near 1 (or no number at all): the lane's elements are then read again.
+  if (__ballot(!(fabsf(m) < TK_FAR) && m != -INFINITY)) s = far_sum(p, n, sp, wid, lane, m);
+  else if (m != -INFINITY) s *= __builtin_amdgcn_exp2f(-fmaf(m, LOG2E, -shift));
   const float mb = block_max(m, red);
   s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
   if (parts == 1) {
