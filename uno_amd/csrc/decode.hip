@@ -536,11 +536,11 @@ __global__ __launch_bounds__(256) void decode_prep_kernel(const bf16_t* __restri
       const int kv = hd / rep, rr = hd % rep;
       dst = qd + (TREE ? (int64_t)m * nq + hd : (int64_t)(b * nk + kv) * 128 + rr * L + t) * D;
     } else {
-      if (len + t >= max_len) return;
+      if ((uint64_t)(len + t) >= (uint64_t)max_len) return;   // no such row
       dst = kc + ((int64_t)(b * nk + hd - nq) * max_len + len + t) * D;
     }
   } else {
-    if (len + t >= max_len) return;
+    if ((uint64_t)(len + t) >= (uint64_t)max_len) return;   // no such row
     dst = vc + ((int64_t)(b * nk + hd - nq - nk) * max_len + len + t) * D;
   }
   *(uint4*)(dst + c0) = make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]),

@@ -19,6 +19,10 @@ Kernels:
   the K/V head, at most 128) are laid out as the 128 query rows of one attention workgroup over
   that key range, with per-row key intervals [start, start + cached + j + 1) -- the block-diffusion
   attention kernel then reads each cache row once per pair;
+* a tree of drafted tokens (tree_block) is one pass of the model over all its nodes: a node's position is the committed
+  length plus its depth, node t's K/V go to cache row length + t, and its queries see the committed rows, its ancestors
+  and itself (unok_tree_attn). BlockKVCache.accept then moves the accepted path's rows together and commits them;
+  BlockKVCache.copy_from gives sequences that share a prefix their own copies of it;
 * a prefill (empty caches) is the clean stream's causal forward of the prompt (LoRA off, keys = the
   prompt itself).
 """
@@ -43,6 +47,26 @@ class BlockKVCache:
         self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int64)
         self.batch, self.max_len, self.geo = batch, max_len, geo
+
+    def accept(self, nodes: torch.Tensor, counts: torch.Tensor) -> None:
+        """Commits the accepted nodes of the tree that ``BlockDecoder.tree_block`` wrote: nodes [B, P] int64, of which the
+        first counts[b] (int64 [B], 0 .. P) are sequence b's path from the root down. Their K/V rows become the next
+        committed rows in that order (every row is read before any is written); the tree's other rows are dropped. All
+        on the device, and capturable into a graph."""
+        K.cache_keep(self.k + self.v, self.lengths, nodes, counts)
+        self.lengths += counts.clamp(0, nodes.shape[1])
+
+    def copy_from(self, other: "BlockKVCache", pairs) -> None:
+        """Copies whole sequences: for each (slot of ``other``, slot of this cache) of ``pairs`` the committed rows of all
+        layers and their number. ``other`` may be this cache; then no slot is both read and written. No slot is written
+        twice. (Reads ``other``'s lengths on the host only if it can hold more rows than this cache.)"""
+        pairs = [(int(a), int(b)) for a, b in pairs]
+        if not pairs:
+            return
+        if other.max_len > self.max_len and all(0 <= a < other.batch for a, _ in pairs) and \
+                int(other.lengths[[a for a, _ in pairs]].max()) > self.max_len:
+            raise RuntimeError("the sequences do not fit in the KV cache")
+        K.cache_copy(other.k + other.v, self.k + self.v, other.lengths, self.lengths, pairs)
 
 
 class BlockDecoder:
@@ -91,6 +115,23 @@ class BlockDecoder:
         (see DraftGraph)."""
         return DraftGraph(self, cache, block_size, commit)
 
+    @torch.no_grad()
+    def tree_block(self, cache: BlockKVCache, node_ids: torch.Tensor, parents: torch.Tensor,
+                   lora_mask: torch.Tensor | None = None) -> torch.Tensor:
+        """One pass over a tree of drafted tokens per sequence; returns logits [B, T, V].
+
+        node_ids [B, T] are the nodes' tokens, parents int32 [B, T] (or [T] for one tree of all sequences) the index of
+        each node's parent: an earlier node, -1 for a root, below -1 for padding, whose logits mean nothing. A root
+        follows the committed rows, a node its parent; T <= 256. Usually node 0 is the last sampled token, the one
+        root. Nothing is committed: call ``cache.accept`` with the path that is kept. The LoRA is off (the
+        verifying pass) unless ``lora_mask`` [B, T] turns it on per node."""
+        self._tree_check(cache, node_ids, parents, lora_mask)
+        return self._tree_forward(cache, node_ids, parents, lora_mask)
+
+    def capture_tree(self, cache: BlockKVCache, nodes: int) -> "TreeGraph":
+        """A tree block of [cache.batch, nodes] over ``cache`` captured as one HIP graph (see TreeGraph)."""
+        return TreeGraph(self, cache, nodes)
+
     # ---- the decoder -----------------------------------------------------------------------------
     def _forward(self, cache: BlockKVCache, ids: torch.Tensor, gate: torch.Tensor | None, commit: int, prefill: bool,
                  check: bool = True):
@@ -119,12 +160,46 @@ class BlockDecoder:
             for li, layer in enumerate(dec.layers):
                 lw = layer.weights()
                 h = self._layer(h, lw, li, pos, gate_rows, cache, maps, B, L)
-        x, _ = K.rmsnorm_fwd(h, dec.norm.weight, g.eps)
-        V = self.base.lm_head.weight.shape[0]
-        head = K.gemm_nt_rows if self._rows_path(M, x.dtype, prefill) and V % 4 == 0 else K.gemm_nt
-        logits = head(x, self.base.lm_head.weight)
+        logits = self._head(h, prefill)
         cache.lengths += commit
         return logits.view(B, L, -1)
+
+    def _tree_check(self, cache, ids, parents, lora_mask) -> None:
+        B, T = ids.shape
+        if B != cache.batch:
+            raise RuntimeError(f"tree batch {B} does not match the cache batch {cache.batch}")
+        if not 1 <= T <= 256:
+            raise ValueError(f"trees hold 1 to 256 nodes, got {T}")
+        if parents.dtype != torch.int32 or tuple(parents.shape) not in ((B, T), (T,)):
+            raise RuntimeError(f"parents must be int32 {(B, T)} or {(T,)}, got {parents.dtype} {tuple(parents.shape)}")
+        if lora_mask is not None and tuple(lora_mask.shape) != (B, T):
+            raise RuntimeError(f"LoRA row mask {tuple(lora_mask.shape)} does not match the tree {(B, T)}")
+        if self.geo.d not in (64, 128):
+            raise NotImplementedError(f"tree blocks take head dimensions 64 and 128, not {self.geo.d}")
+        if int(cache.lengths.max()) + T > cache.max_len:
+            raise RuntimeError("the tree does not fit in the KV cache")
+
+    def _tree_forward(self, cache, ids, parents, lora_mask):
+        g, dec = self.geo, self.decoder
+        B, T = ids.shape
+        gate_rows = None if lora_mask is None else lora_mask.to(torch.bool).reshape(-1).contiguous()
+        parents = parents.expand(B, T).contiguous()
+        maps = {"parents": parents, "depths": K.tree_depths(parents)}
+        if cache.k[0].dtype != torch.bfloat16:
+            t = torch.arange(T, device=ids.device)
+            maps["pos"] = (cache.lengths[:, None] + maps["depths"]).reshape(-1)
+            pair = torch.arange(B * g.nk, device=ids.device).view(B, 1, g.nk)
+            maps["store"] = (pair * cache.max_len + (cache.lengths[:, None] + t)[..., None]).reshape(-1).to(torch.int32)
+        h = K.embedding(ids.reshape(-1).contiguous().to(torch.int64), dec.embed_tokens.weight)
+        for li, layer in enumerate(dec.layers):
+            h = self._layer(h, layer.weights(), li, maps.get("pos"), gate_rows, cache, maps, B, T)
+        return self._head(h, False).view(B, T, -1)
+
+    def _head(self, h, prefill: bool):
+        x, _ = K.rmsnorm_fwd(h, self.decoder.norm.weight, self.geo.eps)
+        w = self.base.lm_head.weight
+        head = K.gemm_nt_rows if self._rows_path(x.shape[0], x.dtype, prefill) and w.shape[0] % 4 == 0 else K.gemm_nt
+        return head(x, w)
 
     def _prefill_layers(self, h, cache, B: int, P: int):
         """All layers over B prompts of P tokens into empty caches: the clean stream's layer (no LoRA rows,
@@ -271,7 +346,14 @@ class BlockDecoder:
         qkv_segments = [(q_end, 0), (k_end, r), (k_end + g.kv, 2 * r)]
 
         def linear(x, w, part, segments=None, residual=None, swiglu=False):
-            """Gated LoRA linear: x w^T + (m (.) x A^T)[:, seg] (s B)^T (+ residual)."""
+            """Gated LoRA linear: x w^T + (m (.) x A^T)[:, seg] (s B)^T (+ residual); no LoRA without a gate."""
+            if gate_rows is None:
+                if few:
+                    return K.gemm_nt_rows(x, w, residual=residual, swiglu=swiglu)
+                if swiglu and x.dtype == torch.bfloat16 and K.swiglu_fused_ok(M, g.F, g.H, any_rows=True):
+                    return K.gemm_nt_swiglu(x, w, any_rows=True, plain_rows=True)
+                y = K.gemm_nt(x, w, residual=residual)
+                return K.swiglu_fwd(y, y.shape[1] // 2) if swiglu else y
             if few:
                 return K.gemm_nt_rows(x, w, lora_a=lora.a_c(li, part), lora_b=lora.sb_c(li, part),
                                       segments=segments, residual=residual, gate=gate_rows, swiglu=swiglu)
@@ -293,11 +375,19 @@ class BlockDecoder:
             o = torch.empty((M, g.q), device=qkv.device, dtype=qkv.dtype)
             K.attn_split_combine(od, lse, maps["dst"], QR, S, g.d, o.view(M * g.nq, g.d))
             return self._mlp(o, h0, lw, li, linear)
+        if "parents" in maps and qkv.dtype == torch.bfloat16:
+            q = K.tree_prep(qkv, lw.q_norm, lw.k_norm, cache.lengths, maps["depths"], self.decoder.inv_freq, g.eps,
+                            cache.k[li], cache.v[li], B, L, g.nq, g.nk, g.d)
+            o = K.tree_attn(q, cache.k[li], cache.v[li], cache.lengths, maps["parents"])
+            return self._mlp(o, h0, lw, li, linear)
         q, k, _ = K.qknorm_rope_fwd(qkv, g.nq, g.nk, g.d, lw.q_norm, lw.k_norm, pos, self.decoder.inv_freq, g.eps)
         v = qkv[:, k_end:]
         # the block's K/V into the cache rows (b, head, cached + t)
         K.rows_copy(k.reshape(M * g.nk, g.d), ck, M * g.nk, dmap=maps["store"])
         K.rows_copy(v.contiguous().view(M * g.nk, g.d), cv, M * g.nk, dmap=maps["store"])
+        if "parents" in maps:
+            o = K.tree_attn(q.reshape(M, g.q), cache.k[li], cache.v[li], cache.lengths, maps["parents"])
+            return self._mlp(o, h0, lw, li, linear)
         rows = maps["iv"].shape[0]
         qd = torch.zeros((rows, g.d), device=q.device, dtype=q.dtype)
         K.rows_copy(q.reshape(M * g.nq, g.d), qd, M * g.nq, dmap=maps["qrow"])
@@ -368,4 +458,36 @@ class DraftGraph:
             self.gate.copy_(lora_mask)
         self.graph.replay()
         self._len_max += self.commit
+        return self.logits
+
+
+class TreeGraph:
+    """A tree block of fixed shape [B, T] over one cache, captured as a single HIP graph.
+
+    Positions, cache rows and the attention's key ranges come from ``cache.lengths`` and the parents inside the graph, so
+    each replay verifies one tree at the current lengths, exactly as ``BlockDecoder.tree_block``; it commits nothing.
+
+    ``replay`` returns the graph's own logits buffer [B, T, V], overwritten by the next replay."""
+
+    def __init__(self, decoder: BlockDecoder, cache: BlockKVCache, nodes: int):
+        B, T = cache.batch, nodes
+        dev = cache.lengths.device
+        self.decoder, self.cache = decoder, cache
+        self.ids = torch.zeros((B, T), device=dev, dtype=torch.int64)
+        self.parents = torch.full((B, T), -1, device=dev, dtype=torch.int32)
+        # one eager pass sets each kernel's launch attributes outside the graph; its rows lie past the committed ones
+        decoder.tree_block(cache, self.ids, self.parents)
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph), torch.no_grad():
+            self.logits = decoder._tree_forward(cache, self.ids, self.parents, None)
+
+    def replay(self, node_ids: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
+        """One tree per sequence: node_ids [B, T], parents int32 [B, T] or [T], as ``tree_block`` takes them (LoRA off)."""
+        if tuple(node_ids.shape) != tuple(self.ids.shape):
+            raise RuntimeError(f"tree {tuple(node_ids.shape)} does not match the captured {tuple(self.ids.shape)}")
+        self.decoder._tree_check(self.cache, node_ids, parents, None)
+        self.ids.copy_(node_ids)
+        self.parents.copy_(parents)
+        self.graph.replay()
         return self.logits
