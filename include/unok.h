@@ -412,7 +412,7 @@ int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz,
                      const float* inv_n, float scale, float* row_stat, float* loss, void* workspace, int64_t ws_bytes,
                      void* stream);
 /* grad [R, V] = gscale[0] inv_n[0] scale (q - p), rows without entries 0 (for the gradient, the forward's scale over
- * tau). grad may be z itself. */
+ * tau). grad may be z itself, and otherwise shares no row with it. */
 int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
                      const float* row_stat, const float* gscale, const float* inv_n, float scale, void* grad, int64_t ldg,
                      void* stream);

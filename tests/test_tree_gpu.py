@@ -186,6 +186,78 @@ def test_masked_rows_may_hold_anything(dev, dtype, D):
     assert bool(out[1, 0].isnan().all())
 
 
+@pytest.mark.parametrize("dtype,heads,T", [(BF, (8, 2, 64), 4), (BF, (8, 2, 64), 15), (BF, (8, 2, 128), 16), (BF, (8, 2, 64), 30),
+                                           (BF, (8, 2, 128), 25), (BF, (8, 2, 64), 70), (BF, (8, 2, 128), 70), (BF, (2, 2, 128), 256),
+                                           (F32, (4, 1, 128), 4), (F32, (4, 1, 64), 41), (F32, (2, 2, 128), 200)])
+def test_masked_rows_in_every_kernel(dev, dtype, heads, T):
+    """The same at every number of query rows (with nodes over several key tiles), over several key ranges, one and none
+    committed: a node's NaN reaches those that see it and no other."""
+    print(f"[tree masked] {dtype} heads={heads} T={T}", flush=True)
+    nq, nk, D = heads
+    B, lengths = 3, [1500, 33, 0]
+    q, k, v, n, parents = _case(dev, dtype, B, T, heads, lengths, room=300, pad=1, seed=8)
+    vis = _visible(parents)
+    clean = K.tree_attn(q, k, v, n, parents.to(dev)).view(B, T, nq, D)
+    _check(clean.view(B * T, -1), _reference(q, k, v, n, parents, D ** -0.5), dtype)
+    whole, part = T // 3, T // 2                # a node whose key is NaN, one with odd elements in its value
+    for b, m in enumerate(lengths):
+        k[b, :, m + T:], v[b, :, m + T:] = math.nan, -math.inf
+        if parents[b, T - 1] < -1:
+            k[b, :, m + T - 1], v[b, :, m + T - 1] = math.inf, math.nan
+        k[b, :, m + whole] = math.nan
+        v[b, :, m + part, 5] = math.nan
+        v[b, :, m + part, D - 1] = math.inf
+    out = K.tree_attn(q, k, v, n, parents.to(dev)).view(B, T, nq, D)
+    rest = [d for d in range(D) if d not in (5, D - 1)]
+    for b in range(B):
+        for t in range(T):
+            if parents[b, t] < -1:
+                assert not out[b, t].any()
+            elif vis[b, t, whole]:
+                assert bool(out[b, t].isnan().all()), (b, t)
+            elif vis[b, t, part]:
+                assert bool(out[b, t, :, 5].isnan().all()) and bool((out[b, t, :, D - 1] == math.inf).all()), (b, t)
+                assert torch.equal(out[b, t][:, rest], clean[b, t][:, rest]), (b, t)
+            else:
+                assert torch.equal(out[b, t], clean[b, t]), (b, t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,heads", [(4, (4, 2, 64)), (20, (4, 2, 128)), (40, (4, 2, 64)), (90, (4, 2, 128))])
+@pytest.mark.parametrize("B", [70, 200])
+def test_many_sequences(dev, dtype, B, T, heads):
+    """More sequences than a wave has lanes, of very different lengths: one long, most short, some empty."""
+    print(f"[tree many] {dtype} B={B} T={T} heads={heads}", flush=True)
+    lengths = [(37 * b) % 90 for b in range(B)]
+    lengths[B - 3], lengths[5], lengths[66] = 2900, 0, 1100
+    q, k, v, n, parents = _case(dev, dtype, B, T, heads, lengths, room=1, pad=2)
+    out = K.tree_attn(q, k, v, n, parents.to(dev))
+    _check(out, _reference(q, k, v, n, parents, heads[2] ** -0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_sequences_that_share_their_rows(dev, dtype):
+    """Caches with a batch or head stride of 0: one prefix read by every sequence (its nodes' rows are then the same)."""
+    B, T, nq, nk, D = 4, 9, 8, 2, 64
+    q, k, v, n, parents = _case(dev, dtype, 1, T, (nq, nk, D), [900], room=0)
+    q = q.repeat(B, 1) * torch.arange(1, B + 1, device=dev).repeat_interleave(T)[:, None].to(dtype)
+    n, parents = n.repeat(B), parents.repeat(B, 1)
+    for kk, vv in ((k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1)),
+                   (k[:, :1].expand(B, nk, -1, -1), v[:, :1].expand(B, nk, -1, -1))):
+        out = K.tree_attn(q, kk, vv, n, parents.to(dev))
+        _check(out, _reference(q, kk, vv, n, parents, D ** -0.5), dtype)
+
+
+def test_an_output_over_its_queries_is_refused(dev):
+    q, k, v, n, parents = _case(dev, BF, 2, 6, (4, 2, 64), [40, 3], room=0)
+    with pytest.raises(ValueError, match="overlaps"):
+        K.tree_attn(q, k, v, n, parents.to(dev), out=q)
+    both = torch.zeros(12, 512, device=dev, dtype=BF)    # columns of one tensor do not
+    both[:, :256] = q
+    K.tree_attn(both[:, :256], k, v, n, parents.to(dev), out=both[:, 256:])
+    assert torch.equal(both[:, 256:], K.tree_attn(q, k, v, n, parents.to(dev)))
+
+
 def test_scores_far_apart(dev):
     """Scores spread over thousands, the largest last: weights of the far ones are 0, and the maximum moves in steps."""
     B, T, nk, D, n = 1, 4, 1, 64, 900

@@ -34,6 +34,16 @@ const char* last_error();
 // Converts a hipError_t from a launch into the return convention above.
 int check_launch(const char* what);
 
+// Whether any of `rows` rows of `width` bytes at a, `lda` bytes apart, shares a byte with the rows at b; rows of different
+// strides in one range of memory are taken to.
+inline bool rows_overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t width) {
+  const int64_t d = (const char*)b - (const char*)a, last = rows - 1;
+  if (rows <= 0 || width <= 0 || d >= last * lda + width || -d >= last * ldb + width) return false;
+  if (lda != ldb || lda <= 0) return true;
+  const int64_t at = ((d % lda) + lda) % lda;
+  return at < width || lda - at < width;
+}
+
 }  // namespace unok
 
 #define UNOK_REQUIRE(cond, code, ...)                 \

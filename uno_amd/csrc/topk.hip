@@ -751,7 +751,8 @@ int distill_check(const char* what, int dtype, int R, int V, int k, int64_t ldz,
   UNOK_REQUIRE(R >= 0 && V >= 1 && (R <= 1 || ldz >= V), UNOK_EINVAL, "%s: R=%d V=%d ldz=%lld", what, R, V, (long long)ldz);
   UNOK_REQUIRE(k >= 1 && k <= DK_MAX, UNOK_EINVAL, "%s: k=%d must lie in [1, %d]", what, k, DK_MAX);
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "%s: bad dtype %d", what, dtype);
-  UNOK_REQUIRE(tau > 0.f && tau < INFINITY, UNOK_EINVAL, "%s: temperature %g must be positive", what, (double)tau);
+  UNOK_REQUIRE(tau > 0.f && tau < INFINITY && 1.f / tau < INFINITY, UNOK_EINVAL, "%s: temperature %g must be positive", what,
+               (double)tau);
   return 0;
 }
 
@@ -836,6 +837,9 @@ UNOK_EXPORT int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, 
   if (rc || R == 0) return rc;
   UNOK_REQUIRE(R <= 1 || ldg >= V, UNOK_EINVAL, "distill_bwd: ldg=%lld", (long long)ldg);
   UNOK_REQUIRE(z && t && idx && row_stat && gscale && grad, UNOK_EINVAL, "distill_bwd: null operand");
+  const int64_t es = dtype == UNOK_BF16 ? 2 : 4;
+  UNOK_REQUIRE((grad == z && (ldg == ldz || R == 1)) || !unok::rows_overlap(z, ldz * es, grad, ldg * es, R, V * es), UNOK_EINVAL,
+               "distill_bwd: the gradient overlaps the logits");
   int parts, width;
   distill_split(R, V, parts, width);
   UNOK_REQUIRE((int64_t)R * parts < (1ll << 31), UNOK_EINVAL, "distill_bwd: R=%d", R);

@@ -512,8 +512,8 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
     f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = merge_ml[w][rl][0];
-      sum += mw == -INFINITY ? 0.f : merge_ml[w][rl][1] * __builtin_amdgcn_exp2f(mw - top);
+      const float mw = merge_ml[w][rl][0], lw = merge_ml[w][rl][1];
+      sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);   // no maximum: 0, or NaN from NaN scores alone
       x += *(const f32x4_t*)(merge_o + (w * ROWS + rl) * LDO + d);
     }
     if (whole) {
@@ -801,8 +801,8 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
-      const float mi = ml[(i * RG + rg) * 64 + lq];
-      l += mi == -INFINITY ? 0.f : ml[(i * RG + rg) * 64 + 32 + lq] * __builtin_amdgcn_exp2f(mi - top);
+      const float mi = ml[(i * RG + rg) * 64 + lq], li = ml[(i * RG + rg) * 64 + 32 + lq];
+      l += mi == -INFINITY ? li : li * __builtin_amdgcn_exp2f(mi - top);   // no maximum: 0, or NaN from NaN scores alone
     }
     const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
     m = top;
@@ -870,11 +870,11 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
       const int64_t at = at0 + min(s0 + i, range.y - 1) * step;
       v[i] = *(const f32x4_t*)(a.po + at * D + d);
       ms[i] = s0 + i < range.y ? a.pm[2 * at] : -INFINITY;
-      ls[i] = a.pm[2 * at + 1];
+      ls[i] = s0 + i < range.y ? a.pm[2 * at + 1] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (ms[i] == -INFINITY) continue;
+      if (ms[i] == -INFINITY) { sum += ls[i]; continue; }   // 0, or NaN from NaN scores alone
       const float f = __builtin_amdgcn_exp2f(ms[i] - top);
       sum += ls[i] * f;
       x += v[i] * f;
@@ -944,6 +944,11 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   UNOK_REQUIRE(k_row >= D && v_row >= D && k_row < (1 << 23) && v_row < (1 << 23), UNOK_EINVAL,
                "tree_attn: row strides %lld and %lld must lie in [D, 2^23)", (long long)k_row, (long long)v_row);
   UNOK_REQUIRE(ldp == 0 || ldp >= T, UNOK_EINVAL, "tree_attn: parents' row stride %lld for %d nodes", (long long)ldp, T);
+  const int64_t es = dtype == UNOK_BF16 ? 2 : 4, width = (int64_t)nq * D, rows = (int64_t)B * T;
+  UNOK_REQUIRE(rows == 1 || (ldq >= width && ldo >= width), UNOK_EINVAL, "tree_attn: rows of %lld elements, ldq=%lld ldo=%lld",
+               (long long)width, (long long)ldq, (long long)ldo);
+  UNOK_REQUIRE(!unok::rows_overlap(q, ldq * es, o, ldo * es, rows, width * es), UNOK_EINVAL,
+               "tree_attn: the output overlaps the queries");
   const int per16 = dtype == UNOK_BF16 ? 8 : 4;
   int64_t bits = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15;
   for (int64_t s : {ldq, k_batch, k_head, k_row, v_batch, v_head, v_row, ldo}) bits |= s % per16;

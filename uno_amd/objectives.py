@@ -197,6 +197,8 @@ def _distill_operands(z: torch.Tensor, values: torch.Tensor, indices: torch.Tens
                            f"{tuple(values.shape)} {tuple(indices.shape)} for {tuple(z.shape)}")
     if indices.dtype != torch.int64:
         raise RuntimeError("top-k distillation: teacher indices must be int64")
+    if not values.is_floating_point():
+        raise RuntimeError(f"top-k distillation: teacher values must be floating-point, got {values.dtype}")
     if not 0.0 < temperature < float("inf"):
         raise ValueError("top-k distillation: the temperature must be positive and finite")
     for t in (values, indices):
@@ -206,6 +208,7 @@ def _distill_operands(z: torch.Tensor, values: torch.Tensor, indices: torch.Tens
 
 def _distill_fwd(z, values, indices, inv_n, scale, temperature):
     """(loss, row statistics for _distill_bwd) over [R, V] logits with unit column stride; inv_n None: 1."""
+    K._same_device("top-k distillation", z, values, indices, *(() if inv_n is None else (inv_n,)))
     R, V = z.shape
     f32 = dict(device=z.device, dtype=torch.float32)
     nbytes = N.lib().unok_distill_workspace(R, V)
