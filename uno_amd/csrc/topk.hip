@@ -576,9 +576,11 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ t, const i
   for (int i = 0; i < DK_MAX / 64; ++i)
     if (col[i] >= 0) s += expf(x[i] - m);
   s = wave_sum(s);
-  const float l = m + logf(s);
+  const float l = logf(s);
+  // (from x - m and s: m + log s would be rounded to the size of m, and p by as much)
 #pragma unroll
-  for (int i = 0; i < DK_MAX / 64; ++i) use(lane + 64 * i, col[i], x[i] - l);
+  for (int i = 0; i < DK_MAX / 64; ++i)
+    use(lane + 64 * i, col[i], x[i] - m - l, col[i] >= 0 ? expf(x[i] - m) / s : 0.f);
   return true;
 }
 
@@ -589,12 +591,20 @@ __device__ __forceinline__ float distill_row(const T* __restrict__ z, const floa
                                              float s) {
   const float l = logf(s);
   float acc = 0.f;
-  teacher_row(t, idx, k, V, inv_tau, lane, [&](int, int col, float logp) {
+  teacher_row(t, idx, k, V, inv_tau, lane, [&](int, int col, float logp, float pr) {
     if (col < 0) return;
-    const float pr = expf(logp);
     if (!(pr == 0.f)) acc += pr * (logp - (Elem<T>::load(z + col) * inv_tau - m) + l);
   });
   return wave_sum(acc);
+}
+
+// e^x of a logit less its row's maximum. fp32 gradients show what the product x log2 e and log2 e itself leave out,
+// (|x| + 1) 2^-24 together, so their part is put back; a bf16 gradient is rounded to 2^-8.
+template <typename T> __device__ __forceinline__ float distill_exp(float x) {
+  if constexpr (sizeof(T) == 2) return fast_expf(x);
+  constexpr float L = 1.4426950408889634f, LOW = (float)(1.4426950408889634 - (double)L);
+  const float h = x * L, r = fmaf(x, LOW, fmaf(x, L, -h)), e = __builtin_amdgcn_exp2f(h);
+  return x < -150.f ? 0.f : fmaf(e, r * 0.69314718f, e);
 }
 
 // (max, sum of e^(x - max)) of x = z / tau over a part of a row; one workgroup per (row, part). A row in one part also gets
@@ -618,19 +628,19 @@ __global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict_
     float g = -INFINITY;
 #pragma unroll
     for (int e = 0; e < N; ++e) { v[e] *= inv_tau; g = fmaxf(g, v[e]); }
-    if (g > m) { s *= fast_expf(m - g); m = g; }
+    if (g > m) { s *= distill_exp<T>(m - g); m = g; }
     const float ref = m == -INFINITY ? 0.f : m;        // -inf then adds 0, and a NaN is seen
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += fast_expf(v[e] - ref);
+    for (int e = 0; e < N; ++e) s += distill_exp<T>(v[e] - ref);
   }
   auto single = [&](float v) {
-    if (v > m) { s *= fast_expf(m - v); m = v; }
-    s += fast_expf(v - (m == -INFINITY ? 0.f : m));
+    if (v > m) { s *= distill_exp<T>(m - v); m = v; }
+    s += distill_exp<T>(v - (m == -INFINITY ? 0.f : m));
   };
   for (int j = threadIdx.x; j < sp.head; j += 256) single(Elem<T>::load(p + j) * inv_tau);
   for (int j = sp.tail() + threadIdx.x; j < n; j += 256) single(Elem<T>::load(p + j) * inv_tau);
   const float mb = block_max(m, red);
-  s = block_sum(m == -INFINITY ? s : s * fast_expf(m - mb), red);
+  s = block_sum(m == -INFINITY ? s : s * distill_exp<T>(m - mb), red);
   if (threadIdx.x == 0) stat[blockIdx.x] = make_float2(mb, s);
   if (parts == 1 && threadIdx.x < 64) {
     const float loss = distill_row(p, t + row * k, idx + row * k, k, V, inv_tau, threadIdx.x, mb, s);
@@ -689,9 +699,9 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
   const T* p = z + row * ldz + c0;
   T* g = grad + row * ldg + c0;
   if (threadIdx.x < 64) {
-    const bool any = teacher_row(t + row * k, idx + row * k, k, V, inv_tau, threadIdx.x, [&](int e, int col, float logp) {
+    const bool any = teacher_row(t + row * k, idx + row * k, k, V, inv_tau, threadIdx.x, [&](int e, int col, float, float pr) {
       cols[e] = col;
-      prob[e] = col < 0 ? 0.f : expf(logp);
+      prob[e] = pr;
     });
     if (threadIdx.x == 0) live = any;
   }
@@ -713,7 +723,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
     for (int e = 0; e < k; ++e) psum += cols[e] == col + c0 ? prob[e] : 0.f;
   }
   __syncthreads();
-  auto one = [&](float v) { return cq * fast_expf(v * inv_tau - m); };
+  auto one = [&](float v) { return cq * distill_exp<T>(v * inv_tau - m); };
   if (aligned) {
     const u32x4_t* pv = (const u32x4_t*)(p + sp.head);
     u32x4_t* gv = (u32x4_t*)(g + sp.head);
@@ -731,7 +741,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the columns' first values are stored before the second ones
   __syncthreads();
-  if (mine) Elem<T>::store(g + col, fast_expf(zc * inv_tau - m) / rs.y * c - psum * c);
+  if (mine) Elem<T>::store(g + col, distill_exp<T>(zc * inv_tau - m) / rs.y * c - psum * c);
 }
 
 // Parts of a row of the statistics and the gradient, as topk_parts, of at least 8192 columns.
