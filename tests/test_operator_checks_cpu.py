@@ -105,6 +105,7 @@ OTHERS = {
     "distill index type": lambda: token_normalized_top_k_distillation(torch.zeros(4, 8), torch.zeros(4, 2), _nodes(4, 2, dtype=I32), 4),
     "distill value type": lambda: token_normalized_top_k_distillation(torch.zeros(4, 8), _nodes(4, 2), _nodes(4, 2), 4),
     "distill device": lambda: token_normalized_top_k_distillation(torch.zeros(4, 8), torch.zeros(4, 2), _nodes(4, 2), 4),
+    "distill inv_n": lambda: top_k_distillation_loss(None, torch.zeros(4, 8), torch.zeros(4, 2), _nodes(4, 2), torch.ones(1).double()),
     "distill hidden rows": lambda: top_k_distillation_loss(None, torch.zeros(4, 8), torch.zeros(3, 2), _nodes(3, 2), torch.ones(1)),
 }
 

@@ -219,6 +219,27 @@ def test_distillation_strides(dev, dtype):
         _check_loss(view, values, indices, R, 1.0, loss.detach(), grad)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_distillation_broadcast_inputs(dev, dtype):
+    """One row of logits for all teacher rows, one teacher row for all logits: the shared row's gradient is the sum."""
+    R, V, k = 5, 640, 9
+    g = torch.Generator(device=dev).manual_seed(12)
+    z = torch.randn(1, V, device=dev, generator=g).to(dtype)
+    values, indices = _teacher(torch.randn(R, V, device=dev, generator=g), k, g)
+    leaf = z.clone().requires_grad_(True)
+    wide = leaf.expand(R, V)
+    loss = token_normalized_top_k_distillation(wide, values, indices, R)
+    per_row, shared = torch.autograd.grad(loss, (wide, leaf))
+    _check_loss(z.expand(R, V), values, indices, R, 1.0, loss.detach(), per_row)
+    # autograd's sum of R rows in the leaf's type: each addition rounds by half a step of at most the sum of magnitudes
+    assert bool(((shared.double() - per_row.double().sum(0)).abs() <= R * HALF[dtype] * per_row.double().abs().sum(0)).all())
+    many = torch.randn(R, V, device=dev, generator=g).to(dtype).requires_grad_(True)
+    one = (values[:1].expand(R, k), indices[:1].expand(R, k))
+    loss = token_normalized_top_k_distillation(many, *one, R)
+    (grad,) = torch.autograd.grad(loss, many)
+    _check_loss(many.detach(), *one, R, 1.0, loss.detach(), grad)
+
+
 def test_distillation_gradient_against_differences(dev):
     """Central differences of the loss in 64 bits around the kernel's inputs: step h, so off by h^2 / 6 of a third derivative
     that a softmax bounds by 1, and by the rounding of two losses of 64 bits."""

@@ -253,6 +253,8 @@ def top_k_distillation_loss(lm_head, h_s: torch.Tensor, values: torch.Tensor, in
     whole vocabulary. Entries of value -inf, or with an index outside the vocabulary, do not count; a row without
     entries contributes nothing, to the loss and to the gradient. The teacher is not differentiated."""
     _distill_operands(h_s, values, indices, temperature)
+    if inv_n.dtype != torch.float32 or inv_n.numel() != 1:
+        raise RuntimeError(f"top-k distillation: inv_n must be one fp32 number, got {inv_n.dtype} {tuple(inv_n.shape)}")
     if h_s.shape[0] == 0:
         return h_s.sum() * 0.0
     return TopKDistillation.apply(h_s, values.detach().float().contiguous(), indices.contiguous(), lm_head.weight,
@@ -264,7 +266,7 @@ class LogitsTopKDistillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, z, values, indices, scale, temperature):
-        if z.stride(1) != 1 and z.shape[1] > 1:
+        if (z.stride(1) != 1 and z.shape[1] > 1) or z.stride(0) < z.shape[1]:   # (an expanded row: copied)
             z = z.contiguous()
         loss, stat = _distill_fwd(z, values, indices, None, scale, temperature)
         ctx.save_for_backward(z, values, indices, stat)
