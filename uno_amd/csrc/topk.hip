@@ -26,6 +26,15 @@ template <typename T> __device__ __forceinline__ u32x4_t pack16(const float (&v)
     return u32x4_t{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7])};
 }
 
+// Logits of more than the memory-side cache's 256 MB are read past it (NT), as they cannot be there: 4096 x 151936 bf16
+// (1.2 GB), k = 10 255 -> 239 us, and the distillation's gradient of 1024 x 151936 (311 MB) 196 -> 176 us with its forward;
+// logits that fit are found there: 512 x 151936 (155 MB) 96 us when read past it, 88 when not.
+constexpr int64_t MEMORY_CACHE = 256ll << 20;
+template <bool NT> __device__ __forceinline__ u32x4_t load16(const u32x4_t* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // A span of n elements at p as: head elements up to the first 16-byte boundary, nv vectors of 16 bytes, the rest.
 template <typename T> struct Span {
   int head, nv;
@@ -312,7 +321,7 @@ __device__ __attribute__((noinline)) float far_sum(const T* p, int n, Span<T> sp
 // 256 groups' maxima (each is one element, so k elements reach it). Bound by its vector instructions: unpacking, comparing,
 // the exponential (4096 x 151936 bf16, k = 64: 290 us, 4.3 TB/s; with a subtraction and a product before the exponential 325;
 // six waves a SIMD: with five 310, held to seven or eight 333 and 493 for spilled registers).
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256, 6) void row_topk_kernel(const T* __restrict__ z, int64_t ldz, int V, int k, int parts,
                                                        int width, float* __restrict__ values, int64_t* __restrict__ cols,
                                                        float* __restrict__ lse, uint64_t* __restrict__ ws_key,
@@ -364,7 +373,7 @@ __global__ __launch_bounds__(256, 6) void row_topk_kernel(const T* __restrict__ 
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int q = q0 + i * 64 + lane;
-      raw[i] = q < sp.nv ? pv[q] : u32x4_t{NOTHING, NOTHING, NOTHING, NOTHING};
+      raw[i] = q < sp.nv ? load16<NT>(pv + q) : u32x4_t{NOTHING, NOTHING, NOTHING, NOTHING};
     }
     float gm[U], sm = -INFINITY;
 #pragma unroll
@@ -682,8 +691,9 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(int R, const float* _
 
 // grad = g inv_n scale (q - p) of a part of a row; grad may be z itself. The entries' columns are written after the
 // barrier, once more, from the logits read before it: entries that name the same column each write the sum of
-// all their probabilities.
-template <typename T>
+// all their probabilities. The gradient is stored past the caches: it is the size of the logits, which the writes would drive
+// out (512 x 151936 bf16 with its forward 99 -> 88 us, 4096 x 151936 785 -> 742, and 711 with loads past them too). Bound by HBM.
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ldz, int V, int parts, int width, int k,
                                                           const float2* __restrict__ row_stat, const float* __restrict__ t,
                                                           const int64_t* __restrict__ idx, float inv_tau,
@@ -729,10 +739,10 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
     u32x4_t* gv = (u32x4_t*)(g + sp.head);
     for (int q = threadIdx.x; q < sp.nv; q += 256) {
       float v[N];
-      unpack16<T>(pv[q], v);
+      unpack16<T>(load16<NT>(pv + q), v);
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] = one(v[e]);
-      gv[q] = pack16<T>(v);
+      __builtin_nontemporal_store(pack16<T>(v), gv + q);
     }
     for (int j = threadIdx.x; j < sp.head; j += 256) Elem<T>::store(g + j, one(Elem<T>::load(p + j)));
     for (int j = sp.tail() + threadIdx.x; j < n; j += 256) Elem<T>::store(g + j, one(Elem<T>::load(p + j)));
@@ -791,12 +801,17 @@ UNOK_EXPORT int unok_row_topk(int dtype, int R, int V, int k, const void* z, int
   uint64_t* keys = (uint64_t*)workspace;
   float2* stat = (float2*)(keys + (int64_t)R * parts * k);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == UNOK_BF16)
-    hipLaunchKernelGGL(row_topk_kernel<bf16_t>, dim3((unsigned)(R * used)), dim3(256), 0, st, (const bf16_t*)z, ldz, V, k, used,
+  auto go = [&](auto* zt, auto nt) {
+    using T = std::remove_cv_t<std::remove_pointer_t<decltype(zt)>>;
+    hipLaunchKernelGGL((row_topk_kernel<T, decltype(nt)::value>), dim3((unsigned)(R * used)), dim3(256), 0, st, zt, ldz, V, k, used,
                        width, values, cols, lse, keys, stat);
-  else
-    hipLaunchKernelGGL(row_topk_kernel<float>, dim3((unsigned)(R * used)), dim3(256), 0, st, (const float*)z, ldz, V, k, used,
-                       width, values, cols, lse, keys, stat);
+  };
+  auto by_size = [&](auto* zt) {
+    if ((int64_t)R * V * (int64_t)sizeof(*zt) > MEMORY_CACHE) go(zt, std::true_type{});
+    else go(zt, std::false_type{});
+  };
+  if (dtype == UNOK_BF16) by_size((const bf16_t*)z);
+  else by_size((const float*)z);
   int rc = unok::check_launch("row_topk");
   if (rc || used == 1) return rc;
   hipLaunchKernelGGL(topk_merge_kernel, dim3((unsigned)R), dim3(256), 0, st, keys, stat, k, used, values, cols, lse);
@@ -854,10 +869,14 @@ UNOK_EXPORT int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, 
   distill_split(R, V, parts, width);
   UNOK_REQUIRE((int64_t)R * parts < (1ll << 31), UNOK_EINVAL, "distill_bwd: R=%d", R);
   hipStream_t st = (hipStream_t)stream;
-  auto go = [&](auto* zt, auto* gt) {
+  auto launch = [&](auto* zt, auto* gt, auto nt) {
     using T = std::remove_pointer_t<decltype(gt)>;
-    hipLaunchKernelGGL(distill_bwd_kernel<T>, dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V, parts, width, k,
-                       (const float2*)row_stat, t, idx, 1.f / tau, gscale, inv_n, scale, gt, ldg);
+    hipLaunchKernelGGL((distill_bwd_kernel<T, decltype(nt)::value>), dim3((unsigned)(R * parts)), dim3(256), 0, st, zt, ldz, V,
+                       parts, width, k, (const float2*)row_stat, t, idx, 1.f / tau, gscale, inv_n, scale, gt, ldg);
+  };
+  auto go = [&](auto* zt, auto* gt) {
+    if (R * V * es > MEMORY_CACHE) launch(zt, gt, std::true_type{});
+    else launch(zt, gt, std::false_type{});
   };
   if (dtype == UNOK_BF16) go((const bf16_t*)z, (bf16_t*)grad);
   else go((const float*)z, (float*)grad);
