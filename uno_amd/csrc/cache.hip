@@ -24,7 +24,9 @@ struct KeepArgs {
 // after it, so that any list of nodes (descending, the same node twice) means the gather it says. Entries
 // outside [0, max_len - n) and rows at or past max_len are skipped.
 //
-// Bound by latency: length, count, node list and rows are four dependent loads, and few bytes move.
+// Bound by latency: length, count, node list and rows are four dependent loads, and few bytes move (72 tensors of 8 heads
+// of 128 bf16, 8 sequences, paths of 6: 12 MB, 4 us). The three NI are the registers that paths of up to 16, 64 and 256 rows of 256
+// bytes need.
 template <int NI>
 __global__ __launch_bounds__(256) void cache_keep_kernel(const KeepArgs p) {
   const int pair = blockIdx.x, b = pair / p.nk;
@@ -71,7 +73,9 @@ struct CopyArgs {
 // held in registers: the source is read once for all its destinations. The first workgroup of a group sets
 // the destinations' lengths (no destination is a source where the two lie in the same memory).
 //
-// Bound by HBM: (1 + destinations) x rows.
+// Bound by HBM: (1 + destinations) x rows. The stores go past the caches, where they would drive out the source: 72 tensors of
+// 8 heads of 128 bf16, 2048 rows to 8 slots (2.7 GB) 549 -> 539 us, to one (604 MB) 120 -> 98, 1000 rows to 3 slots (590 MB)
+// 122 -> 90; 300 rows to one (88 MB) 16.9 -> 16.3. (Loads past them too: 579, 109, 114 and 17.5.)
 constexpr int COPY_U = 8, COPY_PIECE = 256 * COPY_U;   // 16-byte chunks
 
 __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
 #pragma unroll
       for (int i = 0; i < COPY_U; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
-        if (c < total) o[c] = v[i];
+        if (c < total) __builtin_nontemporal_store(v[i], o + c);
       }
     }
   }
