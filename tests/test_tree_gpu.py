@@ -289,6 +289,18 @@ def test_long_cache(dev):
     _check(out[:, :, h].reshape(B * T, 2 * D), ref, BF)
 
 
+@pytest.mark.parametrize("dtype,T,heads", [(BF, 1, (8, 4, 128)), (BF, 9, (16, 4, 64)), (BF, 30, (16, 4, 128)), (BF, 60, (8, 4, 128)),
+                                           (F32, 3, (8, 4, 64)), (F32, 20, (8, 4, 128))])
+def test_caches_larger_than_the_memory_side_cache(dev, dtype, T, heads):
+    """1 GB of keys and values in two sequences, the last head's outputs compared."""
+    nq, nk, D = heads
+    rows = 2 ** 30 // (2 * 2 * nk * D * (2 if dtype == BF else 4))
+    q, k, v, n, parents = _case(dev, dtype, 2, T, heads, [rows - 1000, rows // 2 + 77], room=0)
+    out = K.tree_attn(q, k, v, n, parents.to(dev)).view(2 * T, nk, -1)
+    last = q.view(2 * T, nk, -1)[:, -1].contiguous()
+    _check(out[:, -1], _reference(last, k[:, -1:], v[:, -1:], n, parents, D ** -0.5), dtype)
+
+
 def test_tree_depths(dev):
     parents = _parents(5, 256, 11, pad=40)
     parents[2] = torch.arange(256, dtype=torch.int32) - 1

@@ -104,8 +104,8 @@ __device__ __forceinline__ uint32_t dma_lane_off(int64_t ld, int col0, int wid, 
 // One 64-row tile of a row-major [rows, ld] bf16 matrix via buffer loads straight into LDS, at
 // the per-lane offsets of dma_lane_off. The buffer resource starts at row k0 and covers rows
 // [k0, kend), so rows past kend read as zeros without any clamping arithmetic (their keys are
-// masked).
-template <int D, int NW = 4>
+// masked). PAST: non-temporal loads, for rows that no cache holds.
+template <int D, int NW = 4, bool PAST = false>
 __device__ __forceinline__ void dma_tile(const bf16_t* src, int64_t ld, uint32_t lane_off, int k0, int kend,
                                          bf16_t* dst, int wid) {
   constexpr int CPR = D / 8, RPI = 64 / CPR, INS = 64 / (RPI * NW);
@@ -125,6 +125,6 @@ __device__ __forceinline__ void dma_tile(const bf16_t* src, int64_t ld, uint32_t
 #pragma unroll
   for (int i = 0; i < INS; ++i)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (i * NW + wid) * RPI * D),
-                                             16, lane_off + i * step, 0, 0, 0);
+                                             16, lane_off + i * step, 0, 0, PAST ? 2 : 0);
 }
 

@@ -5,17 +5,15 @@
 // The queries of one (sequence, K/V head) pair, rep q heads x T nodes, are the rows of one product, so each
 // cache row is read once per row tile.
 //
-// A workgroup takes one row tile of up to 64 query rows and one range of the keys; its four waves take
-// key tiles in turn, each with its own running maximum and sum, and merge at the end: no barrier in the
-// walk, and no LDS either. K and V go from memory into the registers that the MFMAs read:
-//   S^T = K Q^T   the first operand wants 16 keys x 8 (fp32: 4) consecutive dims per lane: 16-byte loads of K;
-//   O^T = V^T P^T the second operand is P^T as S^T's accumulators hold it (lane: query l % 16, four keys), and the first
-//                 wants, per lane, one dim of eight (four) keys. With the accumulators' dims numbered so that lane
-//                 m = l % 16 owns dims 8 m .. 8 m + 7 (4 m .. + 3 of each 64), those are 16-byte loads of V rows, and a
-//                 bf16 pair of keys is one byte permute.
-// The maximum that a wave's weights refer to moves only when a score exceeds it by 2^8 (the weights stay
-// within fp32 and bf16 range), so that most tiles pass without a reduction across lanes. Scores,
-// statistics and outputs are fp32; the weights of bf16 products are rounded to bf16, as their V is.
+// A workgroup takes one row tile and one range of the keys (see tree_range); ranges of one sequence are merged by a second
+// kernel. Two walks, by the number of rows (see tree_plan):
+// * few rows (16; fp32 32), bound by HBM: tree_attn_kernel, K and V straight into the MFMAs' registers;
+// * more rows, bf16, bound by LDS, MFMA and VALU alike: tree_attn_lds_kernel, K and V tiles shared through LDS.
+// In both S^T = K Q^T and O^T = V^T P^T, so that a query is a column: its maximum and sum are one number in a lane, and S^T's
+// accumulators are P^T's operand as they stand.
+// The maximum that a row's weights refer to moves only when a score exceeds it by 2^8 (the weights stay
+// within fp32 and bf16 range), so that most tiles pass without rescaling. Scores, statistics and outputs are fp32; the
+// weights of bf16 products are rounded to bf16, as their V is.
 #include "common.h"
 #include "lds_tile.h"
 #include "../../include/unok.h"
@@ -43,10 +41,16 @@ struct TreeAttn {
 
 // How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
 // together. A range is at most c blocks of TB keys, c the least from TREE_LEAST on for which all sequences' keys make about
-// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it.
+// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it. (Ranges of less than
+// 256 keys cost more in the merge than they save: one sequence of 4096 rows 20 us, 26 with 64 or 128.)
 constexpr int TB = 128, TREE_LEAST = 2;
 
-struct Range { int b, n, end, first, count, lo, hi; };   // sequence, its lengths, its ranges, this range's keys
+struct Range { int b, n, end, first, count, lo, hi; bool past; };   // sequence, its lengths, its ranges, this range's keys
+
+// Keys and values well above the memory-side cache's 256 MB are read past the caches (8 sequences, 8 heads of 128 bf16 over
+// 16384 rows, 537 MB: 16 nodes 116 -> 103 us, one node 105 -> 98). Below, a part is found there: over 4096 rows (134 MB) 16
+// nodes take 35 us, 41 with such loads, and 4 nodes in fp32 (269 MB) 54 and 66.
+constexpr int64_t TREE_PAST = 384ll << 20;
 
 __device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
   const int64_t len = a.lengths[b];
@@ -84,7 +88,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // Finds range `id`. Every wave of the workgroup does it for itself.
-__device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
+__device__ __forceinline__ Range tree_range(const TreeAttn& a, int id, int row_bytes) {
   const int lane = threadIdx.x & 63;
   int total = 0, n = 0, end = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -99,7 +103,7 @@ __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id) {
       if (__builtin_amdgcn_readlane(wave_scan(count), 63) <= max(a.share, a.B)) break;
       c += (c + 15) / 16;
     }
-  Range r{-1, 0, 0, 0, 0, 0, 0};
+  Range r{-1, 0, 0, 0, 0, 0, 0, (int64_t)total * TB * a.nk * row_bytes * 2 > TREE_PAST};
   int first = 0;
   for (int b0 = 0; b0 < a.B && r.b < 0; b0 += 64) {
     if (a.B > 64) end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
@@ -177,6 +181,11 @@ __device__ __forceinline__ bool tree_sees(const uint32_t* anc, int node, int W, 
   return anc[node * W + i] >> (t & 31) & 1;
 }
 
+template <bool PAST, typename T> __device__ __forceinline__ T tree_load(const T* p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 template <typename T, int D> struct TileOps;
 
 // bf16: tiles of 32 keys. Slot j of lane group g is key 4 g + j (j < 4) or 16 + 4 g + j - 4, in P and in V.
@@ -196,20 +205,20 @@ template <int D> struct TileOps<bf16_t, D> {
 #pragma unroll
     for (int s = 0; s < KS; ++s) q.f[s] = *(const bf16x8_t*)(row + 32 * s + 8 * g);
   }
-  template <typename F> static __device__ __forceinline__ void load_k(K& k, F row, int m, int g) {
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_k(K& k, F row, int m, int g) {
 #pragma unroll
     for (int a = 0; a < NS; ++a) {
       const bf16_t* r = row(16 * a + m);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) k.f[a][s] = *(const bf16x8_t*)(r + 32 * s + 8 * g);
+      for (int s = 0; s < KS; ++s) k.f[a][s] = tree_load<PAST>((const bf16x8_t*)(r + 32 * s + 8 * g));
     }
   }
-  template <typename F> static __device__ __forceinline__ void load_v(V& v, F row, int m, int g) {
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_v(V& v, F row, int m, int g) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const bf16_t* r = row(slot_key(j, g)) + NDT * m;
-      if constexpr (VW == 4) { const u32x4_t u = *(const u32x4_t*)r; v.w[j][0] = u[0]; v.w[j][1] = u[1]; v.w[j][2] = u[2]; v.w[j][3] = u[3]; }
-      else { const u32x2_t u = *(const u32x2_t*)r; v.w[j][0] = u[0]; v.w[j][1] = u[1]; }
+      if constexpr (VW == 4) { const u32x4_t u = tree_load<PAST>((const u32x4_t*)r); v.w[j][0] = u[0]; v.w[j][1] = u[1]; v.w[j][2] = u[2]; v.w[j][3] = u[3]; }
+      else { const u32x2_t u = tree_load<PAST>((const u32x2_t*)r); v.w[j][0] = u[0]; v.w[j][1] = u[1]; }
     }
   }
   static __device__ __forceinline__ Acc score(const K& k, const Q& q, int a) {
@@ -274,17 +283,17 @@ template <int D> struct TileOps<float, D> {
 #pragma unroll
     for (int s = 0; s < KS; ++s) q.f[s] = *(const f32x4_t*)(row + 16 * s + 4 * g);
   }
-  template <typename F> static __device__ __forceinline__ void load_k(K& k, F row, int m, int g) {
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_k(K& k, F row, int m, int g) {
     const float* r = row(m);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k.f[0][s] = *(const f32x4_t*)(r + 16 * s + 4 * g);
+    for (int s = 0; s < KS; ++s) k.f[0][s] = tree_load<PAST>((const f32x4_t*)(r + 16 * s + 4 * g));
   }
-  template <typename F> static __device__ __forceinline__ void load_v(V& v, F row, int m, int g) {
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_v(V& v, F row, int m, int g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float* r = row(slot_key(j, g)) + 4 * m;
 #pragma unroll
-      for (int jj = 0; jj < NJ; ++jj) v.w[j][jj] = *(const f32x4_t*)(r + 64 * jj);
+      for (int jj = 0; jj < NJ; ++jj) v.w[j][jj] = tree_load<PAST>((const f32x4_t*)(r + 64 * jj));
     }
   }
   static __device__ __forceinline__ Acc score(const K& k, const Q& q, int a) {
@@ -321,6 +330,16 @@ template <int D> struct TileOps<float, D> {
   }
 };
 
+// Few query rows (16 QT): the four waves take key tiles in turn, each with its own running maximum and sum, and merge at the end: no
+// barrier in the walk, and no LDS either. K and V go from memory into the registers that the MFMAs read:
+//   S^T = K Q^T   the first operand wants 16 keys x 8 (fp32: 4) consecutive dims per lane: 16-byte loads of K;
+//   O^T = V^T P^T the second operand is P^T as S^T's accumulators hold it (lane: query l % 16, four keys), and the first
+//                 wants, per lane, one dim of eight (four) keys. With the accumulators' dims numbered so that lane
+//                 m = l % 16 owns dims 8 m .. 8 m + 7 (4 m .. + 3 of each 64), those are 16-byte loads of V rows, and a
+//                 bf16 pair of keys is one byte permute.
+// One tile ahead in a second register set. Bound by HBM: 8 sequences, 32 / 8 heads of 128 bf16, one node over 16384 rows 98 us (5.5
+// TB/s), over 4096 rows 32 us with the merge; a single sequence of 130 rows 8 us, which is launch and latency. fp32, 32 rows, bound
+// by its 16x16x4 MFMAs: 16 nodes over 4096 rows 110 us (64 rows a workgroup, which spills: 209).
 template <typename E, int D, int QT>
 __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   using Ops = TileOps<E, D>;
@@ -335,7 +354,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
   int tile, h, id;
   tree_place(a, tile, h, id);
-  const Range range = tree_range(a, id);
+  const Range range = tree_range(a, id, D * (int)sizeof(E));
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, end = range.end, lo = range.lo, hi = range.hi;
   tree_note(a, range, id, h, tile);
@@ -405,10 +424,11 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   // Tiles of committed rows, which every query sees: one tile ahead, in two register sets.
   const int full = hi < n ? hi : n;
   int key = lo + wid * KT;
-  {
+  auto walk = [&](auto past) {
+    constexpr bool PAST = decltype(past)::value;
     auto load = [&](typename Ops::K& k, typename Ops::V& v, int key0) {
-      Ops::load_k(k, [&](int j) { return kbase + (int64_t)(key0 + j) * a.kr; }, m, g);
-      Ops::load_v(v, [&](int j) { return vbase + (int64_t)(key0 + j) * a.vr; }, m, g);
+      Ops::template load_k<PAST>(k, [&](int j) { return kbase + (int64_t)(key0 + j) * a.kr; }, m, g);
+      Ops::template load_v<PAST>(v, [&](int j) { return vbase + (int64_t)(key0 + j) * a.vr; }, m, g);
     };
     auto step = [&](const typename Ops::K& k, const typename Ops::V& v) {
       float p[QT][NP];
@@ -428,14 +448,16 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
       step(k1, v1);
       key += 4 * KT;
     }
-  }
+  };
+  if (range.past) walk(std::true_type{});
+  else walk(std::false_type{});
   // Tiles with tree rows. Keys at or past the end read the last row, at weight 0.
 #pragma unroll 1
   for (; key < hi; key += 4 * KT) {
     typename Ops::K k;
     typename Ops::V v;
-    Ops::load_k(k, [&](int j) { const int r = key + j; return kbase + (int64_t)(r < end ? r : end - 1) * a.kr; }, m, g);
-    Ops::load_v(v, [&](int j) { const int r = key + j; return vbase + (int64_t)(r < end ? r : end - 1) * a.vr; }, m, g);
+    Ops::template load_k<false>(k, [&](int j) { const int r = key + j; return kbase + (int64_t)(r < end ? r : end - 1) * a.kr; }, m, g);
+    Ops::template load_v<false>(v, [&](int j) { const int r = key + j; return vbase + (int64_t)(r < end ? r : end - 1) * a.vr; }, m, g);
     float p[QT][NP];
     scores(k, p);
 #pragma unroll
@@ -538,10 +560,19 @@ __device__ __forceinline__ float half_max(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// bf16, more than 32 query rows: K and V tiles of 64 keys in LDS (two stages, filled by direct-to-LDS loads one tile
-// ahead), 32x32x16 MFMAs, 32 rows per wave. RG = 4: the four waves take four row groups and all keys; RG = 2: two row groups
-// and one half of every tile's keys each, merged at the end. S^T = K Q^T puts a query in a lane's column; P^T goes to the
-// P V product from the accumulators, V's columns come by LDS transpose loads (see lds_tile.h).
+// bf16, more than 16 query rows: K and V tiles in LDS, filled by direct-to-LDS loads ahead of their use, 32x32x16 MFMAs, 32 rows
+// to a wave, RG groups of 32 rows to a workgroup. V's columns come by LDS transpose loads (see lds_tile.h).
+//   RG = 2: 4 waves, tiles of 64 keys in two stages, two workgroups to a CU; a row group's two waves take half of every tile's keys
+//           each. 8 sequences, 32 / 8 heads of 128, 16 nodes over 4096 rows: 25 us and 6.5 for the merge (the 134 MB are
+//           in the memory-side cache; four stages and one workgroup to a CU: 52 us in place of 45 at the time; 8 waves: 64
+//           sequences of 1000 rows 66 us in place of 55); over 16384 rows 103 us, 5.2 TB/s.
+//   RG = 4: 8 waves, tiles of 128 keys in two stages, key halves as above: 32 nodes over 4096 rows 39 us (4 waves, all keys
+//           each: 43).
+//   RG = 8: 8 waves, all keys each, tiles of 64 keys in four stages: 16 sequences, 64 nodes over 16384 rows 265-320 us, 0.85
+//           PFLOP/s (RG = 4 in twice the row tiles: 350). A wave's 64 keys x 32 rows take 1024 cycles of MFMA, as many of LDS
+//           reads and 900 of VALU (the exponentials are half of those), two waves to a SIMD, and the clock falls under the
+//           load: the shorter time is of single calls, the longer of calls back to back. (64 rows a wave in four waves read LDS half
+//           as often, but nothing runs beside a wave's own exponentials: 359 us.)
 template <int D, int RG>
 __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(const TreeAttn a) {
   constexpr int NKS = D / 16, NDT = D / 32, ROWS = 32 * RG, NW = RG == 2 ? 4 : 8;
@@ -559,7 +590,7 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T, W = (T + 31) / 32;
   int tile0, h, id;
   tree_place(a, tile0, h, id);
-  const Range range = tree_range(a, id);
+  const Range range = tree_range(a, id, D * 2);
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, lo = range.lo, hi = range.hi;
   tree_note(a, range, id, h, tile0);
@@ -567,11 +598,15 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
   const bf16_t* vbase = (const bf16_t*)a.v + b * a.vb + h * a.vh;
   const uint32_t ko = dma_lane_off<D, NW>(a.kr, 0, wid, lane), vo = dma_lane_off<D, NW>(a.vr, 0, wid, lane);
   auto fetch = [&](int key, int stage) {               // rows at or past hi read as zeros
+    auto go = [&](auto past) {
 #pragma unroll
-    for (int i = 0; i < TK / 64; ++i) {
-      dma_tile<D, NW>(kbase, a.kr, ko, key + 64 * i, hi, smem + stage * STAGE + 64 * i * D, wid);
-      dma_tile<D, NW>(vbase, a.vr, vo, key + 64 * i, hi, smem + stage * STAGE + TILE + 64 * i * D, wid);
-    }
+      for (int i = 0; i < TK / 64; ++i) {
+        dma_tile<D, NW, decltype(past)::value>(kbase, a.kr, ko, key + 64 * i, hi, smem + stage * STAGE + 64 * i * D, wid);
+        dma_tile<D, NW, decltype(past)::value>(vbase, a.vr, vo, key + 64 * i, hi, smem + stage * STAGE + TILE + 64 * i * D, wid);
+      }
+    };
+    if (range.past) go(std::true_type{});
+    else go(std::false_type{});
   };
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i)
@@ -902,6 +937,10 @@ __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restr
 
 struct TreePlan { int rows, rt, share; int64_t ranges; };   // rows per row tile; most ranges of all sequences
 
+// The row tile is the least that holds a pair's rows, up to what a workgroup can; K and V are read once per tile.
+// 16: the register walk (8 sequences of 4096 rows, 4 nodes of 4 heads, 39 us where the LDS walk took 47; with 32 rows 40, and the LDS
+// walk 32). Head dimension 64 has half the work to a key, and 128 rows are enough. `share` is one round of workgroups, two
+// to a CU for up to 64 rows and one above: with 1.5 to 4 rounds every case was slower.
 TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   const int NR = nq / nk * T;
   TreePlan p;
