@@ -541,7 +541,8 @@ __global__ __launch_bounds__(256) void topk_merge_kernel(const uint64_t* __restr
 }
 
 // Parts of a row: with fewer rows than fill the chip (two workgroups per CU), as many as do, of at least 4096 columns, whose
-// entries the merge holds.
+// entries the merge holds. Rows of 151936, k = 10: 16 rows 18.6 us, 128 rows 33 (for one workgroup per CU 19.4 and 41, for four
+// 19.6 and 31); 4 rows 17 us (parts of 2048 columns 25), one row, k = 5, 14.8 (parts of 8192 columns 16.6).
 int topk_parts(int R, int V, int k) {
   const int want = (512 + R - 1) / (R > 0 ? R : 1), most = V / 4096, room = TK_MERGE / k;
   int p = want < most ? want : most;
@@ -754,7 +755,9 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
   if (mine) Elem<T>::store(g + col, distill_exp<T>(zc * inv_tau - m) / rs.y * c - psum * c);
 }
 
-// Parts of a row of the statistics and the gradient, as topk_parts, of at least 8192 columns.
+// Parts of a row of the statistics and the gradient, as topk_parts, for four workgroups per CU, of at least 8192 columns. 300 rows of
+// 151936, forward and backward: 61 us (for two or eight per CU 65); 16 rows of 32000 23 us (of 16384 columns 25, of 4096 21; no other case
+// moves by more than 1 us).
 int distill_parts(int R, int V) {
   const int want = (1024 + R - 1) / (R > 0 ? R : 1), most = V / 8192;
   const int p = want < most ? want : most;
