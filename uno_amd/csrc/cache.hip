@@ -74,7 +74,7 @@ struct CopyArgs {
 // the destinations' lengths (no destination is a source where the two lie in the same memory).
 //
 // Bound by HBM: (1 + destinations) x rows. The stores go past the caches, where they would drive out the source: 72 tensors of
-// 8 heads of 128 bf16, 2048 rows to 8 slots (2.7 GB) 549 -> 539 us, to one (604 MB) 120 -> 98, 1000 rows to 3 slots (590 MB)
+// 8 heads of 128 bf16, 2048 rows to 8 slots (2.7 GB) 549 -> 539 us or the same, to one (604 MB) 120 -> 98, 1000 rows to 3 (590 MB)
 // 122 -> 90; 300 rows to one (88 MB) 16.9 -> 16.3. (Loads past them too: 579, 109, 114 and 17.5.)
 constexpr int COPY_U = 8, COPY_PIECE = 256 * COPY_U;   // 16-byte chunks
 

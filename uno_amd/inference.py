@@ -38,6 +38,11 @@ from .adapter import MODULES
 from .layers import Geometry, StreamContext, clean_layer
 
 
+# Without the LoRA's side products the few-row products are the faster ones up to this many rows: eight 8B layers and the head over
+# 4096 cached rows, 64 rows 1773 us (the step's GEMMs 1863), 128 rows 2004 (1992), 256 rows 2773 (2386), 512 rows 4315 (3057).
+PLAIN_FEW_ROWS = 128
+
+
 class BlockKVCache:
     """Per-layer K and V, head-major [B, Hkv, max_len, D], and the committed length per sequence."""
 
@@ -193,9 +198,10 @@ class BlockDecoder:
         h = K.embedding(ids.reshape(-1).contiguous().to(torch.int64), dec.embed_tokens.weight)
         for li, layer in enumerate(dec.layers):
             h = self._layer(h, layer.weights(), li, maps.get("pos"), gate_rows, cache, maps, B, T)
-        return self._head(h, False).view(B, T, -1)
+        return self._head(h, gate_rows is None and B * T > PLAIN_FEW_ROWS).view(B, T, -1)
 
     def _head(self, h, prefill: bool):
+        """Logits of the decoder's output rows (``prefill``: not by the few-row products)."""
         x, _ = K.rmsnorm_fwd(h, self.decoder.norm.weight, self.geo.eps)
         w = self.base.lm_head.weight
         head = K.gemm_nt_rows if self._rows_path(x.shape[0], x.dtype, prefill) and w.shape[0] % 4 == 0 else K.gemm_nt
@@ -342,7 +348,7 @@ class BlockDecoder:
         r = lora.rank
         q_end, k_end = g.q, g.q + g.kv
         M = h0.shape[0]
-        few = self._rows_path(M, h0.dtype, False)
+        few = self._rows_path(M, h0.dtype, gate_rows is None and M > PLAIN_FEW_ROWS)
         qkv_segments = [(q_end, 0), (k_end, r), (k_end + g.kv, 2 * r)]
 
         def linear(x, w, part, segments=None, residual=None, swiglu=False):
