@@ -215,7 +215,7 @@ def _prep(**over):
 C = ctypes.c_void_p
 ENTRIES = [
     ("unok_tree_attn", _tree_call, [dict(dtype=7), dict(B=-1), dict(T=-1), dict(T=257), dict(nq=3, nk=2), dict(nk=0), dict(D=96),
-                                    dict(max_len=0), dict(max_len=1 << 30), dict(B=1 << 20, T=256), dict(q=None), dict(k=None),
+                                    dict(max_len=0), dict(max_len=1 << 30), dict(B=1 << 20, T=256), dict(B=1 << 15, max_len=1 << 23), dict(q=None), dict(k=None),
                                     dict(lengths=None), dict(parents=None), dict(o=None), dict(kr=32), dict(vr=32),
                                     dict(kr=1 << 23), dict(ldp=3), dict(q=BASE + 2), dict(k=BASE + 8), dict(ldq=129),
                                     dict(kb=2047), dict(vh=2047), dict(kr=65), dict(ldo=130), dict(max_len=8192),

@@ -217,6 +217,33 @@ def test_captured_trees(dev, dtype, T):
             call()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_draft_graph_follows_accepts_and_copies(dev, dtype):
+    """A captured draft block between accepts and copies: the eager block's logits, and a refusal once the cache is full."""
+    cfg, params, lora, dec = _build(dev, "gqa2", dtype)
+    g = torch.Generator().manual_seed(6)
+    B, P, L = 2, 10, 8
+    prompt = torch.randint(0, cfg.vocab_size - 1, (B, P), generator=g).to(dev)
+    cache = dec.new_cache(B, P + 3 * 4 + L)
+    dec.prefill(cache, prompt)
+    graph = dec.capture_draft(cache, L, commit=0)
+    parents = torch.arange(-1, 3, device=dev, dtype=torch.int32)
+    path, counts = torch.arange(4, device=dev).repeat(B, 1), torch.tensor([4, 0], device=dev)
+    for step in range(4):
+        blk = torch.randint(0, cfg.vocab_size - 1, (B, L), generator=g).to(dev)
+        assert torch.equal(graph.replay(blk).clone(), dec.draft_block(cache, blk, commit=0)), step
+        if step == 3:
+            break
+        dec.tree_block(cache, blk[:, :4], parents)
+        cache.accept(path, counts)
+    assert cache.lengths.tolist() == [P + 12, P]
+    longer = dec.new_cache(1, 2 * cache.max_len)
+    dec.prefill(longer, torch.randint(0, cfg.vocab_size - 1, (1, P + 13), generator=g).to(dev))
+    cache.copy_from(longer, [(0, 1)])
+    with pytest.raises(RuntimeError, match="does not fit"):
+        graph.replay(blk)
+
+
 def test_drafting_with_trees_is_greedy_decoding(dev):
     """The operators as they are used together: the top logits of the last pass become the children of the next tree, one
     pass verifies it, the longest path of the model's own choices is kept. Every token it gives is the oracle's choice

@@ -957,8 +957,8 @@ int tree_sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
                "tree_attn: B=%d T=%d nq=%d nk=%d max_len=%d", B, T, nq, nk, max_len);
   UNOK_REQUIRE(T <= TREE_MAX, UNOK_EUNSUPPORTED, "tree_attn: trees hold at most %d nodes (got %d)", TREE_MAX, T);
   UNOK_REQUIRE(D == 64 || D == 128, UNOK_EINVAL, "tree_attn: head dim %d not in {64,128}", D);
-  UNOK_REQUIRE((int64_t)B * nq * (T > 0 ? T : 1) < (1ll << 24) && max_len < (1 << 30), UNOK_EINVAL,
-               "tree_attn: B=%d T=%d nq=%d max_len=%d exceed the row layout", B, T, nq, max_len);
+  UNOK_REQUIRE((int64_t)B * nq * (T > 0 ? T : 1) < (1ll << 24) && max_len < (1 << 30) && B * (max_len / TB + 1ll) < (1ll << 30),
+               UNOK_EINVAL, "tree_attn: B=%d T=%d nq=%d max_len=%d exceed the row layout", B, T, nq, max_len);
   return 0;
 }
 

@@ -52,6 +52,7 @@ class BlockKVCache:
         self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int64)
         self.batch, self.max_len, self.geo = batch, max_len, geo
+        self.moves = 0                                   # accepts and copies so far: a DraftGraph looks at the lengths again
 
     def accept(self, nodes: torch.Tensor, counts: torch.Tensor) -> None:
         """Commits the accepted nodes of the tree that ``BlockDecoder.tree_block`` wrote: nodes [B, P] int64, of which the
@@ -59,6 +60,7 @@ class BlockKVCache:
         committed rows in that order (every row is read before any is written); the tree's other rows are dropped. All
         on the device, and capturable into a graph."""
         K.cache_keep(self.k + self.v, self.lengths, nodes, counts)
+        self.moves += 1
         self.lengths += counts.clamp(0, nodes.shape[1])
 
     def copy_from(self, other: "BlockKVCache", pairs) -> None:
@@ -71,6 +73,7 @@ class BlockKVCache:
         if other.max_len > self.max_len and all(0 <= a < other.batch for a, _ in pairs) and \
                 int(other.lengths[[a for a, _ in pairs]].max()) > self.max_len:
             raise RuntimeError("the sequences do not fit in the KV cache")
+        self.moves += 1
         K.cache_copy(other.k + other.v, self.k + self.v, other.lengths, self.lengths, pairs)
 
 
@@ -423,8 +426,8 @@ class DraftGraph:
 
     ``replay`` returns the graph's own logits buffer [B, L, V], overwritten by the next replay.
     The cache capacity is checked on the host against the longest committed length read at
-    capture plus the commits since; after changing ``cache.lengths`` by other means, capture
-    again."""
+    capture, or after the cache's last ``accept`` or ``copy_from``, plus the commits since; after
+    changing ``cache.lengths`` by other means, capture again."""
 
     def __init__(self, decoder: BlockDecoder, cache: BlockKVCache, block_size: int, commit: int = 1):
         B, L = cache.batch, block_size
@@ -438,7 +441,7 @@ class DraftGraph:
         self.ids = torch.zeros((B, L), device=dev, dtype=torch.int64)
         self.gate = torch.ones((B, L), device=dev, dtype=torch.bool)
         self.gate[:, 0] = False
-        self._len_max = int(cache.lengths.max())
+        self._len_max, self._moves = int(cache.lengths.max()), cache.moves
         if self._len_max + L > cache.max_len:
             raise RuntimeError("the block does not fit in the KV cache")
         # One eager pass without commit before the capture: it sets each kernel's launch attributes
@@ -455,6 +458,8 @@ class DraftGraph:
         default gate (off on the seed row, on for the noise rows) for this and later replays."""
         if tuple(block_ids.shape) != tuple(self.ids.shape):
             raise RuntimeError(f"block {tuple(block_ids.shape)} does not match the captured {tuple(self.ids.shape)}")
+        if self._moves != self.cache.moves:
+            self._len_max, self._moves = int(self.cache.lengths.max()), self.cache.moves
         if self._len_max + self.block_size > self.cache.max_len:
             raise RuntimeError("the block does not fit in the KV cache")
         self.ids.copy_(block_ids)
