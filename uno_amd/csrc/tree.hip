@@ -41,8 +41,10 @@ struct TreeAttn {
 
 // How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
 // together. A range is at most c blocks of TB keys, c the least from TREE_LEAST on for which all sequences' keys make about
-// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it. (Ranges of less than
-// 256 keys cost more in the merge than they save: one sequence of 4096 rows 20 us, 26 with 64 or 128.)
+// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it. Sequences of three
+// to eight blocks on average are cut into single ones: one sequence of 1000 rows, one node 10.1 us (in ranges of 256 keys
+// 11.1), fp32 37 nodes of three of 901 rows 13.7 (16.7). Longer ones would pay for it in the merge (one of 4096 rows 15.7 in place
+// of 13.1), shorter ones need none at all (130 rows 9.0 and 8.0).
 constexpr int TB = 128, TREE_LEAST = 2;
 
 struct Range { int b, n, end, first, count, lo, hi; bool past; };   // sequence, its lengths, its ranges, this range's keys
@@ -95,7 +97,7 @@ __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id, int row_b
     end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
     total += __builtin_amdgcn_readlane(wave_scan((end + TB - 1) / TB), 63);
   }
-  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), TREE_LEAST);
+  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), total > 2 * a.B && total <= 8 * a.B ? 1 : TREE_LEAST);
   // sequences end inside ranges: larger ones until no more than `share` are left (one round of workgroups)
   if (a.B <= 64)
     for (int i = 0; i < 12; ++i) {
@@ -337,9 +339,9 @@ template <int D> struct TileOps<float, D> {
 //                 wants, per lane, one dim of eight (four) keys. With the accumulators' dims numbered so that lane
 //                 m = l % 16 owns dims 8 m .. 8 m + 7 (4 m .. + 3 of each 64), those are 16-byte loads of V rows, and a
 //                 bf16 pair of keys is one byte permute.
-// One tile ahead in a second register set. Bound by HBM: 8 sequences, 32 / 8 heads of 128 bf16, one node over 16384 rows 98 us (5.5
-// TB/s), over 4096 rows 32 us with the merge; a single sequence of 130 rows 8 us, which is launch and latency. fp32, 32 rows, bound
-// by its 16x16x4 MFMAs: 16 nodes over 4096 rows 110 us (64 rows a workgroup, which spills: 209).
+// One tile ahead in a second register set. Bound by HBM: 8 sequences, 32 / 8 heads of 128 bf16, one node over 16384 rows 96 us (5.6
+// TB/s), over 4096 rows 28 us with the merge; a single sequence of 130 rows 8 us, which is launch and latency. fp32, 32 rows, bound
+// by its 16x16x4 MFMAs: 16 nodes over 4096 rows 108 us (64 rows a workgroup, which spills: 209).
 template <typename E, int D, int QT>
 __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   using Ops = TileOps<E, D>;
@@ -563,7 +565,7 @@ __device__ __forceinline__ float half_max(float v) {
 // bf16, more than 16 query rows: K and V tiles in LDS, filled by direct-to-LDS loads ahead of their use, 32x32x16 MFMAs, 32 rows
 // to a wave, RG groups of 32 rows to a workgroup. V's columns come by LDS transpose loads (see lds_tile.h).
 //   RG = 2: 4 waves, tiles of 64 keys in two stages, two workgroups to a CU; a row group's two waves take half of every tile's keys
-//           each. 8 sequences, 32 / 8 heads of 128, 16 nodes over 4096 rows: 25 us and 6.5 for the merge (the 134 MB are
+//           each. 8 sequences, 32 / 8 heads of 128, 16 nodes over 4096 rows: 25 us and 5.3 for the merge (the 134 MB are
 //           in the memory-side cache; four stages and one workgroup to a CU: 52 us in place of 45 at the time; 8 waves: 64
 //           sequences of 1000 rows 66 us in place of 55); over 16384 rows 103 us, 5.2 TB/s.
 //   RG = 4: 8 waves, tiles of 128 keys in two stages, key halves as above: 32 nodes over 4096 rows 39 us (4 waves, all keys
@@ -883,7 +885,8 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
 }
 
 // The ranges of each query row merged: one thread per four dims, grid (.., sequences). Sequences of one range were
-// written by the kernels above.
+// written by the kernels above. Bound by latency when ranges are many, so eight are read at a time (one at a time: one sequence of
+// 32768 rows 58 us in place of 34, 8 of 4096 rows with 16 nodes 35 in place of 33), and three where that is all there are.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
   const int b = blockIdx.y, rep = a.nq / a.nk, NR = rep * a.T;
@@ -893,28 +896,39 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
   if (row >= a.nk * NR) return;
   const int h = row / NR, r = row % NR, t = r % a.T;
   const int64_t at0 = (int64_t)range.x * a.nk * NR + row, step = (int64_t)a.nk * NR;
-  // four ranges' rows in flight at a time; the ranges are few, so their maxima are read twice
   float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < range.y; ++s) top = fmaxf(top, a.pm[2 * (at0 + s * step)]);
   f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < range.y; s0 += 4) {
-    f32x4_t v[4];
-    float ms[4], ls[4];
+  auto merge = [&](int s0, auto n) {                     // the next n ranges, in flight together
+    constexpr int N = decltype(n)::value;
+    f32x4_t v[N];
+    float2 ml[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int64_t at = at0 + min(s0 + i, range.y - 1) * step;
       v[i] = *(const f32x4_t*)(a.po + at * D + d);
-      ms[i] = s0 + i < range.y ? a.pm[2 * at] : -INFINITY;
-      ls[i] = s0 + i < range.y ? a.pm[2 * at + 1] : 0.f;
+      ml[i] = *(const float2*)(a.pm + 2 * at);
     }
+    float to = top;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (ms[i] == -INFINITY) { sum += ls[i]; continue; }   // 0, or NaN from NaN scores alone
-      const float f = __builtin_amdgcn_exp2f(ms[i] - top);
-      sum += ls[i] * f;
-      x += v[i] * f;
+    for (int i = 0; i < N; ++i) {
+      if (s0 + i >= range.y) ml[i] = make_float2(-INFINITY, 0.f);
+      to = fmaxf(to, ml[i].x);
     }
-  }
+    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - to);   // (without a maximum x is 0, sum 0 or NaN)
+    top = to;
+    sum *= f;
+    x *= f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (ml[i].x == -INFINITY) { sum += ml[i].y; continue; }   // 0, or NaN from NaN scores alone
+      const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
+      sum += ml[i].y * w;
+      x += v[i] * w;
+    }
+  };
+  if (range.y <= 3) merge(0, std::integral_constant<int, 3>{});
+  else
+    for (int s0 = 0; s0 < range.y; s0 += 8) merge(s0, std::integral_constant<int, 8>{});
   const bool none = sum == 0.f || a.parents[b * a.ldp + t] < -1;
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / sum;
