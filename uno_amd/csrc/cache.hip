@@ -6,6 +6,8 @@
 #include "common.h"
 #include "../../include/unok.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -73,9 +75,11 @@ struct CopyArgs {
 // held in registers: the source is read once for all its destinations. The first workgroup of a group sets
 // the destinations' lengths (no destination is a source where the two lie in the same memory).
 //
-// Bound by HBM: (1 + destinations) x rows. The stores go past the caches, where they would drive out the source: 72 tensors of
-// 8 heads of 128 bf16, 2048 rows to 8 slots (2.7 GB) 549 -> 539 us or the same, to one (604 MB) 120 -> 98, 1000 rows to 3 (590 MB)
-// 122 -> 90; 300 rows to one (88 MB) 16.9 -> 16.3. (Loads past them too: 579, 109, 114 and 17.5.)
+// Bound by HBM: (1 + destinations) x rows. Stores of up to 2 GB go past the caches, where they would drive out the source: 72 tensors
+// of 8 heads of 128 bf16, 2048 rows to one slot (604 MB) 121 -> 99 us, to two 183 -> 157, to four (1.5 GB) 306 -> 289. Above, both
+// reach what HBM does, and the order in which such stores arrive decides: to eight slots (2.7 GB) 550 -> 546 us where every
+// tensor is an allocation of its own, 549 -> 575 where all lie in one. (Loads past the caches too: slower at every size.)
+constexpr int64_t COPY_PAST = 2000000000;
 constexpr int COPY_U = 8, COPY_PIECE = 256 * COPY_U;   // 16-byte chunks
 
 __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
@@ -88,22 +92,29 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
   const int64_t total = rows * p.cpr;                  // 16-byte chunks
   const u32x4_t* src = (const u32x4_t*)p.src[blockIdx.z] + ((int64_t)s * p.nk + h) * p.src_max * p.cpr;
   u32x4_t* dst = (u32x4_t*)p.dst[blockIdx.z];
-  for (int64_t c0 = (int64_t)blockIdx.x * COPY_PIECE; c0 < total; c0 += (int64_t)gridDim.x * COPY_PIECE) {
-    u32x4_t v[COPY_U];
-#pragma unroll
-    for (int i = 0; i < COPY_U; ++i) {
-      const int64_t c = c0 + i * 256 + threadIdx.x;
-      v[i] = src[c < total ? c : total - 1];
-    }
-    for (int d = d0; d < d1; ++d) {
-      u32x4_t* o = dst + ((int64_t)p.slot[d] * p.nk + h) * p.dst_max * p.cpr;
+  // (the branch stands outside: of two stores of one value, the compiler makes one, plain)
+  auto move = [&](auto past) {
+    for (int64_t c0 = (int64_t)blockIdx.x * COPY_PIECE; c0 < total; c0 += (int64_t)gridDim.x * COPY_PIECE) {
+      u32x4_t v[COPY_U];
 #pragma unroll
       for (int i = 0; i < COPY_U; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
-        if (c < total) __builtin_nontemporal_store(v[i], o + c);
+        v[i] = src[c < total ? c : total - 1];
+      }
+      for (int d = d0; d < d1; ++d) {
+        u32x4_t* o = dst + ((int64_t)p.slot[d] * p.nk + h) * p.dst_max * p.cpr;
+#pragma unroll
+        for (int i = 0; i < COPY_U; ++i) {
+          const int64_t c = c0 + i * 256 + threadIdx.x;
+          if (c >= total) continue;
+          if constexpr (decltype(past)::value) __builtin_nontemporal_store(v[i], o + c);
+          else o[c] = v[i];
+        }
       }
     }
-  }
+  };
+  if (total * 16 * p.nk * gridDim.z * p.group_first[p.groups] < COPY_PAST) move(std::true_type{});   // (a group's rows for all)
+  else move(std::false_type{});
   if (blockIdx.x == 0 && blockIdx.z == 0 && h == 0 && p.dst_lengths)
     for (int d = d0 + threadIdx.x; d < d1; d += 256) p.dst_lengths[p.slot[d]] = rows;
 }
