@@ -621,7 +621,7 @@ def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.
     lengths int64 [B]. parents int32 [B, T], or [T] for one tree of all sequences: the index of an earlier node,
     -1 for a root, below -1 for padding, whose output rows are 0; a parent that is no earlier node, or is padding,
     ends the chain. A node sees the committed rows, its ancestors and itself; what else the cache holds does not
-    matter. T <= 256, D 64 or 128, fp32 or bf16."""
+    matter. ``out`` shares no row with q. T <= 256, D 64 or 128, fp32 or bf16."""
     _rowmajor(q, "q")
     if k.dim() != 4 or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
         raise RuntimeError(f"tree_attn: k and v must be [B, nk, max_len, D] in the dtype of q, got {tuple(k.shape)} "
@@ -681,7 +681,7 @@ def tree_prep(qkv, wq, wk, lengths, depths, inv_freq, eps: float, kc, vc, B: int
     if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
         raise RuntimeError("tree_prep: fp32 inv_freq [D/2] required")
     q = torch.empty((B * T, nq * D), device=qkv.device, dtype=qkv.dtype)
-    _same_device("tree_prep", qkv, lengths, depths, inv_freq, kc)
+    _same_device("tree_prep", qkv, lengths, depths, inv_freq, kc, *(w for w in (wq, wk) if w is not None))
     N.call("unok_tree_prep", B, T, nq, nk, D, N.ptr(qkv), _ld(qkv), N.ptr(wq), N.ptr(wk), N.ptr(lengths), N.ptr(depths),
            N.ptr(inv_freq), float(eps), N.ptr(kc), N.ptr(vc), kc.shape[2], N.ptr(q), N.stream())
     return q
