@@ -323,3 +323,23 @@ def test_captured_and_replayed(dev):
         for a, b in zip(got, work()):
             assert torch.equal(a, b), i
         torch.randn(4096, device=dev).sum().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [40, 9001, 40009])
+@pytest.mark.parametrize("low", ["lowest", -3e10])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_row_top_k_masked_by_low_values(dev, dtype, V, low, rows):
+    """Columns masked with the type's lowest value (or another whose product with log2 e is no small number): the first half,
+    the first one, all but the last, the second half, all but one in the middle, every one."""
+    low = torch.finfo(dtype).min if low == "lowest" else low
+    g = torch.Generator(device=dev).manual_seed(V)
+    z = (torch.randn(6, V, device=dev, generator=g) * 3).to(dtype)
+    z[0, :V // 2] = low
+    z[1, 0] = low
+    z[2, :-1] = low
+    z[3, V // 2:] = low
+    z[4, :V // 2], z[4, V // 2 + 1:] = low, low
+    z[5] = low
+    z = z.repeat((rows + 5) // 6, 1)
+    _check_top(z, min(V, 20), K.row_top_k(z, min(V, 20)))

@@ -345,10 +345,12 @@ __global__ __launch_bounds__(256, 6) void row_topk_kernel(const T* __restrict__ 
   // rounding of shift left out is put right at the end.
   float m = -INFINITY, s = 0.f, shift = 0.f;
   auto raise = [&](float to) {
+    // (terms that far below weigh nothing, and their sum is no number where m log2 e is too coarse or overflows: masked columns)
+    const bool drop = to - m > 200.f;
     const float before = shift;
     m = to;
     shift = m == -INFINITY ? 0.f : m * LOG2E;            // -inf then adds 0, and a NaN is seen
-    if (s != 0.f) s *= __builtin_amdgcn_exp2f(before - shift);
+    s = drop ? 0.f : s * __builtin_amdgcn_exp2f(before - shift);
   };
   auto power = [&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, LOG2E, -shift)); };
 
