@@ -307,10 +307,10 @@ int unok_draft_layer(const unok_draft_layer_args* args, void* stream);
 /* Attention of a tree of T <= 256 drafted tokens per sequence. Node t's parent parents[b * ldp + t] (ldp 0: one
  * tree for every sequence) is an earlier node, or -1 for a root; below -1 the node is padding. A node attends to
  * cache rows [0, lengths[b]), its ancestors and itself, node a being cache row lengths[b] + a (rows at or past
- * max_len do not exist; a parent that is no earlier node, or is padding, ends the chain): O = softmax(scale Q K^T) V, zeros for
- * padding. Q and O [B T, nq D] with row strides ldq / ldo and no byte in common, q head h reading K/V head h / (nq / nk); K and V row
- * (b, head, j) at b * batch + head * head stride + j * row stride. dtype 0 / 1, D 64 or 128, every operand and stride a multiple of 16
- * bytes. workspace: unok_tree_attn_workspace() bytes, 16-byte aligned (0: none is read). */
+ * max_len do not exist; a parent that is no earlier node, or is padding, ends the chain): O = softmax(scale Q K^T) V, scale any
+ * finite number, zeros for padding. Q and O [B T, nq D] with row strides ldq / ldo and no byte in common, q head h reading K/V
+ * head h / (nq / nk); K and V row (b, head, j) at b * batch + head * head stride + j * row stride. dtype 0 / 1, D 64 or 128,
+ * every operand and stride a multiple of 16 bytes. workspace: unok_tree_attn_workspace() bytes, 16-byte aligned (0: none is read). */
 int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len);
 int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
                    int64_t k_batch, int64_t k_head, int64_t k_row, const void* v, int64_t v_batch, int64_t v_head,

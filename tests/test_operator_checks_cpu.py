@@ -267,3 +267,10 @@ def test_empty_calls_need_nothing():
                        ("unok_cache_keep", _keep(P=0)), ("unok_cache_keep", _keep(n=0)), ("unok_cache_copy", _copy(np=0)),
                        ("unok_row_topk", _topk(R=0)), ("unok_distill_bwd", _dbwd(R=0))):
         assert getattr(lib, name)(*args) == 0, name
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan"), 3e38])
+def test_tree_attention_refuses_scales(scale):
+    lib = N.lib()
+    assert lib.unok_tree_attn(*_tree_call(scale=scale)) == -1
+    assert "must be finite" in lib.unok_last_error().decode()

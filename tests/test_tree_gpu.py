@@ -451,3 +451,16 @@ def test_captured_and_replayed(dev):
         for b, m in enumerate(other_n.tolist()):
             assert torch.equal(got[3][b, :, :m], other[0][b, :, :m]) and torch.equal(got[4][b, :, :m], other[1][b, :, :m])
         torch.randn(4096, device=dev).sum().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,heads", [(4, (8, 2, 64)), (17, (2, 2, 128)), (30, (8, 2, 128)), (70, (4, 2, 64)), (70, (4, 2, 128)),
+                                     (256, (2, 1, 128))])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, -3.0])
+def test_scales_that_are_not_positive(dev, dtype, T, heads, scale):
+    """At every number of query rows, over one key range and several: softmax(scale q.k) is softmax(|scale| (-q).k), and with
+    scale 0 the mean over the visible rows."""
+    print(f"[tree scale] {dtype} T={T} heads={heads} scale={scale}", flush=True)
+    q, k, v, n, parents = _case(dev, dtype, 3, T, heads, [1500, 33, 0], room=300, pad=1, seed=13)
+    out = K.tree_attn(q, k, v, n, parents.to(dev), scale=scale)
+    _check(out, _reference(-q if scale else q * 0, k, v, n, parents, abs(scale) or 1.0), dtype)

@@ -37,6 +37,9 @@ struct TreeAttn {
   int2* table;                                       // each sequence's (first range, ranges); null: never more than one
   float *po, *pm;                                    // partial outputs [range][nk][rep T][D], (max, sum) pairs
   float scale_log2;
+  // The LDS walk masks and compares scores before it scales them, so its scale has to be positive: another one's sign, or its
+  // 0, goes into the queries (exact in bf16).
+  float walk_scale, q_factor;
 };
 
 // How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
@@ -625,6 +628,10 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) q[ks] = *(const bf16x8_t*)(qp + ks * 16 + g * 8);
   }
+  if (a.q_factor != 1.f) {
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) q[ks] *= (__bf16)a.q_factor;
+  }
   float m = -INFINITY, l = 0.f;
   f32x16_t o[NDT];
 #pragma unroll
@@ -721,7 +728,7 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
     for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, s[kk][j]);
-    top = half_max(top) * a.scale_log2;
+    top = half_max(top) * a.walk_scale;
     const bool grow = top > m + 8.f;
     if (__ballot(grow)) {
       // (for the queries that need it alone: a row's result does not depend on the rows beside it)
@@ -739,7 +746,7 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
       float e[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        e[j] = __builtin_amdgcn_exp2f(fmaf(s[kk][j], a.scale_log2, ref));
+        e[j] = __builtin_amdgcn_exp2f(fmaf(s[kk][j], a.walk_scale, ref));
         l += e[j];
       }
 #pragma unroll
@@ -1002,6 +1009,8 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
                (long long)width, (long long)ldq, (long long)ldo);
   UNOK_REQUIRE(!unok::rows_overlap(q, ldq * es, o, ldo * es, rows, width * es), UNOK_EINVAL,
                "tree_attn: the output overlaps the queries");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  UNOK_REQUIRE(scale_log2 - scale_log2 == 0.f, UNOK_EINVAL, "tree_attn: scale %g must be finite", (double)scale);
   const int per16 = dtype == UNOK_BF16 ? 8 : 4;
   int64_t bits = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15;
   for (int64_t s : {ldq, k_batch, k_head, k_row, v_batch, v_head, v_row, ldo}) bits |= s % per16;
@@ -1021,7 +1030,9 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   a.po = (float*)workspace;
   a.pm = a.po + plan.ranges * nq * T * D;
   a.table = plan.ranges > B ? (int2*)(a.pm + plan.ranges * nq * T * 2) : nullptr;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
+  a.walk_scale = scale_log2 > 0.f ? scale_log2 : scale_log2 < 0.f ? -scale_log2 : 1.f;
+  a.q_factor = scale_log2 > 0.f ? 1.f : scale_log2 < 0.f ? -1.f : 0.f;
   const int64_t nb = (plan.ranges * nk + 7) / 8 * 8 * plan.rt;
   UNOK_REQUIRE(nb < (1ll << 31) && B < 65536, UNOK_EINVAL, "tree_attn: grid too large");
   hipStream_t st = (hipStream_t)stream;

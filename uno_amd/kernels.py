@@ -621,7 +621,8 @@ def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.
     lengths int64 [B]. parents int32 [B, T], or [T] for one tree of all sequences: the index of an earlier node,
     -1 for a root, below -1 for padding, whose output rows are 0; a parent that is no earlier node, or is padding,
     ends the chain. A node sees the committed rows, its ancestors and itself; what else the cache holds does not
-    matter. ``out`` shares no row with q. T <= 256, D 64 or 128, fp32 or bf16."""
+    matter. ``out`` shares no row with q. ``scale`` (default D^-0.5) may be any finite number. T <= 256, D 64 or
+    128, fp32 or bf16."""
     _rowmajor(q, "q")
     if k.dim() != 4 or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
         raise RuntimeError(f"tree_attn: k and v must be [B, nk, max_len, D] in the dtype of q, got {tuple(k.shape)} "
