@@ -343,3 +343,36 @@ def test_row_top_k_masked_by_low_values(dev, dtype, V, low, rows):
     z[5] = low
     z = z.repeat((rows + 5) // 6, 1)
     _check_top(z, min(V, 20), K.row_top_k(z, min(V, 20)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,R", [(777, 8), (40009, 8)])
+@pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
+def test_distillation_over_lowest_values(dev, dtype, V, R, tau):
+    """Columns masked with the type's lowest value: most of a student's row, all of it, a teacher's entries but one, all of
+    them (finite, so they count), and a whole row raised to where its values over tau are no numbers of fp32. With z and t the
+    same numbers as in the kernel, q and p are softmaxes of differences, which the reference takes of values less their maximum."""
+    k, n = 12, 5
+    g = torch.Generator(device=dev).manual_seed(V)
+    z = torch.randn(R, V, device=dev, generator=g).to(dtype)
+    values, indices = _teacher(z, k, g)
+    low = torch.finfo(dtype).min
+    kept = torch.zeros(V, device=dev, dtype=torch.bool)
+    kept[indices[0]] = True
+    z[0] = torch.where(kept, z[0], low)
+    z[1] = low
+    values[2, 1:] = torch.finfo(F32).min
+    values[3] = torch.finfo(F32).min
+    z[4], values[5] = 3e38, 3e38
+    leaf = z.clone().requires_grad_(True)
+    loss = token_normalized_top_k_distillation(leaf, values, indices, n, temperature=tau)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    zs = z.double() - z.double().amax(1, keepdim=True)
+    vs = values.double() - values.double().amax(1, keepdim=True)
+    ref, gref, weight, pd = _reference_loss(zs, vs, indices, n, tau)
+    # a row's values less its maximum, where they weigh anything, are of the size of the unmasked ones: below 16
+    E = (V / 256 + 100) * U + 6 * U * 16 / tau
+    assert abs(loss.double() - ref) <= E * weight * (1 + math.log(V)) + 2 * U * abs(ref) + 1e-30
+    bound = HALF[dtype] * gref.abs() + 1.01 * E * (gref.abs() + 2 * pd) + 2.0 ** -126
+    bad = (grad.double() - gref).abs() - bound
+    assert bool((bad <= 0).all()), (bad.max().item(), int((bad > 0).sum()))

@@ -577,7 +577,7 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ t, const i
     x[i] = -INFINITY;
     if (e < k) {
       const int64_t c = idx[e];
-      const float v = t[e] * inv_tau;
+      const float v = t[e];
       if (c >= 0 && c < V && !(v == -INFINITY)) { col[i] = (int)c; x[i] = v; m = fmaxf(m, v); any = true; }
     }
   }
@@ -586,17 +586,16 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ t, const i
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < DK_MAX / 64; ++i)
-    if (col[i] >= 0) s += expf(x[i] - m);
+    if (col[i] >= 0) { x[i] = (x[i] - m) * inv_tau; s += expf(x[i]); }
   s = wave_sum(s);
   const float l = logf(s);
-  // (from x - m and s: m + log s would be rounded to the size of m, and p by as much)
+  // (from x and s: m / tau + log s would be rounded to its size, and p by as much)
 #pragma unroll
-  for (int i = 0; i < DK_MAX / 64; ++i)
-    use(lane + 64 * i, col[i], x[i] - m - l, col[i] >= 0 ? expf(x[i] - m) / s : 0.f);
+  for (int i = 0; i < DK_MAX / 64; ++i) use(lane + 64 * i, col[i], x[i] - l, col[i] >= 0 ? expf(x[i]) / s : 0.f);
   return true;
 }
 
-// sum_i p_i (log p_i - log q_i) of a row, in one wave, from the row's (max, sum of e^(z / tau - max)).
+// sum_i p_i (log p_i - log q_i) of a row, in one wave, from the row's (max, sum of e^((z - max) / tau)).
 template <typename T>
 __device__ __forceinline__ float distill_row(const T* __restrict__ z, const float* __restrict__ t,
                                              const int64_t* __restrict__ idx, int k, int V, float inv_tau, int lane, float m,
@@ -605,7 +604,7 @@ __device__ __forceinline__ float distill_row(const T* __restrict__ z, const floa
   float acc = 0.f;
   teacher_row(t, idx, k, V, inv_tau, lane, [&](int, int col, float logp, float pr) {
     if (col < 0) return;
-    if (!(pr == 0.f)) acc += pr * (logp - (Elem<T>::load(z + col) * inv_tau - m) + l);
+    if (!(pr == 0.f)) acc += pr * (logp - (Elem<T>::load(z + col) - m) * inv_tau + l);
   });
   return wave_sum(acc);
 }
@@ -619,8 +618,8 @@ template <typename T> __device__ __forceinline__ float distill_exp(float x) {
   return x < -150.f ? 0.f : fmaf(e, r * 0.69314718f, e);
 }
 
-// (max, sum of e^(x - max)) of x = z / tau over a part of a row; one workgroup per (row, part). A row in one part also gets
-// its loss. Bound by HBM: 4096 x 151936 bf16 227-240 us, 5.2-5.5 TB/s.
+// (max, sum of e^((z - max) / tau)) over a part of a row; one workgroup per (row, part). A row in one part also gets its loss.
+// (Differences first: z / tau of the types' largest and lowest numbers may be no number.) Bound by HBM: 4096 x 151936 bf16 227-240 us, 5.2-5.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict__ z, int64_t ldz, int V, int parts,
                                                             int width, int k, const float* __restrict__ t,
@@ -639,20 +638,20 @@ __global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict_
     unpack16<T>(pv[q], v);
     float g = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < N; ++e) { v[e] *= inv_tau; g = fmaxf(g, v[e]); }
-    if (g > m) { s *= distill_exp<T>(m - g); m = g; }
+    for (int e = 0; e < N; ++e) g = fmaxf(g, v[e]);
+    if (g > m) { s *= distill_exp<T>((m - g) * inv_tau); m = g; }
     const float ref = m == -INFINITY ? 0.f : m;        // -inf then adds 0, and a NaN is seen
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += distill_exp<T>(v[e] - ref);
+    for (int e = 0; e < N; ++e) s += distill_exp<T>((v[e] - ref) * inv_tau);
   }
   auto single = [&](float v) {
-    if (v > m) { s *= distill_exp<T>(m - v); m = v; }
-    s += distill_exp<T>(v - (m == -INFINITY ? 0.f : m));
+    if (v > m) { s *= distill_exp<T>((m - v) * inv_tau); m = v; }
+    s += distill_exp<T>((v - (m == -INFINITY ? 0.f : m)) * inv_tau);
   };
-  for (int j = threadIdx.x; j < sp.head; j += 256) single(Elem<T>::load(p + j) * inv_tau);
-  for (int j = sp.tail() + threadIdx.x; j < n; j += 256) single(Elem<T>::load(p + j) * inv_tau);
+  for (int j = threadIdx.x; j < sp.head; j += 256) single(Elem<T>::load(p + j));
+  for (int j = sp.tail() + threadIdx.x; j < n; j += 256) single(Elem<T>::load(p + j));
   const float mb = block_max(m, red);
-  s = block_sum(m == -INFINITY ? s : s * distill_exp<T>(m - mb), red);
+  s = block_sum(m == -INFINITY ? s : s * distill_exp<T>((m - mb) * inv_tau), red);
   if (threadIdx.x == 0) stat[blockIdx.x] = make_float2(mb, s);
   if (parts == 1 && threadIdx.x < 64) {
     const float loss = distill_row(p, t + row * k, idx + row * k, k, V, inv_tau, threadIdx.x, mb, s);
@@ -675,7 +674,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(const T* __restrict__
   m = wave_max(m);
   for (int i = lane; i < parts; i += 64) {
     const float2 st = stat[row * parts + i];
-    s += st.x == -INFINITY ? st.y : st.y * fast_expf(st.x - m);
+    s += st.x == -INFINITY ? st.y : st.y * fast_expf((st.x - m) * inv_tau);
   }
   s = wave_sum(s);
   const float loss = distill_row(z + row * ldz, t + row * k, idx + row * k, k, V, inv_tau, lane, m, s);
@@ -736,7 +735,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
     for (int e = 0; e < k; ++e) psum += cols[e] == col + c0 ? prob[e] : 0.f;
   }
   __syncthreads();
-  auto one = [&](float v) { return cq * distill_exp<T>(v * inv_tau - m); };
+  auto one = [&](float v) { return cq * distill_exp<T>((v - m) * inv_tau); };
   if (aligned) {
     const u32x4_t* pv = (const u32x4_t*)(p + sp.head);
     u32x4_t* gv = (u32x4_t*)(g + sp.head);
@@ -754,7 +753,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const T* z, int64_t ld
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the columns' first values are stored before the second ones
   __syncthreads();
-  if (mine) Elem<T>::store(g + col, distill_exp<T>(zc * inv_tau - m) / rs.y * c - psum * c);
+  if (mine) Elem<T>::store(g + col, distill_exp<T>((zc - m) * inv_tau) / rs.y * c - psum * c);
 }
 
 // Parts of a row of the statistics and the gradient, as topk_parts, for four workgroups per CU, of at least 8192 columns. 300 rows of
