@@ -406,7 +406,7 @@ int unok_row_topk(int dtype, int R, int V, int k, const void* z, int64_t ldz, fl
 /* Distillation from a teacher's top logits t [R, k <= 256] at columns idx [R, k]: with p = softmax(t / tau) over a row's
  * entries (t = -inf or a column outside [0, V): no entry) and q = softmax(z / tau) over the row's V columns,
  * loss[0] = scale inv_n[0] sum over rows with entries of sum_i p_i (log p_i - log q_idx_i) (inv_n null: 1); row_stat [R, 2] is
- * what the backward reads. workspace: unok_distill_workspace() bytes, 8-byte aligned. */
+ * what the backward reads. tau, 1 / tau and scale are finite, tau positive. workspace: unok_distill_workspace() bytes, 8-byte aligned. */
 int64_t unok_distill_workspace(int R, int V);
 int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx, float tau,
                      const float* inv_n, float scale, float* row_stat, float* loss, void* workspace, int64_t ws_bytes,

@@ -274,3 +274,12 @@ def test_tree_attention_refuses_scales(scale):
     lib = N.lib()
     assert lib.unok_tree_attn(*_tree_call(scale=scale)) == -1
     assert "must be finite" in lib.unok_last_error().decode()
+
+
+@pytest.mark.parametrize("entry,make", [("unok_distill_fwd", _dfwd), ("unok_distill_bwd", _dbwd)])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan")])
+def test_distillation_refuses_scales(entry, make, scale):
+    """(A temperature whose square is no number of fp32 arrives as such a scale.)"""
+    lib = N.lib()
+    assert getattr(lib, entry)(*make(scale=scale)) == -1
+    assert "must be finite" in lib.unok_last_error().decode()

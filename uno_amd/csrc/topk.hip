@@ -771,12 +771,13 @@ void distill_split(int R, int V, int& parts, int& width) {
   parts = (V + width - 1) / width;                     // a last part may fall away by the rounding
 }
 
-int distill_check(const char* what, int dtype, int R, int V, int k, int64_t ldz, float tau) {
+int distill_check(const char* what, int dtype, int R, int V, int k, int64_t ldz, float tau, float scale) {
   UNOK_REQUIRE(R >= 0 && V >= 1 && (R <= 1 || ldz >= V), UNOK_EINVAL, "%s: R=%d V=%d ldz=%lld", what, R, V, (long long)ldz);
   UNOK_REQUIRE(k >= 1 && k <= DK_MAX, UNOK_EINVAL, "%s: k=%d must lie in [1, %d]", what, k, DK_MAX);
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "%s: bad dtype %d", what, dtype);
   UNOK_REQUIRE(tau > 0.f && tau < INFINITY && 1.f / tau < INFINITY, UNOK_EINVAL, "%s: temperature %g must be positive", what,
                (double)tau);
+  UNOK_REQUIRE(scale - scale == 0.f, UNOK_EINVAL, "%s: scale %g (temperature %g) must be finite", what, (double)scale, (double)tau);
   return 0;
 }
 
@@ -831,7 +832,7 @@ UNOK_EXPORT int64_t unok_distill_workspace(int R, int V) {
 UNOK_EXPORT int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx,
                                  float tau, const float* inv_n, float scale, float* row_stat, float* loss, void* workspace,
                                  int64_t ws_bytes, void* stream) {
-  int rc = distill_check("distill_fwd", dtype, R, V, k, ldz, tau);
+  int rc = distill_check("distill_fwd", dtype, R, V, k, ldz, tau, scale);
   if (rc) return rc;
   UNOK_REQUIRE(loss && (R == 0 || (z && t && idx && row_stat)), UNOK_EINVAL, "distill_fwd: null operand");
   const int64_t need = unok_distill_workspace(R, V);
@@ -862,7 +863,7 @@ UNOK_EXPORT int unok_distill_fwd(int dtype, int R, int V, int k, const void* z, 
 UNOK_EXPORT int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, int64_t ldz, const float* t, const int64_t* idx,
                                  float tau, const float* row_stat, const float* gscale, const float* inv_n, float scale,
                                  void* grad, int64_t ldg, void* stream) {
-  int rc = distill_check("distill_bwd", dtype, R, V, k, ldz, tau);
+  int rc = distill_check("distill_bwd", dtype, R, V, k, ldz, tau, scale);
   if (rc || R == 0) return rc;
   UNOK_REQUIRE(R <= 1 || ldg >= V, UNOK_EINVAL, "distill_bwd: ldg=%lld", (long long)ldg);
   UNOK_REQUIRE(z && t && idx && row_stat && gscale && grad, UNOK_EINVAL, "distill_bwd: null operand");

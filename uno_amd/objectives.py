@@ -251,7 +251,8 @@ def top_k_distillation_loss(lm_head, h_s: torch.Tensor, values: torch.Tensor, in
     """tau^2 inv_n sum over rows of KL(p || q): p = softmax(values / tau) over a row's teacher entries ([R, k] logits and
     their vocabulary indices, k <= 256, as teacher_top_k returns them), q = softmax of the student's logits / tau over the
     whole vocabulary. Entries of value -inf, or with an index outside the vocabulary, do not count; a row without
-    entries contributes nothing, to the loss and to the gradient. The teacher is not differentiated."""
+    entries contributes nothing, to the loss and to the gradient. The teacher is not differentiated. tau is positive, 1 / tau
+    and tau^2 numbers of fp32."""
     _distill_operands(h_s, values, indices, temperature)
     if inv_n.dtype != torch.float32 or inv_n.numel() != 1:
         raise RuntimeError(f"top-k distillation: inv_n must be one fp32 number, got {inv_n.dtype} {tuple(inv_n.shape)}")
