@@ -294,3 +294,38 @@ def test_drafting_with_trees_is_greedy_decoding(dev):
     for i, tok in enumerate(full[P:].tolist()):
         slack = 2 * TOL[F32] * ref[i].norm().item()
         assert ref[i, tok] >= ref[i].max() - slack, i
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_draft_graph_follows_replayed_accepts(dev, dtype):
+    """Tree blocks and accepts replayed from graphs, and a captured draft block between them: the eager block's logits, and a
+    refusal once the cache is full."""
+    cfg, params, lora, dec = _build(dev, "gqa2", dtype)
+    g = torch.Generator().manual_seed(7)
+    B, P, L = 2, 10, 8
+    prompt = torch.randint(0, cfg.vocab_size - 1, (B, P), generator=g).to(dev)
+    cache = dec.new_cache(B, P + 3 * 4 + L)
+    dec.prefill(cache, prompt)
+    draft, tree = dec.capture_draft(cache, L, commit=0), dec.capture_tree(cache, 4)
+    parents = torch.arange(-1, 3, device=dev, dtype=torch.int32)
+    path, counts = torch.arange(4, device=dev).repeat(B, 1), torch.tensor([4, 1], device=dev)
+    lengths, rows = cache.lengths.clone(), [c.clone() for c in cache.k + cache.v]
+    cache.accept(path, counts)                           # once before the capture, and undone
+    cache.lengths.copy_(lengths)
+    for c, r in zip(cache.k + cache.v, rows):
+        c.copy_(r)
+    accept = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(accept):
+        cache.accept(path, counts)
+    assert cache.lengths.tolist() == [P, P]
+    for step in range(4):
+        blk = torch.randint(0, cfg.vocab_size - 1, (B, L), generator=g).to(dev)
+        assert torch.equal(draft.replay(blk).clone(), dec.draft_block(cache, blk, commit=0)), step
+        if step == 3:
+            break
+        tree.replay(blk[:, :4], parents)
+        accept.replay()
+    assert cache.lengths.tolist() == [P + 12, P + 3]
+    accept.replay()
+    with pytest.raises(RuntimeError, match="does not fit"):
+        draft.replay(blk)

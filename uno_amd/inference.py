@@ -43,6 +43,10 @@ from .layers import Geometry, StreamContext, clean_layer
 PLAIN_FEW_ROWS = 128
 
 
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class BlockKVCache:
     """Per-layer K and V, head-major [B, Hkv, max_len, D], and the committed length per sequence."""
 
@@ -52,15 +56,21 @@ class BlockKVCache:
         self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int64)
         self.batch, self.max_len, self.geo = batch, max_len, geo
-        self.moves = 0                                   # accepts and copies so far: a DraftGraph looks at the lengths again
+        # What a DraftGraph, which keeps a bound on the lengths, goes by: how often they were moved so far, and whether a graph
+        # holds an accept or a copy, which moves them unseen.
+        self.moves, self.unseen = 0, False
+
+    def _moved(self) -> None:
+        self.moves += 1
+        self.unseen |= _capturing()
 
     def accept(self, nodes: torch.Tensor, counts: torch.Tensor) -> None:
         """Commits the accepted nodes of the tree that ``BlockDecoder.tree_block`` wrote: nodes [B, P] int64, of which the
         first counts[b] (int64 [B], 0 .. P) are sequence b's path from the root down. Their K/V rows become the next
         committed rows in that order (every row is read before any is written); the tree's other rows are dropped. All
-        on the device, and capturable into a graph."""
+        on the device, and capturable into a graph (a DraftGraph over this cache then reads the lengths at every replay)."""
         K.cache_keep(self.k + self.v, self.lengths, nodes, counts)
-        self.moves += 1
+        self._moved()
         self.lengths += counts.clamp(0, nodes.shape[1])
 
     def copy_from(self, other: "BlockKVCache", pairs) -> None:
@@ -73,7 +83,7 @@ class BlockKVCache:
         if other.max_len > self.max_len and all(0 <= a < other.batch for a, _ in pairs) and \
                 int(other.lengths[[a for a, _ in pairs]].max()) > self.max_len:
             raise RuntimeError("the sequences do not fit in the KV cache")
-        self.moves += 1
+        self._moved()
         K.cache_copy(other.k + other.v, self.k + self.v, other.lengths, self.lengths, pairs)
 
 
@@ -170,6 +180,8 @@ class BlockDecoder:
                 h = self._layer(h, lw, li, pos, gate_rows, cache, maps, B, L)
         logits = self._head(h, prefill)
         cache.lengths += commit
+        if check and commit:                             # (a captured block's commits are counted as it is replayed)
+            cache.moves += 1
         return logits.view(B, L, -1)
 
     def _tree_check(self, cache, ids, parents, lora_mask) -> None:
@@ -425,9 +437,10 @@ class DraftGraph:
     advances them by ``commit``, exactly as ``BlockDecoder.draft_block``.
 
     ``replay`` returns the graph's own logits buffer [B, L, V], overwritten by the next replay.
-    The cache capacity is checked on the host against the longest committed length read at
-    capture, or after the cache's last ``accept`` or ``copy_from``, plus the commits since; after
-    changing ``cache.lengths`` by other means, capture again."""
+    The cache capacity is checked on the host against the longest committed length read at capture plus
+    this graph's commits since; it is read again after any other block, prefill, ``accept`` or
+    ``copy_from`` over the cache, and at every replay once one of the latter two has been captured into
+    a graph. After changing ``cache.lengths`` by other means, capture again."""
 
     def __init__(self, decoder: BlockDecoder, cache: BlockKVCache, block_size: int, commit: int = 1):
         B, L = cache.batch, block_size
@@ -458,8 +471,8 @@ class DraftGraph:
         default gate (off on the seed row, on for the noise rows) for this and later replays."""
         if tuple(block_ids.shape) != tuple(self.ids.shape):
             raise RuntimeError(f"block {tuple(block_ids.shape)} does not match the captured {tuple(self.ids.shape)}")
-        if self._moves != self.cache.moves:
-            self._len_max, self._moves = int(self.cache.lengths.max()), self.cache.moves
+        if self._moves != self.cache.moves or self.cache.unseen:
+            self._len_max = int(self.cache.lengths.max())
         if self._len_max + self.block_size > self.cache.max_len:
             raise RuntimeError("the block does not fit in the KV cache")
         self.ids.copy_(block_ids)
@@ -469,6 +482,9 @@ class DraftGraph:
             self.gate.copy_(lora_mask)
         self.graph.replay()
         self._len_max += self.commit
+        if self.commit:
+            self.cache.moves += 1
+        self._moves = self.cache.moves
         return self.logits
 
 
