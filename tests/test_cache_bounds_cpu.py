@@ -120,3 +120,11 @@ def test_blocks_that_commit_between_replays(cache, monkeypatch):
     dec.draft_block(cache, IDS, commit=1)
     with pytest.raises(RuntimeError, match="does not fit"):
         draft.replay(IDS)
+
+
+def test_accepted_lengths_end_at_the_cache(cache):
+    cache.lengths.copy_(torch.tensor([LEN - 3, LEN]))
+    cache.accept(PATH, torch.tensor([99, 4]))
+    assert cache.lengths.tolist() == [LEN, LEN]
+    cache.accept(PATH, torch.tensor([-7, 0]))
+    assert cache.lengths.tolist() == [LEN, LEN]

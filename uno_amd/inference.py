@@ -67,11 +67,13 @@ class BlockKVCache:
     def accept(self, nodes: torch.Tensor, counts: torch.Tensor) -> None:
         """Commits the accepted nodes of the tree that ``BlockDecoder.tree_block`` wrote: nodes [B, P] int64, of which the
         first counts[b] (int64 [B], 0 .. P) are sequence b's path from the root down. Their K/V rows become the next
-        committed rows in that order (every row is read before any is written); the tree's other rows are dropped. All
-        on the device, and capturable into a graph (a DraftGraph over this cache then reads the lengths at every replay)."""
+        committed rows in that order (every row is read before any is written); the tree's other rows are dropped. No
+        length passes the cache's end. (An entry that is no row behind the committed ones counts all the same, and its new row
+        stays as it was.) All on the device, and capturable into a graph (a DraftGraph over this cache then reads the lengths
+        at every replay)."""
         K.cache_keep(self.k + self.v, self.lengths, nodes, counts)
         self._moved()
-        self.lengths += counts.clamp(0, nodes.shape[1])
+        self.lengths.add_(counts.clamp(0, nodes.shape[1])).clamp_(max=self.max_len)
 
     def copy_from(self, other: "BlockKVCache", pairs) -> None:
         """Copies whole sequences: for each (slot of ``other``, slot of this cache) of ``pairs`` the committed rows of all
