@@ -275,8 +275,8 @@ int unok_attn_split_combine(int QR, int S, int D, const void* opart, int64_t ldp
 /* Key intervals ivs [S * QR, 8] and output rows dst [QR] of a draft block's split-key attention from
  * the committed lengths (QR = 128 B nk): range s of decode row i holds keys [s c, (s + 1) c) of its
  * causal prefix over cache and block, c = lengths[b] / S, the last range the rest; rows past rep * L
- * of each 128 are empty with dst -1, the others go to row (b L + t) nq + head. The cached lengths
- * and block tables of nano_vllm_uno/layers/attention.py:628-668. */
+ * of each 128 are empty with dst -1, the others go to row (b L + t) nq + head. Keys at or past max_len
+ * do not exist. The cached lengths and block tables of nano_vllm_uno/layers/attention.py:628-668. */
 int unok_decode_maps(int B, int L, int nq, int nk, int max_len, int S, const int64_t* lengths, int32_t* ivs,
                      int32_t* dst, void* stream);
 /* One decoder layer of a draft block [B, L] (bf16) over its KV cache: norm, q|k|v, unok_decode_prep,

@@ -128,3 +128,14 @@ def test_accepted_lengths_end_at_the_cache(cache):
     assert cache.lengths.tolist() == [LEN, LEN]
     cache.accept(PATH, torch.tensor([-7, 0]))
     assert cache.lengths.tolist() == [LEN, LEN]
+
+
+def test_maps_stay_in_the_cache(cache):
+    """Key intervals and store rows of an fp32 block over lengths past the cache's end stay in the sequence's own slots."""
+    dec = _decoder()
+    cache.lengths.copy_(torch.tensor([LEN - 2, LEN + 40]))
+    maps = dec._maps(cache, cache.lengths, B, L)
+    iv, store = maps["iv"].view(B, 128, 8), maps["store"].view(B, L)
+    for b in range(B):
+        for m in (iv[b, :, 0], iv[b, :, 1] - 1, store[b]):
+            assert bool(((m >= b * LEN) & (m < (b + 1) * LEN)).all())

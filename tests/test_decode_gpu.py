@@ -303,3 +303,21 @@ def test_split_combine_range_counts(dev, S):
     w = torch.exp2(lse.double() - lse.double().amax(0).clamp_min(-1e30))
     ref = (w[..., None] * o.view(S, QR, D).double()).sum(0) / w.sum(0).clamp_min(1e-30)[:, None]
     assert _rel(out[dst.long()], ref) < 2.0 ** -8      # one bf16 rounding
+
+
+@pytest.mark.parametrize("L,nq,nk,max_len,S", [(8, 4, 2, 100, 4), (16, 8, 1, 40, 8), (1, 2, 2, 9, 1)])
+def test_decode_maps_past_the_cache(dev, L, nq, nk, max_len, S):
+    """Lengths at, past and below the cache's ends: every interval stays in its own slot, and those of lengths that fit with
+    their block are what they were."""
+    lengths = torch.tensor([max_len - L, max_len - L + 1, max_len, max_len + 300, 2 ** 40, -5], device=dev)
+    B = lengths.numel()
+    ivs, dst = K.decode_maps(lengths, B, L, nq, nk, max_len, S)
+    ivs = ivs.view(S, B, nk, 128, 8).cpu()
+    start = (torch.arange(B)[:, None] * nk + torch.arange(nk)).mul(max_len)[None, :, :, None]
+    assert bool((ivs[..., 0] >= start).all()) and bool((ivs[..., 1] >= ivs[..., 0]).all())
+    assert bool((ivs[..., 1] <= start + max_len).all())
+    rows = (nq // nk) * L
+    seen = (ivs[..., 1] - ivs[..., 0]).sum(0)[:, :, :rows]                     # over the ranges: what each row sees
+    t = torch.arange(rows) % L
+    want = (lengths.cpu().clamp(0, max_len)[:, None, None] + t + 1).clamp(max=max_len).expand(B, nk, rows)
+    assert torch.equal(seen, want.to(seen.dtype))

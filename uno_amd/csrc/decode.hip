@@ -558,7 +558,9 @@ __global__ __launch_bounds__(256) void decode_maps_kernel(const int64_t* __restr
   const int s = i / QR, q = i % QR, pair = q / 128, slot = q % 128, rep = nq / nk;
   const bool valid = slot < rep * L;
   const int t = slot % L;
-  const int64_t len = lengths[pair / nk], seen = len + t + 1, c = len / S;
+  // (lengths that leave no room for the block: no row outside the slot)
+  const int64_t len = min(max(lengths[pair / nk], (int64_t)0), (int64_t)max_len);
+  const int64_t seen = min(len + t + 1, (int64_t)max_len), c = len / S;
   const int64_t start = (int64_t)pair * max_len;
   const int64_t lo = s * c, hi = s == S - 1 ? seen : min((s + 1) * c, seen);
   ivs[2 * i] = make_int4((int)(start + (valid ? lo : 0)), (int)(start + (valid ? max(hi, lo) : 0)), 0, 0);

@@ -263,12 +263,14 @@ class BlockDecoder:
         tt = slot % L
         start = pair[:, None] * cache.max_len                                           # [pairs, 1]
         lens = lengths[:, None].expand(B, g.nk).reshape(-1, 1)                          # [pairs, 1]
-        seen = lens + tt[None, :] + 1                                                   # causal over cache + block
+        seen = (lens + tt[None, :] + 1).clamp(1, cache.max_len)                         # causal over cache + block
         b = torch.arange(B, device=dev)[:, None, None]
         t = torch.arange(L, device=dev)[None, :, None]
         kv = torch.arange(g.nk, device=dev)[None, None, :]
         # cache store: key row (b, t, head) of the block -> cache row (b, head, lengths_b + t)
-        out["store"] = ((b * g.nk + kv) * cache.max_len + lengths[:, None, None] + t).reshape(-1).to(**i32)
+        # (lengths that leave no room for the block: no row outside the slot)
+        at = (lengths[:, None, None] + t).clamp(0, cache.max_len - 1)
+        out["store"] = ((b * g.nk + kv) * cache.max_len + at).reshape(-1).to(**i32)
         # decode layout: query (b, t, head h = kv * rep + r) -> row (b * nk + kv) * 128 + r * L + t
         r = torch.arange(rep, device=dev)
         qrow = ((b * g.nk + kv)[..., None] * 128 + r[None, None, None, :] * L + t[..., None])   # [B, L, nk, rep]
