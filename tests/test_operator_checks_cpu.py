@@ -283,3 +283,20 @@ def test_distillation_refuses_scales(entry, make, scale):
     lib = N.lib()
     assert getattr(lib, entry)(*make(scale=scale)) == -1
     assert "must be finite" in lib.unok_last_error().decode()
+
+
+@pytest.mark.parametrize("pairs", [[(2 ** 32, 1)], [(0, 2 ** 32 + 1)], [(-2 ** 32, 1)], [(0, 1, 1)], [(0,)], [(0, 1), (0,), (1, 1, 0)]])
+def test_copies_refuse_pairs(monkeypatch, pairs):
+    """Slots that are no 32-bit numbers (they would arrive as others), and lists that are no pairs."""
+    monkeypatch.setattr(K, "_same_device", lambda *a: None)
+    with pytest.raises((RuntimeError, ValueError), match="cache_copy: "):
+        K.cache_copy(_cache(batch=4), _cache(batch=4), _nodes(4), _nodes(4), pairs)
+
+
+@pytest.mark.parametrize("k", [0, -1, 9, 257, 2 ** 32 + 1])
+def test_top_k_refuses_numbers(monkeypatch, k):
+    """Before results of that size are allocated."""
+    monkeypatch.setattr(K, "_same_device", lambda *a: None)
+    monkeypatch.setattr(K, "_rowmajor", lambda *a: None)
+    with pytest.raises(ValueError, match="row_top_k: k="):
+        K.row_top_k(torch.zeros(2, 8 if k < 257 else 300), k)

@@ -717,9 +717,11 @@ def cache_copy(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], src_len
     _int64_vector("cache_copy", "source lengths", src_lengths, s.shape[0])
     _int64_vector("cache_copy", "destination lengths", dst_lengths, d.shape[0])
     _same_device("cache_copy", s, d, src_lengths, dst_lengths)
-    flat = [int(i) for pair in pairs for i in pair]
-    if len(flat) != 2 * len(pairs):
+    if any(len(pair) != 2 for pair in pairs):
         raise RuntimeError("cache_copy: pairs must be (source slot, destination slot)")
+    flat = [int(i) for pair in pairs for i in pair]
+    if flat and not (0 <= min(flat[::2]) and max(flat[::2]) < s.shape[0] and 0 <= min(flat[1::2]) and max(flat[1::2]) < d.shape[0]):
+        raise ValueError(f"cache_copy: slots {list(pairs)} of batches {s.shape[0]} -> {d.shape[0]}")
     N.call("unok_cache_copy", len(src), N.ptr_array(src), N.ptr_array(dst), s.shape[3] * s.element_size(), s.shape[1],
            s.shape[0], s.shape[2], d.shape[0], d.shape[2], N.ptr(src_lengths), N.ptr(dst_lengths), len(pairs),
            N.int_array(flat), N.stream())
@@ -732,6 +734,8 @@ def row_top_k(z: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torc
     _rowmajor(z, "z")
     R, V = z.shape
     _same_device("row_top_k", z)
+    if not 1 <= k <= min(256, V):
+        raise ValueError(f"row_top_k: k={k} must lie in [1, min(256, V={V})]")
     values = torch.empty((R, k), device=z.device, dtype=torch.float32)
     cols = torch.empty((R, k), device=z.device, dtype=torch.int64)
     lse = torch.empty(R, device=z.device, dtype=torch.float32)
