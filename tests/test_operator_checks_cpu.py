@@ -300,3 +300,24 @@ def test_top_k_refuses_numbers(monkeypatch, k):
     monkeypatch.setattr(K, "_rowmajor", lambda *a: None)
     with pytest.raises(ValueError, match="row_top_k: k="):
         K.row_top_k(torch.zeros(2, 8 if k < 257 else 300), k)
+
+
+META = dict(device="meta")
+
+
+@pytest.mark.parametrize("call", [
+    lambda: K.row_top_k(torch.empty(1, 2 ** 32 + 5, **META), 2), lambda: K.row_top_k(torch.empty(2 ** 32 + 5, 4, **META), 2),
+    lambda: token_normalized_top_k_distillation(torch.empty(1, 2 ** 32 + 5, **META), torch.empty(1, 2, **META),
+                                                torch.empty(1, 2, dtype=I64, **META), 4),
+    lambda: token_normalized_top_k_distillation(torch.empty(2 ** 32 + 5, 4, **META), torch.empty(2 ** 32 + 5, 2, **META),
+                                                torch.empty(2 ** 32 + 5, 2, dtype=I64, **META), 4),
+    lambda: token_normalized_top_k_distillation(torch.empty(1, 4, **META), torch.empty(1, 2 ** 32 + 5, **META),
+                                                torch.empty(1, 2 ** 32 + 5, dtype=I64, **META), 4),
+    lambda: K.cache_keep(_cache(), _nodes(B), torch.empty(B, 2 ** 32 + 2, dtype=I64, **META), _nodes(B))],
+    ids=["top k columns", "top k rows", "distill columns", "distill rows", "distill entries", "keep nodes"])
+def test_sizes_beyond_32_bits_are_refused(monkeypatch, call):
+    """(They would arrive as others.)"""
+    monkeypatch.setattr(K, "_same_device", lambda *a: None)
+    monkeypatch.setattr(K, "_rowmajor", lambda *a: None)
+    with pytest.raises((RuntimeError, ValueError), match="at most|exceed"):
+        call()

@@ -592,6 +592,12 @@ def _same_device(what: str, *tensors: torch.Tensor) -> None:
             raise RuntimeError(f"{what}: operands must be on the current device, got {t.device}")
 
 
+def _sizes(what: str, *sizes: int) -> None:
+    """Sizes that travel as 32-bit numbers."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{what}: sizes {sizes} exceed 2^31 - 1")
+
+
 def _int64_vector(what: str, name: str, t: torch.Tensor, n: int) -> None:
     if t.dtype != torch.int64 or tuple(t.shape) != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{what}: {name} must be contiguous int64 [{n}], got {t.dtype} {tuple(t.shape)}")
@@ -699,6 +705,8 @@ def cache_keep(caches: Sequence[torch.Tensor], lengths: torch.Tensor, nodes: tor
     _int64_vector("cache_keep", "counts", counts, B)
     if nodes.dtype != torch.int64 or nodes.dim() != 2 or nodes.shape[0] != B or not nodes.is_contiguous():
         raise RuntimeError(f"cache_keep: nodes must be contiguous int64 [{B}, P], got {nodes.dtype} {tuple(nodes.shape)}")
+    if nodes.shape[1] > 256:
+        raise RuntimeError(f"cache_keep: paths hold at most 256 nodes, got {nodes.shape[1]}")
     _same_device("cache_keep", c, lengths, nodes, counts)
     N.call("unok_cache_keep", len(caches), N.ptr_array(caches), D * c.element_size(), B, nk, max_len, nodes.shape[1],
            N.ptr(lengths), N.ptr(nodes), N.ptr(counts), N.stream())
@@ -734,6 +742,7 @@ def row_top_k(z: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torc
     _rowmajor(z, "z")
     R, V = z.shape
     _same_device("row_top_k", z)
+    _sizes("row_top_k", R, V)
     if not 1 <= k <= min(256, V):
         raise ValueError(f"row_top_k: k={k} must lie in [1, min(256, V={V})]")
     values = torch.empty((R, k), device=z.device, dtype=torch.float32)

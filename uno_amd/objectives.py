@@ -210,6 +210,7 @@ def _distill_fwd(z, values, indices, inv_n, scale, temperature):
     """(loss, row statistics for _distill_bwd) over [R, V] logits with unit column stride; inv_n None: 1."""
     K._same_device("top-k distillation", z, values, indices, *(() if inv_n is None else (inv_n,)))
     R, V = z.shape
+    K._sizes("top-k distillation", R, V, values.shape[1])
     f32 = dict(device=z.device, dtype=torch.float32)
     nbytes = N.lib().unok_distill_workspace(R, V)
     stat, loss, ws = torch.empty((R, 2), **f32), torch.empty((), **f32), torch.empty(nbytes // 4, **f32)
