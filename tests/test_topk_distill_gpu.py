@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from uno_amd import kernels as K
+from uno_amd import kernels as K, objectives
 from uno_amd.objectives import teacher_top_k, top_k_distillation_loss
 from uno_amd.training.losses import token_normalized_top_k_distillation
 
@@ -376,3 +376,29 @@ def test_distillation_over_lowest_values(dev, dtype, V, R, tau):
     bound = HALF[dtype] * gref.abs() + 1.01 * E * (gref.abs() + 2 * pd) + 2.0 ** -126
     bad = (grad.double() - gref).abs() - bound
     assert bool((bad <= 0).all()), (bad.max().item(), int((bad > 0).sum()))
+
+
+def test_more_than_two_to_the_31_logits(dev):
+    """14,140 rows of 151936: the loss over all rows, the gradient of the first, the last and those around element 2^31."""
+    R, V, k, n = 14140, 151936, 7, 14140
+    assert R * V > 2 ** 31
+    g = torch.Generator(device=dev).manual_seed(4)
+    z = torch.empty(R, V, device=dev, dtype=BF)
+    for r in range(0, R, 1000):
+        z[r:r + 1000].normal_(generator=g)
+    values = torch.randn(R, k, device=dev, generator=g)
+    indices = torch.randint(0, V, (R, k), device=dev, generator=g)
+    z.requires_grad_(True)
+    loss = token_normalized_top_k_distillation(z, values, indices, n)
+    (grad,) = torch.autograd.grad(loss, z)
+    zd = z.detach()
+    ref = weight = 0.0
+    for r in range(0, R, 500):
+        part = _reference_loss(zd[r:r + 500], values[r:r + 500], indices[r:r + 500], n, 1.0)
+        ref, weight = ref + part[0], weight + part[2]
+    E = (V / 256 + 100) * U + 6 * U * zd.abs().max().double()
+    assert abs(loss.detach().double() - ref) <= E * weight * (1 + math.log(V)) + 2 * U * abs(ref)
+    for r in (0, 2 ** 31 // V - 1, 2 ** 31 // V, 2 ** 31 // V + 1, R - 1):
+        row = slice(r, r + 1)
+        one = token_normalized_top_k_distillation(zd[row], values[row], indices[row], n)
+        _check_loss(zd[row], values[row], indices[row], n, 1.0, one, grad[row])

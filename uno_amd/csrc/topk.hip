@@ -880,7 +880,7 @@ UNOK_EXPORT int unok_distill_bwd(int dtype, int R, int V, int k, const void* z, 
                        parts, width, k, (const float2*)row_stat, t, idx, 1.f / tau, gscale, inv_n, scale, gt, ldg);
   };
   auto go = [&](auto* zt, auto* gt) {
-    if (R * V * es > MEMORY_CACHE) launch(zt, gt, std::true_type{});
+    if ((int64_t)R * V * es > MEMORY_CACHE) launch(zt, gt, std::true_type{});
     else launch(zt, gt, std::false_type{});
   };
   if (dtype == UNOK_BF16) go((const bf16_t*)z, (bf16_t*)grad);
