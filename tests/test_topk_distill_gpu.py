@@ -378,6 +378,23 @@ def test_distillation_over_lowest_values(dev, dtype, V, R, tau):
     assert bool((bad <= 0).all()), (bad.max().item(), int((bad > 0).sum()))
 
 
+@pytest.mark.parametrize("dtype,R", [(BF, 900), (F32, 450)])
+@pytest.mark.parametrize("extra", [0, 5])
+def test_logits_larger_than_the_memory_side_cache(dev, dtype, R, extra):
+    """More than 256 MB, rows with and without elements between them: top logits, loss, gradient."""
+    V, k, tau = 151936, 40, 1.5
+    print(f"[large] {dtype} R={R} extra={extra}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(R)
+    z = (torch.randn(R, V + extra, device=dev, generator=g) * 3).to(dtype)[:, :V]
+    assert R * V * z.element_size() > 2 ** 28
+    _check_top(z, k, K.row_top_k(z, k))
+    values, indices = _teacher(z, k, g)
+    leaf = z.detach().requires_grad_(True)
+    loss = token_normalized_top_k_distillation(leaf, values, indices, R, temperature=tau)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    _check_loss(z, values, indices, R, tau, loss.detach(), grad)
+
+
 def test_more_than_two_to_the_31_logits(dev):
     """14,140 rows of 151936: the loss over all rows, the gradient of the first, the last and those around element 2^31."""
     R, V, k, n = 14140, 151936, 7, 14140
@@ -402,3 +419,27 @@ def test_more_than_two_to_the_31_logits(dev):
         row = slice(r, r + 1)
         one = token_normalized_top_k_distillation(zd[row], values[row], indices[row], n)
         _check_loss(zd[row], values[row], indices[row], n, 1.0, one, grad[row])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [5000, 32000, 151936])
+@pytest.mark.parametrize("R", [1, 16, 300])
+@pytest.mark.parametrize("extra,offset", [(0, 0), (1, 0), (13, 3)])
+def test_gradient_in_the_logits_place(dev, dtype, V, R, extra, offset):
+    """As the loss over the LM head takes it, rows in one part and in several, at any alignment: bit for bit the gradient in a
+    tensor of its own; what lies between the rows stays as it was."""
+    k, tau = 30, 0.8
+    g = torch.Generator(device=dev).manual_seed(V + R)
+    buf = torch.full((R * (V + extra) + offset,), 7.0, device=dev, dtype=dtype)
+    z = buf[offset:].view(R, V + extra)[:, :V]
+    z.copy_(torch.randn(R, V, device=dev, generator=g) * 3)
+    values, indices = _teacher(z, k, g)
+    indices[0, 3] = indices[0, 0]
+    inv_n, up = torch.full((), 1 / 9, device=dev), torch.full((), 1.5, device=dev)
+    loss, stat = objectives._distill_fwd(z, values, indices, inv_n, 1.0, tau)
+    apart = objectives._distill_bwd(z, values, indices, stat, up, inv_n, 1.0, tau, torch.empty(R, V, device=dev, dtype=dtype))
+    ref, gref, _, _ = _reference_loss(z, values, indices, 9, tau)
+    assert ((apart.double() - 1.5 * gref).norm() / (1.5 * gref).norm()).item() < HALF[dtype] + 1e-5
+    objectives._distill_bwd(z, values, indices, stat, up, inv_n, 1.0, tau, z)
+    assert torch.equal(z, apart)
+    assert bool((buf[:offset] == 7).all()) and bool((buf[offset:].view(R, V + extra)[:, V:] == 7).all())

@@ -464,3 +464,15 @@ def test_scales_that_are_not_positive(dev, dtype, T, heads, scale):
     q, k, v, n, parents = _case(dev, dtype, 3, T, heads, [1500, 33, 0], room=300, pad=1, seed=13)
     out = K.tree_attn(q, k, v, n, parents.to(dev), scale=scale)
     _check(out, _reference(-q if scale else q * 0, k, v, n, parents, abs(scale) or 1.0), dtype)
+
+
+def test_copies_of_more_than_two_gigabytes(dev):
+    """One sequence to eight slots, 2.1 GB: committed rows moved, others as they were."""
+    nk, D, rows = 8, 128, 32768
+    src = [torch.empty(1, nk, rows, D, device=dev, dtype=BF).normal_() for _ in range(4)]
+    dst = [torch.full((9, nk, rows + 1, D), 7.0, device=dev, dtype=BF) for _ in range(4)]
+    n, m = torch.tensor([rows], device=dev), torch.zeros(9, device=dev, dtype=torch.int64)
+    K.cache_copy(src, dst, n, m, [(0, d) for d in range(1, 9)])
+    assert m.tolist() == [0] + [rows] * 8
+    for s, d in zip(src, dst):
+        assert bool((d[1:, :, :rows] == s).all()) and bool((d[:, :, rows] == 7).all()) and bool((d[0] == 7).all())

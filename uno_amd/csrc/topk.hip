@@ -74,8 +74,8 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// The greatest t with at least k of the wave's N x 64 values v >= t, where `on` (0: a value that does not count, which no t
-// may reach); 0 if fewer than k count. SH low bits of t are not looked for: they are those of every value.
+// The greatest t with at least k of the wave's N x 64 values v >= t (0: a value that does not count, which no t may reach; the
+// callers see to it that k do, as with fewer t is the least of them). SH low bits of t are not looked for, and come as 0.
 template <int N, int SH>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[N], int used, int k) {
   uint32_t top = 0, low = 0;                             // low: ~ of the least value that counts
