@@ -443,3 +443,16 @@ def test_gradient_in_the_logits_place(dev, dtype, V, R, extra, offset):
     objectives._distill_bwd(z, values, indices, stat, up, inv_n, 1.0, tau, z)
     assert torch.equal(z, apart)
     assert bool((buf[:offset] == 7).all()) and bool((buf[offset:].view(R, V + extra)[:, V:] == 7).all())
+
+
+def test_a_second_derivative_is_refused(dev):
+    """With create_graph the gradient is the same, and a derivative of it refused."""
+    R, V, k = 4, 300, 7
+    g = torch.Generator(device=dev).manual_seed(3)
+    z = torch.randn(R, V, device=dev, generator=g).requires_grad_(True)
+    values, indices = _teacher(z.detach(), k, g)
+    (plain,) = torch.autograd.grad(token_normalized_top_k_distillation(z, values, indices, R), z)
+    (grad,) = torch.autograd.grad(token_normalized_top_k_distillation(z, values, indices, R), z, create_graph=True)
+    assert torch.equal(plain, grad) and not plain.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (grad.sum() + (z ** 2).sum()).backward()

@@ -228,6 +228,23 @@ def _distill_bwd(z, values, indices, stat, g, inv_n, scale, temperature, grad):
     return grad
 
 
+class _OnceDifferentiable(torch.autograd.Function):
+    """A gradient that has no derivative of its own; one that passes here is refused."""
+
+    @staticmethod
+    def forward(ctx, grad, anchor):
+        return grad
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("top-k distillation is differentiable once")
+
+
+def _once(grad: torch.Tensor) -> torch.Tensor:
+    """``grad``; under create_graph, a second derivative through it is refused instead of left out."""
+    return _OnceDifferentiable.apply(grad, grad.new_empty(0).requires_grad_()) if torch.is_grad_enabled() else grad
+
+
 class TopKDistillation(torch.autograd.Function):
     """Distillation from a teacher's top logits over the LM head: logits from h_s (differentiable), gradient formed in
     their place. See top_k_distillation_loss."""
@@ -241,10 +258,12 @@ class TopKDistillation(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        if ctx.save is None:
+            raise RuntimeError("top-k distillation: backward a second time, but the first one overwrote the logits")
         z, values, indices, stat, inv_n, w_lm_t, temperature = ctx.save
         ctx.save = None
         _distill_bwd(z, values, indices, stat, g, inv_n, 1.0, temperature, z)
-        return K.gemm_nt(z, w_lm_t), None, None, None, None, None, None
+        return _once(K.gemm_nt(z, w_lm_t)), None, None, None, None, None, None
 
 
 def top_k_distillation_loss(lm_head, h_s: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, inv_n: torch.Tensor,
@@ -279,7 +298,7 @@ class LogitsTopKDistillation(torch.autograd.Function):
     def backward(ctx, g):
         z, values, indices, stat = ctx.saved_tensors
         grad = torch.empty(z.shape, device=z.device, dtype=z.dtype)
-        return _distill_bwd(z, values, indices, stat, g, None, ctx.scale, ctx.temperature, grad), None, None, None, None
+        return _once(_distill_bwd(z, values, indices, stat, g, None, ctx.scale, ctx.temperature, grad)), None, None, None, None
 
 
 class DistributionLoss(torch.autograd.Function):
