@@ -476,3 +476,15 @@ def test_copies_of_more_than_two_gigabytes(dev):
     assert m.tolist() == [0] + [rows] * 8
     for s, d in zip(src, dst):
         assert bool((d[1:, :, :rows] == s).all()) and bool((d[:, :, rows] == 7).all()) and bool((d[0] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,heads,length", [(1, 16, (32, 8, 128), 1000), (4, 16, (32, 8, 128), 500), (5, 16, (32, 8, 128), 890),
+                                              (8, 16, (32, 8, 128), 500), (8, 16, (32, 8, 128), 1000), (16, 3, (4, 2, 64), 900),
+                                              (33, 3, (4, 2, 64), 1000), (1, 2, (4, 2, 64), 255), (2, 3, (4, 2, 64), 260)])
+def test_sequences_of_few_key_blocks(dev, dtype, B, T, heads, length):
+    """Numbers and lengths of sequences on both sides of the lines where their keys are cut into single blocks."""
+    print(f"[tree blocks] {dtype} B={B} T={T} length={length}", flush=True)
+    q, k, v, n, parents = _case(dev, dtype, B, T, heads, [length - b for b in range(B)], room=0)
+    out = K.tree_attn(q, k, v, n, parents.to(dev))
+    _check(out, _reference(q, k, v, n, parents, heads[2] ** -0.5), dtype)

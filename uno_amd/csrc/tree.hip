@@ -45,9 +45,11 @@ struct TreeAttn {
 // How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
 // together. A range is at most c blocks of TB keys, c the least from TREE_LEAST on for which all sequences' keys make about
 // `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it. Sequences of three
-// to eight blocks on average are cut into single ones: one sequence of 1000 rows, one node 10.1 us (in ranges of 256 keys
-// 11.1), fp32 37 nodes of three of 901 rows 13.7 (16.7). Longer ones would pay for it in the merge (one of 4096 rows 15.7 in place
-// of 13.1), shorter ones need none at all (130 rows 9.0 and 8.0).
+// to eight blocks on average are cut into single ones while these are no more than half a round of workgroups: one sequence of
+// 1000 rows, one node 10.1 us (in ranges of 256 keys 11.1), fp32 37 nodes of three of 901 rows 13.7 (16.7). Longer ones would pay
+// for it in the merge (one of 1150 rows 11.4 and 10.6, of 4096 15.7 and 13.1), shorter ones need none at all (130 rows 9.0 and
+// 8.0), and so would more of them (16 nodes, 8 sequences of 1000 rows 23.9 and 21.5, of 500 rows 23.1 and 19.9; of four of 500
+// rows, a third of a round, 18.0 and 18.2).
 constexpr int TB = 128, TREE_LEAST = 2;
 
 struct Range { int b, n, end, first, count, lo, hi; bool past; };   // sequence, its lengths, its ranges, this range's keys
@@ -100,7 +102,8 @@ __device__ __forceinline__ Range tree_range(const TreeAttn& a, int id, int row_b
     end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
     total += __builtin_amdgcn_readlane(wave_scan((end + TB - 1) / TB), 63);
   }
-  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), total > 2 * a.B && total <= 8 * a.B ? 1 : TREE_LEAST);
+  const bool single = total > 2 * a.B && total <= min(8 * a.B, a.share / 2);
+  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), single ? 1 : TREE_LEAST);
   // sequences end inside ranges: larger ones until no more than `share` are left (one round of workgroups)
   if (a.B <= 64)
     for (int i = 0; i < 12; ++i) {
