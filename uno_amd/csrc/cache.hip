@@ -27,7 +27,7 @@ struct KeepArgs {
 // outside [0, max_len - n) and rows at or past max_len are skipped.
 //
 // Bound by latency: length, count, node list and rows are four dependent loads, and few bytes move (72 tensors of 8 heads
-// of 128 bf16, 8 sequences, paths of 6: 12 MB, 4 us). The three NI are the registers that paths of up to 16, 64 and 256 rows of 256
+// of 128 bf16, 8 sequences, paths of 6: 12 MB, 5 us). The three NI are the registers that paths of up to 16, 64 and 256 rows of 256
 // bytes need.
 template <int NI>
 __global__ __launch_bounds__(256) void cache_keep_kernel(const KeepArgs p) {
@@ -75,10 +75,13 @@ struct CopyArgs {
 // held in registers: the source is read once for all its destinations. The first workgroup of a group sets
 // the destinations' lengths (no destination is a source where the two lie in the same memory).
 //
-// Bound by HBM: (1 + destinations) x rows. Stores of up to 2 GB go past the caches, where they would drive out the source: 72 tensors
-// of 8 heads of 128 bf16, 2048 rows to one slot (604 MB) 121 -> 99 us, to two 183 -> 157, to four (1.5 GB) 306 -> 289. Above, both
-// reach what HBM does, and the order in which such stores arrive decides: to eight slots (2.7 GB) 550 -> 546 us where every
-// tensor is an allocation of its own, 549 -> 575 where all lie in one. (Loads past the caches too: slower at every size.)
+// Bound by HBM: (1 + destinations) x rows. Stores of up to 2 GB go past the caches, where they would drive out a source that is
+// there, as one just written or copied before: the same copy again, 72 tensors of 8 heads of 128 bf16, 2048 rows to one slot (604 MB)
+// 121 -> 99-106 us, to four (1.5 GB) 305 -> 289-297, to six (2.1 GB) 430 -> 416-427, and no difference from seven slots on. A source
+// that no cache holds gains nothing (three copies in turn, 0.6 and 1.2 GB written: 1.00 to 1.06 of the plain stores' time).
+// Above 2 GB no cache holds what matters, and plain stores are the faster ones on the whole (past the caches 1.03 of their time on
+// average, 0.94 to 1.21, over 20 shapes in one allocation and in 72; one prompt of 2048 rows to eight slots in turn 576 and 550 us).
+// (Loads past the caches too: slower at every size.)
 constexpr int64_t COPY_PAST = 2000000000;
 constexpr int COPY_U = 8, COPY_PIECE = 256 * COPY_U;   // 16-byte chunks
 

@@ -619,7 +619,8 @@ template <typename T> __device__ __forceinline__ float distill_exp(float x) {
 }
 
 // (max, sum of e^((z - max) / tau)) over a part of a row; one workgroup per (row, part). A row in one part also gets its loss.
-// (Differences first: z / tau of the types' largest and lowest numbers may be no number.) Bound by HBM: 4096 x 151936 bf16 227-240 us, 5.2-5.5 TB/s.
+// (Differences first: z / tau of the types' largest and lowest numbers may be no number.) Bound by HBM: 4096 x 151936 bf16
+// 227-240 us, 5.2-5.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_stats_kernel(const T* __restrict__ z, int64_t ldz, int V, int parts,
                                                             int width, int k, const float* __restrict__ t,

@@ -12,8 +12,13 @@
 // In both S^T = K Q^T and O^T = V^T P^T, so that a query is a column: its maximum and sum are one number in a lane, and S^T's
 // accumulators are P^T's operand as they stand.
 // The maximum that a row's weights refer to moves only when a score exceeds it by 2^8 (the weights stay
-// within fp32 and bf16 range), so that most tiles pass without rescaling. Scores, statistics and outputs are fp32; the
-// weights of bf16 products are rounded to bf16, as their V is.
+// within fp32 and bf16 range), so that most tiles pass without rescaling. Scores, statistics and outputs are fp32.
+//
+// The weights of bf16 products are rounded to bf16 (half a step, 2^-8 of each; their sum is not), as in the framework's other bf16
+// attention: the output's error against 64 bits is 2.3e-3 of its size, where its own rounding to bf16 makes 1.7e-3. A second
+// product with what the rounding leaves makes it 1.7e-3, for a quarter more time where the matrix cores bind: 8 sequences of 4096
+// rows, 16 nodes 33.4 -> 34.6 us, 32 nodes 38.2 -> 42.8, 16 sequences of 16384 rows, 64 nodes 330 -> 416. And what is left of a
+// weight may be 0 or negative, so that an infinite committed value would give NaN. fp32 products have fp32 weights.
 #include "common.h"
 #include "lds_tile.h"
 #include "../../include/unok.h"
@@ -55,8 +60,8 @@ constexpr int TB = 128, TREE_LEAST = 2;
 struct Range { int b, n, end, first, count, lo, hi; bool past; };   // sequence, its lengths, its ranges, this range's keys
 
 // Keys and values well above the memory-side cache's 256 MB are read past the caches (8 sequences, 8 heads of 128 bf16 over
-// 16384 rows, 537 MB: 16 nodes 116 -> 103 us, one node 105 -> 98). Below, a part is found there: over 4096 rows (134 MB) 16
-// nodes take 35 us, 41 with such loads, and 4 nodes in fp32 (269 MB) 54 and 66.
+// 16384 rows, 537 MB: 16 nodes 115 -> 103 us, one node 101 -> 94). Below, a part is found there: over 4096 rows (134 MB) 16
+// nodes take 33 us, 39 with such loads, and 4 nodes in fp32 (269 MB) 53 and 63.
 constexpr int64_t TREE_PAST = 384ll << 20;
 
 __device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
@@ -67,8 +72,8 @@ __device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
 
 // A workgroup's row tile, K/V head and range. Workgroups go round the 8 XCDs: eight in a row take different (range,
 // head) pairs, and the row tiles of a pair follow on the same XCD, where they share its L2. (With neighbouring pairs on
-// one XCD instead, streams that are whole cache slots apart meet in the same memory channels: 8 sequences of
-// 4096 rows 46 us, this way 37; 16384 rows 141 and 117.)
+// one XCD instead, streams that are whole cache slots apart meet in the same memory channels: with the walk of
+// that time, 8 sequences of 4096 rows 46 us, this way 37; 16384 rows 141 and 117.)
 __device__ __forceinline__ void tree_place(const TreeAttn& a, int& tile, int& h, int& id) {
   const int x = blockIdx.x, unit = x / (8 * a.rt) * 8 + x % 8;
   tile = x / 8 % a.rt;
@@ -962,9 +967,11 @@ __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restr
 struct TreePlan { int rows, rt, share; int64_t ranges; };   // rows per row tile; most ranges of all sequences
 
 // The row tile is the least that holds a pair's rows, up to what a workgroup can; K and V are read once per tile.
-// 16: the register walk (8 sequences of 4096 rows, 4 nodes of 4 heads, 39 us where the LDS walk took 47; with 32 rows 40, and the LDS
-// walk 32). Head dimension 64 has half the work to a key, and 128 rows are enough. `share` is one round of workgroups, two
-// to a CU for up to 64 rows and one above: with 1.5 to 4 rounds every case was slower.
+// 16: the register walk (one sequence of 1000 rows, one node 9.8 us, with the LDS walk 13.1; 4 sequences of 2000, 32 K/V heads, 16
+// nodes 28.3 and 32.4; 8 sequences of 4096, 4 nodes of 4 heads 28.0 and 29.1; over 16384 rows, where both are at HBM, 95 and 93).
+// With 32 rows the register walk took 40 us where the LDS walk took 32. Head dimension 64 has half the work to a key, and 128 rows are
+// enough. `share` is one round of workgroups, two to a CU for up to 64 rows and one above: with 1.5 to 4 rounds every case was
+// slower.
 TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   const int NR = nq / nk * T;
   TreePlan p;
