@@ -15,7 +15,8 @@ import math
 import pytest
 import torch
 
-from uno_amd import kernels as K, objectives
+from uno_amd import kernels as K
+from uno_amd import objectives
 from uno_amd.objectives import teacher_top_k, top_k_distillation_loss
 from uno_amd.training.losses import token_normalized_top_k_distillation
 
