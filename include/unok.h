@@ -337,6 +337,46 @@ int unok_cache_copy(int ntensors, const void* const* src, void* const* dst, int 
                     int dst_batch, int dst_max, const int64_t* src_lengths, int64_t* dst_lengths, int npairs,
                     const int* pairs, void* stream);
 
+/* Caches in 4 bits: a row of D elements is D / 2 bytes of codes (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 as 0 .. 7, bit 3 the sign; the even
+ * element in the low half) and D / 32 scale bytes, 2^(byte - 127) for 32 elements each; codes [B, nk, max_len, D / 2] and scales [B,
+ * nk, max_len, D / 32] are contiguous and 16-byte aligned. The scale is the least power of two (of 2^-125 .. 2^125) of which the
+ * largest magnitude is below seven; elements round to the nearest, ties to the even code; an infinity or NaN makes its 32 elements
+ * NaN (byte 255).
+ * unok_cache4_store: element row b T + t of rows[i] ([B T, nk D], row stride ld[i] elements) into cache row starts[b] + t of codes[i]
+ * and scales[i], for ntensors tensors; rows that do not exist in the cache are skipped. What is written shares no memory with
+ * anything else. unok_cache4_load: the numbers of those cache rows into rows[i]; rows that do not exist read as zeros. rows, ld,
+ * codes, scales are host arrays. */
+int unok_cache4_store(int dtype, int ntensors, const void* const* rows, const int64_t* ld, void* const* codes, void* const* scales,
+                      int B, int T, int nk, int D, int max_len, const int64_t* starts, void* stream);
+int unok_cache4_load(int dtype, int ntensors, void* const* rows, const int64_t* ld, const void* const* codes,
+                     const void* const* scales, int B, int T, int nk, int D, int max_len, const int64_t* starts, void* stream);
+/* unok_tree_attn over such caches. */
+int64_t unok_tree_attn4_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len);
+int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k, const void* k_scales,
+                    const void* v, const void* v_scales, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp,
+                    float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream);
+/* Verification of drafted tokens against the target's logits z (V columns, element strides between rows) from random numbers u
+ * in [0, 1). A row's weights at temperature t > 0 are exp((z - max z) / t), those below e^-700 zero; drawing a token at u takes the
+ * lowest column at which their running sum exceeds u times their sum (fp64; u below 0 counts as 0, from 1 on it takes the last column with a weight); t = 0 takes the largest logit, the lowest column of equal
+ * ones. t is temperatures[b] (device; what is not positive counts as 0), or `temperature` for all. A row with a NaN or +inf, or with
+ * -inf alone, has no distribution: nothing is drawn from it (-1). workspace: the bytes that _workspace() says, 16-byte aligned.
+ * unok_verify_draft: sequence b's rows b (L + 1) .. of z are the target's at its counts[b] <= L (null: L) drafted tokens [B, L] and
+ * behind the last; rows b L .. of y the drafter's logits, from which the tokens were drawn (null: they were chosen, q is 1 there).
+ * Token i is accepted while u[b, i] q_i < p_i; accepted[b] is their number, token[b] is drawn at u[b, L] from max(p - q, 0) at the
+ * refused token (from p where that sums to less than 2^-40) or from p behind the last. At t = 0 a token is accepted if it is the
+ * target's largest, and y is not read.
+ * unok_verify_tree: row b T + i of z is node i's. From node 0 on, the token drawn at u[b, i] leads to the first later node whose parent
+ * is i and whose token it is; nodes [B, T] is the path (-1 behind it), counts[b] its length (0: node 0 is padding), token[b] what was
+ * drawn at its end. parents as in unok_tree_attn. */
+int64_t unok_verify_draft_workspace(int dtype, int B, int L, int V);
+int unok_verify_draft(int dtype, int B, int L, int V, const void* z, int64_t ldz, const void* y, int64_t ldy, const int64_t* tokens,
+                      const int64_t* counts, const float* u, float temperature, const float* temperatures, int64_t* accepted,
+                      int64_t* token, void* workspace, int64_t ws_bytes, void* stream);
+int64_t unok_verify_tree_workspace(int dtype, int B, int T, int V);
+int unok_verify_tree(int dtype, int B, int T, int V, const void* z, int64_t ldz, const int64_t* tokens, const int32_t* parents,
+                     int64_t ldp, const float* u, float temperature, const float* temperatures, int64_t* nodes, int64_t* counts,
+                     int64_t* token, void* workspace, int64_t ws_bytes, void* stream);
+
 /* ---- Block-diffusion batch preparation ----------------------------------------------------- */
 
 /* Noising, [noisy | clean] concatenation, stream maps and interval tables of one batch.

@@ -18,7 +18,7 @@ _EINVAL, _EALIGN, _EUNSUPPORTED = -1, -2, -3
 
 _i, _i64, _p, _f = C.c_int, C.c_int64, C.c_void_p, C.c_float
 _u64 = C.c_uint64
-_ip, _pp = C.POINTER(C.c_int), C.POINTER(C.c_void_p)
+_ip, _pp, _i64p = C.POINTER(C.c_int), C.POINTER(C.c_void_p), C.POINTER(C.c_int64)
 
 
 class DraftLayerArgs(C.Structure):
@@ -72,6 +72,14 @@ SIGNATURES: dict[str, tuple] = {
     "unok_tree_attn_workspace": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
     "unok_tree_attn": (_i, [_i, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _i64,
                             _f, _p, _i64, _p, _i64, _p]),
+    "unok_tree_attn4_workspace": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
+    "unok_tree_attn4": (_i, [_i, _i, _i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _i, _p, _p, _i64, _f, _p, _i64, _p, _i64, _p]),
+    "unok_cache4_store": (_i, [_i, _i, _pp, _i64p, _pp, _pp, _i, _i, _i, _i, _i, _p, _p]),
+    "unok_cache4_load": (_i, [_i, _i, _pp, _i64p, _pp, _pp, _i, _i, _i, _i, _i, _p, _p]),
+    "unok_verify_draft_workspace": (_i64, [_i, _i, _i, _i]),
+    "unok_verify_draft": (_i, [_i, _i, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _f, _p, _p, _p, _p, _i64, _p]),
+    "unok_verify_tree_workspace": (_i64, [_i, _i, _i, _i]),
+    "unok_verify_tree": (_i, [_i, _i, _i, _i, _p, _i64, _p, _p, _i64, _p, _f, _p, _p, _p, _p, _p, _i64, _p]),
     "unok_tree_depths": (_i, [_i, _i, _p, _p, _p]),
     "unok_tree_prep": (_i, [_i, _i, _i, _i, _i, _p, _i64, _p, _p, _p, _p, _p, _f, _p, _p, _i, _p, _p]),
     "unok_cache_keep": (_i, [_i, _pp, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
@@ -172,6 +180,10 @@ def stream() -> int:
 
 def ptr_array(tensors) -> C.Array:
     return (C.c_void_p * max(1, len(tensors)))(*[t.data_ptr() for t in tensors])
+
+
+def int64_array(values) -> C.Array:
+    return (C.c_int64 * max(1, len(values)))(*values)
 
 
 def int_array(values) -> C.Array:

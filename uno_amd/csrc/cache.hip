@@ -17,7 +17,7 @@ constexpr int COPY_TENSORS = 96, COPY_DST = 64;      // per launch
 
 struct KeepArgs {
   char* t[KEEP_TENSORS];
-  int nk, max_len, P, cpr;                            // cpr: 16-byte chunks per row
+  int nk, max_len, P, cpr;                            // cpr: units (16 bytes, or a row of less) per row
   const int64_t *lengths, *nodes, *counts;
 };
 
@@ -28,8 +28,8 @@ struct KeepArgs {
 //
 // Bound by latency: length, count, node list and rows are four dependent loads, and few bytes move (72 tensors of 8 heads
 // of 128 bf16, 8 sequences, paths of 6: 12 MB, 5 us). The three NI are the registers that paths of up to 16, 64 and 256 rows of 256
-// bytes need.
-template <int NI>
+// bytes need. Rows of 2, 4 or 8 bytes (the scales of 4-bit rows) are one unit U each.
+template <typename U, int NI>
 __global__ __launch_bounds__(256) void cache_keep_kernel(const KeepArgs p) {
   const int pair = blockIdx.x, b = pair / p.nk;
   const int64_t n = p.lengths[b];
@@ -38,10 +38,10 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(const KeepArgs p) {
   const int64_t want = p.counts[b];
   const int cnt = (int)(want < 0 ? 0 : want < p.P ? want : p.P);
   const int rows = (int)(cnt < room ? cnt : room);
-  char* base = p.t[blockIdx.y] + ((int64_t)pair * p.max_len + n) * p.cpr * 16;
+  U* base = (U*)p.t[blockIdx.y] + ((int64_t)pair * p.max_len + n) * p.cpr;
   const int64_t* nodes = p.nodes + (int64_t)b * p.P;
   // (the room is at least one row, so a load that nothing needs reads row n)
-  u32x4_t v[NI];
+  U v[NI];
   int64_t from[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
@@ -52,13 +52,13 @@ __global__ __launch_bounds__(256) void cache_keep_kernel(const KeepArgs p) {
   for (int i = 0; i < NI; ++i) {
     const int c = (threadIdx.x + i * blockDim.x) % p.cpr;
     from[i] = from[i] < room ? from[i] : -1;
-    v[i] = *(const u32x4_t*)(base + ((from[i] < 0 ? 0 : from[i]) * p.cpr + c) * 16);
+    v[i] = base[(from[i] < 0 ? 0 : from[i]) * p.cpr + c];
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every row is here before any wave writes
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NI; ++i)
-    if (from[i] >= 0) *(u32x4_t*)(base + (int64_t)(threadIdx.x + i * blockDim.x) * 16) = v[i];
+    if (from[i] >= 0) base[(int64_t)(threadIdx.x + i * blockDim.x)] = v[i];
 }
 
 struct CopyArgs {
@@ -85,27 +85,28 @@ struct CopyArgs {
 constexpr int64_t COPY_PAST = 2000000000;
 constexpr int COPY_U = 8, COPY_PIECE = 256 * COPY_U;   // 16-byte chunks
 
-__global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
+// U: 16 bytes, or the whole row where it is 2, 4 or 8.
+template <typename U> __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
   const int g = blockIdx.y / p.nk, h = blockIdx.y % p.nk;
   const int s = p.group_src[g], d0 = p.group_first[g], d1 = p.group_first[g + 1];
   int64_t rows = p.src_lengths[s];
   rows = rows < 0 ? 0 : rows;
   rows = rows < p.src_max ? rows : p.src_max;
   rows = rows < p.dst_max ? rows : p.dst_max;
-  const int64_t total = rows * p.cpr;                  // 16-byte chunks
-  const u32x4_t* src = (const u32x4_t*)p.src[blockIdx.z] + ((int64_t)s * p.nk + h) * p.src_max * p.cpr;
-  u32x4_t* dst = (u32x4_t*)p.dst[blockIdx.z];
+  const int64_t total = rows * p.cpr;                  // units
+  const U* src = (const U*)p.src[blockIdx.z] + ((int64_t)s * p.nk + h) * p.src_max * p.cpr;
+  U* dst = (U*)p.dst[blockIdx.z];
   // (the branch stands outside: of two stores of one value, the compiler makes one, plain)
   auto move = [&](auto past) {
     for (int64_t c0 = (int64_t)blockIdx.x * COPY_PIECE; c0 < total; c0 += (int64_t)gridDim.x * COPY_PIECE) {
-      u32x4_t v[COPY_U];
+      U v[COPY_U];
 #pragma unroll
       for (int i = 0; i < COPY_U; ++i) {
         const int64_t c = c0 + i * 256 + threadIdx.x;
         v[i] = src[c < total ? c : total - 1];
       }
       for (int d = d0; d < d1; ++d) {
-        u32x4_t* o = dst + ((int64_t)p.slot[d] * p.nk + h) * p.dst_max * p.cpr;
+        U* o = dst + ((int64_t)p.slot[d] * p.nk + h) * p.dst_max * p.cpr;
 #pragma unroll
         for (int i = 0; i < COPY_U; ++i) {
           const int64_t c = c0 + i * 256 + threadIdx.x;
@@ -116,10 +117,23 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(const CopyArgs p) {
       }
     }
   };
-  if (total * 16 * p.nk * gridDim.z * p.group_first[p.groups] < COPY_PAST) move(std::true_type{});   // (a group's rows for all)
+  if (total * (int64_t)sizeof(U) * p.nk * gridDim.z * p.group_first[p.groups] < COPY_PAST) move(std::true_type{});   // (a group's rows for all)
   else move(std::false_type{});
   if (blockIdx.x == 0 && blockIdx.z == 0 && h == 0 && p.dst_lengths)
     for (int d = d0 + threadIdx.x; d < d1; d += 256) p.dst_lengths[p.slot[d]] = rows;
+}
+
+// Bytes of a row's units; 0: not a row that these kernels move.
+int unit_bytes(int row_bytes) {
+  return row_bytes > 0 && row_bytes % 16 == 0 ? 16 : row_bytes == 2 || row_bytes == 4 || row_bytes == 8 ? row_bytes : 0;
+}
+
+// Runs f with a value of the unit's type.
+template <typename F> void with_unit(int bytes, F f) {
+  if (bytes == 16) f(u32x4_t{});
+  else if (bytes == 8) f(uint64_t{});
+  else if (bytes == 4) f(uint32_t{});
+  else f(uint16_t{});
 }
 
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -134,8 +148,8 @@ UNOK_EXPORT int unok_cache_keep(int ntensors, void* const* caches, int row_bytes
   UNOK_REQUIRE(ntensors >= 0 && B >= 0 && nk > 0 && max_len >= 0 && P >= 0, UNOK_EINVAL,
                "cache_keep: tensors=%d B=%d nk=%d max_len=%d P=%d", ntensors, B, nk, max_len, P);
   UNOK_REQUIRE(P <= KEEP_PATH, UNOK_EUNSUPPORTED, "cache_keep: paths hold at most %d nodes (got %d)", KEEP_PATH, P);
-  UNOK_REQUIRE(row_bytes > 0 && row_bytes % 16 == 0 && row_bytes <= 512, UNOK_EALIGN,
-               "cache_keep: rows of %d bytes (a multiple of 16, at most 512)", row_bytes);
+  UNOK_REQUIRE(unit_bytes(row_bytes) && row_bytes <= 512, UNOK_EALIGN,
+               "cache_keep: rows of %d bytes (2, 4, 8 or a multiple of 16, at most 512)", row_bytes);
   UNOK_REQUIRE((int64_t)B * nk < (1ll << 31), UNOK_EINVAL, "cache_keep: B=%d nk=%d", B, nk);
   if (ntensors == 0 || B == 0 || P == 0 || max_len == 0) return 0;
   UNOK_REQUIRE(caches && lengths && nodes && counts, UNOK_EINVAL, "cache_keep: null operand");
@@ -146,7 +160,7 @@ UNOK_EXPORT int unok_cache_keep(int ntensors, void* const* caches, int row_bytes
       UNOK_REQUIRE(!overlap(caches[i], bytes, caches[j], bytes), UNOK_EINVAL, "cache_keep: caches %d and %d overlap", j, i);
   }
   KeepArgs a{};
-  a.nk = nk; a.max_len = max_len; a.P = P; a.cpr = row_bytes / 16;
+  a.nk = nk; a.max_len = max_len; a.P = P; a.cpr = row_bytes / unit_bytes(row_bytes);
   a.lengths = lengths; a.nodes = nodes; a.counts = counts;
   const int items = P * a.cpr, nt = items <= 64 ? 64 : items <= 128 ? 128 : 256, ni = (items + nt - 1) / nt;
   hipStream_t st = (hipStream_t)stream;
@@ -154,9 +168,14 @@ UNOK_EXPORT int unok_cache_keep(int ntensors, void* const* caches, int row_bytes
     const int nt_here = ntensors - t0 < KEEP_TENSORS ? ntensors - t0 : KEEP_TENSORS;
     for (int i = 0; i < nt_here; ++i) a.t[i] = (char*)caches[t0 + i];
     const dim3 grid((unsigned)(B * nk), (unsigned)nt_here), block((unsigned)nt);
-    if (ni <= 1) hipLaunchKernelGGL(cache_keep_kernel<1>, grid, block, 0, st, a);
-    else if (ni <= 4) hipLaunchKernelGGL(cache_keep_kernel<4>, grid, block, 0, st, a);
-    else hipLaunchKernelGGL(cache_keep_kernel<32>, grid, block, 0, st, a);
+    with_unit(unit_bytes(row_bytes), [&](auto u) {
+      using U = decltype(u);
+      if (ni <= 1) hipLaunchKernelGGL((cache_keep_kernel<U, 1>), grid, block, 0, st, a);
+      else if constexpr (sizeof(U) == 16) {              // (a path of smaller rows is one unit to a thread)
+        if (ni <= 4) hipLaunchKernelGGL((cache_keep_kernel<U, 4>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((cache_keep_kernel<U, 32>), grid, block, 0, st, a);
+      }
+    });
   }
   return unok::check_launch("cache_keep");
 }
@@ -167,7 +186,7 @@ UNOK_EXPORT int unok_cache_copy(int ntensors, const void* const* src, void* cons
   UNOK_REQUIRE(ntensors >= 0 && nk > 0 && src_batch >= 0 && src_max >= 0 && dst_batch >= 0 && dst_max >= 0 && npairs >= 0,
                UNOK_EINVAL, "cache_copy: tensors=%d nk=%d batch %d -> %d max_len %d -> %d pairs=%d", ntensors, nk, src_batch,
                dst_batch, src_max, dst_max, npairs);
-  UNOK_REQUIRE(row_bytes > 0 && row_bytes % 16 == 0, UNOK_EALIGN, "cache_copy: rows of %d bytes (a multiple of 16)", row_bytes);
+  UNOK_REQUIRE(unit_bytes(row_bytes), UNOK_EALIGN, "cache_copy: rows of %d bytes (2, 4, 8 or a multiple of 16)", row_bytes);
   UNOK_REQUIRE(nk <= 65535 / COPY_DST, UNOK_EINVAL, "cache_copy: nk=%d", nk);
   if (npairs == 0 || ntensors == 0) return 0;
   UNOK_REQUIRE(src && dst && src_lengths && pairs, UNOK_EINVAL, "cache_copy: null operand");
@@ -197,7 +216,7 @@ UNOK_EXPORT int unok_cache_copy(int ntensors, const void* const* src, void* cons
     }
   }
   CopyArgs a{};
-  a.nk = nk; a.src_max = src_max; a.dst_max = dst_max; a.cpr = row_bytes / 16;
+  a.nk = nk; a.src_max = src_max; a.dst_max = dst_max; a.cpr = row_bytes / unit_bytes(row_bytes);
   a.src_lengths = src_lengths; a.dst_lengths = dst_lengths;
   const int64_t most = (int64_t)(src_max < dst_max ? src_max : dst_max) * a.cpr;
   hipStream_t st = (hipStream_t)stream;
@@ -224,7 +243,10 @@ UNOK_EXPORT int unok_cache_copy(int ntensors, const void* const* src, void* cons
       const int64_t gy = (int64_t)a.groups * nk, pieces = (most + COPY_PIECE - 1) / COPY_PIECE;
       int64_t gx = 8192 / (gy * nt);                   // a few rounds of workgroups; each strides over its pieces
       gx = gx > pieces ? pieces : gx;
-      hipLaunchKernelGGL(cache_copy_kernel, dim3((unsigned)(gx < 1 ? 1 : gx), (unsigned)gy, (unsigned)nt), dim3(256), 0, st, a);
+      with_unit(unit_bytes(row_bytes), [&](auto u) {
+        hipLaunchKernelGGL(cache_copy_kernel<decltype(u)>, dim3((unsigned)(gx < 1 ? 1 : gx), (unsigned)gy, (unsigned)nt),
+                           dim3(256), 0, st, a);
+      });
     }
   }
   return unok::check_launch("cache_copy");

@@ -21,6 +21,7 @@
 // weight may be 0 or negative, so that an infinite committed value would give NaN. fp32 products have fp32 weights.
 #include "common.h"
 #include "lds_tile.h"
+#include "cache4.h"
 #include "../../include/unok.h"
 
 #include <type_traits>
@@ -35,6 +36,7 @@ struct TreeAttn {
   const void* q; int64_t ldq;                        // [B T, nq D]
   const void *k, *v;                                 // row (b, h, j) at b * s_b + h * s_h + j * s_r
   int64_t kb, kh, kr, vb, vh, vr;
+  const uint8_t *ks, *vs;                            // 4-bit caches: their scales (k and v then hold the codes)
   const int64_t* lengths;
   const int32_t* parents; int64_t ldp;               // row stride 0: one tree for all sequences
   int B, T, nq, nk, max_len, rt, share;              // row tiles per (sequence, K/V head); ranges to make of all keys
@@ -199,6 +201,30 @@ template <bool PAST, typename T> __device__ __forceinline__ T tree_load(const T*
   else return *p;
 }
 
+// The rows of one (sequence, K/V head) pair: in the type of the queries, or in 4 bits (cache4.h).
+template <typename E> struct RowsOf {
+  const E *kp, *vp;
+  int64_t kr, vr;
+  __device__ __forceinline__ RowsOf(const TreeAttn& a, int b, int h)
+      : kp((const E*)a.k + b * a.kb + h * a.kh), vp((const E*)a.v + b * a.vb + h * a.vh), kr(a.kr), vr(a.vr) {}
+  __device__ __forceinline__ const E* k(int j) const { return kp + j * kr; }
+  __device__ __forceinline__ const E* v(int j) const { return vp + j * vr; }
+  static __device__ __forceinline__ float value(const E* row, int d) { return Elem<E>::load(row + d); }
+};
+template <int D> struct RowsOf4 {
+  const uint8_t *kp, *vp, *ksp, *vsp;
+  __device__ __forceinline__ RowsOf4(const TreeAttn& a, int b, int h) {
+    const int64_t r = ((int64_t)b * a.nk + h) * a.max_len;
+    kp = (const uint8_t*)a.k + r * (D / 2);
+    vp = (const uint8_t*)a.v + r * (D / 2);
+    ksp = a.ks + r * (D / GROUP4);
+    vsp = a.vs + r * (D / GROUP4);
+  }
+  __device__ __forceinline__ Row4 k(int j) const { return {kp + (int64_t)j * (D / 2), ksp + (int64_t)j * (D / GROUP4)}; }
+  __device__ __forceinline__ Row4 v(int j) const { return {vp + (int64_t)j * (D / 2), vsp + (int64_t)j * (D / GROUP4)}; }
+  static __device__ __forceinline__ float value(Row4 row, int d) { return value4(row, d); }
+};
+
 template <typename T, int D> struct TileOps;
 
 // bf16: tiles of 32 keys. Slot j of lane group g is key 4 g + j (j < 4) or 16 + 4 g + j - 4, in P and in V.
@@ -209,6 +235,12 @@ template <int D> struct TileOps<bf16_t, D> {
   struct K { bf16x8_t f[NS][KS]; };
   struct V { uint32_t w[8][VW]; };
   typedef f32x4_t Acc;
+  // what is loaded, and its form for the products
+  typedef K KRaw;
+  typedef V VRaw;
+  typedef RowsOf<bf16_t> Rows;
+  static __device__ __forceinline__ const K& open_k(const K& k) { return k; }
+  static __device__ __forceinline__ const V& open_v(const V& v) { return v; }
 
   static __device__ __forceinline__ int slot_key(int j, int g) { return j < 4 ? 4 * g + j : 12 + 4 * g + j; }
   // The dim of accumulator element e of output tile c
@@ -287,6 +319,11 @@ template <int D> struct TileOps<float, D> {
   struct K { f32x4_t f[1][KS]; };
   struct V { f32x4_t w[4][NJ]; };
   typedef f32x4_t Acc;
+  typedef K KRaw;
+  typedef V VRaw;
+  typedef RowsOf<float> Rows;
+  static __device__ __forceinline__ const K& open_k(const K& k) { return k; }
+  static __device__ __forceinline__ const V& open_v(const V& v) { return v; }
 
   static __device__ __forceinline__ int slot_key(int j, int g) { return 4 * g + j; }
   // output tile c = 4 jj + x holds dims 64 jj + 4 m + x
@@ -343,6 +380,134 @@ template <int D> struct TileOps<float, D> {
   }
 };
 
+// 4-bit caches, bf16 or fp32 queries. The numbers of a 4-bit row are exact in bf16, so the products are the bf16 ones; the
+// conversion is one instruction for two elements and their scale. An fp32 query is the sum of three bf16 numbers (each what the ones
+// before it leave), and so is a weight: three products take the place of one, exact but for their sums.
+//   K: the 32-dim steps of S may take the dims in any order that Q takes too. Lane group g has dims D/4 g .. of its key: one load,
+//      one scale.
+//   V: lane m owns dims D/16 m .., as in bf16: one load of four (two) bytes to a key, one scale.
+template <typename E, int D> struct TileOps4 {
+  typedef TileOps<bf16_t, D> Base;
+  static constexpr int KT = Base::KT, NS = Base::NS, NDT = Base::NDT, KS = Base::KS, VW = Base::VW;
+  static constexpr int PARTS = sizeof(E) == 4 ? 3 : 1;
+  struct Q { bf16x8_t f[PARTS][KS]; };
+  typedef typename Base::K K;
+  typedef typename Base::V V;
+  typedef f32x4_t Acc;
+  typedef std::conditional_t<D == 128, uint32_t, uint16_t> VCode;
+  struct KRaw { uint32_t w[NS][KS]; uint32_t s[NS]; };
+  struct VRaw { VCode w[8]; uint32_t s[8]; };
+  typedef RowsOf4<D> Rows;
+
+  static __device__ __forceinline__ int slot_key(int j, int g) { return Base::slot_key(j, g); }
+  static __device__ __forceinline__ int dim(int c, int e, int g) { return Base::dim(c, e, g); }
+
+  // The leading bf16 part of x; x becomes what it leaves.
+  static __device__ __forceinline__ __bf16 part(float& x) {
+    const uint32_t u = __float_as_uint(x) & 0xffff0000u;
+    x -= __uint_as_float(u);
+    return __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
+  }
+  static __device__ __forceinline__ void load_q(Q& q, const E* row, int g) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const E* p = row + D / 4 * g + 8 * s;
+      if constexpr (PARTS == 1) q.f[0][s] = *(const bf16x8_t*)p;
+      else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = p[i];
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q.f[n][s][i] = part(x[i]);
+      }
+    }
+  }
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_k(KRaw& k, F row, int m, int g) {
+#pragma unroll
+    for (int a = 0; a < NS; ++a) {
+      const Row4 r = row(16 * a + m);
+      if constexpr (D == 128) {
+        const u32x4_t u = tree_load<PAST>((const u32x4_t*)(r.codes + 16 * g));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k.w[a][s] = u[s];
+      } else {
+        const u32x2_t u = tree_load<PAST>((const u32x2_t*)(r.codes + 8 * g));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k.w[a][s] = u[s];
+      }
+      k.s[a] = tree_load<PAST>(r.scales + D / 4 * g / GROUP4);
+    }
+  }
+  template <bool PAST, typename F> static __device__ __forceinline__ void load_v(VRaw& v, F row, int m, int g) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const Row4 r = row(slot_key(j, g));
+      v.w[j] = tree_load<PAST>((const VCode*)r.codes + m);
+      v.s[j] = tree_load<PAST>(r.scales + NDT * m / GROUP4);
+    }
+  }
+  static __device__ __forceinline__ K open_k(const KRaw& r) {
+    K k;
+#pragma unroll
+    for (int a = 0; a < NS; ++a) {
+      const float s = scale4(r.s[a]);
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+        k.f[a][i] = __builtin_bit_cast(bf16x8_t, u32x4_t{pair4<0>(r.w[a][i], s), pair4<1>(r.w[a][i], s), pair4<2>(r.w[a][i], s),
+                                                         pair4<3>(r.w[a][i], s)});
+    }
+    return k;
+  }
+  static __device__ __forceinline__ V open_v(const VRaw& r) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = scale4(r.s[j]);
+      v.w[j][0] = pair4<0>(r.w[j], s);
+      v.w[j][1] = pair4<1>(r.w[j], s);
+      if constexpr (VW == 4) {
+        v.w[j][2] = pair4<2>(r.w[j], s);
+        v.w[j][3] = pair4<3>(r.w[j], s);
+      }
+    }
+    return v;
+  }
+  static __device__ __forceinline__ Acc score(const K& k, const Q& q, int a) {
+    Acc s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = PARTS - 1; n >= 0; --n)                   // small parts first
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.f[a][i], q.f[n][i], s, 0, 0, 0);
+    return s;
+  }
+  template <int QT> static __device__ __forceinline__ void add_pv(const V& v, const float (&p)[QT][8], Acc (&o)[QT][NDT]) {
+    if constexpr (PARTS == 1) Base::template add_pv<QT>(v, p, o);
+    else {
+      float left[QT][8];
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) left[i][j] = p[i][j];
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n) {
+        float now[QT][8];
+#pragma unroll
+        for (int i = 0; i < QT; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            now[i][j] = __uint_as_float(__float_as_uint(left[i][j]) & 0xffff0000u);
+            left[i][j] -= now[i][j];
+          }
+        Base::template add_pv<QT>(v, now, o);
+      }
+    }
+  }
+  static __device__ __forceinline__ bool odd(const V& v) { return Base::odd(v); }
+  static __device__ __forceinline__ void clean(V& v) { Base::clean(v); }
+};
+
 // Few query rows (16 QT): the four waves take key tiles in turn, each with its own running maximum and sum, and merge at the end: no
 // barrier in the walk, and no LDS either. K and V go from memory into the registers that the MFMAs read:
 //   S^T = K Q^T   the first operand wants 16 keys x 8 (fp32: 4) consecutive dims per lane: 16-byte loads of K;
@@ -353,9 +518,8 @@ template <int D> struct TileOps<float, D> {
 // One tile ahead in a second register set. Bound by HBM: 8 sequences, 32 / 8 heads of 128 bf16, one node over 16384 rows 96 us (5.6
 // TB/s), over 4096 rows 28 us with the merge; a single sequence of 130 rows 8 us, which is launch and latency. fp32, 32 rows, bound
 // by its 16x16x4 MFMAs: 16 nodes over 4096 rows 108 us (64 rows a workgroup, which spills: 209).
-template <typename E, int D, int QT>
-__global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
-  using Ops = TileOps<E, D>;
+template <typename E, typename Ops, int D, int QT>
+__global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int row_bytes) {
   constexpr int KT = Ops::KT, NS = Ops::NS, NDT = Ops::NDT, NP = 4 * NS, ROWS = 16 * QT, LDO = D + 4;
   extern __shared__ __attribute__((aligned(16))) float merge_o[];     // [4][ROWS][LDO]
   __shared__ float merge_ml[4][ROWS][2];
@@ -367,7 +531,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
   int tile, h, id;
   tree_place(a, tile, h, id);
-  const Range range = tree_range(a, id, D * (int)sizeof(E));
+  const Range range = tree_range(a, id, row_bytes);
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, end = range.end, lo = range.lo, hi = range.hi;
   tree_note(a, range, id, h, tile);
@@ -386,8 +550,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
     if (threadIdx.x < 16) merge_pad[16 * i + m] = a.parents[b * a.ldp + node[i]] < -1;
   }
 
-  const E* kbase = (const E*)a.k + b * a.kb + h * a.kh;
-  const E* vbase = (const E*)a.v + b * a.vb + h * a.vh;
+  const typename Ops::Rows src(a, b, h);
   typename Ops::Acc o[QT][NDT];
   float mref[QT], l[QT];
 #pragma unroll
@@ -439,18 +602,18 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   int key = lo + wid * KT;
   auto walk = [&](auto past) {
     constexpr bool PAST = decltype(past)::value;
-    auto load = [&](typename Ops::K& k, typename Ops::V& v, int key0) {
-      Ops::template load_k<PAST>(k, [&](int j) { return kbase + (int64_t)(key0 + j) * a.kr; }, m, g);
-      Ops::template load_v<PAST>(v, [&](int j) { return vbase + (int64_t)(key0 + j) * a.vr; }, m, g);
+    auto load = [&](typename Ops::KRaw& k, typename Ops::VRaw& v, int key0) {
+      Ops::template load_k<PAST>(k, [&](int j) { return src.k(key0 + j); }, m, g);
+      Ops::template load_v<PAST>(v, [&](int j) { return src.v(key0 + j); }, m, g);
     };
-    auto step = [&](const typename Ops::K& k, const typename Ops::V& v) {
+    auto step = [&](const typename Ops::KRaw& k, const typename Ops::VRaw& v) {
       float p[QT][NP];
-      scores(k, p);
+      scores(Ops::open_k(k), p);
       weights(p);
-      Ops::template add_pv<QT>(v, p, o);
+      Ops::template add_pv<QT>(Ops::open_v(v), p, o);
     };
-    typename Ops::K k0, k1;
-    typename Ops::V v0, v1;
+    typename Ops::KRaw k0, k1;
+    typename Ops::VRaw v0, v1;
     if (key + KT <= full) load(k0, v0, key);
     while (key + KT <= full) {
       if (key + 5 * KT <= full) load(k1, v1, key + 4 * KT);
@@ -467,12 +630,13 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
   // Tiles with tree rows. Keys at or past the end read the last row, at weight 0.
 #pragma unroll 1
   for (; key < hi; key += 4 * KT) {
-    typename Ops::K k;
-    typename Ops::V v;
-    Ops::template load_k<false>(k, [&](int j) { const int r = key + j; return kbase + (int64_t)(r < end ? r : end - 1) * a.kr; }, m, g);
-    Ops::template load_v<false>(v, [&](int j) { const int r = key + j; return vbase + (int64_t)(r < end ? r : end - 1) * a.vr; }, m, g);
+    typename Ops::KRaw kraw;
+    typename Ops::VRaw vraw;
+    Ops::template load_k<false>(kraw, [&](int j) { const int r = key + j; return src.k(r < end ? r : end - 1); }, m, g);
+    Ops::template load_v<false>(vraw, [&](int j) { const int r = key + j; return src.v(r < end ? r : end - 1); }, m, g);
+    typename Ops::V v = Ops::open_v(vraw);
     float p[QT][NP];
-    scores(k, p);
+    scores(Ops::open_k(kraw), p);
 #pragma unroll
     for (int i = 0; i < QT; ++i)
 #pragma unroll
@@ -496,12 +660,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
 #pragma unroll 1
       for (int j = 0; j < KT && key + j < hi; ++j) {
         const int t = key + j - n;
-        const E* row = vbase + (int64_t)(key + j) * a.vr;
+        const auto row = src.v(key + j);
 #pragma unroll
         for (int c = 0; c < NDT; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = Elem<E>::load(row + Ops::dim(c, e, g));
+            const float x = Ops::Rows::value(row, Ops::dim(c, e, g));
             if (!__ballot(!(fabsf(x) < INFINITY))) continue;
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
@@ -983,55 +1147,55 @@ TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int D, int max_len) 
   return p;
 }
 
-int tree_sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
+int tree_sizes_ok(const char* what, int B, int T, int nq, int nk, int D, int max_len) {
   UNOK_REQUIRE(B >= 0 && T >= 0 && nq > 0 && nk > 0 && nq % nk == 0 && max_len >= 1, UNOK_EINVAL,
-               "tree_attn: B=%d T=%d nq=%d nk=%d max_len=%d", B, T, nq, nk, max_len);
-  UNOK_REQUIRE(T <= TREE_MAX, UNOK_EUNSUPPORTED, "tree_attn: trees hold at most %d nodes (got %d)", TREE_MAX, T);
-  UNOK_REQUIRE(D == 64 || D == 128, UNOK_EINVAL, "tree_attn: head dim %d not in {64,128}", D);
+               "%s: B=%d T=%d nq=%d nk=%d max_len=%d", what, B, T, nq, nk, max_len);
+  UNOK_REQUIRE(T <= TREE_MAX, UNOK_EUNSUPPORTED, "%s: trees hold at most %d nodes (got %d)", what, TREE_MAX, T);
+  UNOK_REQUIRE(D == 64 || D == 128, UNOK_EINVAL, "%s: head dim %d not in {64,128}", what, D);
   UNOK_REQUIRE((int64_t)B * nq * (T > 0 ? T : 1) < (1ll << 24) && max_len < (1 << 30) && B * (max_len / TB + 1ll) < (1ll << 30),
-               UNOK_EINVAL, "tree_attn: B=%d T=%d nq=%d max_len=%d exceed the row layout", B, T, nq, max_len);
+               UNOK_EINVAL, "%s: B=%d T=%d nq=%d max_len=%d exceed the row layout", what, B, T, nq, max_len);
   return 0;
 }
 
-}  // namespace
+// Workgroups of a walk: (range, head) units in eights, times the row tiles (see tree_place).
+int64_t tree_blocks(const TreeAttn& a, const TreePlan& p) { return (p.ranges * a.nk + 7) / 8 * 8 * p.rt; }
 
-UNOK_EXPORT int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
-  if (tree_sizes_ok(B, T, nq, nk, D, max_len)) return -1;
-  if (B == 0 || T == 0) return 0;
-  const TreePlan p = tree_plan(dtype, B, T, nq, nk, D, max_len);
+// Over 4-bit caches.
+TreePlan tree_plan4(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
+  const int NR = nq / nk * T;
+  TreePlan p;
+  p.rows = NR <= 16 ? 16 : 32;
+  p.rt = (NR + p.rows - 1) / p.rows;
+  const int64_t share = 512 / ((int64_t)nk * p.rt);
+  p.share = share > 1 ? (int)share : 1;
+  p.ranges = max_len <= TREE_LEAST * TB ? B : B + p.share;
+  return p;
+}
+
+int64_t plan_workspace(const TreePlan& p, int B, int T, int nq, int D) {
   return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
 }
 
-UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
-                               int64_t k_batch, int64_t k_head, int64_t k_row, const void* v, int64_t v_batch, int64_t v_head,
-                               int64_t v_row, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp,
-                               float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream) {
-  int rc = tree_sizes_ok(B, T, nq, nk, D, max_len);
-  if (rc) return rc;
-  UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn: bad dtype %d", dtype);
-  if (B == 0 || T == 0) return 0;
-  UNOK_REQUIRE(q && k && v && lengths && parents && o, UNOK_EINVAL, "tree_attn: null operand");
-  UNOK_REQUIRE(k_row >= D && v_row >= D && k_row < (1 << 23) && v_row < (1 << 23), UNOK_EINVAL,
-               "tree_attn: row strides %lld and %lld must lie in [D, 2^23)", (long long)k_row, (long long)v_row);
-  UNOK_REQUIRE(ldp == 0 || ldp >= T, UNOK_EINVAL, "tree_attn: parents' row stride %lld for %d nodes", (long long)ldp, T);
+// What both cache formats check and fill in: queries, trees, outputs, workspace. `what` names the entry point.
+int tree_setup(TreeAttn& a, const char* what, const TreePlan& plan, int dtype, int B, int T, int nq, int nk, int D, const void* q,
+               int64_t ldq, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp, float scale, void* o,
+               int64_t ldo, void* workspace, int64_t ws_bytes) {
+  UNOK_REQUIRE(q && lengths && parents && o, UNOK_EINVAL, "%s: null operand", what);
+  UNOK_REQUIRE(ldp == 0 || ldp >= T, UNOK_EINVAL, "%s: parents' row stride %lld for %d nodes", what, (long long)ldp, T);
   const int64_t es = dtype == UNOK_BF16 ? 2 : 4, width = (int64_t)nq * D, rows = (int64_t)B * T;
-  UNOK_REQUIRE(rows == 1 || (ldq >= width && ldo >= width), UNOK_EINVAL, "tree_attn: rows of %lld elements, ldq=%lld ldo=%lld",
+  UNOK_REQUIRE(rows == 1 || (ldq >= width && ldo >= width), UNOK_EINVAL, "%s: rows of %lld elements, ldq=%lld ldo=%lld", what,
                (long long)width, (long long)ldq, (long long)ldo);
   UNOK_REQUIRE(!unok::rows_overlap(q, ldq * es, o, ldo * es, rows, width * es), UNOK_EINVAL,
-               "tree_attn: the output overlaps the queries");
+               "%s: the output overlaps the queries", what);
   const float scale_log2 = scale * 1.4426950408889634f;
-  UNOK_REQUIRE(scale_log2 - scale_log2 == 0.f, UNOK_EINVAL, "tree_attn: scale %g must be finite", (double)scale);
+  UNOK_REQUIRE(scale_log2 - scale_log2 == 0.f, UNOK_EINVAL, "%s: scale %g must be finite", what, (double)scale);
   const int per16 = dtype == UNOK_BF16 ? 8 : 4;
-  int64_t bits = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) & 15;
-  for (int64_t s : {ldq, k_batch, k_head, k_row, v_batch, v_head, v_row, ldo}) bits |= s % per16;
-  UNOK_REQUIRE(bits == 0, UNOK_EALIGN, "tree_attn: operands and their strides must be multiples of 16 bytes");
-  const int64_t need = unok_tree_attn_workspace(dtype, B, T, nq, nk, D, max_len);
+  UNOK_REQUIRE((((uintptr_t)q | (uintptr_t)o) & 15) == 0 && ldq % per16 == 0 && ldo % per16 == 0, UNOK_EALIGN,
+               "%s: queries and outputs and their strides must be multiples of 16 bytes", what);
+  const int64_t need = plan_workspace(plan, B, T, nq, D);
   UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0), UNOK_EINVAL,
-               "tree_attn: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)need, (long long)ws_bytes);
-  const TreePlan plan = tree_plan(dtype, B, T, nq, nk, D, max_len);
-  TreeAttn a{};
-  a.q = q; a.ldq = ldq; a.k = k; a.v = v;
-  a.kb = k_batch; a.kh = k_head; a.kr = k_row; a.vb = v_batch; a.vh = v_head; a.vr = v_row;
+               "%s: workspace of %lld bytes (16-byte aligned) required, got %lld", what, (long long)need, (long long)ws_bytes);
+  a.q = q; a.ldq = ldq;
   a.lengths = lengths; a.parents = parents; a.ldp = ldp;
   a.B = B; a.T = T; a.nq = nq; a.nk = nk; a.max_len = max_len;
   a.rt = plan.rt;
@@ -1043,45 +1207,115 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   a.scale_log2 = scale_log2;
   a.walk_scale = scale_log2 > 0.f ? scale_log2 : scale_log2 < 0.f ? -scale_log2 : 1.f;
   a.q_factor = scale_log2 > 0.f ? 1.f : scale_log2 < 0.f ? -1.f : 0.f;
-  const int64_t nb = (plan.ranges * nk + 7) / 8 * 8 * plan.rt;
-  UNOK_REQUIRE(nb < (1ll << 31) && B < 65536, UNOK_EINVAL, "tree_attn: grid too large");
+  UNOK_REQUIRE(tree_blocks(a, plan) < (1ll << 31) && B < 65536, UNOK_EINVAL, "%s: grid too large", what);
+  return 0;
+}
+
+template <typename E, typename Ops, int D, int QT> void launch_registers(const TreeAttn& a, int64_t nb, int row_bytes, hipStream_t st) {
+  constexpr size_t lds = 4ull * 16 * QT * (D + 4) * sizeof(float);
+  UNOK_SET_LDS_ONCE((tree_attn_kernel<E, Ops, D, QT>), lds);
+  hipLaunchKernelGGL((tree_attn_kernel<E, Ops, D, QT>), dim3((unsigned)nb), dim3(256), lds, st, a, row_bytes);
+}
+template <int D, int RG> void launch_lds(const TreeAttn& a, int64_t nb, hipStream_t st) {
+  constexpr size_t lds = (RG == 2 ? 128ull : 256ull) * 2 * D * sizeof(bf16_t);   // all stages' keys
+  UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<D, RG>), lds);
+  hipLaunchKernelGGL((tree_attn_lds_kernel<D, RG>), dim3((unsigned)nb), dim3(RG == 2 ? 256 : 512), lds, st, a);
+}
+template <typename E, int D> void launch_combine(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
+  if (plan.ranges > a.B)
+    hipLaunchKernelGGL((tree_combine_kernel<E, D>), dim3((unsigned)(((int64_t)a.nq * a.T * (D / 4) + 255) / 256), (unsigned)a.B),
+                       dim3(256), 0, st, a);
+}
+
+template <typename E, int D> void launch_tree(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
+  const int64_t nb = tree_blocks(a, plan);
+  using Ops = TileOps<E, D>;
+  constexpr int bytes = D * (int)sizeof(E);
+  if (plan.rows == 16) {
+    launch_registers<E, Ops, D, 1>(a, nb, bytes, st);
+  } else if constexpr (sizeof(E) == 4) {
+    launch_registers<E, Ops, D, 2>(a, nb, bytes, st);
+  } else {
+    if (plan.rows == 64) launch_lds<D, 2>(a, nb, st);
+    else if (plan.rows == 128) launch_lds<D, 4>(a, nb, st);
+    else if constexpr (D == 128) launch_lds<D, 8>(a, nb, st);
+  }
+  launch_combine<E, D>(a, plan, st);
+}
+
+template <typename E, int D> void launch_tree4(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
+  const int64_t nb = tree_blocks(a, plan);
+  using Ops = TileOps4<E, D>;
+  constexpr int bytes = D / 2 + D / GROUP4;
+  if (plan.rows == 16) launch_registers<E, Ops, D, 1>(a, nb, bytes, st);
+  else launch_registers<E, Ops, D, 2>(a, nb, bytes, st);
+  launch_combine<E, D>(a, plan, st);
+}
+
+}  // namespace
+
+UNOK_EXPORT int64_t unok_tree_attn_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
+  if (tree_sizes_ok("tree_attn", B, T, nq, nk, D, max_len)) return -1;
+  if (B == 0 || T == 0) return 0;
+  return plan_workspace(tree_plan(dtype, B, T, nq, nk, D, max_len), B, T, nq, D);
+}
+
+UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
+                               int64_t k_batch, int64_t k_head, int64_t k_row, const void* v, int64_t v_batch, int64_t v_head,
+                               int64_t v_row, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp,
+                               float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream) {
+  int rc = tree_sizes_ok("tree_attn", B, T, nq, nk, D, max_len);
+  if (rc) return rc;
+  UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn: bad dtype %d", dtype);
+  if (B == 0 || T == 0) return 0;
+  UNOK_REQUIRE(k && v, UNOK_EINVAL, "tree_attn: null operand");
+  UNOK_REQUIRE(k_row >= D && v_row >= D && k_row < (1 << 23) && v_row < (1 << 23), UNOK_EINVAL,
+               "tree_attn: row strides %lld and %lld must lie in [D, 2^23)", (long long)k_row, (long long)v_row);
+  const int per16 = dtype == UNOK_BF16 ? 8 : 4;
+  int64_t bits = ((uintptr_t)k | (uintptr_t)v) & 15;
+  for (int64_t s : {k_batch, k_head, k_row, v_batch, v_head, v_row}) bits |= s % per16;
+  UNOK_REQUIRE(bits == 0, UNOK_EALIGN, "tree_attn: operands and their strides must be multiples of 16 bytes");
+  const TreePlan plan = tree_plan(dtype, B, T, nq, nk, D, max_len);
+  TreeAttn a{};
+  a.k = k; a.v = v;
+  a.kb = k_batch; a.kh = k_head; a.kr = k_row; a.vb = v_batch; a.vh = v_head; a.vr = v_row;
+  rc = tree_setup(a, "tree_attn", plan, dtype, B, T, nq, nk, D, q, ldq, max_len, lengths, parents, ldp, scale, o, ldo, workspace,
+                  ws_bytes);
+  if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)nb), block(256);
-  auto run = [&](auto e, auto d) {
-    using E = decltype(e);
-    constexpr int DD = decltype(d)::value;
-    auto registers = [&](auto t) {
-      constexpr int QT = decltype(t)::value;
-      constexpr size_t lds = 4ull * 16 * QT * (DD + 4) * sizeof(float);
-      UNOK_SET_LDS_ONCE((tree_attn_kernel<E, DD, QT>), lds);
-      hipLaunchKernelGGL((tree_attn_kernel<E, DD, QT>), grid, block, lds, st, a);
-    };
-    if (plan.rows == 16) {
-      registers(std::integral_constant<int, 1>{});
-    } else if constexpr (sizeof(E) == 4) {
-      registers(std::integral_constant<int, 2>{});
-    } else {
-      auto tiles = [&](auto g) {
-        constexpr int RG = decltype(g)::value;
-        constexpr size_t lds = (RG == 2 ? 128ull : 256ull) * 2 * DD * sizeof(bf16_t);   // all stages' keys
-        UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<DD, RG>), lds);
-        hipLaunchKernelGGL((tree_attn_lds_kernel<DD, RG>), grid, dim3(RG == 2 ? 256 : 512), lds, st, a);
-      };
-      if (plan.rows == 64) tiles(std::integral_constant<int, 2>{});
-      else if (plan.rows == 128) tiles(std::integral_constant<int, 4>{});
-      else if constexpr (DD == 128) tiles(std::integral_constant<int, 8>{});
-    }
-    if (plan.ranges > B)
-      hipLaunchKernelGGL((tree_combine_kernel<E, DD>), dim3((unsigned)(((int64_t)nq * T * (DD / 4) + 255) / 256), (unsigned)B),
-                         block, 0, st, a);
-  };
-  auto by_dim = [&](auto e) {
-    if (D == 128) run(e, std::integral_constant<int, 128>{});
-    else run(e, std::integral_constant<int, 64>{});
-  };
-  if (dtype == UNOK_BF16) by_dim(bf16_t{});
-  else by_dim(float{});
+  if (dtype == UNOK_BF16) D == 128 ? launch_tree<bf16_t, 128>(a, plan, st) : launch_tree<bf16_t, 64>(a, plan, st);
+  else D == 128 ? launch_tree<float, 128>(a, plan, st) : launch_tree<float, 64>(a, plan, st);
   return unok::check_launch("tree_attn");
+}
+
+UNOK_EXPORT int64_t unok_tree_attn4_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
+  if (tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len)) return -1;
+  if (B == 0 || T == 0) return 0;
+  return plan_workspace(tree_plan4(dtype, B, T, nq, nk, D, max_len), B, T, nq, D);
+}
+
+UNOK_EXPORT int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
+                                const void* k_scales, const void* v, const void* v_scales, int max_len, const int64_t* lengths,
+                                const int32_t* parents, int64_t ldp, float scale, void* o, int64_t ldo, void* workspace,
+                                int64_t ws_bytes, void* stream) {
+  int rc = tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len);
+  if (rc) return rc;
+  UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn4: bad dtype %d", dtype);
+  if (B == 0 || T == 0) return 0;
+  UNOK_REQUIRE(k && v && k_scales && v_scales, UNOK_EINVAL, "tree_attn4: null operand");
+  UNOK_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) == 0, UNOK_EALIGN,
+               "tree_attn4: codes and scales must be 16-byte aligned");
+  const TreePlan plan = tree_plan4(dtype, B, T, nq, nk, D, max_len);
+  TreeAttn a{};
+  a.k = k; a.v = v;
+  a.ks = (const uint8_t*)k_scales; a.vs = (const uint8_t*)v_scales;
+  rc = tree_setup(a, "tree_attn4", plan, dtype, B, T, nq, nk, D, q, ldq, max_len, lengths, parents, ldp, scale, o, ldo, workspace,
+                  ws_bytes);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == UNOK_BF16) D == 128 ? launch_tree4<bf16_t, 128>(a, plan, st) : launch_tree4<bf16_t, 64>(a, plan, st);
+  else D == 128 ? launch_tree4<float, 128>(a, plan, st) : launch_tree4<float, 64>(a, plan, st);
+  return unok::check_launch("tree_attn4");
 }
 
 UNOK_EXPORT int unok_tree_depths(int B, int T, const int32_t* parents, int32_t* depths, void* stream) {

@@ -7,7 +7,7 @@ non-HIP code path.
 from __future__ import annotations
 
 from functools import lru_cache
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -618,6 +618,35 @@ def _check_caches(what: str, caches: Sequence[torch.Tensor]) -> torch.Tensor:
     return c
 
 
+def _parents(what: str, parents: torch.Tensor, B: int) -> int:
+    """Checks parents int32 [B, T] or [T]; returns the stride between their rows (0: one tree for all)."""
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or (parents.dim() == 2 and parents.shape[0] != B) \
+            or (parents.shape[-1] > 1 and parents.stride(-1) != 1):
+        raise RuntimeError(f"{what}: parents must be int32 [{B}, T] or [T], got {parents.dtype} {tuple(parents.shape)}")
+    return parents.stride(0) if parents.dim() == 2 and B > 1 else 0
+
+
+def _tree_operands(what: str, q: torch.Tensor, B: int, nk: int, D: int, lengths: torch.Tensor,
+                   parents: torch.Tensor) -> tuple[int, int, int]:
+    """Checks the queries, lengths and trees of an attention over caches [B, nk, max_len, D]; returns (nq, T, parents' row stride)."""
+    _int64_vector(what, "lengths", lengths, B)
+    ldp = _parents(what, parents, B)
+    T = parents.shape[-1]
+    nq = q.shape[1] // D if D else 0
+    if q.shape[0] != B * T or nk == 0 or nq == 0 or nq % nk or nq * D != q.shape[1]:
+        raise RuntimeError(f"{what}: q must be [{B} * {T}, nq * {D}] with nq a multiple of {nk}, got {tuple(q.shape)}")
+    return nq, T, ldp
+
+
+def _tree_out(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _rowmajor(out, "out")
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise RuntimeError(f"{what}: out must have the shape and dtype of q")
+    return out
+
+
 def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *,
               scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of a tree of drafted tokens over a KV cache; returns [B*T, nq*D].
@@ -636,20 +665,8 @@ def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.
     B, nk, max_len, D = k.shape
     if D > 1 and (k.stride(3) != 1 or v.stride(3) != 1):
         raise RuntimeError("tree_attn: k and v must have unit stride along their last dimension")
-    _int64_vector("tree_attn", "lengths", lengths, B)
-    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or (parents.dim() == 2 and parents.shape[0] != B) \
-            or (parents.shape[-1] > 1 and parents.stride(-1) != 1):
-        raise RuntimeError(f"tree_attn: parents must be int32 [{B}, T] or [T], got {parents.dtype} {tuple(parents.shape)}")
-    T = parents.shape[-1]
-    ldp = parents.stride(0) if parents.dim() == 2 and B > 1 else 0
-    nq = q.shape[1] // D if D else 0
-    if q.shape[0] != B * T or nk == 0 or nq == 0 or nq % nk or nq * D != q.shape[1]:
-        raise RuntimeError(f"tree_attn: q must be [{B} * {T}, nq * {D}] with nq a multiple of {nk}, got {tuple(q.shape)}")
-    if out is None:
-        out = torch.empty((B * T, nq * D), device=q.device, dtype=q.dtype)
-    _rowmajor(out, "out")
-    if out.shape != (B * T, nq * D) or out.dtype != q.dtype:
-        raise RuntimeError("tree_attn: out must have the shape and dtype of q")
+    nq, T, ldp = _tree_operands("tree_attn", q, B, nk, D, lengths, parents)
+    out = _tree_out("tree_attn", q, out)
     _same_device("tree_attn", q, k, v, lengths, parents, out)
     ks, vs = ((*t.stride()[:2], t.stride(2) if max_len > 1 else D) for t in (k, v))
     nbytes = N.lib().unok_tree_attn_workspace(N.dtype_code(q.dtype), B, T, nq, nk, D, max_len)
@@ -733,6 +750,173 @@ def cache_copy(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], src_len
     N.call("unok_cache_copy", len(src), N.ptr_array(src), N.ptr_array(dst), s.shape[3] * s.element_size(), s.shape[1],
            s.shape[0], s.shape[2], d.shape[0], d.shape[2], N.ptr(src_lengths), N.ptr(dst_lengths), len(pairs),
            N.int_array(flat), N.stream())
+
+
+# ------------------------------------------------------------------------------------------
+# KV caches in 4 bits
+# ------------------------------------------------------------------------------------------
+class Rows4(NamedTuple):
+    """A cache tensor in 4 bits: codes uint8 [B, nk, max_len, D/2] and scales uint8 [B, nk, max_len, D/32], contiguous.
+
+    32 consecutive elements share the scale 2^(byte - 127), the least power of two of which the largest magnitude is below
+    seven; an element is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 scales (codes 0 .. 7, ties to the even one, bit 3 the sign; the
+    even element is its byte's low half). An infinity or NaN makes its 32 elements NaN (byte 255)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _check_caches4(what: str, caches: Sequence[Rows4]) -> tuple[int, int, int, int]:
+    """4-bit caches of one shape; returns (B, nk, max_len, D)."""
+    c = _check_caches(what, [x.codes for x in caches])
+    s = _check_caches(what, [x.scales for x in caches])
+    B, nk, max_len, half = c.shape
+    if c.dtype != torch.uint8 or s.dtype != torch.uint8 or half not in (32, 64) or s.shape != (B, nk, max_len, half // 16):
+        raise RuntimeError(f"{what}: uint8 codes [B, nk, max_len, D/2] and scales [B, nk, max_len, D/32] of D 64 or 128 required, "
+                           f"got {c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
+    return B, nk, max_len, 2 * half
+
+
+def cache4_store(rows: Sequence[torch.Tensor], caches: Sequence[Rows4], starts: torch.Tensor) -> None:
+    """Puts rows into 4-bit caches (see Rows4): row b*T + t of each of ``rows`` ([B*T, nk*D], fp32 or bf16, rows on 16 bytes)
+    becomes cache row starts[b] + t of its cache; rows that the cache does not have are skipped. starts int64 [B]."""
+    if len(rows) != len(caches):
+        raise RuntimeError(f"cache4_store: {len(rows)} tensors for {len(caches)} caches")
+    B, nk, max_len, D = _check_caches4("cache4_store", caches)
+    _int64_vector("cache4_store", "starts", starts, B)
+    for x in rows:
+        _rowmajor(x, "cache4_store: rows")
+        if x.shape != rows[0].shape or x.dtype != rows[0].dtype or x.shape[1] != nk * D or (x.shape[0] % B if B else x.shape[0]):
+            raise RuntimeError(f"cache4_store: rows must be [{B} * T, {nk * D}] of one type, got {x.dtype} {tuple(x.shape)}")
+    _same_device("cache4_store", starts, *rows, *(t for c in caches for t in c))
+    T = rows[0].shape[0] // B if B else 0
+    _sizes("cache4_store", B, T, nk, max_len)
+    N.call("unok_cache4_store", N.dtype_code(rows[0].dtype), len(rows), N.ptr_array(rows), N.int64_array([_ld(x) for x in rows]),
+           N.ptr_array([c.codes for c in caches]), N.ptr_array([c.scales for c in caches]), B, T, nk, D, max_len, N.ptr(starts),
+           N.stream())
+
+
+def cache4_load(caches: Sequence[Rows4], starts: torch.Tensor, T: int, dtype: torch.dtype = torch.bfloat16) -> list[torch.Tensor]:
+    """The numbers that rows starts[b] .. starts[b] + T - 1 of 4-bit caches stand for, [B*T, nk*D] each (fp32 or bf16, both exact);
+    rows that the cache does not have are zeros."""
+    B, nk, max_len, D = _check_caches4("cache4_load", caches)
+    _int64_vector("cache4_load", "starts", starts, B)
+    code = N.dtype_code(dtype)
+    if T < 0:
+        raise ValueError(f"cache4_load: {T} rows")
+    _sizes("cache4_load", B, T, nk, max_len)
+    _same_device("cache4_load", starts, *(t for c in caches for t in c))
+    rows = [torch.empty((B * T, nk * D), device=starts.device, dtype=dtype) for _ in caches]
+    N.call("unok_cache4_load", code, len(rows), N.ptr_array(rows), N.int64_array([nk * D] * len(rows)),
+           N.ptr_array([c.codes for c in caches]), N.ptr_array([c.scales for c in caches]), B, T, nk, D, max_len, N.ptr(starts),
+           N.stream())
+    return rows
+
+
+def tree_attn4(q: torch.Tensor, k: Rows4, v: Rows4, lengths: torch.Tensor, parents: torch.Tensor, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``tree_attn`` over caches in 4 bits (Rows4): the same queries, trees, lengths and output; fp32 or bf16 queries over either."""
+    _rowmajor(q, "q")
+    B, nk, max_len, D = _check_caches4("tree_attn4", (k, v))
+    nq, T, ldp = _tree_operands("tree_attn4", q, B, nk, D, lengths, parents)
+    out = _tree_out("tree_attn4", q, out)
+    _same_device("tree_attn4", q, *k, *v, lengths, parents, out)
+    _sizes("tree_attn4", B, T, nq, max_len)
+    code = N.dtype_code(q.dtype)
+    nbytes = N.lib().unok_tree_attn4_workspace(code, B, T, nq, nk, D, max_len)
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    N.call("unok_tree_attn4", code, B, T, nq, nk, D, N.ptr(q), _ld(q), N.ptr(k.codes), N.ptr(k.scales), N.ptr(v.codes),
+           N.ptr(v.scales), max_len, N.ptr(lengths), N.ptr(parents), ldp, float(D ** -0.5 if scale is None else scale), N.ptr(out),
+           _ld(out), N.ptr(ws), max(nbytes, 0), N.stream())
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# Verification of drafted tokens
+# ------------------------------------------------------------------------------------------
+def _verify_operands(what: str, z: torch.Tensor, rows: int, u: torch.Tensor, shape: tuple[int, int],
+                     temperature: float | torch.Tensor) -> tuple[float, torch.Tensor | None]:
+    """Checks logits, random numbers and temperature; returns the temperature for the library."""
+    _rowmajor(z, f"{what}: logits")
+    if z.shape[0] != rows or z.shape[1] == 0:
+        raise RuntimeError(f"{what}: logits must be [{rows}, V], got {tuple(z.shape)}")
+    N.dtype_code(z.dtype)
+    if u.dtype != torch.float32 or tuple(u.shape) != shape or not u.is_contiguous():
+        raise RuntimeError(f"{what}: u must be contiguous fp32 {shape}, got {u.dtype} {tuple(u.shape)}")
+    _sizes(what, *shape, z.shape[1])
+    if not torch.is_tensor(temperature):
+        if not 0 <= temperature < float("inf"):
+            raise ValueError(f"{what}: temperature {temperature} must be finite and not negative")
+        return float(temperature), None
+    if temperature.dtype != torch.float32 or tuple(temperature.shape) != shape[:1] or not temperature.is_contiguous():
+        raise RuntimeError(f"{what}: temperatures must be contiguous fp32 {shape[:1]}, got {temperature.dtype} "
+                           f"{tuple(temperature.shape)}")
+    return 0.0, temperature
+
+
+def verify_draft(logits: torch.Tensor, draft_logits: torch.Tensor | None, tokens: torch.Tensor, u: torch.Tensor, *,
+                 counts: torch.Tensor | None = None, temperature: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Accepts drafted tokens against the target's logits: (accepted int64 [B], next token int64 [B]).
+
+    logits [B*(L+1), V] (fp32 or bf16): row b*(L+1) + i is the target's at drafted token i of tokens int64 [B, L], the last
+    one behind them all. draft_logits [B*L, V] of the same type: what each token was drawn from at the same temperature; None
+    for tokens that were chosen, not drawn. counts int64 [B]: sequence b drafted its first counts[b] tokens only (its rows
+    behind counts[b] are not read). u fp32 [B, L+1] in [0, 1).
+
+    Token i is accepted while u[b, i] < p_i / q_i (of its target and draft probability; q_i = 1 without draft_logits). The next token
+    is drawn at u[b, L]: at the refused token from max(p - q, 0), so that every token is distributed as the target says, or from p
+    behind the last. Drawing takes the lowest token at which the distribution function exceeds u (below 0: as 0; 1 and above: the last
+    token with a probability), all in fp64. temperature: a number or
+    fp32 [B]; 0 accepts what the target's largest logit says, and takes that (draft_logits are not read). A row of logits with
+    a NaN or +inf, or of -inf alone, ends its sequence there, and the next token is -1."""
+    if tokens.dtype != torch.int64 or tokens.dim() != 2 or not tokens.is_contiguous():
+        raise RuntimeError(f"verify_draft: tokens must be contiguous int64 [B, L], got {tokens.dtype} {tuple(tokens.shape)}")
+    B, L = tokens.shape
+    temp, temps = _verify_operands("verify_draft", logits, B * (L + 1), u, (B, L + 1), temperature)
+    if draft_logits is not None:
+        _rowmajor(draft_logits, "verify_draft: draft_logits")
+        if tuple(draft_logits.shape) != (B * L, logits.shape[1]) or draft_logits.dtype != logits.dtype:
+            raise RuntimeError(f"verify_draft: draft_logits must be {logits.dtype} {(B * L, logits.shape[1])}, got "
+                               f"{draft_logits.dtype} {tuple(draft_logits.shape)}")
+    if counts is not None:
+        _int64_vector("verify_draft", "counts", counts, B)
+    _same_device("verify_draft", logits, tokens, u, *(t for t in (draft_logits, counts, temps) if t is not None))
+    V, code, dev = logits.shape[1], N.dtype_code(logits.dtype), logits.device
+    accepted, token = (torch.empty(B, device=dev, dtype=torch.int64) for _ in range(2))
+    nbytes = N.lib().unok_verify_draft_workspace(code, B, L, V)
+    ws = torch.empty(max(nbytes, 0), device=dev, dtype=torch.uint8)
+    N.call("unok_verify_draft", code, B, L, V, N.ptr(logits), _ld(logits), N.ptr(draft_logits),
+           _ld(draft_logits) if draft_logits is not None else 0, N.ptr(tokens), N.ptr(counts), N.ptr(u), temp, N.ptr(temps),
+           N.ptr(accepted), N.ptr(token), N.ptr(ws), nbytes, N.stream())
+    return accepted, token
+
+
+def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, u: torch.Tensor, *,
+                temperature: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Follows drafted trees along tokens drawn from the target's logits: (nodes int64 [B, T], counts int64 [B], next token int64
+    [B]), the first two as ``cache_keep`` takes them.
+
+    logits [B*T, V] (fp32 or bf16): row b*T + t is node t's. tokens int64 [B, T] and parents int32 [B, T] (or [T]) as tree_attn
+    reads them; T <= 256. From node 0, the one root that counts, the token drawn at a node (at u fp32 [B, T], in [0, 1)) leads
+    to its first child that holds it; the next token is what was drawn at the path's end, and nodes are -1 behind the path. Every
+    token is distributed as the target says, whatever the tree holds. With T = 1 this samples one token for each row. Drawing,
+    temperature and rows without a distribution (which end the path, next token -1) as in ``verify_draft``. A sequence whose node
+    0 is padding has the count 0 and the next token -1."""
+    if tokens.dtype != torch.int64 or tokens.dim() != 2 or not tokens.is_contiguous() or tokens.shape[1] == 0:
+        raise RuntimeError(f"verify_tree: tokens must be contiguous int64 [B, T], got {tokens.dtype} {tuple(tokens.shape)}")
+    B, T = tokens.shape
+    ldp = _parents("verify_tree", parents, B)
+    if parents.shape[-1] != T:
+        raise RuntimeError(f"verify_tree: parents {tuple(parents.shape)} do not match the tokens {(B, T)}")
+    temp, temps = _verify_operands("verify_tree", logits, B * T, u, (B, T), temperature)
+    _same_device("verify_tree", logits, tokens, parents, u, *(() if temps is None else (temps,)))
+    V, code, dev = logits.shape[1], N.dtype_code(logits.dtype), logits.device
+    nodes = torch.empty((B, T), device=dev, dtype=torch.int64)
+    counts, token = (torch.empty(B, device=dev, dtype=torch.int64) for _ in range(2))
+    nbytes = N.lib().unok_verify_tree_workspace(code, B, T, V)
+    ws = torch.empty(max(nbytes, 0), device=dev, dtype=torch.uint8)
+    N.call("unok_verify_tree", code, B, T, V, N.ptr(logits), _ld(logits), N.ptr(tokens), N.ptr(parents), ldp, N.ptr(u), temp,
+           N.ptr(temps), N.ptr(nodes), N.ptr(counts), N.ptr(token), N.ptr(ws), nbytes, N.stream())
+    return nodes, counts, token
 
 
 def row_top_k(z: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
