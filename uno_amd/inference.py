@@ -23,6 +23,10 @@ Kernels:
   length plus its depth, node t's K/V go to cache row length + t, and its queries see the committed rows, its ancestors
   and itself (unok_tree_attn). BlockKVCache.accept then moves the accepted path's rows together and commits them;
   BlockKVCache.copy_from gives sequences that share a prefix their own copies of it;
+* what of a drafted tree or block is accepted is drawn from its logits and given random numbers (verify_tree, verify_draft on
+  unok_verify_tree and unok_verify_draft), and kept;
+* a cache in 4 bits (new_cache(bits=4)) holds 3.76 times as many bf16 rows: blocks and trees store their rows quantised
+  (unok_cache4_store), and attend over the cache by unok_tree_attn4, a draft block as a chain of its rows;
 * a prefill (empty caches) is the clean stream's causal forward of the prompt (LoRA off, keys = the
   prompt itself).
 """
@@ -51,14 +55,20 @@ class BlockKVCache:
     """Per-layer K and V, head-major [B, Hkv, max_len, D], and the committed length per sequence."""
 
     def __init__(self, geo: Geometry, layers: int, batch: int, max_len: int, device, dtype):
-        shape = (batch, geo.nk, max_len, geo.d)
-        self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
-        self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
+        self.k, self.v = ([self._rows((batch, geo.nk, max_len, geo.d), device, dtype) for _ in range(layers)] for _ in "kv")
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int64)
         self.batch, self.max_len, self.geo = batch, max_len, geo
         # What a DraftGraph, which keeps a bound on the lengths, goes by: how often they were moved so far, and whether a graph
         # holds an accept or a copy, which moves them unseen.
         self.moves, self.unseen = 0, False
+
+    @staticmethod
+    def _rows(shape, device, dtype):
+        return torch.zeros(shape, device=device, dtype=dtype)
+
+    def _tensors(self) -> list[list[torch.Tensor]]:
+        """The caches' tensors, a list to each kind of row."""
+        return [self.k + self.v]
 
     def _moved(self) -> None:
         self.moves += 1
@@ -71,14 +81,18 @@ class BlockKVCache:
         length passes the cache's end. (An entry that is no row behind the committed ones counts all the same, and its new row
         stays as it was.) All on the device, and capturable into a graph (a DraftGraph over this cache then reads the lengths
         at every replay)."""
-        K.cache_keep(self.k + self.v, self.lengths, nodes, counts)
+        for tensors in self._tensors():
+            K.cache_keep(tensors, self.lengths, nodes, counts)
         self._moved()
         self.lengths.add_(counts.clamp(0, nodes.shape[1])).clamp_(max=self.max_len)
 
     def copy_from(self, other: "BlockKVCache", pairs) -> None:
         """Copies whole sequences: for each (slot of ``other``, slot of this cache) of ``pairs`` the committed rows of all
         layers and their number. ``other`` may be this cache; then no slot is both read and written. No slot is written
-        twice. (Reads ``other``'s lengths on the host only if it can hold more rows than this cache.)"""
+        twice. Both hold their rows in the same form. (Reads ``other``'s lengths on the host only if it can hold more rows than
+        this cache.)"""
+        if type(other) is not type(self):
+            raise RuntimeError(f"rows of a {type(other).__name__} do not go into a {type(self).__name__}")
         pairs = [(int(a), int(b)) for a, b in pairs]
         if not pairs:
             return
@@ -86,7 +100,23 @@ class BlockKVCache:
                 int(other.lengths[[a for a, _ in pairs]].max()) > self.max_len:
             raise RuntimeError("the sequences do not fit in the KV cache")
         self._moved()
-        K.cache_copy(other.k + other.v, self.k + self.v, other.lengths, self.lengths, pairs)
+        for src, dst in zip(other._tensors(), self._tensors()):
+            K.cache_copy(src, dst, other.lengths, self.lengths, pairs)
+
+
+class BlockKVCache4(BlockKVCache):
+    """A BlockKVCache whose K and V rows are held in 4 bits (kernels.Rows4): 4.25 bits an element, scales included."""
+
+    @staticmethod
+    def _rows(shape, device, dtype):
+        *rows, d = shape
+        if d not in (64, 128):
+            raise NotImplementedError(f"4-bit caches take head dimensions 64 and 128, not {d}")
+        return K.Rows4(*(torch.zeros((*rows, n), device=device, dtype=torch.uint8) for n in (d // 2, d // 32)))
+
+    def _tensors(self) -> list[list[torch.Tensor]]:
+        rows = self.k + self.v
+        return [[r.codes for r in rows], [r.scales for r in rows]]
 
 
 class BlockDecoder:
@@ -102,8 +132,12 @@ class BlockDecoder:
             raise RuntimeError("BlockDecoder needs a model with a LoRA adapter attached (create_lora_model).")
         self.geo = self.decoder.geo
 
-    def new_cache(self, batch: int, max_len: int) -> BlockKVCache:
-        return BlockKVCache(self.geo, len(self.decoder.layers), batch, max_len, self.base.device, self.base.dtype)
+    def new_cache(self, batch: int, max_len: int, bits: int | None = None) -> BlockKVCache:
+        """Empty caches of ``batch`` slots; ``bits`` = 4 holds their rows in 4 bits, otherwise they have the model's type."""
+        if bits not in (None, 4):
+            raise ValueError(f"caches hold rows in the model's type or in 4 bits, not in {bits}")
+        kind = BlockKVCache if bits is None else BlockKVCache4
+        return kind(self.geo, len(self.decoder.layers), batch, max_len, self.base.device, self.base.dtype)
 
     # ---- public entry points ------------------------------------------------------------------
     @torch.no_grad()
@@ -152,6 +186,35 @@ class BlockDecoder:
         """A tree block of [cache.batch, nodes] over ``cache`` captured as one HIP graph (see TreeGraph)."""
         return TreeGraph(self, cache, nodes)
 
+    @torch.no_grad()
+    def verify_tree(self, cache: BlockKVCache, node_ids: torch.Tensor, parents: torch.Tensor, u: torch.Tensor,
+                    temperature: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Verifies a drafted tree per sequence and keeps what is accepted: ``tree_block``, then the path along tokens drawn from its
+        logits at u fp32 [B, T] in [0, 1) (kernels.verify_tree), which ``cache.accept`` commits. Node 0 is the last token of the
+        sequence, always kept. Returns (nodes [B, T], counts [B], next token [B]): the path, -1 behind it, its length, and the token
+        drawn at its end, the next tree's node 0 (-1: its logits are no distribution). temperature: a number or fp32 [B]."""
+        logits = self.tree_block(cache, node_ids, parents)
+        nodes, counts, token = K.verify_tree(logits.flatten(0, 1), node_ids.to(torch.int64).contiguous(), parents, u, temperature=temperature)
+        cache.accept(nodes, counts)
+        return nodes, counts, token
+
+    @torch.no_grad()
+    def verify_draft(self, cache: BlockKVCache, block_ids: torch.Tensor, u: torch.Tensor, draft_logits: torch.Tensor | None = None,
+                     counts: torch.Tensor | None = None, temperature: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Verifies a drafted block per sequence and keeps what is accepted. block_ids [B, L+1] are the last token of each sequence
+        and its L drafted ones, draft_logits [B, L, V] what these were drawn from (None: they were chosen), counts [B] how many there
+        are (None: L). One pass over the block (LoRA off), then kernels.verify_draft at u fp32 [B, L+1]; the last token and the
+        accepted ones are committed. Returns (accepted [B], next token [B])."""
+        B, rows = block_ids.shape
+        if not 1 <= rows <= 256:
+            raise ValueError(f"blocks hold 1 to 256 rows, got {rows}")
+        chain = torch.arange(-1, rows - 1, device=block_ids.device, dtype=torch.int32)
+        logits = self.tree_block(cache, block_ids, chain)
+        accepted, token = K.verify_draft(logits.flatten(0, 1), None if draft_logits is None else draft_logits.flatten(0, 1),
+                                         block_ids[:, 1:].to(torch.int64).contiguous(), u, counts=counts, temperature=temperature)
+        cache.accept((chain.long() + 1).expand(B, rows).contiguous(), accepted + 1)
+        return accepted, token
+
     # ---- the decoder -----------------------------------------------------------------------------
     def _forward(self, cache: BlockKVCache, ids: torch.Tensor, gate: torch.Tensor | None, commit: int, prefill: bool,
                  check: bool = True):
@@ -162,11 +225,13 @@ class BlockDecoder:
         lengths = cache.lengths
         if check and int(lengths.max()) + L > cache.max_len:
             raise RuntimeError("the block does not fit in the KV cache")
-        rep = g.nq // g.nk
-        if not prefill and rep * L > 128:
-            raise NotImplementedError(f"draft blocks hold at most 128 / {rep} rows per sequence (got {L})")
+        if not prefill:
+            self._check_block(cache, L)
         dev = ids.device
         M = B * L
+        if isinstance(cache, BlockKVCache4) and not prefill:
+            chain = torch.arange(-1, L - 1, device=dev, dtype=torch.int32).expand(B, L).contiguous()
+            return self._commit(cache, self._tree_layers(ids, cache, chain, gate.reshape(-1).contiguous()), B, L, commit, prefill, check)
         h = K.embedding(ids.reshape(-1).contiguous().to(torch.int64), dec.embed_tokens.weight)
         if prefill:
             h = self._prefill_layers(h, cache, B, L)
@@ -180,11 +245,24 @@ class BlockDecoder:
             for li, layer in enumerate(dec.layers):
                 lw = layer.weights()
                 h = self._layer(h, lw, li, pos, gate_rows, cache, maps, B, L)
+        return self._commit(cache, h, B, L, commit, prefill, check)
+
+    def _commit(self, cache, h, B: int, L: int, commit: int, prefill: bool, check: bool):
+        """A block's logits; its first ``commit`` rows are the sequences' next ones."""
         logits = self._head(h, prefill)
         cache.lengths += commit
         if check and commit:                             # (a captured block's commits are counted as it is replayed)
             cache.moves += 1
         return logits.view(B, L, -1)
+
+    def _check_block(self, cache, L: int) -> None:
+        """Draft blocks that the attention takes: one workgroup's query rows, or over a 4-bit cache a tree."""
+        rep = self.geo.nq // self.geo.nk
+        if isinstance(cache, BlockKVCache4):
+            if L > 256:
+                raise NotImplementedError(f"draft blocks hold at most 256 rows per sequence (got {L})")
+        elif rep * L > 128:
+            raise NotImplementedError(f"draft blocks hold at most 128 / {rep} rows per sequence (got {L})")
 
     def _tree_check(self, cache, ids, parents, lora_mask) -> None:
         B, T = ids.shape
@@ -201,20 +279,27 @@ class BlockDecoder:
         if int(cache.lengths.max()) + T > cache.max_len:
             raise RuntimeError("the tree does not fit in the KV cache")
 
-    def _tree_forward(self, cache, ids, parents, lora_mask):
-        g, dec = self.geo, self.decoder
+    def _tree_layers(self, ids, cache, parents, gate_rows):
+        """Embedding and all layers over trees of tokens ids [B, T] (parents int32 [B, T])."""
+        g = self.geo
         B, T = ids.shape
-        gate_rows = None if lora_mask is None else lora_mask.to(torch.bool).reshape(-1).contiguous()
-        parents = parents.expand(B, T).contiguous()
         maps = {"parents": parents, "depths": K.tree_depths(parents)}
-        if cache.k[0].dtype != torch.bfloat16:
-            t = torch.arange(T, device=ids.device)
+        in4 = isinstance(cache, BlockKVCache4)
+        if in4 or cache.k[0].dtype != torch.bfloat16:
             maps["pos"] = (cache.lengths[:, None] + maps["depths"]).reshape(-1)
+        if not in4 and cache.k[0].dtype != torch.bfloat16:
+            t = torch.arange(T, device=ids.device)
             pair = torch.arange(B * g.nk, device=ids.device).view(B, 1, g.nk)
             maps["store"] = (pair * cache.max_len + (cache.lengths[:, None] + t)[..., None]).reshape(-1).to(torch.int32)
-        h = K.embedding(ids.reshape(-1).contiguous().to(torch.int64), dec.embed_tokens.weight)
-        for li, layer in enumerate(dec.layers):
+        h = K.embedding(ids.reshape(-1).contiguous().to(torch.int64), self.decoder.embed_tokens.weight)
+        for li, layer in enumerate(self.decoder.layers):
             h = self._layer(h, layer.weights(), li, maps.get("pos"), gate_rows, cache, maps, B, T)
+        return h
+
+    def _tree_forward(self, cache, ids, parents, lora_mask):
+        B, T = ids.shape
+        gate_rows = None if lora_mask is None else lora_mask.to(torch.bool).reshape(-1).contiguous()
+        h = self._tree_layers(ids, cache, parents.expand(B, T).contiguous(), gate_rows)
         return self._head(h, gate_rows is None and B * T > PLAIN_FEW_ROWS).view(B, T, -1)
 
     def _head(self, h, prefill: bool):
@@ -241,6 +326,9 @@ class BlockDecoder:
         rows = B * P * g.nk
         for li, layer in enumerate(dec.layers):
             h, k, v = clean_layer(h, layer.weights(), g, sc)
+            if isinstance(cache, BlockKVCache4):
+                K.cache4_store((k.view(B * P, g.kv), v.reshape(B * P, g.kv)), (cache.k[li], cache.v[li]), cache.lengths)
+                continue
             K.rows_copy(k.reshape(rows, g.d), cache.k[li].view(-1, g.d), rows, dmap=store)
             K.rows_copy(v.reshape(rows, g.d), cache.v[li].view(-1, g.d), rows, dmap=store)
         return h
@@ -353,7 +441,7 @@ class BlockDecoder:
 
     def _split_path(self, dev, cache) -> bool:
         """bf16 draft blocks run the attention as prep + split-key attention + combine."""
-        return cache.k[0].dtype == torch.bfloat16 and self.geo.d in (64, 128)
+        return not isinstance(cache, BlockKVCache4) and cache.k[0].dtype == torch.bfloat16 and self.geo.d in (64, 128)
 
     def _rows_path(self, M: int, dtype, prefill: bool) -> bool:
         """Draft blocks in bf16 take the few-row products (K ranges over the whole chip) when every
@@ -388,6 +476,11 @@ class BlockDecoder:
 
         x1, _ = K.rmsnorm_fwd(h0, lw.ln_in, g.eps)
         qkv = linear(x1, lw.w_qkv, "qkv", qkv_segments)
+        if isinstance(cache, BlockKVCache4):
+            q, k, _ = K.qknorm_rope_fwd(qkv, g.nq, g.nk, g.d, lw.q_norm, lw.k_norm, pos, self.decoder.inv_freq, g.eps)
+            K.cache4_store((k, qkv[:, k_end:]), (cache.k[li], cache.v[li]), cache.lengths)
+            o = K.tree_attn4(q, cache.k[li], cache.v[li], cache.lengths, maps["parents"])
+            return self._mlp(o, h0, lw, li, linear)
         ck = cache.k[li].view(-1, g.d)
         cv = cache.v[li].view(-1, g.d)
         if "ivs" in maps:
@@ -448,9 +541,7 @@ class DraftGraph:
 
     def __init__(self, decoder: BlockDecoder, cache: BlockKVCache, block_size: int, commit: int = 1):
         B, L = cache.batch, block_size
-        rep = decoder.geo.nq // decoder.geo.nk
-        if rep * L > 128:
-            raise NotImplementedError(f"draft blocks hold at most 128 / {rep} rows per sequence (got {L})")
+        decoder._check_block(cache, L)
         if not 0 <= commit <= L:
             raise ValueError(f"commit must lie in [0, {L}]")
         dev = cache.lengths.device
