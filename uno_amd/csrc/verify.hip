@@ -33,32 +33,52 @@ struct Verify {
   const float* temps; float temp;                     // per sequence, or one
   int B, T, V, nch;                                   // T: nodes of a tree, or drafted tokens
   Part* parts;                                        // [target rows, then the drafter's][nch]
+  uint32_t* arrived;                                  // of a tree's rows, drawn; 0 before
   int64_t *nodes, *out_counts, *out_token;
 };
 
-// 2^x for -1022 <= x <= 0: 2^n (1 + r q(r)), r = x - n in [-1/2, 1/2], q the polynomial through (2^r - 1) / r at ten Chebyshev
-// points. Relative error 6.4e-16; exactly 1 at 0.
-__device__ __forceinline__ double exp2_64(double x) {
-  const double n = __builtin_rint(x), r = x - n;
-  double q = 0x1.e5e9f548e5725p-28;
-  q = fma(q, r, 0x1.b6571de2f2351p-24);
-  q = fma(q, r, 0x1.62bfe46117445p-20);
-  q = fma(q, r, 0x1.ffcb76789860fp-17);
-  q = fma(q, r, 0x1.4309130378460p-13);
-  q = fma(q, r, 0x1.5d87fe908f88ap-10);
-  q = fma(q, r, 0x1.3b2ab6fba385fp-7);
-  q = fma(q, r, 0x1.c6b08d7044119p-5);
-  q = fma(q, r, 0x1.ebfbdff82c590p-3);
-  q = fma(q, r, 0x1.62e42fefa39f7p-1);
-  const double p = fma(q, r, 1.0);
-  return __hiloint2double(__double2hiint(p) + (int)n * (1 << 20), __double2loint(p));
+// 2^x at x = d c, -1022 <= x <= 0, of N numbers side by side: 2^n (1 + r q(r)), r = x - n in [-1/2, 1/2], q the polynomial through
+// (2^r - 1) / r at eight Chebyshev points. Relative error 2.1e-12, of both signs in turn (at 150 thousand columns it moves less than
+// one token in 10^6; another degree, 3.7e-14, takes 5% more time); exactly 1 at 0. n is the low half of x + 1.5 2^52.
+template <int N> __device__ __forceinline__ void exp2_64(double (&d)[N], double c) {
+  constexpr double ROUND = 0x1.8p52;
+  constexpr double Q[8] = {0x1.62e42fef9cc69p-1, 0x1.ebfbdff82a734p-3, 0x1.c6b08da70cce3p-5, 0x1.3b2ab70ad2565p-7,
+                           0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13, 0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
+  double t[N], r[N], q[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = fma(d[i], c, ROUND);
+    r[i] = fma(d[i], c, ROUND - t[i]);
+    q[i] = Q[7];
+  }
+#pragma unroll
+  for (int k = 6; k >= 0; --k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = fma(q[i], r[i], Q[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double p = fma(q[i], r[i], 1.0);
+    d[i] = __hiloint2double(__double2hiint(p) + __double2loint(t[i]) * (1 << 20), __double2loint(p));
+  }
 }
-// The weight of z relative to m, c = log2(e) / T.
+// The weights of z relative to m, c = log2(e) / T.
+template <int N> __device__ __forceinline__ void weights(const float (&z)[N], double m, double c, double (&w)[N]) {
+  bool some[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = (double)z[i] - m;
+    some[i] = w[i] * c >= LOWEST;
+    w[i] = some[i] ? w[i] : 0.0;
+  }
+  exp2_64<N>(w, c);
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = some[i] ? w[i] : 0.0;
+}
 __device__ __forceinline__ double weight(float z, double m, double c) {
-  const double x = ((double)z - m) * c;
-  const bool some = x >= LOWEST;
-  const double w = exp2_64(some ? x : 0.0);
-  return some ? w : 0.0;
+  const float a[1] = {z};
+  double w[1];
+  weights<1>(a, m, c, w);
+  return w[0];
 }
 
 __device__ __forceinline__ double rate(const Verify& a, int b) {        // log2(e) / T; 0: the largest logit is taken
@@ -103,8 +123,6 @@ __device__ __forceinline__ int wave_min(int v) {
   for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
   return v;
 }
-__device__ __forceinline__ int wave_or(bool v) { return __ballot(v) != 0; }
-
 // The parts of one chunk of a row, by one wave.
 template <typename T> __device__ __forceinline__ Part chunk_part(const T* row, int V, int nch, int chunk, double c) {
   using C = Chunks<T>;
@@ -112,50 +130,68 @@ template <typename T> __device__ __forceinline__ Part chunk_part(const T* row, i
   const C ch(row, V, nch);
   const int lane = threadIdx.x & 63, v0 = chunk * C::VPC;
   const u32x4_t* vec = (const u32x4_t*)(row + ch.head);
-  u32x4_t raw[NL];
+  constexpr int N = NL * C::VN;
+  float z[N];
+  const bool edge = chunk == 0 ? ch.head > 0 : false, last = chunk == nch - 1 && ch.tail() < V;
+  const float zh = edge && lane < ch.head ? at(row, lane) : -INFINITY;
+  const float zt = last && ch.tail() + lane < V ? at(row, ch.tail() + lane) : -INFINITY;
+  auto unpack = [&](auto whole) {
+    u32x4_t raw[NL];
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int v = v0 + 64 * i + lane;
-    raw[i] = v < ch.nv ? vec[v] : u32x4_t{0, 0, 0, 0};
-  }
-  float z[NL * C::VN + 2];
-  z[NL * C::VN] = chunk == 0 && lane < ch.head ? at(row, lane) : -INFINITY;
-  z[NL * C::VN + 1] = chunk == nch - 1 && ch.tail() + lane < V ? at(row, ch.tail() + lane) : -INFINITY;
+    for (int i = 0; i < NL; ++i) {
+      const int v = v0 + 64 * i + lane;
+      raw[i] = decltype(whole)::value || v < ch.nv ? vec[v] : u32x4_t{0, 0, 0, 0};
+    }
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const bool in = v0 + 64 * i + lane < ch.nv;
+    for (int i = 0; i < NL; ++i) {
+      const bool in = decltype(whole)::value || v0 + 64 * i + lane < ch.nv;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (C::VN == 4) z[4 * i + k] = in ? __uint_as_float(raw[i][k]) : -INFINITY;
-      else {
-        z[8 * i + 2 * k] = in ? __uint_as_float(raw[i][k] << 16) : -INFINITY;
-        z[8 * i + 2 * k + 1] = in ? __uint_as_float(raw[i][k] & 0xffff0000u) : -INFINITY;
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (C::VN == 4) z[4 * i + k] = in ? __uint_as_float(raw[i][k]) : -INFINITY;
+        else {
+          z[8 * i + 2 * k] = in ? __uint_as_float(raw[i][k] << 16) : -INFINITY;
+          z[8 * i + 2 * k + 1] = in ? __uint_as_float(raw[i][k] & 0xffff0000u) : -INFINITY;
+        }
       }
     }
-  }
-  float m = -INFINITY;
-  bool bad = false;
+  };
+  if (v0 + C::VPC <= ch.nv) unpack(std::true_type{});
+  else unpack(std::false_type{});
+  float m = -INFINITY;                                   // (NaN passes through this maximum)
 #pragma unroll
-  for (int i = 0; i < NL * C::VN + 2; ++i) {
-    m = fmaxf(m, z[i]);
-    bad |= !(z[i] < INFINITY);
-  }
-  m = wave_max(m);
+  for (int i = 0; i < N; ++i) m = __builtin_elementwise_maximum(m, z[i]);
+  m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(zh, zt));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o, 64));
   Part p{m, 0, 0.0};
-  if (wave_or(bad)) p.m = __uint_as_float(0x7fc00000u);
+  if (!(m < INFINITY)) p.m = __uint_as_float(0x7fc00000u);
   else if (m > -INFINITY) {
     if (c == 0.0) {
       int first = INT32_MAX;                             // the lowest column of the largest logit
 #pragma unroll
-      for (int i = NL * C::VN - 1; i >= 0; --i)
+      for (int i = N - 1; i >= 0; --i)
         if (z[i] == m) first = ch.head + (v0 + 64 * (i / C::VN) + lane) * C::VN + i % C::VN;
-      if (z[NL * C::VN] == m) first = lane;
-      if (first == INT32_MAX && z[NL * C::VN + 1] == m) first = ch.tail() + lane;
+      if (zh == m) first = lane;
+      if (first == INT32_MAX && zt == m) first = ch.tail() + lane;
       p.arg = wave_min(first);
     } else {
+      // (beside the chunk's largest, whose weight is 1, what lies below the lowest weight need not be exactly 0)
+      const double least = LOWEST / c;
       double s = 0.0;
+      constexpr int G = 4;
 #pragma unroll
-      for (int i = 0; i < NL * C::VN + 2; ++i) s += weight(z[i], (double)m, c);
+      for (int i = 0; i < N; i += G) {
+        double w[G];
+#pragma unroll
+        for (int k = 0; k < G; ++k) w[k] = fmax((double)z[i + k] - (double)m, least);
+        exp2_64<G>(w, c);
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      if (edge || last) {
+        double w[2] = {fmax((double)zh - (double)m, least), fmax((double)zt - (double)m, least)};
+        exp2_64<2>(w, c);
+        s += w[0] + w[1];
+      }
       p.s = wave_sum64(s);
     }
   }
@@ -171,6 +207,7 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
   int b;
   if constexpr (TREE) {
     b = row / a.T;
+    if (row % a.T == 0 && chunk == 0 && (threadIdx.x & 63) == 0) a.arrived[b] = 0;
     if (a.parents[b * a.ldp + row % a.T] < -1) return;   // padding
     z = (const T*)a.z + (int64_t)row * a.ldz;
   } else {
@@ -189,190 +226,207 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
   if ((threadIdx.x & 63) == 0) a.parts[(int64_t)row * a.nch + chunk] = p;
 }
 
-// ---- workgroup-wide steps (256 threads) ---------------------------------------------------------
-struct Shared { double wave[4]; float fmax[4]; int flag[4], win, last; };
-
-__device__ __forceinline__ double scan64(double v, Shared& sh, double& total) {   // sum over threads 0 .. this one
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// ---- one wave's steps ------------------------------------------------------------------------------
+__device__ __forceinline__ double wave_scan64(double v) {                // sum over lanes 0 .. this one
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const double below = __shfl_up(v, o, 64);
     if (lane >= o) v += below;
   }
-  __syncthreads();
-  if (lane == 63) sh.wave[w] = v;
-  __syncthreads();
-  double before = 0.0;
-  total = 0.0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < w) before += sh.wave[i];
-    total += sh.wave[i];
-  }
-  return before + v;
+  return v;
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
 
-// The lowest index j of [lo, hi) at which base plus the weights up to j exceeds t, or where none does, the last with a weight
-// (-1: no weight at all). `of` gives an index's weight. `start` becomes base plus the weights before j.
-template <typename F> __device__ int pick(int lo, int hi, double base, double t, Shared& sh, F of, double& start) {
-  const int n = hi - lo, per = (n + 255) / 256;
-  const int first = lo + min(n, (int)threadIdx.x * per), end = min(hi, first + per);
-  double sum = 0.0, total;
-  int some = -1;
-  for (int j = first; j < end; ++j) {
-    const double w = of(j);
-    sum += w;
-    some = w > 0.0 ? j : some;
+// A number that a workgroup on another XCD reads in the same launch: stored past this one's caches, and read past its own.
+template <typename V> __device__ __forceinline__ void hand_over(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ V taken(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// A list of n values that the wave goes through in order: lane l holds values [l per, (l + 1) per), the first K of them in registers.
+__device__ __forceinline__ Part listed(const Part* p) { return *p; }
+__device__ __forceinline__ double2 listed(const double2* p) { return make_double2(taken(&p->x), taken(&p->y)); }
+template <typename P, int K> struct Listed {
+  const P* p;
+  P v[K];
+  int first, end;
+  __device__ __forceinline__ Listed(const P* p_, int n) : p(p_) {
+    const int per = (n + 63) / 64;
+    first = min(n, (int)(threadIdx.x & 63) * per);
+    end = min(n, first + per);
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = listed(p + min(first + k, n - 1));
   }
-  const double upto = base + scan64(sum, sh, total);
-  if (threadIdx.x == 0) { sh.win = INT32_MAX; sh.last = -1; }
-  __syncthreads();
-  if (some >= 0) {
-    atomicMax(&sh.last, some);
-    if (upto > t) atomicMin(&sh.win, (int)threadIdx.x);
+  template <typename F> __device__ __forceinline__ void each(F f) const {   // f(index, value), in order
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (first + k < end) f(first + k, v[k]);
+    for (int i = first + K; i < end; ++i) f(i, listed(p + i));
   }
-  __syncthreads();
-  const int win = sh.win, last = sh.last;
-  // the thread that holds the index goes through its weights again
-  __syncthreads();
-  if (win == INT32_MAX ? (last >= first && last < end) : win == (int)threadIdx.x) {
+};
+
+// Of values in order across the lanes (each lane's `sum`, and `each` to go through them: f(index, weight)), the lowest index at
+// which base plus the sum so far exceeds t; where none does, the last with a weight; -1: there is none. All lanes get the index,
+// and in base the sum before it.
+template <typename F> __device__ __forceinline__ int pick(double& base, double t, double sum, int last, F each) {
+  const int lane = threadIdx.x & 63;
+  const double upto = base + wave_scan64(sum);
+  const uint64_t any = __ballot(last >= 0), over = __ballot(last >= 0 && upto > t);
+  if (any == 0) return -1;
+  const int win = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+  int found = -1;
+  double before = 0.0;
+  if (lane == win) {
     double run = upto - sum;
-    int j = first, found = some;
-    double before = run;
-    for (; j < end; ++j) {
-      const double w = of(j);
-      if (w > 0.0) {
+    bool done = false;
+    each([&](int j, double w) {
+      if (!done && w > 0.0) {
+        found = j;
         before = run;
-        if (win != INT32_MAX && run + w > t) { found = j; break; }
+        done = over && run + w > t;
       }
       run += w;
-    }
-    sh.last = found;
-    sh.wave[0] = before;
+    });
   }
-  __syncthreads();
-  const int found = sh.last;
-  start = sh.wave[0];
-  __syncthreads();
-  return found;
+  base = lane_value(before, win);
+  return __builtin_amdgcn_readlane(found, win);
 }
 
-// A row's largest logit over its parts (NaN: no distribution).
-__device__ __forceinline__ float row_max(const Part* parts, int nch, Shared& sh) {
-  float m = -INFINITY;
-  bool bad = false;
-  for (int c = threadIdx.x; c < nch; c += 256) {
-    const float x = parts[c].m;
-    bad |= x != x;
-    m = fmaxf(m, x);
+// The same over columns [lo, hi), at most 64 K of them: get(j) loads what weigh(j, values, weights) makes the weights of G columns
+// from j on from.
+template <int K, int G, typename F, typename W> __device__ __forceinline__ int pick_column(int lo, int hi, double base, double t, F get, W weigh) {
+  constexpr int KG = (K + G - 1) / G;
+  const int per = (hi - lo + 63) / 64, first = lo + min(hi - lo, (int)(threadIdx.x & 63) * per), end = min(hi, first + per);
+  decltype(get(0)) raw[KG][G];
+#pragma unroll
+  for (int k = 0; k < KG * G; ++k) raw[k / G][k % G] = get(min(first + k, hi - 1));
+  double sum = 0.0, w[KG][G];
+  int last = -1;
+#pragma unroll
+  for (int g = 0; g < KG; ++g) {
+    weigh(first + g * G, raw[g], w[g]);
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      const int j = first + g * G + k;
+      w[g][k] = j < end ? w[g][k] : 0.0;
+      sum += w[g][k];
+      last = w[g][k] > 0.0 ? j : last;
+    }
   }
-  m = wave_max(m);
-  const int any = wave_or(bad);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) { sh.fmax[threadIdx.x >> 6] = m; sh.flag[threadIdx.x >> 6] = any; }
-  __syncthreads();
-  m = fmaxf(fmaxf(sh.fmax[0], sh.fmax[1]), fmaxf(sh.fmax[2], sh.fmax[3]));
-  return sh.flag[0] | sh.flag[1] | sh.flag[2] | sh.flag[3] || m == -INFINITY ? __uint_as_float(0x7fc00000u) : m;
+  return pick(base, t, sum, last, [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < KG * G; ++k)
+      if (first + k < end) f(first + k, w[k / G][k % G]);
+  });
 }
+
 __device__ __forceinline__ double part_sum(const Part& p, double m, double c) { return p.s > 0.0 ? p.s * weight(p.m, m, c) : 0.0; }
 
-// The token of each node: one workgroup per row. (-1: padding, or no distribution.)
-template <typename T> __global__ __launch_bounds__(256) void verify_draw_kernel(const Verify a, int32_t* drawn) {
-  __shared__ Shared sh;
-  const int row = blockIdx.x, b = row / a.T;
-  if (a.parents[b * a.ldp + row % a.T] < -1) {
-    if (threadIdx.x == 0) drawn[row] = -1;
-    return;
+// A row's largest logit, its lowest column, and the sum of its weights, from its parts. bad: the row has no distribution.
+struct Row { float m; int arg; double s; bool bad; };
+template <int K> __device__ __forceinline__ Row row_of(const Listed<Part, K>& parts, double c) {
+  Row r{-INFINITY, INT32_MAX, 0.0, false};
+  parts.each([&](int, const Part& p) { r.m = __builtin_elementwise_maximum(r.m, p.m); });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) r.m = __builtin_elementwise_maximum(r.m, __shfl_xor(r.m, o, 64));
+  r.bad = !(r.m < INFINITY && r.m > -INFINITY);
+  if (r.bad) return r;
+  if (c == 0.0) {
+    parts.each([&](int, const Part& p) { if (p.m == r.m) r.arg = min(r.arg, p.arg); });
+    r.arg = wave_min(r.arg);
+  } else {
+    parts.each([&](int, const Part& p) { r.s += part_sum(p, r.m, c); });
   }
-  const Part* parts = a.parts + (int64_t)row * a.nch;
-  const double c = rate(a, b);
-  const float m = row_max(parts, a.nch, sh);
-  int token = -1;
-  if (m == m) {
-    if (c == 0.0) {
-      int first = INT32_MAX;
-      for (int i = threadIdx.x; i < a.nch; i += 256)
-        if (parts[i].m == m) first = min(first, parts[i].arg);
-      first = wave_min(first);
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) sh.flag[threadIdx.x >> 6] = first;
-      __syncthreads();
-      token = min(min(sh.flag[0], sh.flag[1]), min(sh.flag[2], sh.flag[3]));
-    } else {
-      double sum = 0.0, total, start;
-      for (int i = threadIdx.x; i < a.nch; i += 256) sum += part_sum(parts[i], m, c);
-      (void)scan64(sum, sh, total);
-      const double t = random_at(a, row) * total;
-      const int ch = pick(0, a.nch, 0.0, t, sh, [&](int i) { return part_sum(parts[i], m, c); }, start);
-      const T* z = (const T*)a.z + (int64_t)row * a.ldz;
-      const Chunks<T> cs(z, a.V, a.nch);
-      if (ch >= 0) token = pick(cs.lo(ch), cs.hi(ch), start, t, sh, [&](int j) { return weight(at(z, j), m, c); }, start);
-    }
-  }
-  if (threadIdx.x == 0) drawn[row] = token;
+  return r;
 }
 
-// From node 0 on: the token drawn at a node leads to its first child that holds it. One workgroup per sequence, a thread to a node.
-__global__ __launch_bounds__(256) void verify_walk_kernel(const Verify a, const int32_t* drawn) {
-  __shared__ int next;
-  const int b = blockIdx.x, t = threadIdx.x, T = a.T;
-  const bool node = t < T;
-  const int parent = node ? a.parents[b * a.ldp + t] : -2;
-  const int64_t token = node ? a.tokens[(int64_t)b * T + t] : -1;
-  if (node) a.nodes[(int64_t)b * T + t] = -1;
-  __syncthreads();
-  const bool none = a.parents[b * a.ldp] < -1;           // no root
-  int at = 0, n = none ? 0 : 1, got = none ? -1 : drawn[(int64_t)b * T];
-  if (!none && t == 0) a.nodes[(int64_t)b * T] = 0;
-  while (n > 0 && got >= 0) {                            // (ends: a child's index is larger than its parent's)
-    __syncthreads();
-    if (t == 0) next = T;
-    __syncthreads();
-    if (node && t > at && parent == at && token == got) atomicMin(&next, t);
-    __syncthreads();
-    if (next == T) break;
-    at = next;
-    got = drawn[(int64_t)b * T + at];
-    if (t == 0) a.nodes[(int64_t)b * T + n] = at;
-    ++n;
+// Counts one arrival of `all`; whether it is the last. What the others handed over before theirs is then there: each waited for its
+// stores before it counted. (Release and acquire fences write back and drop whole L2s: 1024 of them took 30 us.) Called by one wave.
+__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t all) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  uint32_t n = 0;
+  if ((threadIdx.x & 63) == 0) n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __builtin_amdgcn_readfirstlane(n) + 1 == all;
+}
+
+// From node 0 on: the token drawn at a node leads to its first child that holds it. One wave; lane l has nodes l, l + 64, ..
+__device__ void walk(const Verify& a, int b, const int32_t* drawn) {
+  constexpr int NK = VERIFY_NODES / 64;
+  const int lane = threadIdx.x & 63, T = a.T;
+  int parent[NK], got[NK];
+  int64_t token[NK];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    const int t = min(64 * k + lane, T - 1);
+    parent[k] = 64 * k + lane < T ? a.parents[b * a.ldp + t] : -2;
+    token[k] = a.tokens[(int64_t)b * T + t];
+    got[k] = taken(drawn + (int64_t)b * T + t);
   }
-  if (t == 0) { a.out_counts[b] = n; a.out_token[b] = got; }
+  int64_t path[NK];
+  int at = 0, n = 0, next = -1;
+#pragma unroll
+  for (int k = 0; k < NK; ++k) path[k] = -1;
+  if (__builtin_amdgcn_readfirstlane(parent[0]) >= -1) {
+    while (true) {                                       // (ends: a child's index is larger than its parent's)
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        if (n / 64 == k && n % 64 == lane) path[k] = at;
+        if (at / 64 == k) next = __builtin_amdgcn_readlane(got[k], at % 64);
+      }
+      ++n;
+      if (next < 0) break;
+      int child = T;
+#pragma unroll
+      for (int k = NK - 1; k >= 0; --k) {
+        const uint64_t hit = __ballot(parent[k] == at && 64 * k + lane > at && token[k] == next);
+        if (hit) child = 64 * k + __builtin_ctzll(hit);
+      }
+      if (child == T) break;
+      at = child;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+    if (64 * k + lane < T) a.nodes[(int64_t)b * T + 64 * k + lane] = path[k];
+  if (lane == 0) { a.out_counts[b] = n; a.out_token[b] = next; }
+}
+
+// The token of each node, one wave per row (-1: padding, or no distribution); the last of a sequence's rows follows the tree.
+template <typename T> __global__ __launch_bounds__(64) void verify_draw_kernel(const Verify a, int32_t* drawn, uint32_t* arrived) {
+  const int row = blockIdx.x, b = row / a.T;
+  int token = -1;
+  if (a.parents[b * a.ldp + row % a.T] >= -1) {
+    const double c = rate(a, b), u = random_at(a, row);
+    const Listed<Part, 4> parts(a.parts + (int64_t)row * a.nch, a.nch);
+    const Row r = row_of(parts, c);
+    if (!r.bad && c == 0.0) token = r.arg;
+    else if (!r.bad) {
+      const double m = r.m, t = u * lane_value(wave_scan64(r.s), 63);
+      double base = 0.0;
+      int last = -1;
+      parts.each([&](int i, const Part& p) { if (part_sum(p, m, c) > 0.0) last = i; });
+      const int ch = pick(base, t, r.s, last, [&](auto f) { parts.each([&](int i, const Part& p) { f(i, part_sum(p, m, c)); }); });
+      const T* z = (const T*)a.z + (int64_t)row * a.ldz;
+      const Chunks<T> cs(z, a.V, a.nch);
+      if (ch >= 0)
+        token = pick_column<(CHUNK + 14 + 63) / 64, 6>(cs.lo(ch), cs.hi(ch), base, t, [&](int j) { return at(z, j); },
+                                                       [&](int, const float (&x)[6], double (&w)[6]) { weights<6>(x, m, c, w); });
+    }
+  }
+  if (threadIdx.x == 0) hand_over(drawn + row, token);
+  if (last_to_arrive(arrived + b, a.T)) walk(a, b, drawn);
 }
 
 // ---- drafted blocks ------------------------------------------------------------------------------
-// Where a block's verification ended: row n of the target, and what the next token is drawn from.
-struct Ended { int n, mode, token, rest; double c, mp, sp, mq, sq; };
+// Where a block's verification ended: row n of the target, and what the next token is drawn from (with the rows' largest logits
+// and one over their sums).
+struct Ended { int n, mode, token, rest; double c, mp, ip, mq, iq; };
 enum : int { ENDED_KNOWN = 0, ENDED_P = 1, ENDED_ROW = 2, ENDED_POINT = 3 };   // token known; p; max(p - q, 0), q a row or one token
 
-// The largest logit and the sum of a row by one wave.
-__device__ __forceinline__ void wave_row(const Part* parts, int nch, double c, double& m, double& s, int& arg, bool& bad) {
-  const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  bool odd = false;
-  for (int i = lane; i < nch; i += 64) {
-    const float x = parts[i].m;
-    odd |= x != x;
-    top = fmaxf(top, x);
-  }
-  top = wave_max(top);
-  bad = wave_or(odd) || top == -INFINITY;
-  m = top;
-  s = 0.0;
-  arg = -1;
-  if (bad) return;
-  if (c == 0.0) {
-    int first = INT32_MAX;
-    for (int i = lane; i < nch; i += 64)
-      if (parts[i].m == top) first = min(first, parts[i].arg);
-    arg = wave_min(first);
-  } else {
-    for (int i = lane; i < nch; i += 64) s += part_sum(parts[i], m, c);
-    s = wave_sum64(s);
-  }
-}
-
-// Accepts drafted tokens in order: one workgroup of 16 waves per sequence, a wave to a row at a time.
-template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kernel(const Verify a, Ended* ended) {
+// Accepts drafted tokens in order: one workgroup of 16 waves per sequence, a wave to a row at a time. Bound by latency: every load
+// of a row is issued before the first is waited for.
+template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kernel(const Verify a, Ended* ended, uint32_t* arrived) {
   __shared__ Ended rows[VERIFY_NODES + 1];
   __shared__ bool stop[VERIFY_NODES + 1];
   const int b = blockIdx.x, wid = threadIdx.x >> 6, lane = threadIdx.x & 63, L = a.T, n = drafted(a, b);
@@ -380,30 +434,42 @@ template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kern
   const Part* targets = a.parts + (int64_t)b * (L + 1) * a.nch;
   const Part* drafts = a.parts + ((int64_t)a.B * (L + 1) + (int64_t)b * L) * a.nch;
   for (int i = wid; i <= n; i += 16) {
-    Ended e{i, ENDED_P, -1, 0, c, 0.0, 1.0, 0.0, 1.0};
-    bool bad, stops = true;
-    int arg;
-    wave_row(targets + (int64_t)i * a.nch, a.nch, c, e.mp, e.sp, arg, bad);
+    const bool row = a.y && i < n && c != 0.0;           // the drafter's row is read
     const int64_t x = i < n ? a.tokens[(int64_t)b * L + i] : -1;
     const bool in = x >= 0 && x < a.V;
-    if (bad) e.mode = ENDED_KNOWN;
+    const double u = random_at(a, (int64_t)b * (L + 1) + i);
+    const Listed<Part, 2> tp(targets + (int64_t)i * a.nch, a.nch), dp(row ? drafts + (int64_t)i * a.nch : targets, a.nch);
+    const float zx = at((const T*)a.z + ((int64_t)b * (L + 1) + i) * a.ldz, in ? (int)x : 0);
+    const float yx = row ? at((const T*)a.y + ((int64_t)b * L + i) * a.ldy, in ? (int)x : 0) : 0.f;
+    Ended e{i, ENDED_P, -1, 0, c, 0.0, 1.0, 0.0, 1.0};
+    const Row p = row_of(tp, c);
+    bool stops = true;
+    if (p.bad) e.mode = ENDED_KNOWN;
     else if (c == 0.0) {
       e.mode = ENDED_KNOWN;
-      e.token = arg;
-      stops = !(i < n && x == arg);
-    } else if (i < n) {
-      const T* z = (const T*)a.z + ((int64_t)b * (L + 1) + i) * a.ldz;
-      const double p = in ? weight(at(z, (int)x), e.mp, c) / e.sp : 0.0;
-      double q = in ? 1.0 : 0.0;
-      e.mode = ENDED_POINT;
-      e.token = in ? (int)x : -1;
-      if (a.y) {
-        wave_row(drafts + (int64_t)i * a.nch, a.nch, c, e.mq, e.sq, arg, bad);
-        e.mode = ENDED_ROW;
-        if (bad) { e.mode = ENDED_KNOWN; e.token = -1; }
-        else q = in ? weight(at((const T*)a.y + ((int64_t)b * L + i) * a.ldy, (int)x), e.mq, c) / e.sq : 0.0;
+      e.token = p.arg;
+      stops = !(i < n && x == p.arg);
+    } else {
+      e.mp = p.m;
+      e.ip = 1.0 / wave_sum64(p.s);
+      if (i < n) {
+        e.mode = ENDED_POINT;
+        e.token = in ? (int)x : -1;
+        double px = in ? weight(zx, e.mp, c) * e.ip : 0.0, qx = in ? 1.0 : 0.0;
+        bool bad = false;
+        if (row) {
+          const Row q = row_of(dp, c);
+          bad = q.bad;
+          e.mode = bad ? ENDED_KNOWN : ENDED_ROW;
+          if (bad) e.token = -1;
+          else {
+            e.mq = q.m;
+            e.iq = 1.0 / wave_sum64(q.s);
+            qx = in ? weight(yx, e.mq, c) * e.iq : 0.0;
+          }
+        }
+        stops = bad || !(u * qx < px);
       }
-      stops = bad || !(random_at(a, (int64_t)b * (L + 1) + i) * q < p);
     }
     if (lane == 0) { rows[i] = e; stop[i] = stops; }
   }
@@ -412,8 +478,9 @@ template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kern
     int i = 0;
     while (i < n && !stop[i]) ++i;
     ended[b] = rows[i];
+    arrived[b] = 0;
     a.out_counts[b] = i;
-    a.out_token[b] = rows[i].mode == ENDED_KNOWN ? rows[i].token : -1;
+    if (rows[i].mode == ENDED_KNOWN) a.out_token[b] = rows[i].token;
   }
 }
 
@@ -421,57 +488,101 @@ template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kern
 template <typename T> struct Left {
   const T *z, *y;
   Ended e;
+  struct Raw { float z, y; };
   __device__ __forceinline__ Left(const Verify& a, const Ended& e_, int b) : e(e_) {
     z = (const T*)a.z + ((int64_t)b * (a.T + 1) + e.n) * a.ldz;
-    y = e.mode == ENDED_ROW ? (const T*)a.y + ((int64_t)b * a.T + e.n) * a.ldy : nullptr;
+    y = e.mode == ENDED_ROW ? (const T*)a.y + ((int64_t)b * a.T + e.n) * a.ldy : z;
   }
-  __device__ __forceinline__ double p(int j) const { return weight(at(z, j), e.mp, e.c) / e.sp; }
-  __device__ __forceinline__ double left(int j) const {
-    const double x = p(j);
-    if (e.mode == ENDED_P) return x;
-    if (e.mode == ENDED_POINT) return j == e.token ? 0.0 : x;
-    const double d = x - weight(at(y, j), e.mq, e.c) / e.sq;
-    return d > 0.0 ? d : 0.0;
+  __device__ __forceinline__ Raw get(int j) const { return {at(z, j), at(y, j)}; }
+  // Of columns j, j + step, ..
+  template <int N> __device__ __forceinline__ void of(int j, int step, const Raw (&v)[N], double (&p)[N], double (&left)[N]) const {
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = v[i].z;
+    weights<N>(x, e.mp, e.c, p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) left[i] = p[i] *= e.ip;
+    if (e.mode == ENDED_POINT) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) left[i] = j + i * step == e.token ? 0.0 : p[i];
+    } else if (e.mode == ENDED_ROW) {
+      double q[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = v[i].y;
+      weights<N>(x, e.mq, e.c, q);
+#pragma unroll
+      for (int i = 0; i < N; ++i) left[i] = fmax(p[i] - q[i] * e.iq, 0.0);
+    }
   }
 };
 
-// Sums of p and of what is left of it, a wave to a chunk: grid (chunks / 4, sequences).
-template <typename T> __global__ __launch_bounds__(256) void verify_left_kernel(const Verify a, const Ended* ended, double2* sums) {
-  const int b = blockIdx.y, chunk = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (chunk >= a.nch || ended[b].mode == ENDED_KNOWN) return;
-  const Left<T> row(a, ended[b], b);
-  const Chunks<T> cs(row.z, a.V, a.nch);
-  const int lo = cs.lo(chunk), hi = cs.hi(chunk);
-  double p = 0.0, left = 0.0;
-  for (int j = lo + lane; j < hi; j += 64) {
-    p += row.p(j);
-    left += row.left(j);
+// Sums of p and of what is left of it, a wave to PIECE columns, grid (pieces / 4, sequences); the last workgroup of a sequence
+// draws its next token. Pieces are short, as one row of each sequence has to fill the chip.
+constexpr int PIECE = 512;
+template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(const Verify a, const Ended* ended, double2* sums,
+                                                                                uint32_t* arrived) {
+  const int b = blockIdx.y, wid = threadIdx.x >> 6, lane = threadIdx.x & 63, pieces = (a.V + PIECE - 1) / PIECE;
+  const Ended e = ended[b];
+  if (e.mode == ENDED_KNOWN) return;
+  __shared__ bool last;
+  const Left<T> row(a, e, b);
+  double2* mine = sums + (int64_t)b * pieces;
+  const int piece = blockIdx.x * 4 + wid;
+  if (piece < pieces) {
+    const int lo = piece * PIECE, hi = min(lo + PIECE, a.V);
+    constexpr int G = 4;
+    typename Left<T>::Raw raw[PIECE / 64 / G][G];
+#pragma unroll
+    for (int k = 0; k < PIECE / 64; ++k) raw[k / G][k % G] = row.get(min(lo + 64 * k + lane, hi - 1));
+    double p = 0.0, left = 0.0;
+#pragma unroll
+    for (int k = 0; k < PIECE / 64; k += G) {
+      double x[G], l[G];
+      row.template of<G>(lo + 64 * k + lane, 64, raw[k / G], x, l);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const bool in = lo + 64 * (k + i) + lane < hi;
+        p += in ? x[i] : 0.0;
+        left += in ? l[i] : 0.0;
+      }
+    }
+    p = wave_sum64(p);
+    left = wave_sum64(left);
+    if (lane == 0) {
+      hand_over(&mine[piece].x, left);
+      hand_over(&mine[piece].y, p);
+    }
   }
-  p = wave_sum64(p);
-  left = wave_sum64(left);
-  if (lane == 0) sums[(int64_t)b * a.nch + chunk] = make_double2(left, p);
-}
-
-// The next token: one workgroup per sequence.
-template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(const Verify a, const Ended* ended, const double2* sums) {
-  __shared__ Shared sh;
-  const int b = blockIdx.x;
-  if (ended[b].mode == ENDED_KNOWN) return;
-  Left<T> row(a, ended[b], b);
-  const double2* mine = sums + (int64_t)b * a.nch;
-  double l = 0.0, p = 0.0, left, whole, start;
-  for (int i = threadIdx.x; i < a.nch; i += 256) { l += mine[i].x; p += mine[i].y; }
-  (void)scan64(l, sh, left);
-  (void)scan64(p, sh, whole);
-  if (left < LEAST) row.e.mode = ENDED_P;
-  const bool all = row.e.mode == ENDED_P;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (wid == 0) {
+    const bool mylast = last_to_arrive(arrived + b, gridDim.x);
+    if (lane == 0) last = mylast;
+  }
+  __syncthreads();
+  if (!last || wid != 0) return;
+  const Listed<double2, 5> list(mine, pieces);
+  double l = 0.0, p = 0.0;
+  list.each([&](int, const double2& s) { l += s.x; p += s.y; });
+  const double left = wave_sum64(l), whole = wave_sum64(p);
+  const bool all = e.mode == ENDED_P || left < LEAST;
   const double t = random_at(a, (int64_t)b * (a.T + 1) + a.T) * (all ? whole : left);
-  const int ch = pick(0, a.nch, 0.0, t, sh, [&](int i) { return all ? mine[i].y : mine[i].x; }, start);
-  const Chunks<T> cs(row.z, a.V, a.nch);
-  const int token = ch < 0 ? -1 : pick(cs.lo(ch), cs.hi(ch), start, t, sh, [&](int j) { return row.left(j); }, start);
-  if (threadIdx.x == 0) a.out_token[b] = token;
+  int some = -1;
+  list.each([&](int i, const double2& s) { if ((all ? s.y : s.x) > 0.0) some = i; });
+  double base = 0.0;
+  const int at = pick(base, t, all ? p : l, some, [&](auto f) { list.each([&](int i, const double2& s) { f(i, all ? s.y : s.x); }); });
+  int token = -1;
+  if (at >= 0)
+    token = pick_column<PIECE / 64, 4>(at * PIECE, min(at * PIECE + PIECE, a.V), base, t, [&](int j) { return row.get(j); },
+                                       [&](int j, const typename Left<T>::Raw (&v)[4], double (&w)[4]) {
+                                         double x[4];
+                                         row.template of<4>(j, 1, v, x, w);
+                                         if (all) for (int i = 0; i < 4; ++i) w[i] = x[i];
+                                       });
+  if (lane == 0) a.out_token[b] = token;
 }
 
+int64_t pieces_of(int V) { return ((int64_t)V + PIECE - 1) / PIECE; }
 int64_t chunks_of(int V) { return ((int64_t)V + CHUNK - 1) / CHUNK; }
 
 int verify_sizes_ok(const char* what, int dtype, int B, int T, int V, int64_t rows) {
@@ -506,7 +617,7 @@ int verify_setup(Verify& a, const char* what, int dtype, int B, int T, int V, co
 
 UNOK_EXPORT int64_t unok_verify_tree_workspace(int dtype, int B, int T, int V) {
   if (verify_sizes_ok("verify_tree", dtype, B, T, V, (int64_t)B * T)) return -1;
-  return ((int64_t)B * T * (chunks_of(V) * (int64_t)sizeof(Part) + (int64_t)sizeof(int32_t)) + 15) / 16 * 16;
+  return ((int64_t)B * T * (chunks_of(V) * (int64_t)sizeof(Part) + (int64_t)sizeof(int32_t)) + B * 4ll + 15) / 16 * 16;
 }
 
 UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, int64_t ldz, const int64_t* tokens,
@@ -527,23 +638,23 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
   a.parents = parents; a.ldp = ldp;
   a.nodes = nodes;
   int32_t* drawn = (int32_t*)(a.parts + rows * a.nch);
+  a.arrived = (uint32_t*)(drawn + rows);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(rows * ((a.nch + 3) / 4))), block(256);
   auto run = [&](auto e) {
     using E = decltype(e);
     hipLaunchKernelGGL((verify_parts_kernel<E, true>), grid, block, 0, st, a);
-    hipLaunchKernelGGL(verify_draw_kernel<E>, dim3((unsigned)rows), block, 0, st, a, drawn);
+    hipLaunchKernelGGL(verify_draw_kernel<E>, dim3((unsigned)rows), dim3(64), 0, st, a, drawn, a.arrived);
   };
   if (dtype == UNOK_BF16) run(bf16_t{});
   else run(float{});
-  hipLaunchKernelGGL(verify_walk_kernel, dim3((unsigned)B), block, 0, st, a, drawn);
   return unok::check_launch("verify_tree");
 }
 
 UNOK_EXPORT int64_t unok_verify_draft_workspace(int dtype, int B, int L, int V) {
   if (verify_sizes_ok("verify_draft", dtype, B, L, V, (int64_t)B * (2 * L + 1))) return -1;
-  return (int64_t)B * ((2 * L + 1) * chunks_of(V) * (int64_t)sizeof(Part) + chunks_of(V) * (int64_t)sizeof(double2) +
-                       (int64_t)sizeof(Ended));
+  return ((int64_t)B * ((2 * L + 1) * chunks_of(V) * (int64_t)sizeof(Part) + pieces_of(V) * (int64_t)sizeof(double2) +
+                        (int64_t)sizeof(Ended) + 4) + 15) / 16 * 16;
 }
 
 UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z, int64_t ldz, const void* y, int64_t ldy,
@@ -563,16 +674,17 @@ UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z,
   a.y = y; a.ldy = ldy;
   a.counts = counts;
   double2* sums = (double2*)(a.parts + (targets + drafts) * a.nch);
-  Ended* ended = (Ended*)(sums + (int64_t)B * a.nch);
+  Ended* ended = (Ended*)(sums + (int64_t)B * pieces_of(V));
+  uint32_t* arrived = (uint32_t*)(ended + B);
   hipStream_t st = (hipStream_t)stream;
   const int groups = (a.nch + 3) / 4;
   const dim3 grid((unsigned)((targets + (y ? drafts : 0)) * groups)), block(256);
   auto run = [&](auto e) {
     using E = decltype(e);
     hipLaunchKernelGGL((verify_parts_kernel<E, false>), grid, block, 0, st, a);
-    hipLaunchKernelGGL(verify_accept_kernel<E>, dim3((unsigned)B), dim3(1024), 0, st, a, ended);
-    hipLaunchKernelGGL(verify_left_kernel<E>, dim3((unsigned)groups, (unsigned)B), block, 0, st, a, ended, sums);
-    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)B), block, 0, st, a, ended, sums);
+    hipLaunchKernelGGL(verify_accept_kernel<E>, dim3((unsigned)B), dim3(1024), 0, st, a, ended, arrived);
+    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)((pieces_of(V) + 3) / 4), (unsigned)B), block, 0, st, a, ended, sums,
+                       arrived);
   };
   if (dtype == UNOK_BF16) run(bf16_t{});
   else run(float{});
