@@ -175,7 +175,7 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def ptr_array(tensors) -> C.Array:

@@ -42,6 +42,7 @@ def _hipcc() -> str:
 FILE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "tree4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

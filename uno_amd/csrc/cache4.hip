@@ -9,7 +9,7 @@ namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int TENSORS4 = 64;                          // per launch
+constexpr int TENSORS4 = 16;                          // per launch (their addresses are arguments)
 
 struct Move4 {
   void* rows[TENSORS4]; int64_t ld[TENSORS4];         // [B T, nk D]

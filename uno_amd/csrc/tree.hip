@@ -19,211 +19,10 @@
 // product with what the rounding leaves makes it 1.7e-3, for a quarter more time where the matrix cores bind: 8 sequences of 4096
 // rows, 16 nodes 33.4 -> 34.6 us, 32 nodes 38.2 -> 42.8, 16 sequences of 16384 rows, 64 nodes 330 -> 416. And what is left of a
 // weight may be 0 or negative, so that an infinite committed value would give NaN. fp32 products have fp32 weights.
-#include "common.h"
-#include "lds_tile.h"
-#include "cache4.h"
+#include "tree.h"
 #include "../../include/unok.h"
 
-#include <type_traits>
-
 namespace {
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-constexpr int TREE_MAX = 256, TREE_WORDS = TREE_MAX / 32;
-
-struct TreeAttn {
-  const void* q; int64_t ldq;                        // [B T, nq D]
-  const void *k, *v;                                 // row (b, h, j) at b * s_b + h * s_h + j * s_r
-  int64_t kb, kh, kr, vb, vh, vr;
-  const uint8_t *ks, *vs;                            // 4-bit caches: their scales (k and v then hold the codes)
-  const int64_t* lengths;
-  const int32_t* parents; int64_t ldp;               // row stride 0: one tree for all sequences
-  int B, T, nq, nk, max_len, rt, share;              // row tiles per (sequence, K/V head); ranges to make of all keys
-  void* o; int64_t ldo;
-  int2* table;                                       // each sequence's (first range, ranges); null: never more than one
-  float *po, *pm;                                    // partial outputs [range][nk][rep T][D], (max, sum) pairs
-  float scale_log2;
-  // The LDS walk masks and compares scores before it scales them, so its scale has to be positive: another one's sign, or its
-  // 0, goes into the queries (exact in bf16).
-  float walk_scale, q_factor;
-};
-
-// How the keys are divided: in ranges of equal size, whatever the sequences' lengths, so that workgroups end
-// together. A range is at most c blocks of TB keys, c the least from TREE_LEAST on for which all sequences' keys make about
-// `share` ranges; a sequence's ranges are evened out, and numbered after those of the sequences before it. Sequences of three
-// to eight blocks on average are cut into single ones while these are no more than half a round of workgroups: one sequence of
-// 1000 rows, one node 10.1 us (in ranges of 256 keys 11.1), fp32 37 nodes of three of 901 rows 13.7 (16.7). Longer ones would pay
-// for it in the merge (one of 1150 rows 11.4 and 10.6, of 4096 15.7 and 13.1), shorter ones need none at all (130 rows 9.0 and
-// 8.0), and so would more of them (16 nodes, 8 sequences of 1000 rows 23.9 and 21.5, of 500 rows 23.1 and 19.9; of four of 500
-// rows, a third of a round, 18.0 and 18.2).
-constexpr int TB = 128, TREE_LEAST = 2;
-
-struct Range { int b, n, end, first, count, lo, hi; bool past; };   // sequence, its lengths, its ranges, this range's keys
-
-// Keys and values well above the memory-side cache's 256 MB are read past the caches (8 sequences, 8 heads of 128 bf16 over
-// 16384 rows, 537 MB: 16 nodes 115 -> 103 us, one node 101 -> 94). Below, a part is found there: over 4096 rows (134 MB) 16
-// nodes take 33 us, 39 with such loads, and 4 nodes in fp32 (269 MB) 53 and 63.
-constexpr int64_t TREE_PAST = 384ll << 20;
-
-__device__ __forceinline__ int tree_end(const TreeAttn& a, int b, int& n) {
-  const int64_t len = a.lengths[b];
-  n = (int)(len < 0 ? 0 : len < a.max_len ? len : a.max_len);
-  return n + a.T < a.max_len ? n + a.T : a.max_len;
-}
-
-// A workgroup's row tile, K/V head and range. Workgroups go round the 8 XCDs: eight in a row take different (range,
-// head) pairs, and the row tiles of a pair follow on the same XCD, where they share its L2. (With neighbouring pairs on
-// one XCD instead, streams that are whole cache slots apart meet in the same memory channels: with the walk of
-// that time, 8 sequences of 4096 rows 46 us, this way 37; 16384 rows 141 and 117.)
-__device__ __forceinline__ void tree_place(const TreeAttn& a, int& tile, int& h, int& id) {
-  const int x = blockIdx.x, unit = x / (8 * a.rt) * 8 + x % 8;
-  tile = x / 8 % a.rt;
-  h = unit % a.nk;
-  id = unit / a.nk;
-}
-
-// Notes a sequence's ranges for the kernel that merges them.
-__device__ __forceinline__ void tree_note(const TreeAttn& a, const Range& r, int id, int h, int tile) {
-  if (a.table && id == r.first && h == 0 && tile == 0 && threadIdx.x == 0) a.table[r.b] = make_int2(r.first, r.count);
-}
-
-// Sum over lanes 0 .. l in lane l, by data-parallel moves within the wave.
-__device__ __forceinline__ int wave_scan(int v) {
-#define TREE_ADD(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
-  TREE_ADD(0x111, 0xf);                                  // row_shr 1, 2, 4, 8
-  TREE_ADD(0x112, 0xf);
-  TREE_ADD(0x114, 0xf);
-  TREE_ADD(0x118, 0xf);
-  TREE_ADD(0x142, 0xa);                                  // row_bcast 15 into rows 1 and 3
-  TREE_ADD(0x143, 0xc);                                  // row_bcast 31 into rows 2 and 3
-#undef TREE_ADD
-  return v;
-}
-
-// Finds range `id`. Every wave of the workgroup does it for itself.
-__device__ __forceinline__ Range tree_range(const TreeAttn& a, int id, int row_bytes) {
-  const int lane = threadIdx.x & 63;
-  int total = 0, n = 0, end = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
-    total += __builtin_amdgcn_readlane(wave_scan((end + TB - 1) / TB), 63);
-  }
-  const bool single = total > 2 * a.B && total <= min(8 * a.B, a.share / 2);
-  int c = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), single ? 1 : TREE_LEAST);
-  // sequences end inside ranges: larger ones until no more than `share` are left (one round of workgroups)
-  if (a.B <= 64)
-    for (int i = 0; i < 12; ++i) {
-      const int count = (int)((uint32_t)((end + TB - 1) / TB + c - 1) / (uint32_t)c);
-      if (__builtin_amdgcn_readlane(wave_scan(count), 63) <= max(a.share, a.B)) break;
-      c += (c + 15) / 16;
-    }
-  Range r{-1, 0, 0, 0, 0, 0, 0, (int64_t)total * TB * a.nk * row_bytes * 2 > TREE_PAST};
-  int first = 0;
-  for (int b0 = 0; b0 < a.B && r.b < 0; b0 += 64) {
-    if (a.B > 64) end = b0 + lane < a.B ? tree_end(a, b0 + lane, n) : 0;
-    const int count = (int)((uint32_t)((end + TB - 1) / TB + c - 1) / (uint32_t)c);
-    const int upto = wave_scan(count);                   // ranges of the sequences up to this lane's
-    const uint64_t hit = __ballot(id < first + upto);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      r.b = b0 + l;
-      r.n = __builtin_amdgcn_readlane(n, l);
-      r.end = __builtin_amdgcn_readlane(end, l);
-      r.count = __builtin_amdgcn_readlane(count, l);
-      r.first = first + __builtin_amdgcn_readlane(upto, l) - r.count;
-    }
-    first += __builtin_amdgcn_readlane(upto, 63);
-  }
-  if (r.b >= 0) {
-    const int blocks = (r.end + TB - 1) / TB, per = (int)((uint32_t)(blocks + r.count - 1) / (uint32_t)r.count);
-    r.lo = (id - r.first) * per * TB;
-    r.hi = min(r.lo + per * TB, r.end);
-  }
-  return r;
-}
-
-// Each node's ancestors (itself among them) as bits, by pointer doubling: thread t holds node t's set and how far
-// its chain is followed. A padding node's set is empty; a parent that is no earlier node ends the chain. All
-// threads of the workgroup call it.
-__device__ __forceinline__ void tree_ancestors(const int32_t* parents, int T, uint32_t* anc, int* next) {
-  const int t = threadIdx.x, W = (T + 31) / 32;
-  bool real = false;
-  int p = -1;
-  uint32_t w[TREE_WORDS];
-#pragma unroll
-  for (int i = 0; i < TREE_WORDS; ++i) w[i] = 0;
-  if (t < T) {
-    p = parents[t];
-    real = p >= -1;
-    next[t] = p;
-  }
-  __syncthreads();
-  const bool cut = t < T && (p >= t || p < 0 || next[p] < -1);
-  __syncthreads();
-  if (t < T) {
-    if (cut) p = -1;
-#pragma unroll
-    for (int i = 0; i < TREE_WORDS; ++i) w[i] = real && t / 32 == i ? 1u << (t % 32) : 0u;
-    for (int i = 0; i < W; ++i) anc[t * W + i] = real && t / 32 == i ? 1u << (t % 32) : 0u;
-    next[t] = p;
-  }
-  __syncthreads();
-  for (int hops = 1; hops < T; hops *= 2) {
-    int far = -1;
-    if (p >= 0) {
-#pragma unroll
-      for (int i = 0; i < TREE_WORDS; ++i)
-        if (i < W) w[i] |= anc[p * W + i];
-      far = next[p];
-    }
-    __syncthreads();
-    if (p >= 0) {
-#pragma unroll
-      for (int i = 0; i < TREE_WORDS; ++i)
-        if (i < W) anc[t * W + i] = w[i];
-      next[t] = far;
-      p = far;
-    }
-    __syncthreads();
-  }
-}
-
-// Whether node t is among the ancestors of `node` (t outside the tree: some bit or other; no branch, so that it can stand in a
-// select).
-__device__ __forceinline__ bool tree_sees(const uint32_t* anc, int node, int W, int t) {
-  const int i = min(max(t >> 5, 0), W - 1);
-  return anc[node * W + i] >> (t & 31) & 1;
-}
-
-template <bool PAST, typename T> __device__ __forceinline__ T tree_load(const T* p) {
-  if constexpr (PAST) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-
-// The rows of one (sequence, K/V head) pair: in the type of the queries, or in 4 bits (cache4.h).
-template <typename E> struct RowsOf {
-  const E *kp, *vp;
-  int64_t kr, vr;
-  __device__ __forceinline__ RowsOf(const TreeAttn& a, int b, int h)
-      : kp((const E*)a.k + b * a.kb + h * a.kh), vp((const E*)a.v + b * a.vb + h * a.vh), kr(a.kr), vr(a.vr) {}
-  __device__ __forceinline__ const E* k(int j) const { return kp + j * kr; }
-  __device__ __forceinline__ const E* v(int j) const { return vp + j * vr; }
-  static __device__ __forceinline__ float value(const E* row, int d) { return Elem<E>::load(row + d); }
-};
-template <int D> struct RowsOf4 {
-  const uint8_t *kp, *vp, *ksp, *vsp;
-  __device__ __forceinline__ RowsOf4(const TreeAttn& a, int b, int h) {
-    const int64_t r = ((int64_t)b * a.nk + h) * a.max_len;
-    kp = (const uint8_t*)a.k + r * (D / 2);
-    vp = (const uint8_t*)a.v + r * (D / 2);
-    ksp = a.ks + r * (D / GROUP4);
-    vsp = a.vs + r * (D / GROUP4);
-  }
-  __device__ __forceinline__ Row4 k(int j) const { return {kp + (int64_t)j * (D / 2), ksp + (int64_t)j * (D / GROUP4)}; }
-  __device__ __forceinline__ Row4 v(int j) const { return {vp + (int64_t)j * (D / 2), vsp + (int64_t)j * (D / GROUP4)}; }
-  static __device__ __forceinline__ float value(Row4 row, int d) { return value4(row, d); }
-};
 
 template <typename T, int D> struct TileOps;
 
@@ -235,12 +34,6 @@ template <int D> struct TileOps<bf16_t, D> {
   struct K { bf16x8_t f[NS][KS]; };
   struct V { uint32_t w[8][VW]; };
   typedef f32x4_t Acc;
-  // what is loaded, and its form for the products
-  typedef K KRaw;
-  typedef V VRaw;
-  typedef RowsOf<bf16_t> Rows;
-  static __device__ __forceinline__ const K& open_k(const K& k) { return k; }
-  static __device__ __forceinline__ const V& open_v(const V& v) { return v; }
 
   static __device__ __forceinline__ int slot_key(int j, int g) { return j < 4 ? 4 * g + j : 12 + 4 * g + j; }
   // The dim of accumulator element e of output tile c
@@ -319,11 +112,6 @@ template <int D> struct TileOps<float, D> {
   struct K { f32x4_t f[1][KS]; };
   struct V { f32x4_t w[4][NJ]; };
   typedef f32x4_t Acc;
-  typedef K KRaw;
-  typedef V VRaw;
-  typedef RowsOf<float> Rows;
-  static __device__ __forceinline__ const K& open_k(const K& k) { return k; }
-  static __device__ __forceinline__ const V& open_v(const V& v) { return v; }
 
   static __device__ __forceinline__ int slot_key(int j, int g) { return 4 * g + j; }
   // output tile c = 4 jj + x holds dims 64 jj + 4 m + x
@@ -380,134 +168,6 @@ template <int D> struct TileOps<float, D> {
   }
 };
 
-// 4-bit caches, bf16 or fp32 queries. The numbers of a 4-bit row are exact in bf16, so the products are the bf16 ones; the
-// conversion is one instruction for two elements and their scale. An fp32 query is the sum of three bf16 numbers (each what the ones
-// before it leave), and so is a weight: three products take the place of one, exact but for their sums.
-//   K: the 32-dim steps of S may take the dims in any order that Q takes too. Lane group g has dims D/4 g .. of its key: one load,
-//      one scale.
-//   V: lane m owns dims D/16 m .., as in bf16: one load of four (two) bytes to a key, one scale.
-template <typename E, int D> struct TileOps4 {
-  typedef TileOps<bf16_t, D> Base;
-  static constexpr int KT = Base::KT, NS = Base::NS, NDT = Base::NDT, KS = Base::KS, VW = Base::VW;
-  static constexpr int PARTS = sizeof(E) == 4 ? 3 : 1;
-  struct Q { bf16x8_t f[PARTS][KS]; };
-  typedef typename Base::K K;
-  typedef typename Base::V V;
-  typedef f32x4_t Acc;
-  typedef std::conditional_t<D == 128, uint32_t, uint16_t> VCode;
-  struct KRaw { uint32_t w[NS][KS]; uint32_t s[NS]; };
-  struct VRaw { VCode w[8]; uint32_t s[8]; };
-  typedef RowsOf4<D> Rows;
-
-  static __device__ __forceinline__ int slot_key(int j, int g) { return Base::slot_key(j, g); }
-  static __device__ __forceinline__ int dim(int c, int e, int g) { return Base::dim(c, e, g); }
-
-  // The leading bf16 part of x; x becomes what it leaves.
-  static __device__ __forceinline__ __bf16 part(float& x) {
-    const uint32_t u = __float_as_uint(x) & 0xffff0000u;
-    x -= __uint_as_float(u);
-    return __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
-  }
-  static __device__ __forceinline__ void load_q(Q& q, const E* row, int g) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const E* p = row + D / 4 * g + 8 * s;
-      if constexpr (PARTS == 1) q.f[0][s] = *(const bf16x8_t*)p;
-      else {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = p[i];
-#pragma unroll
-        for (int n = 0; n < PARTS; ++n)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) q.f[n][s][i] = part(x[i]);
-      }
-    }
-  }
-  template <bool PAST, typename F> static __device__ __forceinline__ void load_k(KRaw& k, F row, int m, int g) {
-#pragma unroll
-    for (int a = 0; a < NS; ++a) {
-      const Row4 r = row(16 * a + m);
-      if constexpr (D == 128) {
-        const u32x4_t u = tree_load<PAST>((const u32x4_t*)(r.codes + 16 * g));
-#pragma unroll
-        for (int s = 0; s < KS; ++s) k.w[a][s] = u[s];
-      } else {
-        const u32x2_t u = tree_load<PAST>((const u32x2_t*)(r.codes + 8 * g));
-#pragma unroll
-        for (int s = 0; s < KS; ++s) k.w[a][s] = u[s];
-      }
-      k.s[a] = tree_load<PAST>(r.scales + D / 4 * g / GROUP4);
-    }
-  }
-  template <bool PAST, typename F> static __device__ __forceinline__ void load_v(VRaw& v, F row, int m, int g) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const Row4 r = row(slot_key(j, g));
-      v.w[j] = tree_load<PAST>((const VCode*)r.codes + m);
-      v.s[j] = tree_load<PAST>(r.scales + NDT * m / GROUP4);
-    }
-  }
-  static __device__ __forceinline__ K open_k(const KRaw& r) {
-    K k;
-#pragma unroll
-    for (int a = 0; a < NS; ++a) {
-      const float s = scale4(r.s[a]);
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-        k.f[a][i] = __builtin_bit_cast(bf16x8_t, u32x4_t{pair4<0>(r.w[a][i], s), pair4<1>(r.w[a][i], s), pair4<2>(r.w[a][i], s),
-                                                         pair4<3>(r.w[a][i], s)});
-    }
-    return k;
-  }
-  static __device__ __forceinline__ V open_v(const VRaw& r) {
-    V v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = scale4(r.s[j]);
-      v.w[j][0] = pair4<0>(r.w[j], s);
-      v.w[j][1] = pair4<1>(r.w[j], s);
-      if constexpr (VW == 4) {
-        v.w[j][2] = pair4<2>(r.w[j], s);
-        v.w[j][3] = pair4<3>(r.w[j], s);
-      }
-    }
-    return v;
-  }
-  static __device__ __forceinline__ Acc score(const K& k, const Q& q, int a) {
-    Acc s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int n = PARTS - 1; n >= 0; --n)                   // small parts first
-#pragma unroll
-      for (int i = 0; i < KS; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.f[a][i], q.f[n][i], s, 0, 0, 0);
-    return s;
-  }
-  template <int QT> static __device__ __forceinline__ void add_pv(const V& v, const float (&p)[QT][8], Acc (&o)[QT][NDT]) {
-    if constexpr (PARTS == 1) Base::template add_pv<QT>(v, p, o);
-    else {
-      float left[QT][8];
-#pragma unroll
-      for (int i = 0; i < QT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) left[i][j] = p[i][j];
-#pragma unroll
-      for (int n = 0; n < PARTS; ++n) {
-        float now[QT][8];
-#pragma unroll
-        for (int i = 0; i < QT; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            now[i][j] = __uint_as_float(__float_as_uint(left[i][j]) & 0xffff0000u);
-            left[i][j] -= now[i][j];
-          }
-        Base::template add_pv<QT>(v, now, o);
-      }
-    }
-  }
-  static __device__ __forceinline__ bool odd(const V& v) { return Base::odd(v); }
-  static __device__ __forceinline__ void clean(V& v) { Base::clean(v); }
-};
-
 // Few query rows (16 QT): the four waves take key tiles in turn, each with its own running maximum and sum, and merge at the end: no
 // barrier in the walk, and no LDS either. K and V go from memory into the registers that the MFMAs read:
 //   S^T = K Q^T   the first operand wants 16 keys x 8 (fp32: 4) consecutive dims per lane: 16-byte loads of K;
@@ -518,8 +178,9 @@ template <typename E, int D> struct TileOps4 {
 // One tile ahead in a second register set. Bound by HBM: 8 sequences, 32 / 8 heads of 128 bf16, one node over 16384 rows 96 us (5.6
 // TB/s), over 4096 rows 28 us with the merge; a single sequence of 130 rows 8 us, which is launch and latency. fp32, 32 rows, bound
 // by its 16x16x4 MFMAs: 16 nodes over 4096 rows 108 us (64 rows a workgroup, which spills: 209).
-template <typename E, typename Ops, int D, int QT>
-__global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int row_bytes) {
+template <typename E, int D, int QT>
+__global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a) {
+  using Ops = TileOps<E, D>;
   constexpr int KT = Ops::KT, NS = Ops::NS, NDT = Ops::NDT, NP = 4 * NS, ROWS = 16 * QT, LDO = D + 4;
   extern __shared__ __attribute__((aligned(16))) float merge_o[];     // [4][ROWS][LDO]
   __shared__ float merge_ml[4][ROWS][2];
@@ -531,7 +192,7 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
   const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
   int tile, h, id;
   tree_place(a, tile, h, id);
-  const Range range = tree_range(a, id, row_bytes);
+  const Range range = tree_range(a, id, D * (int)sizeof(E));
   if (range.b < 0 || range.lo >= range.hi) return;
   const int b = range.b, n = range.n, end = range.end, lo = range.lo, hi = range.hi;
   tree_note(a, range, id, h, tile);
@@ -550,7 +211,8 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
     if (threadIdx.x < 16) merge_pad[16 * i + m] = a.parents[b * a.ldp + node[i]] < -1;
   }
 
-  const typename Ops::Rows src(a, b, h);
+  const E* kbase = (const E*)a.k + b * a.kb + h * a.kh;
+  const E* vbase = (const E*)a.v + b * a.vb + h * a.vh;
   typename Ops::Acc o[QT][NDT];
   float mref[QT], l[QT];
 #pragma unroll
@@ -602,18 +264,18 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
   int key = lo + wid * KT;
   auto walk = [&](auto past) {
     constexpr bool PAST = decltype(past)::value;
-    auto load = [&](typename Ops::KRaw& k, typename Ops::VRaw& v, int key0) {
-      Ops::template load_k<PAST>(k, [&](int j) { return src.k(key0 + j); }, m, g);
-      Ops::template load_v<PAST>(v, [&](int j) { return src.v(key0 + j); }, m, g);
+    auto load = [&](typename Ops::K& k, typename Ops::V& v, int key0) {
+      Ops::template load_k<PAST>(k, [&](int j) { return kbase + (int64_t)(key0 + j) * a.kr; }, m, g);
+      Ops::template load_v<PAST>(v, [&](int j) { return vbase + (int64_t)(key0 + j) * a.vr; }, m, g);
     };
-    auto step = [&](const typename Ops::KRaw& k, const typename Ops::VRaw& v) {
+    auto step = [&](const typename Ops::K& k, const typename Ops::V& v) {
       float p[QT][NP];
-      scores(Ops::open_k(k), p);
+      scores(k, p);
       weights(p);
-      Ops::template add_pv<QT>(Ops::open_v(v), p, o);
+      Ops::template add_pv<QT>(v, p, o);
     };
-    typename Ops::KRaw k0, k1;
-    typename Ops::VRaw v0, v1;
+    typename Ops::K k0, k1;
+    typename Ops::V v0, v1;
     if (key + KT <= full) load(k0, v0, key);
     while (key + KT <= full) {
       if (key + 5 * KT <= full) load(k1, v1, key + 4 * KT);
@@ -630,13 +292,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
   // Tiles with tree rows. Keys at or past the end read the last row, at weight 0.
 #pragma unroll 1
   for (; key < hi; key += 4 * KT) {
-    typename Ops::KRaw kraw;
-    typename Ops::VRaw vraw;
-    Ops::template load_k<false>(kraw, [&](int j) { const int r = key + j; return src.k(r < end ? r : end - 1); }, m, g);
-    Ops::template load_v<false>(vraw, [&](int j) { const int r = key + j; return src.v(r < end ? r : end - 1); }, m, g);
-    typename Ops::V v = Ops::open_v(vraw);
+    typename Ops::K k;
+    typename Ops::V v;
+    Ops::template load_k<false>(k, [&](int j) { const int r = key + j; return kbase + (int64_t)(r < end ? r : end - 1) * a.kr; }, m, g);
+    Ops::template load_v<false>(v, [&](int j) { const int r = key + j; return vbase + (int64_t)(r < end ? r : end - 1) * a.vr; }, m, g);
     float p[QT][NP];
-    scores(Ops::open_k(kraw), p);
+    scores(k, p);
 #pragma unroll
     for (int i = 0; i < QT; ++i)
 #pragma unroll
@@ -660,12 +321,12 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
 #pragma unroll 1
       for (int j = 0; j < KT && key + j < hi; ++j) {
         const int t = key + j - n;
-        const auto row = src.v(key + j);
+        const E* row = vbase + (int64_t)(key + j) * a.vr;
 #pragma unroll
         for (int c = 0; c < NDT; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = Ops::Rows::value(row, Ops::dim(c, e, g));
+            const float x = Elem<E>::load(row + Ops::dim(c, e, g));
             if (!__ballot(!(fabsf(x) < INFINITY))) continue;
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
@@ -678,57 +339,8 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(const TreeAttn a, int
     }
   }
 
-  // merge: every wave's outputs relative to the common maximum, summed in wave order
-#pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    l[i] += __shfl_xor(l[i], 16, 64);
-    l[i] += __shfl_xor(l[i], 32, 64);
-    if (g == 0) { merge_ml[wid][16 * i + m][0] = mref[i]; merge_ml[wid][16 * i + m][1] = l[i]; }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    const int r = 16 * i + m;
-    float top = merge_ml[0][r][0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, merge_ml[w][r][0]);
-    const float f = mref[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref[i] - top);
-    float* dst = merge_o + (wid * ROWS + r) * LDO;
-#pragma unroll
-    for (int c = 0; c < NDT; c += 4)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *(f32x4_t*)(dst + Ops::dim(c, e, g)) = f32x4_t{o[i][c][e] * f, o[i][c + 1][e] * f, o[i][c + 2][e] * f, o[i][c + 3][e] * f};
-  }
-  __syncthreads();
-  const bool whole = range.count == 1;
-  for (int it = threadIdx.x; it < ROWS * (D / 4); it += 256) {
-    const int rl = it / (D / 4), d = it % (D / 4) * 4, r = tile * ROWS + rl;
-    if (r >= NR) continue;
-    float top = merge_ml[0][rl][0], sum = 0.f;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, merge_ml[w][rl][0]);
-    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = merge_ml[w][rl][0], lw = merge_ml[w][rl][1];
-      sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - top);   // no maximum: 0, or NaN from NaN scores alone
-      x += *(const f32x4_t*)(merge_o + (w * ROWS + rl) * LDO + d);
-    }
-    if (whole) {
-      const int t = r % T;
-      const bool none = sum == 0.f || merge_pad[rl];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / sum;
-      E* dst = (E*)a.o + ((int64_t)b * T + t) * a.ldo + ((int64_t)h * rep + r / T) * D + d;
-      if constexpr (sizeof(E) == 2) *(u32x2_t*)dst = u32x2_t{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
-      else *(f32x4_t*)dst = x;
-    } else {
-      const int64_t at = ((int64_t)id * a.nk + h) * NR + r;
-      *(f32x4_t*)(a.po + at * D + d) = x;
-      if (d == 0) { a.pm[2 * at] = top; a.pm[2 * at + 1] = sum; }
-    }
-  }
+  tree_merge<E, D, QT>(a, range, tile, h, id, o, mref, l, merge_o, merge_ml, merge_pad,
+                       [](int c, int e, int g) { return Ops::dim(c, e, g); });
 }
 
 // max over lanes l and l ^ 32
@@ -1063,59 +675,6 @@ __global__ __launch_bounds__(RG == 2 ? 256 : 512, 2) void tree_attn_lds_kernel(c
   }
 }
 
-// The ranges of each query row merged: one thread per four dims, grid (.., sequences). Sequences of one range were
-// written by the kernels above. Bound by latency when ranges are many, so eight are read at a time (one at a time: one sequence of
-// 32768 rows 58 us in place of 34, 8 of 4096 rows with 16 nodes 35 in place of 33), and three where that is all there are.
-template <typename E, int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeAttn a) {
-  const int b = blockIdx.y, rep = a.nq / a.nk, NR = rep * a.T;
-  const int2 range = a.table[b];                       // first, count
-  if (range.y <= 1) return;
-  const int it = blockIdx.x * 256 + threadIdx.x, row = it / (D / 4), d = it % (D / 4) * 4;
-  if (row >= a.nk * NR) return;
-  const int h = row / NR, r = row % NR, t = r % a.T;
-  const int64_t at0 = (int64_t)range.x * a.nk * NR + row, step = (int64_t)a.nk * NR;
-  float top = -INFINITY, sum = 0.f;
-  f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-  auto merge = [&](int s0, auto n) {                     // the next n ranges, in flight together
-    constexpr int N = decltype(n)::value;
-    f32x4_t v[N];
-    float2 ml[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t at = at0 + min(s0 + i, range.y - 1) * step;
-      v[i] = *(const f32x4_t*)(a.po + at * D + d);
-      ml[i] = *(const float2*)(a.pm + 2 * at);
-    }
-    float to = top;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (s0 + i >= range.y) ml[i] = make_float2(-INFINITY, 0.f);
-      to = fmaxf(to, ml[i].x);
-    }
-    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - to);   // (without a maximum x is 0, sum 0 or NaN)
-    top = to;
-    sum *= f;
-    x *= f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (ml[i].x == -INFINITY) { sum += ml[i].y; continue; }   // 0, or NaN from NaN scores alone
-      const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
-      sum += ml[i].y * w;
-      x += v[i] * w;
-    }
-  };
-  if (range.y <= 3) merge(0, std::integral_constant<int, 3>{});
-  else
-    for (int s0 = 0; s0 < range.y; s0 += 8) merge(s0, std::integral_constant<int, 8>{});
-  const bool none = sum == 0.f || a.parents[b * a.ldp + t] < -1;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = none ? 0.f : x[e] / sum;
-  E* dst = (E*)a.o + ((int64_t)b * a.T + t) * a.ldo + ((int64_t)h * rep + r / a.T) * D + d;
-  if constexpr (sizeof(E) == 2) *(u32x2_t*)dst = u32x2_t{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
-  else *(f32x4_t*)dst = x;
-}
-
 // Depth of every node: the number of its ancestors (0 for roots and padding). One workgroup per tree.
 __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restrict__ parents, int T, int32_t* depths) {
   __shared__ uint32_t anc[TREE_MAX * TREE_WORDS];
@@ -1127,8 +686,6 @@ __global__ __launch_bounds__(256) void tree_depths_kernel(const int32_t* __restr
   for (int i = 0; i < W; ++i) n += __popc(anc[t * W + i]);
   depths[(int64_t)blockIdx.x * T + t] = n > 0 ? n - 1 : 0;
 }
-
-struct TreePlan { int rows, rt, share; int64_t ranges; };   // rows per row tile; most ranges of all sequences
 
 // The row tile is the least that holds a pair's rows, up to what a workgroup can; K and V are read once per tile.
 // 16: the register walk (one sequence of 1000 rows, one node 9.8 us, with the LDS walk 13.1; 4 sequences of 2000, 32 K/V heads, 16
@@ -1147,108 +704,29 @@ TreePlan tree_plan(int dtype, int B, int T, int nq, int nk, int D, int max_len) 
   return p;
 }
 
-int tree_sizes_ok(const char* what, int B, int T, int nq, int nk, int D, int max_len) {
-  UNOK_REQUIRE(B >= 0 && T >= 0 && nq > 0 && nk > 0 && nq % nk == 0 && max_len >= 1, UNOK_EINVAL,
-               "%s: B=%d T=%d nq=%d nk=%d max_len=%d", what, B, T, nq, nk, max_len);
-  UNOK_REQUIRE(T <= TREE_MAX, UNOK_EUNSUPPORTED, "%s: trees hold at most %d nodes (got %d)", what, TREE_MAX, T);
-  UNOK_REQUIRE(D == 64 || D == 128, UNOK_EINVAL, "%s: head dim %d not in {64,128}", what, D);
-  UNOK_REQUIRE((int64_t)B * nq * (T > 0 ? T : 1) < (1ll << 24) && max_len < (1 << 30) && B * (max_len / TB + 1ll) < (1ll << 30),
-               UNOK_EINVAL, "%s: B=%d T=%d nq=%d max_len=%d exceed the row layout", what, B, T, nq, max_len);
-  return 0;
-}
-
-// Workgroups of a walk: (range, head) units in eights, times the row tiles (see tree_place).
-int64_t tree_blocks(const TreeAttn& a, const TreePlan& p) { return (p.ranges * a.nk + 7) / 8 * 8 * p.rt; }
-
-// Over 4-bit caches.
-TreePlan tree_plan4(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
-  const int NR = nq / nk * T;
-  TreePlan p;
-  p.rows = NR <= 16 ? 16 : 32;
-  p.rt = (NR + p.rows - 1) / p.rows;
-  const int64_t share = 512 / ((int64_t)nk * p.rt);
-  p.share = share > 1 ? (int)share : 1;
-  p.ranges = max_len <= TREE_LEAST * TB ? B : B + p.share;
-  return p;
-}
-
-int64_t plan_workspace(const TreePlan& p, int B, int T, int nq, int D) {
-  return p.ranges == B ? 0 : p.ranges * nq * T * (D + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(int2);
-}
-
-// What both cache formats check and fill in: queries, trees, outputs, workspace. `what` names the entry point.
-int tree_setup(TreeAttn& a, const char* what, const TreePlan& plan, int dtype, int B, int T, int nq, int nk, int D, const void* q,
-               int64_t ldq, int max_len, const int64_t* lengths, const int32_t* parents, int64_t ldp, float scale, void* o,
-               int64_t ldo, void* workspace, int64_t ws_bytes) {
-  UNOK_REQUIRE(q && lengths && parents && o, UNOK_EINVAL, "%s: null operand", what);
-  UNOK_REQUIRE(ldp == 0 || ldp >= T, UNOK_EINVAL, "%s: parents' row stride %lld for %d nodes", what, (long long)ldp, T);
-  const int64_t es = dtype == UNOK_BF16 ? 2 : 4, width = (int64_t)nq * D, rows = (int64_t)B * T;
-  UNOK_REQUIRE(rows == 1 || (ldq >= width && ldo >= width), UNOK_EINVAL, "%s: rows of %lld elements, ldq=%lld ldo=%lld", what,
-               (long long)width, (long long)ldq, (long long)ldo);
-  UNOK_REQUIRE(!unok::rows_overlap(q, ldq * es, o, ldo * es, rows, width * es), UNOK_EINVAL,
-               "%s: the output overlaps the queries", what);
-  const float scale_log2 = scale * 1.4426950408889634f;
-  UNOK_REQUIRE(scale_log2 - scale_log2 == 0.f, UNOK_EINVAL, "%s: scale %g must be finite", what, (double)scale);
-  const int per16 = dtype == UNOK_BF16 ? 8 : 4;
-  UNOK_REQUIRE((((uintptr_t)q | (uintptr_t)o) & 15) == 0 && ldq % per16 == 0 && ldo % per16 == 0, UNOK_EALIGN,
-               "%s: queries and outputs and their strides must be multiples of 16 bytes", what);
-  const int64_t need = plan_workspace(plan, B, T, nq, D);
-  UNOK_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0), UNOK_EINVAL,
-               "%s: workspace of %lld bytes (16-byte aligned) required, got %lld", what, (long long)need, (long long)ws_bytes);
-  a.q = q; a.ldq = ldq;
-  a.lengths = lengths; a.parents = parents; a.ldp = ldp;
-  a.B = B; a.T = T; a.nq = nq; a.nk = nk; a.max_len = max_len;
-  a.rt = plan.rt;
-  a.share = plan.share;
-  a.o = o; a.ldo = ldo;
-  a.po = (float*)workspace;
-  a.pm = a.po + plan.ranges * nq * T * D;
-  a.table = plan.ranges > B ? (int2*)(a.pm + plan.ranges * nq * T * 2) : nullptr;
-  a.scale_log2 = scale_log2;
-  a.walk_scale = scale_log2 > 0.f ? scale_log2 : scale_log2 < 0.f ? -scale_log2 : 1.f;
-  a.q_factor = scale_log2 > 0.f ? 1.f : scale_log2 < 0.f ? -1.f : 0.f;
-  UNOK_REQUIRE(tree_blocks(a, plan) < (1ll << 31) && B < 65536, UNOK_EINVAL, "%s: grid too large", what);
-  return 0;
-}
-
-template <typename E, typename Ops, int D, int QT> void launch_registers(const TreeAttn& a, int64_t nb, int row_bytes, hipStream_t st) {
-  constexpr size_t lds = 4ull * 16 * QT * (D + 4) * sizeof(float);
-  UNOK_SET_LDS_ONCE((tree_attn_kernel<E, Ops, D, QT>), lds);
-  hipLaunchKernelGGL((tree_attn_kernel<E, Ops, D, QT>), dim3((unsigned)nb), dim3(256), lds, st, a, row_bytes);
-}
-template <int D, int RG> void launch_lds(const TreeAttn& a, int64_t nb, hipStream_t st) {
-  constexpr size_t lds = (RG == 2 ? 128ull : 256ull) * 2 * D * sizeof(bf16_t);   // all stages' keys
-  UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<D, RG>), lds);
-  hipLaunchKernelGGL((tree_attn_lds_kernel<D, RG>), dim3((unsigned)nb), dim3(RG == 2 ? 256 : 512), lds, st, a);
-}
-template <typename E, int D> void launch_combine(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
-  if (plan.ranges > a.B)
-    hipLaunchKernelGGL((tree_combine_kernel<E, D>), dim3((unsigned)(((int64_t)a.nq * a.T * (D / 4) + 255) / 256), (unsigned)a.B),
-                       dim3(256), 0, st, a);
-}
-
 template <typename E, int D> void launch_tree(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
-  const int64_t nb = tree_blocks(a, plan);
-  using Ops = TileOps<E, D>;
-  constexpr int bytes = D * (int)sizeof(E);
+  const dim3 grid((unsigned)tree_blocks(a, plan));
+  auto registers = [&](auto t) {
+    constexpr int QT = decltype(t)::value;
+    constexpr size_t lds = 4ull * 16 * QT * (D + 4) * sizeof(float);
+    UNOK_SET_LDS_ONCE((tree_attn_kernel<E, D, QT>), lds);
+    hipLaunchKernelGGL((tree_attn_kernel<E, D, QT>), grid, dim3(256), lds, st, a);
+  };
   if (plan.rows == 16) {
-    launch_registers<E, Ops, D, 1>(a, nb, bytes, st);
+    registers(std::integral_constant<int, 1>{});
   } else if constexpr (sizeof(E) == 4) {
-    launch_registers<E, Ops, D, 2>(a, nb, bytes, st);
+    registers(std::integral_constant<int, 2>{});
   } else {
-    if (plan.rows == 64) launch_lds<D, 2>(a, nb, st);
-    else if (plan.rows == 128) launch_lds<D, 4>(a, nb, st);
-    else if constexpr (D == 128) launch_lds<D, 8>(a, nb, st);
+    auto tiles = [&](auto g) {
+      constexpr int RG = decltype(g)::value;
+      constexpr size_t lds = (RG == 2 ? 128ull : 256ull) * 2 * D * sizeof(bf16_t);   // all stages' keys
+      UNOK_SET_LDS_ONCE((tree_attn_lds_kernel<D, RG>), lds);
+      hipLaunchKernelGGL((tree_attn_lds_kernel<D, RG>), grid, dim3(RG == 2 ? 256 : 512), lds, st, a);
+    };
+    if (plan.rows == 64) tiles(std::integral_constant<int, 2>{});
+    else if (plan.rows == 128) tiles(std::integral_constant<int, 4>{});
+    else if constexpr (D == 128) tiles(std::integral_constant<int, 8>{});
   }
-  launch_combine<E, D>(a, plan, st);
-}
-
-template <typename E, int D> void launch_tree4(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
-  const int64_t nb = tree_blocks(a, plan);
-  using Ops = TileOps4<E, D>;
-  constexpr int bytes = D / 2 + D / GROUP4;
-  if (plan.rows == 16) launch_registers<E, Ops, D, 1>(a, nb, bytes, st);
-  else launch_registers<E, Ops, D, 2>(a, nb, bytes, st);
   launch_combine<E, D>(a, plan, st);
 }
 
@@ -1286,36 +764,6 @@ UNOK_EXPORT int unok_tree_attn(int dtype, int B, int T, int nq, int nk, int D, c
   if (dtype == UNOK_BF16) D == 128 ? launch_tree<bf16_t, 128>(a, plan, st) : launch_tree<bf16_t, 64>(a, plan, st);
   else D == 128 ? launch_tree<float, 128>(a, plan, st) : launch_tree<float, 64>(a, plan, st);
   return unok::check_launch("tree_attn");
-}
-
-UNOK_EXPORT int64_t unok_tree_attn4_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
-  if (tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len)) return -1;
-  if (B == 0 || T == 0) return 0;
-  return plan_workspace(tree_plan4(dtype, B, T, nq, nk, D, max_len), B, T, nq, D);
-}
-
-UNOK_EXPORT int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
-                                const void* k_scales, const void* v, const void* v_scales, int max_len, const int64_t* lengths,
-                                const int32_t* parents, int64_t ldp, float scale, void* o, int64_t ldo, void* workspace,
-                                int64_t ws_bytes, void* stream) {
-  int rc = tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len);
-  if (rc) return rc;
-  UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn4: bad dtype %d", dtype);
-  if (B == 0 || T == 0) return 0;
-  UNOK_REQUIRE(k && v && k_scales && v_scales, UNOK_EINVAL, "tree_attn4: null operand");
-  UNOK_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) == 0, UNOK_EALIGN,
-               "tree_attn4: codes and scales must be 16-byte aligned");
-  const TreePlan plan = tree_plan4(dtype, B, T, nq, nk, D, max_len);
-  TreeAttn a{};
-  a.k = k; a.v = v;
-  a.ks = (const uint8_t*)k_scales; a.vs = (const uint8_t*)v_scales;
-  rc = tree_setup(a, "tree_attn4", plan, dtype, B, T, nq, nk, D, q, ldq, max_len, lengths, parents, ldp, scale, o, ldo, workspace,
-                  ws_bytes);
-  if (rc) return rc;
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == UNOK_BF16) D == 128 ? launch_tree4<bf16_t, 128>(a, plan, st) : launch_tree4<bf16_t, 64>(a, plan, st);
-  else D == 128 ? launch_tree4<float, 128>(a, plan, st) : launch_tree4<float, 64>(a, plan, st);
-  return unok::check_launch("tree_attn4");
 }
 
 UNOK_EXPORT int unok_tree_depths(int B, int T, const int32_t* parents, int32_t* depths, void* stream) {

@@ -1,0 +1,424 @@
+// Attention of a tree of drafted tokens over a KV cache in 4 bits: tree.hip's operator over rows as cache4.h describes them.
+//
+// The numbers of a 4-bit row are exact in bf16, so the products are bf16 ones, and the conversion is one instruction for two elements
+// and their scale. A wave loads codes from memory into registers, converts them there, and keeps 16 QT query rows: no LDS and no barrier
+// in the walk. (A walk that shares converted tiles through LDS, as the bf16 cache's does, spends its time on LDS reads of numbers four
+// times as large as their codes: 16 sequences, 64 nodes of 32 / 8 heads of 128 over 16384 rows 418 us.)
+//
+// fp32 queries: a query is the sum of three bf16 numbers (each what the ones before it leave, 8 of its 24 bits), and so is a weight;
+// three products take the place of one, exact but for their sums.
+#include "tree.h"
+#include "cache4.h"
+#include "../../include/unok.h"
+#include <stdlib.h>
+
+namespace {
+
+// Rows of K and V of one (sequence, K/V head) pair, loaded through buffers that end behind the last row: what lies past it reads as
+// zeros, and a lane's place in a tile is one offset for all tiles.
+struct Buffer4 {
+  __amdgpu_buffer_rsrc_t codes, scales;
+};
+template <int D> __device__ __forceinline__ Buffer4 buffer4(const void* codes, const uint8_t* scales, int64_t row, int rows) {
+  auto make = [&](const uint8_t* p, int bytes) {
+    const uintptr_t at = (uintptr_t)(p + row * bytes);
+    const uintptr_t u = ((uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, __builtin_amdgcn_readfirstlane(rows) * bytes, 0x00020000);
+  };
+  return {make((const uint8_t*)codes, D / 2), make(scales, D / GROUP4)};
+}
+
+// Tiles of 32 keys: codes and scales go from memory straight into LDS, NST - 1 tiles ahead, each wave's into its own part, so that
+// nothing but the wave's own counter of loads is waited for. (Two tiles in registers, one of them on its way: 16 sequences, 64 nodes over
+// 16384 rows 309 us.) A stage: K's codes, V's codes, a dword to a key for its scales of K, and of V. A lane (m, g), m < 16, g < 4, reads
+//   K (S^T = K Q^T, first operand: 16 keys x 8 dims a lane): the dims of a product may come in any order that Q takes too; lane group g
+//     has dims D/4 g .. of key m and of key 16 + m: one read each, of one scale;
+//   V (O^T = V^T P^T, first operand: one dim x 8 keys): lane m has dims D/16 m .. of keys 4 g .. + 3 and 16 + 4 g .. + 3, which are
+//     those of its accumulators of S^T. Row 4 g + j of each 16 lies at place 4 j + g, so that the four rows read together are in
+//     different banks. Four keys' scales are one read, and a rotation brings the byte of the lane's dims into the exponent (the
+//     conversions read no other bit).
+template <int D> struct Tile4 {
+  static constexpr int KT = 32, KS = D / 32, NDT = D / 16, CR = D / 2, SR = D / GROUP4, NST = 3;
+  static constexpr int CODES = KT * CR, SCALES = 256, STAGE = 2 * CODES + 2 * SCALES, LOADS = 2 * CODES / 1024 + 2;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  typedef std::conditional_t<D == 128, u4, u2> KCodes;
+  KCodes k[2];
+  uint32_t ks[2], v[8];
+  u4 vs[2];
+
+  // The wave's loads of the tile at `key` into a stage; lane offsets as `places` gives them.
+  static __device__ __forceinline__ int2 places(int lane) {
+    const int place = lane * 16 / CR, q = place % 16, row = place / 16 * 16 + 4 * (q % 4) + q / 4;
+    return make_int2(lane * 16, row * CR + lane * 16 % CR);
+  }
+  static __device__ __forceinline__ void issue(const Buffer4& kb, const Buffer4& vb, int key, int2 at, int lane, char* stage) {
+    typedef __attribute__((address_space(3))) void* Lds;
+#pragma unroll
+    for (int i = 0; i < CODES / 1024; ++i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.codes, (Lds)(stage + 1024 * i), 16, at.x, key * CR + 1024 * i, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.codes, (Lds)(stage + CODES + 1024 * i), 16, at.y, key * CR + 1024 * i, 0, 0);
+    }
+    const Lds kx = (Lds)(stage + 2 * CODES), vx = (Lds)(stage + 2 * CODES + SCALES);
+    if constexpr (D == 128) {                            // (the size has to be a literal)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.scales, kx, 4, lane * SR, key * SR, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.scales, vx, 4, lane * SR, key * SR, 0, 0);
+    } else {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.scales, kx, 2, lane * SR, key * SR, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.scales, vx, 2, lane * SR, key * SR, 0, 0);
+    }
+  }
+  // Reads the stage at LDS address `at` once its loads have arrived (the later tiles' may be on their way; the compiler, which cannot
+  // tell the stages apart, would wait for those too).
+  __device__ __forceinline__ void read(uint32_t at, int m, int g) {
+    const uint32_t ka = at + m * CR + CR / 4 * g, kx = at + 2 * CODES + 4 * m + D / 4 * g / GROUP4;
+    const uint32_t va = at + CODES + g * CR + NDT / 2 * m, vx = at + 2 * CODES + SCALES + 16 * g;
+    if constexpr (D == 128) {
+      u2 a, b, c, d;
+      asm volatile(
+          "s_waitcnt vmcnt(%14)\n\t"
+          "ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:1024\n\t"
+          "ds_read_u8 %2, %11\n\tds_read_u8 %3, %11 offset:64\n\t"
+          "ds_read2st64_b32 %4, %12 offset0:0 offset1:1\n\tds_read2st64_b32 %5, %12 offset0:2 offset1:3\n\t"
+          "ds_read2st64_b32 %6, %12 offset0:4 offset1:5\n\tds_read2st64_b32 %7, %12 offset0:6 offset1:7\n\t"
+          "ds_read_b128 %8, %13\n\tds_read_b128 %9, %13 offset:64\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(k[0]), "=&v"(k[1]), "=&v"(ks[0]), "=&v"(ks[1]), "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(vs[0]), "=&v"(vs[1])
+          : "v"(ka), "v"(kx), "v"(va), "v"(vx), "i"((NST - 1) * LOADS)
+          : "memory");
+      v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+      v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
+    } else {
+      asm volatile(
+          "s_waitcnt vmcnt(%18)\n\t"
+          "ds_read_b64 %0, %14\n\tds_read_b64 %1, %14 offset:512\n\t"
+          "ds_read_u8 %2, %15\n\tds_read_u8 %3, %15 offset:64\n\t"
+          "ds_read_u16 %4, %16\n\tds_read_u16 %5, %16 offset:128\n\tds_read_u16 %6, %16 offset:256\n\t"
+          "ds_read_u16 %7, %16 offset:384\n\tds_read_u16 %8, %16 offset:512\n\tds_read_u16 %9, %16 offset:640\n\t"
+          "ds_read_u16 %10, %16 offset:768\n\tds_read_u16 %11, %16 offset:896\n\t"
+          "ds_read_b128 %12, %17\n\tds_read_b128 %13, %17 offset:64\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(k[0]), "=&v"(k[1]), "=&v"(ks[0]), "=&v"(ks[1]), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]),
+            "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(vs[0]), "=&v"(vs[1])
+          : "v"(ka), "v"(kx), "v"(va), "v"(vx), "i"((NST - 1) * LOADS)
+          : "memory");
+    }
+  }
+  // Key j's scale of V for the conversions (more than its exponent bits may be set), and its byte.
+  static __device__ __forceinline__ int group(int m) { return NDT * m / GROUP4; }
+  __device__ __forceinline__ float v_scale(int j, int m) const {
+    return __uint_as_float(__builtin_amdgcn_alignbit(vs[j / 4][j % 4], vs[j / 4][j % 4], (8 * group(m) + 9) & 31));
+  }
+  __device__ __forceinline__ uint32_t v_byte(int j, int m) const { return vs[j / 4][j % 4] >> (8 * group(m)) & 255; }
+  __device__ __forceinline__ static int slot_key(int j, int g) { return j < 4 ? 4 * g + j : 12 + 4 * g + j; }
+};
+
+// Eight elements of codes as a product's operand.
+__device__ __forceinline__ bf16x8_t eight4(uint32_t codes, float scale) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(bf16x8_t, u4{pair4<0>(codes, scale), pair4<1>(codes, scale), pair4<2>(codes, scale), pair4<3>(codes, scale)});
+}
+template <int I> __device__ __forceinline__ uint32_t pair_at(uint32_t codes, float scale) { return pair4<I>(codes, scale); }
+
+template <typename E, int D, int QT>
+__global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_attn4_kernel(const TreeAttn a) {
+  using Tile = Tile4<D>;
+  constexpr int KT = Tile::KT, KS = Tile::KS, NDT = Tile::NDT, ROWS = 16 * QT, PARTS = sizeof(E) == 4 ? 3 : 1;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  extern __shared__ __attribute__((aligned(1024))) char lds[];          // the waves' stages; at the end [4][ROWS][D + 4] floats
+  __shared__ float merge_ml[4][ROWS][2];
+  __shared__ bool merge_pad[ROWS];
+  __shared__ uint32_t anc[TREE_MAX * TREE_WORDS];
+  __shared__ int next[TREE_MAX];
+
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+  const int rep = a.nq / a.nk, T = a.T, NR = rep * T;
+  int tile, h, id;
+  tree_place(a, tile, h, id);
+  const Range range = tree_range(a, id, Tile::CR + Tile::SR);
+  if (range.b < 0 || range.lo >= range.hi) return;
+  const int b = range.b, n = range.n, lo = range.lo, hi = range.hi;
+  tree_note(a, range, id, h, tile);
+
+  // from the range's first row on: the buffers' offsets are 32-bit
+  const int64_t row0 = ((int64_t)b * a.nk + h) * a.max_len + lo;
+  const Buffer4 kb = buffer4<D>(a.k, a.ks, row0, hi - lo), vb = buffer4<D>(a.v, a.vs, row0, hi - lo);
+  const int full = min(hi, n) - lo, all = hi - lo;       // committed rows, which every query sees, and rows, of this range
+  char* const mine = lds + wid * Tile::NST * Tile::STAGE;
+  const int2 place = Tile::places(lane);
+  int key = wid * KT, stage = 0;
+#pragma unroll
+  for (int i = 0; i < Tile::NST; ++i) Tile::issue(kb, vb, key + 4 * i * KT, place, lane, mine + i * Tile::STAGE);
+
+  if (hi > n) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
+  const int W = (T + 31) / 32;
+
+  // this lane's query of each 16-row subtile (rows past the pair's last repeat it; their results are dropped)
+  bf16x8_t q[QT][PARTS][KS];
+  int node[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const int r = tile * ROWS + 16 * i + m, rc = r < NR ? r : NR - 1;
+    node[i] = rc % T;
+    const E* row = (const E*)a.q + ((int64_t)b * T + node[i]) * a.ldq + ((int64_t)h * rep + rc / T) * D + D / 4 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (PARTS == 1) {
+        q[i][0][s] = *(const bf16x8_t*)(row + 8 * s);
+        if (a.q_factor != 1.f) q[i][0][s] *= (__bf16)a.q_factor;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = row[8 * s + e] * a.q_factor;
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            const uint32_t u = __float_as_uint(x) & 0xffff0000u;
+            x -= __uint_as_float(u);
+            q[i][p][s][e] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
+          }
+        }
+      }
+    }
+    if (threadIdx.x < 16) merge_pad[16 * i + m] = a.parents[b * a.ldp + node[i]] < -1;
+  }
+  f32x4_t o[QT][NDT];
+  float mref[QT], l[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    mref[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NDT; ++c) o[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto scores = [&](const Tile& t, f32x4_t (&s)[QT][2]) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float f = scale4(t.ks[x]);
+#pragma unroll
+      for (int i = 0; i < QT; ++i) s[i][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const bf16x8_t kf = eight4(t.k[x][k], f);
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p)               // small parts first
+#pragma unroll
+          for (int i = 0; i < QT; ++i) s[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i][p][k], s[i][x], 0, 0, 0);
+      }
+    }
+  };
+  // Scores become weights; the reference moves only where one exceeds it by 2^8 (see tree.hip).
+  auto weights = [&](f32x4_t (&s)[QT][2], float (&p)[QT][8]) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      // (a maximum that NaN passes through: a row with a NaN score is NaN whatever its reference)
+      float mx = s[i][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx = __builtin_elementwise_maximum(mx, s[i][j / 4][j % 4]);
+      mx *= a.walk_scale;
+      if (__ballot(mx > mref[i] + 8.f)) {
+        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 16, 64));
+        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+        // (for the queries that need it alone: a row's result does not depend on the rows beside it)
+        const float to = mx > mref[i] + 8.f ? mx : mref[i];
+        const float f = to == mref[i] ? 1.f : mref[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref[i] - to);
+        mref[i] = to;
+        l[i] *= f;
+#pragma unroll
+        for (int c = 0; c < NDT; ++c) o[i][c] *= f;
+      }
+      const float ref = mref[i] == -INFINITY ? 0.f : -mref[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j / 4][j % 4], a.walk_scale, ref));
+        l[i] += p[i][j];
+      }
+    }
+  };
+  // Keys in pairs: two dims of eight keys become, by a permute to a dim and pair, two operands.
+  auto add_pv = [&](const Tile& t, const float (&vf)[8], float (&p)[QT][8]) {
+    bf16x8_t pf[QT][PARTS];
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        u4 u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (PARTS == 1) u[j] = pack2_bf16(p[i][2 * j], p[i][2 * j + 1]);
+          else {
+            const uint32_t x = __float_as_uint(p[i][2 * j]) & 0xffff0000u, y = __float_as_uint(p[i][2 * j + 1]) & 0xffff0000u;
+            p[i][2 * j] -= __uint_as_float(x);
+            p[i][2 * j + 1] -= __uint_as_float(y);
+            u[j] = x >> 16 | y;
+          }
+        }
+        pf[i][part] = __builtin_bit_cast(bf16x8_t, u);
+      }
+    auto dims = [&](auto pair) {
+      constexpr int C = decltype(pair)::value;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = pair_at<C>(t.v[j], vf[j]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        u4 u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], c ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+          for (int i = 0; i < QT; ++i)
+            o[i][2 * C + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, u), pf[i][part], o[i][2 * C + c], 0, 0, 0);
+      }
+    };
+    dims(std::integral_constant<int, 0>{});
+    dims(std::integral_constant<int, 1>{});
+    if constexpr (D == 128) {
+      dims(std::integral_constant<int, 2>{});
+      dims(std::integral_constant<int, 3>{});
+    }
+  };
+
+  const uint32_t at = lds_addr(mine);
+  auto next_tile = [&] {                                  // its stage gets the tile NST behind it (zeros past the end)
+    Tile::issue(kb, vb, key + 4 * Tile::NST * KT, place, lane, mine + stage * Tile::STAGE);
+    key += 4 * KT;
+    stage = stage + 1 < Tile::NST ? stage + 1 : 0;
+  };
+  // Tiles of committed rows.
+#pragma unroll 1
+  while (key + KT <= full) {
+    Tile t;
+    t.read(at + stage * Tile::STAGE, m, g);
+    f32x4_t s[QT][2];
+    float p[QT][8], vf[8];
+    scores(t, s);
+    weights(s, p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vf[j] = t.v_scale(j, m);
+    add_pv(t, vf, p);
+    next_tile();
+  }
+  // Tiles with tree rows, and rows at or past hi, which read as zeros, at weight 0.
+#pragma unroll 1
+  while (key < all) {
+    Tile t;
+    t.read(at + stage * Tile::STAGE, m, g);
+    f32x4_t s[QT][2];
+    float p[QT][8], vf[8];
+    scores(t, s);
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = key + Tile::slot_key(j, g), x = r + lo - n;
+        s[i][j / 4][j % 4] = r < all && ((x < 0) | tree_sees(anc, node[i], W, x)) ? s[i][j / 4][j % 4] : -INFINITY;
+      }
+    weights(s, p);
+    // A scale of NaN, or one too large for numbers, in a row that some queries do not see: 0 in the product, and added where it is
+    // seen. The weights go through the tile's stage, 16 rows at a time.
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t byte = t.v_byte(j, m);
+      odd |= byte > SCALE4_MAX;
+      vf[j] = scale4(byte > SCALE4_MAX ? 0 : byte);
+    }
+    odd = __ballot(odd) != 0;
+    if (odd) {
+      float* ps = (float*)(mine + stage * Tile::STAGE);
+      static_assert(16 * (KT + 1) * 4 <= Tile::STAGE, "the weights of 16 rows fit in a stage");
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ps[m * (KT + 1) + Tile::slot_key(j, g)] = p[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int j = 0; j < KT && key + j < all; ++j) {
+          const int x = key + j + lo - n;
+          const bool seen = (x < 0) | tree_sees(anc, node[i], W, x);
+          const int64_t r = row0 + key + j;
+          const Row4 row{(const uint8_t*)a.v + r * Tile::CR, a.vs + r * Tile::SR};
+          const float w = ps[m * (KT + 1) + j];
+#pragma unroll
+          for (int c = 0; c < NDT; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = (4 * g + e) * NDT + c;
+              if (seen && row.scales[d / GROUP4] > SCALE4_MAX) o[i][c][e] += w * value4(row, d);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    add_pv(t, vf, p);
+    next_tile();
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // no load is on its way into what becomes the merge's
+  tree_merge<E, D, QT>(a, range, tile, h, id, o, mref, l, (float*)lds, merge_ml, merge_pad,
+                       [](int c, int e, int g) { return (4 * g + e) * NDT + c; });
+}
+
+// Query rows of a workgroup, and one round of workgroups.
+TreePlan tree_plan4(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
+  const int NR = nq / nk * T;
+  TreePlan p;
+  p.rows = NR <= 16 ? 16 : NR <= 32 || dtype == UNOK_F32 ? 32 : 64;
+  if (getenv("W2") && p.rows == 64) p.rows = 32;
+  p.rt = (NR + p.rows - 1) / p.rows;
+  const int64_t share = (p.rows > 32 || dtype == UNOK_F32 ? 256 : 512) / ((int64_t)nk * p.rt);
+  p.share = share > 1 ? (int)share : 1;
+  p.ranges = max_len <= TREE_LEAST * TB ? B : B + p.share;
+  return p;
+}
+
+template <typename E, int D> void launch_tree4(const TreeAttn& a, const TreePlan& plan, hipStream_t st) {
+  const dim3 grid((unsigned)tree_blocks(a, plan));
+  auto walk = [&](auto t) {
+    constexpr int QT = decltype(t)::value;
+    constexpr size_t merge = 4ull * 16 * QT * (D + 4) * sizeof(float), stages = 4ull * Tile4<D>::NST * Tile4<D>::STAGE;
+    constexpr size_t lds = merge > stages ? merge : stages;
+    UNOK_SET_LDS_ONCE((tree_attn4_kernel<E, D, QT>), lds);
+    hipLaunchKernelGGL((tree_attn4_kernel<E, D, QT>), grid, dim3(256), lds, st, a);
+  };
+  if (plan.rows == 16) walk(std::integral_constant<int, 1>{});
+  else if (plan.rows == 32) walk(std::integral_constant<int, 2>{});
+  else if constexpr (sizeof(E) == 2) walk(std::integral_constant<int, 4>{});
+  launch_combine<E, D>(a, plan, st);
+}
+
+}  // namespace
+
+UNOK_EXPORT int64_t unok_tree_attn4_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
+  if (tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len)) return -1;
+  if (B == 0 || T == 0) return 0;
+  return plan_workspace(tree_plan4(dtype, B, T, nq, nk, D, max_len), B, T, nq, D);
+}
+
+UNOK_EXPORT int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, const void* q, int64_t ldq, const void* k,
+                                const void* k_scales, const void* v, const void* v_scales, int max_len, const int64_t* lengths,
+                                const int32_t* parents, int64_t ldp, float scale, void* o, int64_t ldo, void* workspace,
+                                int64_t ws_bytes, void* stream) {
+  int rc = tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len);
+  if (rc) return rc;
+  UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn4: bad dtype %d", dtype);
+  UNOK_REQUIRE(max_len <= 1 << 24, UNOK_EINVAL, "tree_attn4: caches hold at most 2^24 rows (got %d)", max_len);
+  if (B == 0 || T == 0) return 0;
+  UNOK_REQUIRE(k && v && k_scales && v_scales, UNOK_EINVAL, "tree_attn4: null operand");
+  UNOK_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) == 0, UNOK_EALIGN,
+               "tree_attn4: codes and scales must be 16-byte aligned");
+  const TreePlan plan = tree_plan4(dtype, B, T, nq, nk, D, max_len);
+  TreeAttn a{};
+  a.k = k; a.v = v;
+  a.ks = (const uint8_t*)k_scales; a.vs = (const uint8_t*)v_scales;
+  rc = tree_setup(a, "tree_attn4", plan, dtype, B, T, nq, nk, D, q, ldq, max_len, lengths, parents, ldp, scale, o, ldo, workspace,
+                  ws_bytes);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == UNOK_BF16) D == 128 ? launch_tree4<bf16_t, 128>(a, plan, st) : launch_tree4<bf16_t, 64>(a, plan, st);
+  else D == 128 ? launch_tree4<float, 128>(a, plan, st) : launch_tree4<float, 64>(a, plan, st);
+  return unok::check_launch("tree_attn4");
+}

@@ -586,9 +586,9 @@ def decode_maps(lengths, B: int, L: int, nq: int, nk: int, max_len: int, S: int)
 # ------------------------------------------------------------------------------------------
 def _same_device(what: str, *tensors: torch.Tensor) -> None:
     """The operands lie on the current device, whose current stream the kernels are enqueued on."""
-    dev = torch.cuda.current_device() if tensors and tensors[0].is_cuda else None
+    dev = torch._C._cuda_getDevice() if tensors and tensors[0].is_cuda else None
     for t in tensors:
-        if not t.is_cuda or t.device.index != dev:
+        if t.get_device() != dev:                        # (-1 for a host tensor)
             raise RuntimeError(f"{what}: operands must be on the current device, got {t.device}")
 
 
@@ -640,7 +640,7 @@ def _tree_operands(what: str, q: torch.Tensor, B: int, nk: int, D: int, lengths:
 
 def _tree_out(what: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        return q.new_empty(q.shape)
     _rowmajor(out, "out")
     if out.shape != q.shape or out.dtype != q.dtype:
         raise RuntimeError(f"{what}: out must have the shape and dtype of q")
@@ -767,13 +767,19 @@ class Rows4(NamedTuple):
 
 def _check_caches4(what: str, caches: Sequence[Rows4]) -> tuple[int, int, int, int]:
     """4-bit caches of one shape; returns (B, nk, max_len, D)."""
-    c = _check_caches(what, [x.codes for x in caches])
-    s = _check_caches(what, [x.scales for x in caches])
-    B, nk, max_len, half = c.shape
-    if c.dtype != torch.uint8 or s.dtype != torch.uint8 or half not in (32, 64) or s.shape != (B, nk, max_len, half // 16):
+    if not caches:
+        raise RuntimeError(f"{what}: no cache tensors")
+    first, fscales = caches[0]
+    shape, sshape = first.shape, fscales.shape
+    if len(shape) != 4 or shape[3] not in (32, 64) or sshape != (*shape[:3], shape[3] // 16):
         raise RuntimeError(f"{what}: uint8 codes [B, nk, max_len, D/2] and scales [B, nk, max_len, D/32] of D 64 or 128 required, "
-                           f"got {c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
-    return B, nk, max_len, 2 * half
+                           f"got {tuple(shape)} and {tuple(sshape)}")
+    for c, s in caches:
+        if c.dtype != torch.uint8 or s.dtype != torch.uint8 or not c.is_contiguous() or not s.is_contiguous() \
+                or (c is not first and (c.shape != shape or s.shape != sshape)) or (s is not fscales and s.shape != sshape):
+            raise RuntimeError(f"{what}: caches must be contiguous uint8 codes {tuple(shape)} and scales {tuple(sshape)}, got "
+                               f"{c.dtype} {tuple(c.shape)} and {s.dtype} {tuple(s.shape)}")
+    return shape[0], shape[1], shape[2], 2 * shape[3]
 
 
 def cache4_store(rows: Sequence[torch.Tensor], caches: Sequence[Rows4], starts: torch.Tensor) -> None:
@@ -783,16 +789,21 @@ def cache4_store(rows: Sequence[torch.Tensor], caches: Sequence[Rows4], starts: 
         raise RuntimeError(f"cache4_store: {len(rows)} tensors for {len(caches)} caches")
     B, nk, max_len, D = _check_caches4("cache4_store", caches)
     _int64_vector("cache4_store", "starts", starts, B)
+    shape, dtype = rows[0].shape, rows[0].dtype
     for x in rows:
         _rowmajor(x, "cache4_store: rows")
-        if x.shape != rows[0].shape or x.dtype != rows[0].dtype or x.shape[1] != nk * D or (x.shape[0] % B if B else x.shape[0]):
-            raise RuntimeError(f"cache4_store: rows must be [{B} * T, {nk * D}] of one type, got {x.dtype} {tuple(x.shape)}")
-    _same_device("cache4_store", starts, *rows, *(t for c in caches for t in c))
-    T = rows[0].shape[0] // B if B else 0
+        if x.shape != shape or x.dtype != dtype:
+            raise RuntimeError(f"cache4_store: rows must be of one shape and type, got {dtype} {tuple(shape)} and {x.dtype} "
+                               f"{tuple(x.shape)}")
+    M, width = shape
+    if width != nk * D or (M % B if B else M):
+        raise RuntimeError(f"cache4_store: rows must be [{B} * T, {nk * D}], got {tuple(shape)}")
+    codes, scales = [c.codes for c in caches], [c.scales for c in caches]
+    _same_device("cache4_store", starts, *rows, *codes, *scales)
+    T = M // B if B else 0
     _sizes("cache4_store", B, T, nk, max_len)
-    N.call("unok_cache4_store", N.dtype_code(rows[0].dtype), len(rows), N.ptr_array(rows), N.int64_array([_ld(x) for x in rows]),
-           N.ptr_array([c.codes for c in caches]), N.ptr_array([c.scales for c in caches]), B, T, nk, D, max_len, N.ptr(starts),
-           N.stream())
+    N.call("unok_cache4_store", N.dtype_code(dtype), len(rows), N.ptr_array(rows), N.int64_array([_ld(x) for x in rows]),
+           N.ptr_array(codes), N.ptr_array(scales), B, T, nk, D, max_len, N.ptr(starts), N.stream())
 
 
 def cache4_load(caches: Sequence[Rows4], starts: torch.Tensor, T: int, dtype: torch.dtype = torch.bfloat16) -> list[torch.Tensor]:
@@ -804,11 +815,11 @@ def cache4_load(caches: Sequence[Rows4], starts: torch.Tensor, T: int, dtype: to
     if T < 0:
         raise ValueError(f"cache4_load: {T} rows")
     _sizes("cache4_load", B, T, nk, max_len)
-    _same_device("cache4_load", starts, *(t for c in caches for t in c))
-    rows = [torch.empty((B * T, nk * D), device=starts.device, dtype=dtype) for _ in caches]
-    N.call("unok_cache4_load", code, len(rows), N.ptr_array(rows), N.int64_array([nk * D] * len(rows)),
-           N.ptr_array([c.codes for c in caches]), N.ptr_array([c.scales for c in caches]), B, T, nk, D, max_len, N.ptr(starts),
-           N.stream())
+    codes, scales = [c.codes for c in caches], [c.scales for c in caches]
+    _same_device("cache4_load", starts, *codes, *scales)
+    rows = [starts.new_empty((B * T, nk * D), dtype=dtype) for _ in caches]
+    N.call("unok_cache4_load", code, len(rows), N.ptr_array(rows), N.int64_array([nk * D] * len(rows)), N.ptr_array(codes),
+           N.ptr_array(scales), B, T, nk, D, max_len, N.ptr(starts), N.stream())
     return rows
 
 
@@ -823,7 +834,7 @@ def tree_attn4(q: torch.Tensor, k: Rows4, v: Rows4, lengths: torch.Tensor, paren
     _sizes("tree_attn4", B, T, nq, max_len)
     code = N.dtype_code(q.dtype)
     nbytes = N.lib().unok_tree_attn4_workspace(code, B, T, nq, nk, D, max_len)
-    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
     N.call("unok_tree_attn4", code, B, T, nq, nk, D, N.ptr(q), _ld(q), N.ptr(k.codes), N.ptr(k.scales), N.ptr(v.codes),
            N.ptr(v.scales), max_len, N.ptr(lengths), N.ptr(parents), ldp, float(D ** -0.5 if scale is None else scale), N.ptr(out),
            _ld(out), N.ptr(ws), max(nbytes, 0), N.stream())
@@ -880,10 +891,10 @@ def verify_draft(logits: torch.Tensor, draft_logits: torch.Tensor | None, tokens
     if counts is not None:
         _int64_vector("verify_draft", "counts", counts, B)
     _same_device("verify_draft", logits, tokens, u, *(t for t in (draft_logits, counts, temps) if t is not None))
-    V, code, dev = logits.shape[1], N.dtype_code(logits.dtype), logits.device
-    accepted, token = (torch.empty(B, device=dev, dtype=torch.int64) for _ in range(2))
+    V, code = logits.shape[1], N.dtype_code(logits.dtype)
+    accepted, token = tokens.new_empty(B), tokens.new_empty(B)
     nbytes = N.lib().unok_verify_draft_workspace(code, B, L, V)
-    ws = torch.empty(max(nbytes, 0), device=dev, dtype=torch.uint8)
+    ws = tokens.new_empty(max(nbytes, 0), dtype=torch.uint8)
     N.call("unok_verify_draft", code, B, L, V, N.ptr(logits), _ld(logits), N.ptr(draft_logits),
            _ld(draft_logits) if draft_logits is not None else 0, N.ptr(tokens), N.ptr(counts), N.ptr(u), temp, N.ptr(temps),
            N.ptr(accepted), N.ptr(token), N.ptr(ws), nbytes, N.stream())
@@ -909,11 +920,10 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         raise RuntimeError(f"verify_tree: parents {tuple(parents.shape)} do not match the tokens {(B, T)}")
     temp, temps = _verify_operands("verify_tree", logits, B * T, u, (B, T), temperature)
     _same_device("verify_tree", logits, tokens, parents, u, *(() if temps is None else (temps,)))
-    V, code, dev = logits.shape[1], N.dtype_code(logits.dtype), logits.device
-    nodes = torch.empty((B, T), device=dev, dtype=torch.int64)
-    counts, token = (torch.empty(B, device=dev, dtype=torch.int64) for _ in range(2))
+    V, code = logits.shape[1], N.dtype_code(logits.dtype)
+    nodes, counts, token = torch.empty_like(tokens), tokens.new_empty(B), tokens.new_empty(B)
     nbytes = N.lib().unok_verify_tree_workspace(code, B, T, V)
-    ws = torch.empty(max(nbytes, 0), device=dev, dtype=torch.uint8)
+    ws = tokens.new_empty(max(nbytes, 0), dtype=torch.uint8)
     N.call("unok_verify_tree", code, B, T, V, N.ptr(logits), _ld(logits), N.ptr(tokens), N.ptr(parents), ldp, N.ptr(u), temp,
            N.ptr(temps), N.ptr(nodes), N.ptr(counts), N.ptr(token), N.ptr(ws), nbytes, N.stream())
     return nodes, counts, token
