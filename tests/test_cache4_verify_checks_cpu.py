@@ -209,14 +209,14 @@ ENTRIES = [
     ("unok_cache4_store", _move, [*MOVES, dict(codes=_at(8192, 8192)), dict(codes=_at(8192, 8448)), dict(scales=_at(16384, 16384))]),
     ("unok_cache4_load", _move, [*MOVES, dict(rows=_at(0, 0)), dict(rows=_at(0, 256))]),
     ("unok_tree_attn4", _attn, [dict(dtype=7), dict(B=-1), dict(T=257), dict(nq=3, nk=2), dict(nk=0), dict(D=96), dict(max_len=0),
-                                dict(max_len=1 << 30), dict(B=1 << 20, T=256), dict(q=None), dict(k=None), dict(ks=None), dict(v=None),
+                                dict(max_len=1 << 30), dict(max_len=(1 << 24) + 1, ws=BASE + 65536, nws=1 << 40), dict(B=1 << 20, T=256), dict(q=None), dict(k=None), dict(ks=None), dict(v=None),
                                 dict(vs=None), dict(lengths=None), dict(parents=None), dict(o=None), dict(ldp=3), dict(q=BASE + 2),
                                 dict(k=BASE + 4104), dict(ks=BASE + 8194), dict(ldq=129), dict(ldo=130), dict(ldq=64), dict(ldo=64),
                                 dict(o=BASE), dict(o=BASE + 128), dict(max_len=8192), dict(max_len=8192, ws=BASE, nws=64),
                                 dict(scale=float("inf")), dict(scale=float("nan")), dict(scale=3e38)]),
     ("unok_tree_attn4_workspace", lambda **o: [{**dict(dtype=1, B=1, T=4, nq=2, nk=1, D=64, max_len=8), **o}[n] for n in
                                                ("dtype", "B", "T", "nq", "nk", "D", "max_len")],
-     [dict(T=257), dict(D=32), dict(nq=3, nk=2), dict(max_len=0)]),
+     [dict(T=257), dict(D=32), dict(nq=3, nk=2), dict(max_len=0), dict(max_len=(1 << 24) + 1)]),
     ("unok_verify_draft", _draft, [dict(dtype=5), dict(B=-1), dict(L=-1), dict(L=257), dict(V=0), dict(V=(1 << 30) + 1), dict(B=1 << 16),
                                    dict(B=60000, L=200, V=1 << 24), dict(z=None), dict(tokens=None), dict(u=None), dict(accepted=None),
                                    dict(token=None), dict(ws=None), dict(nws=8), dict(ws=BASE + 16392), dict(ldz=49), dict(ldy=49),

@@ -1,16 +1,21 @@
 // Attention of a tree of drafted tokens over a KV cache in 4 bits: tree.hip's operator over rows as cache4.h describes them.
 //
 // The numbers of a 4-bit row are exact in bf16, so the products are bf16 ones, and the conversion is one instruction for two elements
-// and their scale. A wave loads codes from memory into registers, converts them there, and keeps 16 QT query rows: no LDS and no barrier
-// in the walk. (A walk that shares converted tiles through LDS, as the bf16 cache's does, spends its time on LDS reads of numbers four
-// times as large as their codes: 16 sequences, 64 nodes of 32 / 8 heads of 128 over 16384 rows 418 us.)
+// and their scale. Each of a workgroup's four waves walks its own tiles of a range: codes come into its part of LDS, are converted in
+// registers, and serve the wave's 16 QT query rows; no barrier in the walk. (Converted tiles shared through LDS, as the bf16 cache's are,
+// cost LDS reads of numbers four times as large as their codes: 16 sequences, 64 nodes of 32 / 8 heads of 128 over 16384 rows 418 us,
+// this 257.)
+//
+// Measured: one node of 4 sequences over 65536 rows 44 us (232 MB of codes and scales, 5.3 TB/s: what a large copy reaches); 64 nodes of 16
+// sequences over 16384 rows 257 us (820 TFLOP/s; conversions, weights and their rounding, some 200 vector instructions to 32 keys and 32
+// rows, bound it: the products alone would take 173); 16 nodes of 8 sequences over 4096 rows 22 us (6 at the copy's rate: 16 tiles to a
+// wave, the rest is the queries, the join and the launch).
 //
 // fp32 queries: a query is the sum of three bf16 numbers (each what the ones before it leave, 8 of its 24 bits), and so is a weight;
 // three products take the place of one, exact but for their sums.
 #include "tree.h"
 #include "cache4.h"
 #include "../../include/unok.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -31,7 +36,7 @@ template <int D> __device__ __forceinline__ Buffer4 buffer4(const void* codes, c
 
 // Tiles of 32 keys: codes and scales go from memory straight into LDS, NST - 1 tiles ahead, each wave's into its own part, so that
 // nothing but the wave's own counter of loads is waited for. (Two tiles in registers, one of them on its way: 16 sequences, 64 nodes over
-// 16384 rows 309 us.) A stage: K's codes, V's codes, a dword to a key for its scales of K, and of V. A lane (m, g), m < 16, g < 4, reads
+// 16384 rows 309 us, three spill: 518.) A stage: K's codes, V's codes, a dword to a key for its scales of K, and of V. A lane (m, g), m < 16, g < 4, reads
 //   K (S^T = K Q^T, first operand: 16 keys x 8 dims a lane): the dims of a product may come in any order that Q takes too; lane group g
 //     has dims D/4 g .. of key m and of key 16 + m: one read each, of one scale;
 //   V (O^T = V^T P^T, first operand: one dim x 8 keys): lane m has dims D/16 m .. of keys 4 g .. + 3 and 16 + 4 g .. + 3, which are
@@ -119,10 +124,9 @@ __device__ __forceinline__ bf16x8_t eight4(uint32_t codes, float scale) {
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(bf16x8_t, u4{pair4<0>(codes, scale), pair4<1>(codes, scale), pair4<2>(codes, scale), pair4<3>(codes, scale)});
 }
-template <int I> __device__ __forceinline__ uint32_t pair_at(uint32_t codes, float scale) { return pair4<I>(codes, scale); }
 
 template <typename E, int D, int QT>
-__global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_attn4_kernel(const TreeAttn a) {
+__global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_attn4_kernel(const TreeAttn a) {
   using Tile = Tile4<D>;
   constexpr int KT = Tile::KT, KS = Tile::KS, NDT = Tile::NDT, ROWS = 16 * QT, PARTS = sizeof(E) == 4 ? 3 : 1;
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -208,69 +212,19 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
       }
     }
   };
-  // Scores become weights; the reference moves only where one exceeds it by 2^8 (see tree.hip).
-  auto weights = [&](f32x4_t (&s)[QT][2], float (&p)[QT][8]) {
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-      // (a maximum that NaN passes through: a row with a NaN score is NaN whatever its reference)
-      float mx = s[i][0][0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = __builtin_elementwise_maximum(mx, s[i][j / 4][j % 4]);
-      mx *= a.walk_scale;
-      if (__ballot(mx > mref[i] + 8.f)) {
-        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 16, 64));
-        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
-        // (for the queries that need it alone: a row's result does not depend on the rows beside it)
-        const float to = mx > mref[i] + 8.f ? mx : mref[i];
-        const float f = to == mref[i] ? 1.f : mref[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref[i] - to);
-        mref[i] = to;
-        l[i] *= f;
-#pragma unroll
-        for (int c = 0; c < NDT; ++c) o[i][c] *= f;
-      }
-      const float ref = mref[i] == -INFINITY ? 0.f : -mref[i];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j / 4][j % 4], a.walk_scale, ref));
-        l[i] += p[i][j];
-      }
-    }
-  };
-  // Keys in pairs: two dims of eight keys become, by a permute to a dim and pair, two operands.
-  auto add_pv = [&](const Tile& t, const float (&vf)[8], float (&p)[QT][8]) {
-    bf16x8_t pf[QT][PARTS];
-#pragma unroll
-    for (int i = 0; i < QT; ++i)
-#pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
-        u4 u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (PARTS == 1) u[j] = pack2_bf16(p[i][2 * j], p[i][2 * j + 1]);
-          else {
-            const uint32_t x = __float_as_uint(p[i][2 * j]) & 0xffff0000u, y = __float_as_uint(p[i][2 * j + 1]) & 0xffff0000u;
-            p[i][2 * j] -= __uint_as_float(x);
-            p[i][2 * j + 1] -= __uint_as_float(y);
-            u[j] = x >> 16 | y;
-          }
-        }
-        pf[i][part] = __builtin_bit_cast(bf16x8_t, u);
-      }
+  // V's operands: keys in pairs, two dims of eight keys by a permute to a dim and pair.
+  auto values = [&](const Tile& t, const float (&vf)[8], bf16x8_t (&v)[NDT]) {
     auto dims = [&](auto pair) {
       constexpr int C = decltype(pair)::value;
       uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = pair_at<C>(t.v[j], vf[j]);
+      for (int j = 0; j < 8; ++j) w[j] = pair4<C>(t.v[j], vf[j]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         u4 u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], c ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-          for (int i = 0; i < QT; ++i)
-            o[i][2 * C + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, u), pf[i][part], o[i][2 * C + c], 0, 0, 0);
+        v[2 * C + c] = __builtin_bit_cast(bf16x8_t, u);
       }
     };
     dims(std::integral_constant<int, 0>{});
@@ -279,6 +233,64 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
       dims(std::integral_constant<int, 2>{});
       dims(std::integral_constant<int, 3>{});
     }
+  };
+  // The reference that a row's weights are relative to moves only where a score exceeds it by 2^8 (see tree.hip).
+  auto reference = [&](const f32x4_t (&s)[QT][2]) {
+    float mx[QT];
+    bool grow = false;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      // (a maximum that NaN passes through: a row with a NaN score is NaN whatever its reference)
+      mx[i] = s[i][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx[i] = __builtin_elementwise_maximum(mx[i], s[i][j / 4][j % 4]);
+      mx[i] *= a.walk_scale;
+      grow |= mx[i] > mref[i] + 8.f;
+    }
+    if (__ballot(grow)) {
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        mx[i] = __builtin_elementwise_maximum(mx[i], __shfl_xor(mx[i], 16, 64));
+        mx[i] = __builtin_elementwise_maximum(mx[i], __shfl_xor(mx[i], 32, 64));
+        // (for the queries that need it alone: a row's result does not depend on the rows beside it)
+        const float to = mx[i] > mref[i] + 8.f ? mx[i] : mref[i];
+        const float f = to == mref[i] ? 1.f : mref[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref[i] - to);
+        mref[i] = to;
+        l[i] *= f;
+#pragma unroll
+        for (int c = 0; c < NDT; ++c) o[i][c] *= f;
+      }
+    }
+  };
+  auto weights = [&](int i, const f32x4_t (&s)[2], float (&p)[8]) {
+    const float ref = mref[i] == -INFINITY ? 0.f : -mref[i];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], a.walk_scale, ref));
+      l[i] += p[j];
+    }
+  };
+  auto add_pv = [&](int i, const bf16x8_t (&v)[NDT], float (&p)[8]) {
+    bf16x8_t pf[PARTS];
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      u4 u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (PARTS == 1) u[j] = pack2_bf16(p[2 * j], p[2 * j + 1]);
+        else {
+          const uint32_t x = __float_as_uint(p[2 * j]) & 0xffff0000u, y = __float_as_uint(p[2 * j + 1]) & 0xffff0000u;
+          p[2 * j] -= __uint_as_float(x);
+          p[2 * j + 1] -= __uint_as_float(y);
+          u[j] = x >> 16 | y;
+        }
+      }
+      pf[part] = __builtin_bit_cast(bf16x8_t, u);
+    }
+#pragma unroll
+    for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+      for (int c = 0; c < NDT; ++c) o[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[c], pf[part], o[i][c], 0, 0, 0);
   };
 
   const uint32_t at = lds_addr(mine);
@@ -293,12 +305,41 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
     Tile t;
     t.read(at + stage * Tile::STAGE, m, g);
     f32x4_t s[QT][2];
-    float p[QT][8], vf[8];
-    scores(t, s);
-    weights(s, p);
+    float vf[8];
+    bf16x8_t v[NDT];
 #pragma unroll
     for (int j = 0; j < 8; ++j) vf[j] = t.v_scale(j, m);
-    add_pv(t, vf, p);
+    scores(t, s);
+    values(t, vf, v);
+    // the scores' products run while the codes are converted (held here: the compiler would move V's behind the branch)
+#pragma unroll
+    for (int c = 0; c < NDT; ++c) {
+      u4 u = __builtin_bit_cast(u4, v[c]);
+      asm volatile("" : "+v"(u));
+      v[c] = __builtin_bit_cast(bf16x8_t, u);
+    }
+    __builtin_amdgcn_sched_group_barrier(SG_VALU, 6, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * KS * QT * PARTS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(SG_VALU, QT == 1 ? 12 : 6, 0);
+    }
+    reference(s);
+    // and the weighted values' while the next rows' weights are formed
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      float p[8];
+      weights(i, s[i], p);
+      add_pv(i, v, p);
+    }
+    if constexpr (QT > 1) {
+      __builtin_amdgcn_sched_group_barrier(SG_VALU, 28, 0);
+#pragma unroll
+      for (int i = 0; i < NDT * (QT - 1); ++i) {
+        __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(SG_VALU, 32 / NDT, 0);
+      }
+    }
     next_tile();
   }
   // Tiles with tree rows, and rows at or past hi, which read as zeros, at weight 0.
@@ -307,7 +348,6 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
     Tile t;
     t.read(at + stage * Tile::STAGE, m, g);
     f32x4_t s[QT][2];
-    float p[QT][8], vf[8];
     scores(t, s);
 #pragma unroll
     for (int i = 0; i < QT; ++i)
@@ -316,10 +356,12 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
         const int r = key + Tile::slot_key(j, g), x = r + lo - n;
         s[i][j / 4][j % 4] = r < all && ((x < 0) | tree_sees(anc, node[i], W, x)) ? s[i][j / 4][j % 4] : -INFINITY;
       }
-    weights(s, p);
+    reference(s);
     // A scale of NaN, or one too large for numbers, in a row that some queries do not see: 0 in the product, and added where it is
     // seen. The weights go through the tile's stage, 16 rows at a time.
     bool odd = false;
+    float vf[8];
+    bf16x8_t v[NDT];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t byte = t.v_byte(j, m);
@@ -327,14 +369,17 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
       vf[j] = scale4(byte > SCALE4_MAX ? 0 : byte);
     }
     odd = __ballot(odd) != 0;
-    if (odd) {
-      float* ps = (float*)(mine + stage * Tile::STAGE);
-      static_assert(16 * (KT + 1) * 4 <= Tile::STAGE, "the weights of 16 rows fit in a stage");
+    values(t, vf, v);
+    float* ps = (float*)(mine + stage * Tile::STAGE);
+    static_assert(16 * (KT + 1) * 4 <= Tile::STAGE, "the weights of 16 rows fit in a stage");
 #pragma unroll
-      for (int i = 0; i < QT; ++i) {
+    for (int i = 0; i < QT; ++i) {
+      float p[8];
+      weights(i, s[i], p);
+      if (odd) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ps[m * (KT + 1) + Tile::slot_key(j, g)] = p[i][j];
-        __builtin_amdgcn_wave_barrier();
+        for (int j = 0; j < 8; ++j) ps[m * (KT + 1) + Tile::slot_key(j, g)] = p[j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
         for (int j = 0; j < KT && key + j < all; ++j) {
           const int x = key + j + lo - n;
@@ -350,11 +395,10 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
               if (seen && row.scales[d / GROUP4] > SCALE4_MAX) o[i][c][e] += w * value4(row, d);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      add_pv(i, v, p);
     }
-    add_pv(t, vf, p);
     next_tile();
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // no load is on its way into what becomes the merge's
@@ -362,14 +406,15 @@ __global__ __launch_bounds__(256, QT <= 2 && sizeof(E) == 2 ? 2 : 1) void tree_a
                        [](int c, int e, int g) { return (4 * g + e) * NDT + c; });
 }
 
-// Query rows of a workgroup, and one round of workgroups.
+// Query rows of a workgroup, and one round of workgroups (`share`, two to a CU; fp32 with 128 dims has the registers for one). 32 rows: 64
+// to a wave share a conversion among more products, but leave one wave to a SIMD: 16 sequences, 64 nodes over 16384 rows 273 us (32
+// rows 266), 8 sequences, 16 nodes over 4096 26.2 (22.5).
 TreePlan tree_plan4(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   const int NR = nq / nk * T;
   TreePlan p;
-  p.rows = NR <= 16 ? 16 : NR <= 32 || dtype == UNOK_F32 ? 32 : 64;
-  if (getenv("W2") && p.rows == 64) p.rows = 32;
+  p.rows = NR <= 16 ? 16 : 32;
   p.rt = (NR + p.rows - 1) / p.rows;
-  const int64_t share = (p.rows > 32 || dtype == UNOK_F32 ? 256 : 512) / ((int64_t)nk * p.rt);
+  const int64_t share = (dtype == UNOK_F32 && D == 128 ? 256 : 512) / ((int64_t)nk * p.rt);
   p.share = share > 1 ? (int)share : 1;
   p.ranges = max_len <= TREE_LEAST * TB ? B : B + p.share;
   return p;
@@ -385,15 +430,19 @@ template <typename E, int D> void launch_tree4(const TreeAttn& a, const TreePlan
     hipLaunchKernelGGL((tree_attn4_kernel<E, D, QT>), grid, dim3(256), lds, st, a);
   };
   if (plan.rows == 16) walk(std::integral_constant<int, 1>{});
-  else if (plan.rows == 32) walk(std::integral_constant<int, 2>{});
-  else if constexpr (sizeof(E) == 2) walk(std::integral_constant<int, 4>{});
+  else walk(std::integral_constant<int, 2>{});
   launch_combine<E, D>(a, plan, st);
+}
+
+int sizes_ok(int B, int T, int nq, int nk, int D, int max_len) {
+  UNOK_REQUIRE(max_len <= 1 << 24, UNOK_EINVAL, "tree_attn4: caches hold at most 2^24 rows (got %d)", max_len);   // (32-bit offsets)
+  return tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len);
 }
 
 }  // namespace
 
 UNOK_EXPORT int64_t unok_tree_attn4_workspace(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
-  if (tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len)) return -1;
+  if (sizes_ok(B, T, nq, nk, D, max_len)) return -1;
   if (B == 0 || T == 0) return 0;
   return plan_workspace(tree_plan4(dtype, B, T, nq, nk, D, max_len), B, T, nq, D);
 }
@@ -402,10 +451,9 @@ UNOK_EXPORT int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, 
                                 const void* k_scales, const void* v, const void* v_scales, int max_len, const int64_t* lengths,
                                 const int32_t* parents, int64_t ldp, float scale, void* o, int64_t ldo, void* workspace,
                                 int64_t ws_bytes, void* stream) {
-  int rc = tree_sizes_ok("tree_attn4", B, T, nq, nk, D, max_len);
+  int rc = sizes_ok(B, T, nq, nk, D, max_len);
   if (rc) return rc;
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "tree_attn4: bad dtype %d", dtype);
-  UNOK_REQUIRE(max_len <= 1 << 24, UNOK_EINVAL, "tree_attn4: caches hold at most 2^24 rows (got %d)", max_len);
   if (B == 0 || T == 0) return 0;
   UNOK_REQUIRE(k && v && k_scales && v_scales, UNOK_EINVAL, "tree_attn4: null operand");
   UNOK_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) == 0, UNOK_EALIGN,
