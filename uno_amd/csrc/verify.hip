@@ -21,8 +21,9 @@ constexpr int CHUNK = 2048, VERIFY_NODES = 256;
 constexpr double LOG2E = 1.4426950408889634, LOWEST = -700.0 * LOG2E;   // weights below e^-700 are 0
 constexpr double LEAST = 0x1p-40;                                       // of max(p - q, 0) in all; below, p itself is drawn from
 
-// One chunk of a row: its largest logit (NaN: the row has a NaN or +inf here), its column, the sum of the weights relative to it.
-struct Part { float m; int arg; double s; };
+// One chunk of a row: the sums of its fourths' weights relative to its largest logit, the fourths' largest (NaN passes through), and the
+// column of the largest.
+struct alignas(16) Part { double s[4]; float m[4]; int arg; };
 
 struct Verify {
   const void *z, *y; int64_t ldz, ldy;                // target rows; the drafter's rows (null: none)
@@ -62,13 +63,13 @@ template <int N> __device__ __forceinline__ void exp2_64(double (&d)[N], double 
   }
 }
 // The weights of z relative to m, c = log2(e) / T.
+__device__ __forceinline__ bool counts(float z, double m, double c) { return ((double)z - m) * c >= LOWEST; }
 template <int N> __device__ __forceinline__ void weights(const float (&z)[N], double m, double c, double (&w)[N]) {
   bool some[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    w[i] = (double)z[i] - m;
-    some[i] = w[i] * c >= LOWEST;
-    w[i] = some[i] ? w[i] : 0.0;
+    some[i] = counts(z[i], m, c);
+    w[i] = some[i] ? (double)z[i] - m : 0.0;
   }
   exp2_64<N>(w, c);
 #pragma unroll
@@ -109,22 +110,87 @@ template <typename T> struct Chunks {
     nv = (V - head) / VN;
   }
   __device__ __forceinline__ int tail() const { return head + nv * VN; }
-  __device__ __forceinline__ int lo(int c) const { return c == 0 ? 0 : min(head + c * CHUNK, tail()); }
-  __device__ __forceinline__ int hi(int c) const { return c == nch - 1 ? V : min(head + (c + 1) * CHUNK, tail()); }
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// A value moved between lanes by data-parallel moves; lanes that nothing reaches get 0.
+template <int CTRL, int ROWS = 0xf, typename V> __device__ __forceinline__ V moved(V v) {
+  auto one = [](int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); };
+  if constexpr (sizeof(V) == 8) return __hiloint2double(one(__double2hiint(v)), one(__double2loint(v)));
+  else return __builtin_bit_cast(V, one(__builtin_bit_cast(int, v)));
+}
+// Over each 16 lanes, and over the wave: all of them get the result.
+template <typename V, typename F> __device__ __forceinline__ V row_all(V v, F f) {
+  v = f(v, moved<0xb1>(v));                              // quads 1 0 3 2, then 2 3 0 1, mirrored eights, mirrored rows
+  v = f(v, moved<0x4e>(v));
+  v = f(v, moved<0x141>(v));
+  return f(v, moved<0x140>(v));
+}
+template <typename V, typename F> __device__ __forceinline__ V wave_all(V v, F f) {
+  v = row_all(v, f);
+  v = f(v, __shfl_xor(v, 16, 64));
+  return f(v, __shfl_xor(v, 32, 64));
+}
+constexpr auto add64 = [](double x, double y) { return x + y; };
+__device__ __forceinline__ double wave_sum64(double v) { return wave_all(v, add64); }
+__device__ __forceinline__ int wave_min(int v) { return wave_all(v, [](int x, int y) { return min(x, y); }); }
+constexpr auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };   // (NaN passes through this maximum)
+// Four values over the wave at once: the 16 lanes of row j get that of v[j].
+template <typename V, typename F> __device__ __forceinline__ V four_all(const V (&v)[4], F f) {
+  const bool upper = threadIdx.x & 32, odd = threadIdx.x & 16;
+  const V a = f(upper ? v[2] : v[0], __shfl_xor(upper ? v[0] : v[2], 32, 64));
+  const V b = f(upper ? v[3] : v[1], __shfl_xor(upper ? v[1] : v[3], 32, 64));
+  return row_all(f(odd ? b : a, __shfl_xor(odd ? a : b, 16, 64)), f);
+}
+__device__ __forceinline__ double wave_scan64(double v) {                // sum over lanes 0 .. this one
+  v += moved<0x111>(v);                                  // row_shr 1, 2, 4, 8
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xa>(v);                             // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+  v += moved<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ int wave_min(int v) {
+
+// Sums of weights by a table: 2^x = 2^(N / STEPS) (1 + r q(r)), N + r = STEPS x, r in [-1/2, 1/2], q the polynomial through
+// (2^(r / STEPS) - 1) / r at three Chebyshev points (relative error 9e-12, of both signs in turn). The table holds 2^(j / STEPS) with
+// j / STEPS taken from the exponent, so that N joins it there whole.
+constexpr int STEP_BITS = 6, STEPS = 1 << STEP_BITS;
+struct Steps {
+  uint64_t v[STEPS];
+  constexpr Steps() : v{} {
+    for (int j = 0; j < STEPS; ++j) {
+      const double y = 0.6931471805599453 * j / STEPS;
+      double p = 1.0;
+      for (int k = 20; k > 0; --k) p = 1.0 + p * y / k;
+      v[j] = __builtin_bit_cast(uint64_t, p) - ((uint64_t)j << (52 - STEP_BITS));
+    }
+  }
+};
+__device__ const Steps steps_of_two{};
+
+// s plus the weights of N logits (`least` in place of those below it); c in steps, k = 1.5 2^52 less the reference's whole step.
+template <int N> __device__ __forceinline__ double add_weights(const float* z, float least, double c, double k, const double* table,
+                                                           double s) {
+  constexpr double Q[3] = {0x1.62e42fefa39efp-7, 0x1.ebfc1b10317efp-15, 0x1.c6b0ae350b0b5p-23};
+  double t[N], r[N], w[N];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
+  for (int i = 0; i < N; ++i) {
+    const double x = (double)__builtin_elementwise_maximum(z[i], least);
+    t[i] = fma(x, c, k);
+    r[i] = fma(x, c, k - t[i]);
+    w[i] = table[__double2loint(t[i]) & (STEPS - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double p = fma(fma(fma(Q[2], r[i], Q[1]), r[i], Q[0]), r[i], 1.0);
+    s = fma(__hiloint2double(__double2hiint(w[i]) + (__double2loint(t[i]) << (20 - STEP_BITS)), __double2loint(w[i])), p, s);
+  }
+  return s;
 }
-// The parts of one chunk of a row, by one wave.
-template <typename T> __device__ __forceinline__ Part chunk_part(const T* row, int V, int nch, int chunk, double c) {
+
+// The part of one chunk of a row, by one wave.
+template <typename T> __device__ __forceinline__ void chunk_part(const T* row, int V, int nch, int chunk, double c, const double* table,
+                                                                 Part* to) {
   using C = Chunks<T>;
   constexpr int NL = C::VPC / 64;
   const C ch(row, V, nch);
@@ -157,15 +223,15 @@ template <typename T> __device__ __forceinline__ Part chunk_part(const T* row, i
   };
   if (v0 + C::VPC <= ch.nv) unpack(std::true_type{});
   else unpack(std::false_type{});
-  float m = -INFINITY;                                   // (NaN passes through this maximum)
+  float top[4] = {zh, -INFINITY, -INFINITY, zt};
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = __builtin_elementwise_maximum(m, z[i]);
-  m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(zh, zt));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o, 64));
-  Part p{m, 0, 0.0};
-  if (!(m < INFINITY)) p.m = __uint_as_float(0x7fc00000u);
-  else if (m > -INFINITY) {
+  for (int i = 0; i < N; ++i) top[i * 4 / N] = larger(top[i * 4 / N], z[i]);
+  const float fourth = four_all(top, larger);
+  float m = larger(fourth, __shfl_xor(fourth, 16, 64));
+  m = larger(m, __shfl_xor(m, 32, 64));
+  int arg = 0;
+  double sum = 0.0;
+  if (m < INFINITY && m > -INFINITY) {
     if (c == 0.0) {
       int first = INT32_MAX;                             // the lowest column of the largest logit
 #pragma unroll
@@ -173,35 +239,46 @@ template <typename T> __device__ __forceinline__ Part chunk_part(const T* row, i
         if (z[i] == m) first = ch.head + (v0 + 64 * (i / C::VN) + lane) * C::VN + i % C::VN;
       if (zh == m) first = lane;
       if (first == INT32_MAX && zt == m) first = ch.tail() + lane;
-      p.arg = wave_min(first);
+      arg = wave_min(first);
     } else {
       // (beside the chunk's largest, whose weight is 1, what lies below the lowest weight need not be exactly 0)
-      const double least = LOWEST / c;
-      double s = 0.0;
-      constexpr int G = 4;
+      const double cs = c * STEPS, whole = rint((double)m * cs), low = (double)m + LOWEST / c;
+      double s[4] = {0.0, 0.0, 0.0, 0.0};
+      if (fabs(whole) < 0x1p50 && low > -3e38) {
+        const double k = 0x1.8p52 - whole;
+        const float least = (float)low;
 #pragma unroll
-      for (int i = 0; i < N; i += G) {
-        double w[G];
+        for (int i = 0; i < N; i += 4) s[i * 4 / N] = add_weights<4>(z + i, least, cs, k, table, s[i * 4 / N]);
+        if (edge) s[0] = add_weights<1>(&zh, least, cs, k, table, s[0]);
+        if (last) s[3] = add_weights<1>(&zt, least, cs, k, table, s[3]);
+        double f[1] = {-fma((double)m, cs, -whole)};     // (these are relative to the whole step next to m)
+        exp2_64<1>(f, 1.0 / STEPS);
+        sum = four_all(s, add64) * f[0];
+      } else {                                           // temperatures so low or high that steps or `low` leave their formats
 #pragma unroll
-        for (int k = 0; k < G; ++k) w[k] = fmax((double)z[i + k] - (double)m, least);
-        exp2_64<G>(w, c);
-        s += (w[0] + w[1]) + (w[2] + w[3]);
+        for (int i = 0; i < N; i += 4) {
+          const float x[4] = {z[i], z[i + 1], z[i + 2], z[i + 3]};
+          double w[4];
+          weights<4>(x, m, c, w);
+          s[i * 4 / N] += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        s[0] += weight(zh, m, c);
+        s[3] += weight(zt, m, c);
+        sum = four_all(s, add64);
       }
-      if (edge || last) {
-        double w[2] = {fmax((double)zh - (double)m, least), fmax((double)zt - (double)m, least)};
-        exp2_64<2>(w, c);
-        s += w[0] + w[1];
-      }
-      p.s = wave_sum64(s);
     }
   }
-  return p;
+  if (lane == 0) to->arg = arg;
+  if ((lane & 15) == 0) { to->s[lane >> 4] = sum; to->m[lane >> 4] = fourth; }
 }
 
 // One wave to a chunk; workgroups go through a row's chunks first.
 template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_parts_kernel(const Verify a) {
   const int groups = (a.nch + 3) / 4, row = blockIdx.x / groups;
   const int chunk = blockIdx.x % groups * 4 + (threadIdx.x >> 6);
+  __shared__ double table[STEPS];
+  if (threadIdx.x < STEPS) table[threadIdx.x] = __builtin_bit_cast(double, steps_of_two.v[threadIdx.x]);
+  __syncthreads();
   if (chunk >= a.nch) return;
   const T* z;
   int b;
@@ -222,20 +299,10 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
       z = (const T*)a.y + (int64_t)(row - targets) * a.ldy;
     }
   }
-  const Part p = chunk_part(z, a.V, a.nch, chunk, rate(a, b));
-  if ((threadIdx.x & 63) == 0) a.parts[(int64_t)row * a.nch + chunk] = p;
+  chunk_part(z, a.V, a.nch, chunk, rate(a, b), table, a.parts + (int64_t)row * a.nch + chunk);
 }
 
 // ---- one wave's steps ------------------------------------------------------------------------------
-__device__ __forceinline__ double wave_scan64(double v) {                // sum over lanes 0 .. this one
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double below = __shfl_up(v, o, 64);
-    if (lane >= o) v += below;
-  }
-  return v;
-}
 __device__ __forceinline__ double lane_value(double v, int lane) {
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
 }
@@ -244,41 +311,48 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 template <typename V> __device__ __forceinline__ void hand_over(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename V> __device__ __forceinline__ V taken(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// A list of n values that the wave goes through in order: lane l holds values [l per, (l + 1) per), the first K of them in registers.
-__device__ __forceinline__ Part listed(const Part* p) { return *p; }
-__device__ __forceinline__ double2 listed(const double2* p) { return make_double2(taken(&p->x), taken(&p->y)); }
-template <typename P, int K> struct Listed {
-  const P* p;
-  P v[K];
+// A list of n values that the wave goes through in order: lane l holds values [l per, (l + 1) per), the first K of them in registers;
+// get(i) loads one.
+template <typename G, int K> struct Listed {
+  G get;
+  decltype(get(0)) v[K];
   int first, end;
-  __device__ __forceinline__ Listed(const P* p_, int n) : p(p_) {
+  __device__ __forceinline__ Listed(G get_, int n) : get(get_) {
     const int per = (n + 63) / 64;
     first = min(n, (int)(threadIdx.x & 63) * per);
     end = min(n, first + per);
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = listed(p + min(first + k, n - 1));
+    for (int k = 0; k < K; ++k) v[k] = get(min(first + k, n - 1));
   }
   template <typename F> __device__ __forceinline__ void each(F f) const {   // f(index, value), in order
 #pragma unroll
     for (int k = 0; k < K; ++k)
       if (first + k < end) f(first + k, v[k]);
-    for (int i = first + K; i < end; ++i) f(i, listed(p + i));
+    for (int i = first + K; i < end; ++i) f(i, get(i));
   }
 };
+struct Parts {
+  const Part* p;
+  __device__ __forceinline__ Part operator()(int i) const { return p[i]; }
+};
+struct Pairs {                                           // sums that other workgroups of this launch handed over
+  const double2* p;
+  __device__ __forceinline__ double2 operator()(int i) const { return make_double2(taken(&p[i].x), taken(&p[i].y)); }
+};
 
-// Of values in order across the lanes (each lane's `sum`, and `each` to go through them: f(index, weight)), the lowest index at
-// which base plus the sum so far exceeds t; where none does, the last with a weight; -1: there is none. All lanes get the index,
-// and in base the sum before it.
-template <typename F> __device__ __forceinline__ int pick(double& base, double t, double sum, int last, F each) {
+// Of values in order across the lanes (`upto` the sum up to each lane's end, `sum` its own, `last` its last index with a weight, and
+// `each` to go through them: f(index, weight)), the lowest index at which base plus the sum so far exceeds t; where none does, the last
+// with a weight, and `over` is false; -1: there is none. All lanes get the index, and in base the sum before it.
+template <typename F> __device__ __forceinline__ int pick(double& base, bool& over, double t, double upto, double sum, int last, F each) {
   const int lane = threadIdx.x & 63;
-  const double upto = base + wave_scan64(sum);
-  const uint64_t any = __ballot(last >= 0), over = __ballot(last >= 0 && upto > t);
+  const uint64_t any = __ballot(last >= 0), past = __ballot(last >= 0 && base + upto > t);
+  over = past != 0;
   if (any == 0) return -1;
-  const int win = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+  const int win = over ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
   int found = -1;
   double before = 0.0;
   if (lane == win) {
-    double run = upto - sum;
+    double run = base + (upto - sum);
     bool done = false;
     each([&](int j, double w) {
       if (!done && w > 0.0) {
@@ -314,29 +388,30 @@ template <int K, int G, typename F, typename W> __device__ __forceinline__ int p
       last = w[g][k] > 0.0 ? j : last;
     }
   }
-  return pick(base, t, sum, last, [&](auto f) {
+  bool over;
+  return pick(base, over, t, wave_scan64(sum), sum, last, [&](auto f) {
 #pragma unroll
     for (int k = 0; k < KG * G; ++k)
       if (first + k < end) f(first + k, w[k / G][k % G]);
   });
 }
 
-__device__ __forceinline__ double part_sum(const Part& p, double m, double c) { return p.s > 0.0 ? p.s * weight(p.m, m, c) : 0.0; }
+__device__ __forceinline__ double part_sum(const Part& p) { return (p.s[0] + p.s[1]) + (p.s[2] + p.s[3]); }
+__device__ __forceinline__ float part_max(const Part& p) { return larger(larger(p.m[0], p.m[1]), larger(p.m[2], p.m[3])); }
 
 // A row's largest logit, its lowest column, and the sum of its weights, from its parts. bad: the row has no distribution.
 struct Row { float m; int arg; double s; bool bad; };
-template <int K> __device__ __forceinline__ Row row_of(const Listed<Part, K>& parts, double c) {
+template <int K> __device__ __forceinline__ Row row_of(const Listed<Parts, K>& parts, double c) {
   Row r{-INFINITY, INT32_MAX, 0.0, false};
-  parts.each([&](int, const Part& p) { r.m = __builtin_elementwise_maximum(r.m, p.m); });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) r.m = __builtin_elementwise_maximum(r.m, __shfl_xor(r.m, o, 64));
+  parts.each([&](int, const Part& p) { r.m = larger(r.m, part_max(p)); });
+  r.m = wave_all(r.m, larger);
   r.bad = !(r.m < INFINITY && r.m > -INFINITY);
   if (r.bad) return r;
   if (c == 0.0) {
-    parts.each([&](int, const Part& p) { if (p.m == r.m) r.arg = min(r.arg, p.arg); });
+    parts.each([&](int, const Part& p) { if (part_max(p) == r.m) r.arg = min(r.arg, p.arg); });
     r.arg = wave_min(r.arg);
   } else {
-    parts.each([&](int, const Part& p) { r.s += part_sum(p, r.m, c); });
+    parts.each([&](int, const Part& p) { r.s += part_sum(p) * weight(part_max(p), r.m, c); });
   }
   return r;
 }
@@ -392,27 +467,85 @@ __device__ void walk(const Verify& a, int b, const int32_t* drawn) {
   if (lane == 0) { a.out_counts[b] = n; a.out_token[b] = next; }
 }
 
+// The token drawn from a row, by one wave: the fourth of a chunk in which the running sum exceeds t, then its columns, a vector or two
+// to a lane (before the first one those up to the first boundary, after the last one the rest).
+template <typename T> __device__ __forceinline__ int draw(const T* z, const Verify& a, const Listed<Parts, 2>& parts, double c, double u) {
+  const Row r = row_of(parts, c);
+  if (r.bad || c == 0.0) return r.bad ? -1 : r.arg;
+  const int lane = threadIdx.x & 63;
+  const double m = r.m, upto = wave_scan64(r.s), t = u * lane_value(upto, 63);
+  auto fourths = [&](auto f) {
+    parts.each([&](int i, const Part& p) {
+      const double w = weight(part_max(p), m, c);
+      // (of a fourth in which no column counts, some columns' lowest weights may have been added)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f(4 * i + k, counts(p.m[k], m, c) ? p.s[k] * w : 0.0);
+    });
+  };
+  int last = -1;
+  fourths([&](int i, double w) { last = w > 0.0 ? i : last; });
+  double base = 0.0;
+  bool over;
+  const int at4 = pick(base, over, t, upto, r.s, last, fourths);
+  if (at4 < 0) return -1;
+  using C = Chunks<T>;
+  constexpr int COLS = CHUNK / 4 / 64;                   // to a lane
+  const C ch(z, a.V, a.nch);
+  const int body = ch.head + at4 * (CHUNK / 4);
+  int token = -1;
+  double start = base;
+  for (int step = at4 == 0 && ch.head > 0 ? 0 : 1; step < 3; ++step) {   // head, vectors, rest
+    if (step == 2 && (at4 != 4 * ch.nch - 1 || ch.tail() == ch.V)) break;
+    const int j = step == 0 ? lane : step == 1 ? body + COLS * lane : ch.tail() + lane;
+    const int n = step == 0 ? lane < ch.head : step == 1 ? max(0, min(COLS, ch.tail() - j)) : j < ch.V;
+    float x[COLS];
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) x[k] = -INFINITY;
+    if (step != 1) {
+      if (n) x[0] = at(z, j);
+    } else {
+#pragma unroll
+      for (int v = 0; v < COLS / C::VN; ++v)
+        if (n >= (v + 1) * C::VN) {
+          const u32x4_t raw = *(const u32x4_t*)(z + j + v * C::VN);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (C::VN == 4) x[4 * v + k] = __uint_as_float(raw[k]);
+            else { x[2 * k] = __uint_as_float(raw[k] << 16); x[2 * k + 1] = __uint_as_float(raw[k] & 0xffff0000u); }
+          }
+        }
+    }
+    double w[COLS], sum = 0.0;
+    int some = -1;
+    weights<COLS>(x, m, c, w);
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) {
+      sum += w[k];
+      some = w[k] > 0.0 ? j + k : some;
+    }
+    const double all = wave_scan64(sum);
+    double before = start;
+    const int got = pick(before, over, t, all, sum, some, [&](auto f) {
+#pragma unroll
+      for (int k = 0; k < COLS; ++k) f(j + k, w[k]);
+    });
+    if (got >= 0) token = got;
+    if (over) break;
+    start += lane_value(all, 63);
+  }
+  return token;
+}
+
 // The token of each node, one wave per row (-1: padding, or no distribution); the last of a sequence's rows follows the tree.
 template <typename T> __global__ __launch_bounds__(64) void verify_draw_kernel(const Verify a, int32_t* drawn, uint32_t* arrived) {
   const int row = blockIdx.x, b = row / a.T;
-  int token = -1;
-  if (a.parents[b * a.ldp + row % a.T] >= -1) {
-    const double c = rate(a, b), u = random_at(a, row);
-    const Listed<Part, 4> parts(a.parts + (int64_t)row * a.nch, a.nch);
-    const Row r = row_of(parts, c);
-    if (!r.bad && c == 0.0) token = r.arg;
-    else if (!r.bad) {
-      const double m = r.m, t = u * lane_value(wave_scan64(r.s), 63);
-      double base = 0.0;
-      int last = -1;
-      parts.each([&](int i, const Part& p) { if (part_sum(p, m, c) > 0.0) last = i; });
-      const int ch = pick(base, t, r.s, last, [&](auto f) { parts.each([&](int i, const Part& p) { f(i, part_sum(p, m, c)); }); });
-      const T* z = (const T*)a.z + (int64_t)row * a.ldz;
-      const Chunks<T> cs(z, a.V, a.nch);
-      if (ch >= 0)
-        token = pick_column<(CHUNK + 14 + 63) / 64, 6>(cs.lo(ch), cs.hi(ch), base, t, [&](int j) { return at(z, j); },
-                                                       [&](int, const float (&x)[6], double (&w)[6]) { weights<6>(x, m, c, w); });
-    }
+  const Listed<Parts, 2> parts(Parts{a.parts + (int64_t)row * a.nch}, a.nch);
+  const double c = rate(a, b), u = random_at(a, row);
+  const int parent = a.parents[b * a.ldp + row % a.T];
+  const int token = parent >= -1 ? draw((const T*)a.z + (int64_t)row * a.ldz, a, parts, c, u) : -1;
+  if (a.T == 1) {                                        // (no one to wait for)
+    if (threadIdx.x == 0) { a.nodes[b] = parent >= -1 ? 0 : -1; a.out_counts[b] = parent >= -1; a.out_token[b] = token; }
+    return;
   }
   if (threadIdx.x == 0) hand_over(drawn + row, token);
   if (last_to_arrive(arrived + b, a.T)) walk(a, b, drawn);
@@ -438,7 +571,7 @@ template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kern
     const int64_t x = i < n ? a.tokens[(int64_t)b * L + i] : -1;
     const bool in = x >= 0 && x < a.V;
     const double u = random_at(a, (int64_t)b * (L + 1) + i);
-    const Listed<Part, 2> tp(targets + (int64_t)i * a.nch, a.nch), dp(row ? drafts + (int64_t)i * a.nch : targets, a.nch);
+    const Listed<Parts, 2> tp(Parts{targets + (int64_t)i * a.nch}, a.nch), dp(Parts{row ? drafts + (int64_t)i * a.nch : targets}, a.nch);
     const float zx = at((const T*)a.z + ((int64_t)b * (L + 1) + i) * a.ldz, in ? (int)x : 0);
     const float yx = row ? at((const T*)a.y + ((int64_t)b * L + i) * a.ldy, in ? (int)x : 0) : 0.f;
     Ended e{i, ENDED_P, -1, 0, c, 0.0, 1.0, 0.0, 1.0};
@@ -561,7 +694,7 @@ template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(
   }
   __syncthreads();
   if (!last || wid != 0) return;
-  const Listed<double2, 5> list(mine, pieces);
+  const Listed<Pairs, 5> list(Pairs{mine}, pieces);
   double l = 0.0, p = 0.0;
   list.each([&](int, const double2& s) { l += s.x; p += s.y; });
   const double left = wave_sum64(l), whole = wave_sum64(p);
@@ -570,7 +703,8 @@ template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(
   int some = -1;
   list.each([&](int i, const double2& s) { if ((all ? s.y : s.x) > 0.0) some = i; });
   double base = 0.0;
-  const int at = pick(base, t, all ? p : l, some, [&](auto f) { list.each([&](int i, const double2& s) { f(i, all ? s.y : s.x); }); });
+  bool over;
+  const int at = pick(base, over, t, wave_scan64(all ? p : l), all ? p : l, some, [&](auto f) { list.each([&](int i, const double2& s) { f(i, all ? s.y : s.x); }); });
   int token = -1;
   if (at >= 0)
     token = pick_column<PIECE / 64, 4>(at * PIECE, min(at * PIECE + PIECE, a.V), base, t, [&](int j) { return row.get(j); },
