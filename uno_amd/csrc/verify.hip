@@ -21,9 +21,10 @@ constexpr int CHUNK = 2048, VERIFY_NODES = 256;
 constexpr double LOG2E = 1.4426950408889634, LOWEST = -700.0 * LOG2E;   // weights below e^-700 are 0
 constexpr double LEAST = 0x1p-40;                                       // of max(p - q, 0) in all; below, p itself is drawn from
 
-// One chunk of a row: the sums of its fourths' weights relative to its largest logit, the fourths' largest (NaN passes through), and the
-// column of the largest.
-struct alignas(16) Part { double s[4]; float m[4]; int arg; };
+// One chunk of a row: its largest logit (NaN passes through), the column of that, and the sum of the weights relative to it. For rows
+// that a token may be drawn from, the same of its fourths (the sums relative to the chunk's largest).
+struct alignas(16) Part { double s; float m; int arg; };
+struct alignas(16) Fourths { double s[4]; float m[4]; int arg; };
 
 struct Verify {
   const void *z, *y; int64_t ldz, ldy;                // target rows; the drafter's rows (null: none)
@@ -33,7 +34,8 @@ struct Verify {
   const float* u;
   const float* temps; float temp;                     // per sequence, or one
   int B, T, V, nch;                                   // T: nodes of a tree, or drafted tokens
-  Part* parts;                                        // [target rows, then the drafter's][nch]
+  Part* parts;                                        // drafted blocks: [target rows, then the drafter's][nch]
+  Fourths* fourths;                                   // [target rows][nch]
   uint32_t* arrived;                                  // of a tree's rows, drawn; 0 before
   int64_t *nodes, *out_counts, *out_token;
 };
@@ -190,7 +192,7 @@ template <int N> __device__ __forceinline__ double add_weights(const float* z, f
 
 // The part of one chunk of a row, by one wave.
 template <typename T> __device__ __forceinline__ void chunk_part(const T* row, int V, int nch, int chunk, double c, const double* table,
-                                                                 Part* to) {
+                                                                 Part* to, Fourths* four) {
   using C = Chunks<T>;
   constexpr int NL = C::VPC / 64;
   const C ch(row, V, nch);
@@ -268,8 +270,15 @@ template <typename T> __device__ __forceinline__ void chunk_part(const T* row, i
       }
     }
   }
-  if (lane == 0) to->arg = arg;
-  if ((lane & 15) == 0) { to->s[lane >> 4] = sum; to->m[lane >> 4] = fourth; }
+  if (four) {
+    if ((lane & 15) == 0) { four->s[lane >> 4] = sum; four->m[lane >> 4] = fourth; }
+    if (lane == 0) four->arg = arg;
+  }
+  if (to) {
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane == 0) *to = Part{sum, m, arg};
+  }
 }
 
 // One wave to a chunk; workgroups go through a row's chunks first.
@@ -282,6 +291,7 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
   if (chunk >= a.nch) return;
   const T* z;
   int b;
+  bool target = true;
   if constexpr (TREE) {
     b = row / a.T;
     if (row % a.T == 0 && chunk == 0 && (threadIdx.x & 63) == 0) a.arrived[b] = 0;
@@ -294,12 +304,14 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
       if (row % (a.T + 1) > drafted(a, b)) return;
       z = (const T*)a.z + (int64_t)row * a.ldz;
     } else {
+      target = false;
       b = (row - targets) / a.T;
       if ((row - targets) % a.T >= drafted(a, b) || rate(a, b) == 0.0) return;
       z = (const T*)a.y + (int64_t)(row - targets) * a.ldy;
     }
   }
-  chunk_part(z, a.V, a.nch, chunk, rate(a, b), table, a.parts + (int64_t)row * a.nch + chunk);
+  chunk_part(z, a.V, a.nch, chunk, rate(a, b), table, TREE ? nullptr : a.parts + (int64_t)row * a.nch + chunk,
+             target ? a.fourths + (int64_t)row * a.nch + chunk : nullptr);
 }
 
 // ---- one wave's steps ------------------------------------------------------------------------------
@@ -335,6 +347,14 @@ struct Parts {
   const Part* p;
   __device__ __forceinline__ Part operator()(int i) const { return p[i]; }
 };
+struct FourthParts {
+  const Fourths* p;
+  __device__ __forceinline__ Fourths operator()(int i) const { return p[i]; }
+};
+__device__ __forceinline__ const Part& whole(const Part& p) { return p; }
+__device__ __forceinline__ Part whole(const Fourths& p) {
+  return {(p.s[0] + p.s[1]) + (p.s[2] + p.s[3]), larger(larger(p.m[0], p.m[1]), larger(p.m[2], p.m[3])), p.arg};
+}
 struct Pairs {                                           // sums that other workgroups of this launch handed over
   const double2* p;
   __device__ __forceinline__ double2 operator()(int i) const { return make_double2(taken(&p[i].x), taken(&p[i].y)); }
@@ -396,22 +416,19 @@ template <int K, int G, typename F, typename W> __device__ __forceinline__ int p
   });
 }
 
-__device__ __forceinline__ double part_sum(const Part& p) { return (p.s[0] + p.s[1]) + (p.s[2] + p.s[3]); }
-__device__ __forceinline__ float part_max(const Part& p) { return larger(larger(p.m[0], p.m[1]), larger(p.m[2], p.m[3])); }
-
 // A row's largest logit, its lowest column, and the sum of its weights, from its parts. bad: the row has no distribution.
 struct Row { float m; int arg; double s; bool bad; };
-template <int K> __device__ __forceinline__ Row row_of(const Listed<Parts, K>& parts, double c) {
+template <typename G, int K> __device__ __forceinline__ Row row_of(const Listed<G, K>& parts, double c) {
   Row r{-INFINITY, INT32_MAX, 0.0, false};
-  parts.each([&](int, const Part& p) { r.m = larger(r.m, part_max(p)); });
+  parts.each([&](int, const auto& p) { r.m = larger(r.m, whole(p).m); });
   r.m = wave_all(r.m, larger);
   r.bad = !(r.m < INFINITY && r.m > -INFINITY);
   if (r.bad) return r;
   if (c == 0.0) {
-    parts.each([&](int, const Part& p) { if (part_max(p) == r.m) r.arg = min(r.arg, p.arg); });
+    parts.each([&](int, const auto& p) { if (whole(p).m == r.m) r.arg = min(r.arg, whole(p).arg); });
     r.arg = wave_min(r.arg);
   } else {
-    parts.each([&](int, const Part& p) { r.s += part_sum(p) * weight(part_max(p), r.m, c); });
+    parts.each([&](int, const auto& p) { r.s += whole(p).s * weight(whole(p).m, r.m, c); });
   }
   return r;
 }
@@ -469,14 +486,14 @@ __device__ void walk(const Verify& a, int b, const int32_t* drawn) {
 
 // The token drawn from a row, by one wave: the fourth of a chunk in which the running sum exceeds t, then its columns, a vector or two
 // to a lane (before the first one those up to the first boundary, after the last one the rest).
-template <typename T> __device__ __forceinline__ int draw(const T* z, const Verify& a, const Listed<Parts, 2>& parts, double c, double u) {
+template <typename T> __device__ __forceinline__ int draw(const T* z, const Verify& a, const Listed<FourthParts, 2>& parts, double c, double u) {
   const Row r = row_of(parts, c);
   if (r.bad || c == 0.0) return r.bad ? -1 : r.arg;
   const int lane = threadIdx.x & 63;
   const double m = r.m, upto = wave_scan64(r.s), t = u * lane_value(upto, 63);
   auto fourths = [&](auto f) {
-    parts.each([&](int i, const Part& p) {
-      const double w = weight(part_max(p), m, c);
+    parts.each([&](int i, const Fourths& p) {
+      const double w = weight(whole(p).m, m, c);
       // (of a fourth in which no column counts, some columns' lowest weights may have been added)
 #pragma unroll
       for (int k = 0; k < 4; ++k) f(4 * i + k, counts(p.m[k], m, c) ? p.s[k] * w : 0.0);
@@ -539,7 +556,7 @@ template <typename T> __device__ __forceinline__ int draw(const T* z, const Veri
 // The token of each node, one wave per row (-1: padding, or no distribution); the last of a sequence's rows follows the tree.
 template <typename T> __global__ __launch_bounds__(64) void verify_draw_kernel(const Verify a, int32_t* drawn, uint32_t* arrived) {
   const int row = blockIdx.x, b = row / a.T;
-  const Listed<Parts, 2> parts(Parts{a.parts + (int64_t)row * a.nch}, a.nch);
+  const Listed<FourthParts, 2> parts({a.fourths + (int64_t)row * a.nch}, a.nch);
   const double c = rate(a, b), u = random_at(a, row);
   const int parent = a.parents[b * a.ldp + row % a.T];
   const int token = parent >= -1 ? draw((const T*)a.z + (int64_t)row * a.ldz, a, parts, c, u) : -1;
@@ -649,18 +666,26 @@ template <typename T> struct Left {
   }
 };
 
-// Sums of p and of what is left of it, a wave to PIECE columns, grid (pieces / 4, sequences); the last workgroup of a sequence
+// Sums of p and of what is left of it, a wave to PIECE columns, grid (pieces / WAVES, sequences); the last workgroup of a sequence
 // draws its next token. Pieces are short, as one row of each sequence has to fill the chip.
-constexpr int PIECE = 512;
-template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(const Verify a, const Ended* ended, double2* sums,
+constexpr int PIECE = 512, WAVES = 16;
+template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_kernel(const Verify a, const Ended* ended, double2* sums,
                                                                                 uint32_t* arrived) {
   const int b = blockIdx.y, wid = threadIdx.x >> 6, lane = threadIdx.x & 63, pieces = (a.V + PIECE - 1) / PIECE;
   const Ended e = ended[b];
   if (e.mode == ENDED_KNOWN) return;
+  if (e.mode == ENDED_P) {                               // p's sums are there already
+    if (blockIdx.x || wid) return;
+    const int64_t at = (int64_t)b * (a.T + 1) + e.n;
+    const Listed<FourthParts, 2> parts({a.fourths + at * a.nch}, a.nch);
+    const int token = draw((const T*)a.z + at * a.ldz, a, parts, e.c, random_at(a, (int64_t)b * (a.T + 1) + a.T));
+    if (lane == 0) a.out_token[b] = token;
+    return;
+  }
   __shared__ bool last;
   const Left<T> row(a, e, b);
   double2* mine = sums + (int64_t)b * pieces;
-  const int piece = blockIdx.x * 4 + wid;
+  const int piece = blockIdx.x * WAVES + wid;
   if (piece < pieces) {
     const int lo = piece * PIECE, hi = min(lo + PIECE, a.V);
     constexpr int G = 4;
@@ -698,7 +723,7 @@ template <typename T> __global__ __launch_bounds__(256) void verify_next_kernel(
   double l = 0.0, p = 0.0;
   list.each([&](int, const double2& s) { l += s.x; p += s.y; });
   const double left = wave_sum64(l), whole = wave_sum64(p);
-  const bool all = e.mode == ENDED_P || left < LEAST;
+  const bool all = left < LEAST;
   const double t = random_at(a, (int64_t)b * (a.T + 1) + a.T) * (all ? whole : left);
   int some = -1;
   list.each([&](int i, const double2& s) { if ((all ? s.y : s.x) > 0.0) some = i; });
@@ -742,7 +767,6 @@ int verify_setup(Verify& a, const char* what, int dtype, int B, int T, int V, co
   a.tokens = tokens;
   a.u = u; a.temp = temperature; a.temps = temperatures;
   a.B = B; a.T = T; a.V = V; a.nch = (int)chunks_of(V);
-  a.parts = (Part*)workspace;
   a.out_counts = counts; a.out_token = token;
   return 0;
 }
@@ -751,7 +775,7 @@ int verify_setup(Verify& a, const char* what, int dtype, int B, int T, int V, co
 
 UNOK_EXPORT int64_t unok_verify_tree_workspace(int dtype, int B, int T, int V) {
   if (verify_sizes_ok("verify_tree", dtype, B, T, V, (int64_t)B * T)) return -1;
-  return ((int64_t)B * T * (chunks_of(V) * (int64_t)sizeof(Part) + (int64_t)sizeof(int32_t)) + B * 4ll + 15) / 16 * 16;
+  return ((int64_t)B * T * (chunks_of(V) * (int64_t)sizeof(Fourths) + (int64_t)sizeof(int32_t)) + B * 4ll + 15) / 16 * 16;
 }
 
 UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, int64_t ldz, const int64_t* tokens,
@@ -771,7 +795,8 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
   if (rc) return rc;
   a.parents = parents; a.ldp = ldp;
   a.nodes = nodes;
-  int32_t* drawn = (int32_t*)(a.parts + rows * a.nch);
+  a.fourths = (Fourths*)workspace;
+  int32_t* drawn = (int32_t*)(a.fourths + rows * a.nch);
   a.arrived = (uint32_t*)(drawn + rows);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(rows * ((a.nch + 3) / 4))), block(256);
@@ -787,7 +812,7 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
 
 UNOK_EXPORT int64_t unok_verify_draft_workspace(int dtype, int B, int L, int V) {
   if (verify_sizes_ok("verify_draft", dtype, B, L, V, (int64_t)B * (2 * L + 1))) return -1;
-  return ((int64_t)B * ((2 * L + 1) * chunks_of(V) * (int64_t)sizeof(Part) + pieces_of(V) * (int64_t)sizeof(double2) +
+  return ((int64_t)B * (chunks_of(V) * ((2 * L + 1) * (int64_t)sizeof(Part) + (L + 1) * (int64_t)sizeof(Fourths)) + pieces_of(V) * (int64_t)sizeof(double2) +
                         (int64_t)sizeof(Ended) + 4) + 15) / 16 * 16;
 }
 
@@ -807,7 +832,9 @@ UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z,
   UNOK_REQUIRE(((uintptr_t)y & (dtype == UNOK_BF16 ? 1 : 3)) == 0, UNOK_EALIGN, "verify_draft: logits at a fraction of an element");
   a.y = y; a.ldy = ldy;
   a.counts = counts;
-  double2* sums = (double2*)(a.parts + (targets + drafts) * a.nch);
+  a.parts = (Part*)workspace;
+  a.fourths = (Fourths*)(a.parts + (targets + drafts) * a.nch);
+  double2* sums = (double2*)(a.fourths + targets * a.nch);
   Ended* ended = (Ended*)(sums + (int64_t)B * pieces_of(V));
   uint32_t* arrived = (uint32_t*)(ended + B);
   hipStream_t st = (hipStream_t)stream;
@@ -817,7 +844,7 @@ UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z,
     using E = decltype(e);
     hipLaunchKernelGGL((verify_parts_kernel<E, false>), grid, block, 0, st, a);
     hipLaunchKernelGGL(verify_accept_kernel<E>, dim3((unsigned)B), dim3(1024), 0, st, a, ended, arrived);
-    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)((pieces_of(V) + 3) / 4), (unsigned)B), block, 0, st, a, ended, sums,
+    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)((pieces_of(V) + WAVES - 1) / WAVES), (unsigned)B), dim3(64 * WAVES), 0, st, a, ended, sums,
                        arrived);
   };
   if (dtype == UNOK_BF16) run(bf16_t{});
