@@ -9,27 +9,41 @@ namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
+static_assert(GROUP4 == 32, "rows have 2^(log_d - 5) scales");
 constexpr int TENSORS4 = 16;                          // per launch (their addresses are arguments)
+
+// n / d for 0 <= n < 2^31, d > 0: with 2^(bits - 1) < d <= 2^bits, 2^(31 + bits) / d rounded up has at most 32 bits, and exceeds the quotient
+// by less than 2^bits / 2^(31 + bits) of n, below 1 / d.
+struct Divisor {
+  uint32_t d, factor, bits;
+  __host__ __device__ Divisor() {}
+  explicit Divisor(uint32_t d_) : d(d_), bits(0) {
+    while ((1ull << bits) < d) ++bits;
+    factor = (uint32_t)(((1ull << (31 + bits)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (uint32_t)((uint64_t)n * factor >> (31 + bits)); }
+};
 
 struct Move4 {
   void* rows[TENSORS4]; int64_t ld[TENSORS4];         // [B T, nk D]
   uint8_t *codes[TENSORS4], *scales[TENSORS4];        // [B, nk, max_len, D / 2], [.., D / GROUP4]
   const int64_t* starts;
-  int T, nk, max_len, D;
+  int nk, max_len, log_d;
+  Divisor per_row, per_sequence;                      // threads to a row, rows to a sequence
   uint32_t items;                                     // threads: eight elements each
 };
 
 // The thread's eight elements: row, their offset in it, their cache row (none: negative), and their offset in that.
 struct Eight { int64_t row, cache; int at, d; };
 __device__ __forceinline__ Eight eight(const Move4& p, uint32_t i) {
-  const uint32_t per = (uint32_t)p.nk * p.D / 8;
   Eight e;
-  e.row = i / per;
-  e.at = (int)(i % per) * 8;
-  e.d = e.at % p.D;
-  const int b = (int)(e.row / p.T), t = (int)(e.row % p.T);
-  const int64_t start = p.starts[b], r = start < p.max_len && start > INT32_MIN ? start + t : -1;
-  e.cache = r >= 0 && r < p.max_len ? ((int64_t)b * p.nk + e.at / p.D) * p.max_len + r : -1;
+  const int D = 1 << p.log_d;
+  const uint32_t row = p.per_row.quotient(i), b = p.per_sequence.quotient(row);
+  e.row = row;
+  e.at = (int)(i - row * p.per_row.d) * 8;
+  e.d = e.at & (D - 1);
+  const int64_t start = p.starts[b], r = start < p.max_len && start > INT32_MIN ? start + (row - b * p.per_sequence.d) : -1;
+  e.cache = r >= 0 && r < p.max_len ? ((int64_t)b * p.nk + (e.at >> p.log_d)) * p.max_len + r : -1;
   return e;
 }
 
@@ -65,8 +79,8 @@ template <typename E> __global__ __launch_bounds__(256) void cache4_store_kernel
   codes = codes4<1>(codes, x[2], x[3], s);
   codes = codes4<2>(codes, x[4], x[5], s);
   codes = codes4<3>(codes, x[6], x[7], s);
-  *(uint32_t*)(p.codes[blockIdx.y] + e.cache * (p.D / 2) + e.d / 2) = byte == SCALE4_NAN ? 0u : codes;
-  if (e.d % GROUP4 == 0) p.scales[blockIdx.y][e.cache * (p.D / GROUP4) + e.d / GROUP4] = (uint8_t)byte;
+  *(uint32_t*)(p.codes[blockIdx.y] + (e.cache << (p.log_d - 1)) + e.d / 2) = byte == SCALE4_NAN ? 0u : codes;
+  if (e.d % GROUP4 == 0) p.scales[blockIdx.y][(e.cache << (p.log_d - 5)) + e.d / GROUP4] = (uint8_t)byte;
 }
 
 // Cache rows that do not exist read as zeros.
@@ -76,8 +90,8 @@ template <typename E> __global__ __launch_bounds__(256) void cache4_load_kernel(
   const Eight e = eight(p, i);
   uint32_t codes = 0, byte = SCALE4_MIN;
   if (e.cache >= 0) {
-    codes = *(const uint32_t*)(p.codes[blockIdx.y] + e.cache * (p.D / 2) + e.d / 2);
-    byte = p.scales[blockIdx.y][e.cache * (p.D / GROUP4) + e.d / GROUP4];
+    codes = *(const uint32_t*)(p.codes[blockIdx.y] + (e.cache << (p.log_d - 1)) + e.d / 2);
+    byte = p.scales[blockIdx.y][(e.cache << (p.log_d - 5)) + e.d / GROUP4];
   }
   const float s = scale4(byte);
   const u32x4_t v = {pair4<0>(codes, s), pair4<1>(codes, s), pair4<2>(codes, s), pair4<3>(codes, s)};
@@ -130,7 +144,10 @@ int move4(const char* what, bool store, int dtype, int ntensors, void* const* ro
   }
   Move4 p{};
   p.starts = starts;
-  p.T = T; p.nk = nk; p.max_len = max_len; p.D = D;
+  p.nk = nk; p.max_len = max_len;
+  p.log_d = D == 128 ? 7 : 6;
+  p.per_row = Divisor((uint32_t)(nk * (D / 8)));
+  p.per_sequence = Divisor((uint32_t)T);
   p.items = (uint32_t)(n * nk * (D / 8));
   hipStream_t st = (hipStream_t)stream;
   for (int t0 = 0; t0 < ntensors; t0 += TENSORS4) {
