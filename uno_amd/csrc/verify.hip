@@ -36,7 +36,7 @@ struct Verify {
   int B, T, V, nch;                                   // T: nodes of a tree, or drafted tokens
   Part* parts;                                        // drafted blocks: [target rows, then the drafter's][nch]
   Fourths* fourths;                                   // [target rows][nch]
-  uint32_t* arrived;                                  // of a tree's rows, drawn; 0 before
+  uint32_t* arrived;                                  // [B], 0 after the parts
   int64_t *nodes, *out_counts, *out_token;
 };
 
@@ -301,6 +301,7 @@ template <typename T, bool TREE> __global__ __launch_bounds__(256) void verify_p
     const int targets = a.B * (a.T + 1);
     if (row < targets) {
       b = row / (a.T + 1);
+      if (row % (a.T + 1) == 0 && chunk == 0 && (threadIdx.x & 63) == 0) a.arrived[b] = 0;
       if (row % (a.T + 1) > drafted(a, b)) return;
       z = (const T*)a.z + (int64_t)row * a.ldz;
     } else {
@@ -557,8 +558,7 @@ template <typename T> __device__ __forceinline__ int draw(const T* z, const Veri
 // of a sequence follows the tree. Workgroups that count their arrival in one place wait for each other: 16 sequences of 64 nodes 18 us
 // where each row has its own, in eights 9.3; 8 sequences of 16 nodes 6.8 and 8.0, since there waves of one CU wait for each other more.
 constexpr int DRAW_ALONE = 16, DRAW_ROWS = 8;            // up to DRAW_ALONE nodes each has a workgroup
-template <typename T, int ROWS> __global__ __launch_bounds__(64 * ROWS) void verify_draw_kernel(const Verify a, int32_t* drawn,
-                                                                                               uint32_t* arrived) {
+template <typename T, int ROWS> __global__ __launch_bounds__(64 * ROWS) void verify_draw_kernel(const Verify a, int32_t* drawn) {
   __shared__ int tokens[ROWS];
   const int b = blockIdx.y, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int node0 = blockIdx.x * ROWS, node = min(node0 + wid, a.T - 1);
@@ -576,25 +576,24 @@ template <typename T, int ROWS> __global__ __launch_bounds__(64 * ROWS) void ver
   __syncthreads();
   if (wid != 0) return;
   if (lane < ROWS && node0 + lane < a.T) hand_over(drawn + (int64_t)b * a.T + node0 + lane, tokens[lane]);
-  if (last_to_arrive(arrived + b, gridDim.x)) walk(a, b, drawn);
+  if (last_to_arrive(a.arrived + b, gridDim.x)) walk(a, b, drawn);
 }
 
 // ---- drafted blocks ------------------------------------------------------------------------------
 // Where a block's verification ended: row n of the target, and what the next token is drawn from (with the rows' largest logits
 // and one over their sums).
 struct Ended { int n, mode, token, rest; double c, mp, ip, mq, iq; };
+constexpr int WAVES = 16;
 enum : int { ENDED_KNOWN = 0, ENDED_P = 1, ENDED_ROW = 2, ENDED_POINT = 3 };   // token known; p; max(p - q, 0), q a row or one token
 
-// Accepts drafted tokens in order: one workgroup of 16 waves per sequence, a wave to a row at a time. Bound by latency: every load
-// of a row is issued before the first is waited for.
-template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kernel(const Verify a, Ended* ended, uint32_t* arrived) {
-  __shared__ Ended rows[VERIFY_NODES + 1];
-  __shared__ bool stop[VERIFY_NODES + 1];
-  const int b = blockIdx.x, wid = threadIdx.x >> 6, lane = threadIdx.x & 63, L = a.T, n = drafted(a, b);
+// Accepts drafted tokens in order: a wave of the workgroup to a row at a time. Bound by latency: every load of a row is issued before the
+// first is waited for. All of them get where it ended.
+template <typename T> __device__ __forceinline__ Ended accept(const Verify& a, int b, Ended* rows, bool* stop) {
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, L = a.T, n = drafted(a, b);
   const double c = rate(a, b);
   const Part* targets = a.parts + (int64_t)b * (L + 1) * a.nch;
   const Part* drafts = a.parts + ((int64_t)a.B * (L + 1) + (int64_t)b * L) * a.nch;
-  for (int i = wid; i <= n; i += 16) {
+  for (int i = wid; i <= n; i += WAVES) {
     const bool row = a.y && i < n && c != 0.0;           // the drafter's row is read
     const int64_t x = i < n ? a.tokens[(int64_t)b * L + i] : -1;
     const bool in = x >= 0 && x < a.V;
@@ -635,14 +634,13 @@ template <typename T> __global__ __launch_bounds__(1024) void verify_accept_kern
     if (lane == 0) { rows[i] = e; stop[i] = stops; }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int i = 0;
-    while (i < n && !stop[i]) ++i;
-    ended[b] = rows[i];
-    arrived[b] = 0;
-    a.out_counts[b] = i;
-    if (rows[i].mode == ENDED_KNOWN) a.out_token[b] = rows[i].token;
+  int first = 0;
+  for (int i = 0; i < n; i += 64) {
+    const uint64_t here = __ballot(i + lane < n && stop[i + lane]);
+    first = here ? i + __builtin_ctzll(here) : n;
+    if (here) break;
   }
+  return rows[first];
 }
 
 // p and what is left of it at column j.
@@ -677,13 +675,19 @@ template <typename T> struct Left {
   }
 };
 
-// Sums of p and of what is left of it, a wave to PIECE columns, grid (pieces / WAVES, sequences); the last workgroup of a sequence
-// draws its next token. Pieces are short, as one row of each sequence has to fill the chip.
-constexpr int PIECE = 512, WAVES = 16;
-template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_kernel(const Verify a, const Ended* ended, double2* sums,
-                                                                                uint32_t* arrived) {
+// Finds where a sequence ended (every workgroup for itself: 8 sequences of 15 tokens of 151936 15.3 us, with a kernel before it for that
+// 5.8 + 10.6 and a launch), then sums p and what is left of it, a wave to PIECE columns, grid (pieces / WAVES, sequences); the last
+// workgroup of a sequence draws its next token. Pieces are short, as one row of each sequence has to fill the chip.
+constexpr int PIECE = 512;
+template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_kernel(const Verify a, double2* sums) {
+  __shared__ Ended rows[VERIFY_NODES + 1];
+  __shared__ bool stop[VERIFY_NODES + 1];
   const int b = blockIdx.y, wid = threadIdx.x >> 6, lane = threadIdx.x & 63, pieces = (a.V + PIECE - 1) / PIECE;
-  const Ended e = ended[b];
+  const Ended e = accept<T>(a, b, rows, stop);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.out_counts[b] = e.n;
+    if (e.mode == ENDED_KNOWN) a.out_token[b] = e.token;
+  }
   if (e.mode == ENDED_KNOWN) return;
   if (e.mode == ENDED_P) {                               // p's sums are there already
     if (blockIdx.x || wid) return;
@@ -725,7 +729,7 @@ template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (wid == 0) {
-    const bool mylast = last_to_arrive(arrived + b, gridDim.x);
+    const bool mylast = last_to_arrive(a.arrived + b, gridDim.x);
     if (lane == 0) last = mylast;
   }
   __syncthreads();
@@ -815,10 +819,10 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
     using E = decltype(e);
     hipLaunchKernelGGL((verify_parts_kernel<E, true>), grid, block, 0, st, a);
     if (T <= DRAW_ALONE)
-      hipLaunchKernelGGL((verify_draw_kernel<E, 1>), dim3((unsigned)T, (unsigned)B), dim3(64), 0, st, a, drawn, a.arrived);
+      hipLaunchKernelGGL((verify_draw_kernel<E, 1>), dim3((unsigned)T, (unsigned)B), dim3(64), 0, st, a, drawn);
     else
       hipLaunchKernelGGL((verify_draw_kernel<E, DRAW_ROWS>), dim3((unsigned)((T + DRAW_ROWS - 1) / DRAW_ROWS), (unsigned)B),
-                         dim3(64 * DRAW_ROWS), 0, st, a, drawn, a.arrived);
+                         dim3(64 * DRAW_ROWS), 0, st, a, drawn);
   };
   if (dtype == UNOK_BF16) run(bf16_t{});
   else run(float{});
@@ -828,7 +832,7 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
 UNOK_EXPORT int64_t unok_verify_draft_workspace(int dtype, int B, int L, int V) {
   if (verify_sizes_ok("verify_draft", dtype, B, L, V, (int64_t)B * (2 * L + 1))) return -1;
   return ((int64_t)B * (chunks_of(V) * ((2 * L + 1) * (int64_t)sizeof(Part) + (L + 1) * (int64_t)sizeof(Fourths)) + pieces_of(V) * (int64_t)sizeof(double2) +
-                        (int64_t)sizeof(Ended) + 4) + 15) / 16 * 16;
+                        4) + 15) / 16 * 16;
 }
 
 UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z, int64_t ldz, const void* y, int64_t ldy,
@@ -850,17 +854,15 @@ UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z,
   a.parts = (Part*)workspace;
   a.fourths = (Fourths*)(a.parts + (targets + drafts) * a.nch);
   double2* sums = (double2*)(a.fourths + targets * a.nch);
-  Ended* ended = (Ended*)(sums + (int64_t)B * pieces_of(V));
-  uint32_t* arrived = (uint32_t*)(ended + B);
+  a.arrived = (uint32_t*)(sums + (int64_t)B * pieces_of(V));
   hipStream_t st = (hipStream_t)stream;
   const int groups = (a.nch + 3) / 4;
   const dim3 grid((unsigned)((targets + (y ? drafts : 0)) * groups)), block(256);
   auto run = [&](auto e) {
     using E = decltype(e);
     hipLaunchKernelGGL((verify_parts_kernel<E, false>), grid, block, 0, st, a);
-    hipLaunchKernelGGL(verify_accept_kernel<E>, dim3((unsigned)B), dim3(1024), 0, st, a, ended, arrived);
-    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)((pieces_of(V) + WAVES - 1) / WAVES), (unsigned)B), dim3(64 * WAVES), 0, st, a, ended, sums,
-                       arrived);
+    hipLaunchKernelGGL(verify_next_kernel<E>, dim3((unsigned)((pieces_of(V) + WAVES - 1) / WAVES), (unsigned)B), dim3(64 * WAVES), 0,
+                       st, a, sums);
   };
   if (dtype == UNOK_BF16) run(bf16_t{});
   else run(float{});
