@@ -357,9 +357,11 @@ int unok_tree_attn4(int dtype, int B, int T, int nq, int nk, int D, const void* 
                     float scale, void* o, int64_t ldo, void* workspace, int64_t ws_bytes, void* stream);
 /* Verification of drafted tokens against the target's logits z (V columns, element strides between rows) from random numbers u
  * in [0, 1). A row's weights at temperature t > 0 are exp((z - max z) / t), those below e^-700 zero; drawing a token at u takes the
- * lowest column at which their running sum exceeds u times their sum (fp64; u below 0 counts as 0, from 1 on it takes the last column with a weight); t = 0 takes the largest logit, the lowest column of equal
- * ones. t is temperatures[b] (device; what is not positive counts as 0), or `temperature` for all. A row with a NaN or +inf, or with
- * -inf alone, has no distribution: nothing is drawn from it (-1). workspace: the bytes that _workspace() says, 16-byte aligned.
+ * lowest column at which their running sum exceeds u times their sum (fp64; u below 0 counts as 0, from 1 on it takes the last
+ * column with a weight); t = 0 takes the largest logit, the lowest column of equal ones. t is temperatures[b] (device; what is not
+ * positive counts as 0), or `temperature` for all. A row with a NaN or +inf, or with -inf alone, has no distribution: nothing is
+ * drawn from it (-1). workspace: the bytes that _workspace() says, 16-byte aligned; it and the outputs share no memory with
+ * anything else.
  * unok_verify_draft: sequence b's rows b (L + 1) .. of z are the target's at its counts[b] <= L (null: L) drafted tokens [B, L] and
  * behind the last; rows b L .. of y the drafter's logits, from which the tokens were drawn (null: they were chosen, q is 1 there).
  * Token i is accepted while u[b, i] q_i < p_i; accepted[b] is their number, token[b] is drawn at u[b, L] from max(p - q, 0) at the

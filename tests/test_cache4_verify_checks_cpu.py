@@ -221,10 +221,14 @@ ENTRIES = [
                                    dict(B=60000, L=200, V=1 << 24), dict(z=None), dict(tokens=None), dict(u=None), dict(accepted=None),
                                    dict(token=None), dict(ws=None), dict(nws=8), dict(ws=BASE + 16392), dict(ldz=49), dict(ldy=49),
                                    dict(z=BASE + 2), dict(y=BASE + 4097), dict(temp=-1.0), dict(temp=float("nan")),
-                                   dict(temp=float("inf"))]),
+                                   dict(temp=float("inf")), dict(accepted=BASE + 12544), dict(accepted=BASE + 8200),
+                                   dict(counts=BASE + 12288), dict(token=BASE + 8448), dict(ws=BASE + 8192), dict(ws=BASE),
+                                   dict(y=BASE + 16384), dict(temps=BASE + 12292), dict(accepted=BASE + 596)]),
     ("unok_verify_tree", _tree, [dict(dtype=5), dict(B=-1), dict(T=-1), dict(T=0), dict(T=257), dict(V=0), dict(z=None), dict(tokens=None),
                                  dict(parents=None), dict(u=None), dict(nodes=None), dict(counts=None), dict(token=None), dict(ws=None),
-                                 dict(nws=8), dict(ldp=2), dict(ldz=49), dict(z=BASE + 1), dict(temp=-0.5), dict(temp=float("nan"))]),
+                                 dict(nws=8), dict(ldp=2), dict(ldz=49), dict(z=BASE + 1), dict(temp=-0.5), dict(temp=float("nan")),
+                                 dict(nodes=BASE + 8200), dict(nodes=BASE + 8456), dict(counts=BASE + 12304), dict(token=BASE + 8712),
+                                 dict(ws=BASE + 12288), dict(nodes=BASE), dict(temps=BASE + 16388)]),
     ("unok_verify_draft_workspace", lambda **o: [{**dict(dtype=1, B=1, L=2, V=50), **o}[n] for n in ("dtype", "B", "L", "V")],
      [dict(dtype=3), dict(B=-1), dict(L=257), dict(V=0)]),
     ("unok_verify_tree_workspace", lambda **o: [{**dict(dtype=1, B=1, T=2, V=50), **o}[n] for n in ("dtype", "B", "T", "V")],

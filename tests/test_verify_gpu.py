@@ -194,6 +194,26 @@ def test_extreme_random_numbers(dev, dtype):
         _check_tree(z, x.new_zeros(B, L + 1), torch.tensor([-1, 0, 0, 2], device=dev, dtype=torch.int32), u)
 
 
+@pytest.mark.parametrize("scale,temperature", [(1e9, 1.0), (50.0, 1e-7), (50.0, 1e-12), (1e4, 1e-3), (1e30, 1e30), (3e38, 1e36), (1e-30, 1e-32),
+                                               (1.0, 3e38), (1.0, 1e-38), (700.0, 1.0), (3e38, 1e-30)])
+def test_logits_and_temperatures_of_any_size(dev, scale, temperature):
+    """Logits around +- scale that differ by multiples of an fp32 step, of the temperature, and by infinities."""
+    B, L, V = 3, 4, 4100
+    temperature = float(torch.tensor(temperature))       # as fp32 has it
+    g = torch.Generator("cpu").manual_seed(17)
+    near = max(temperature, scale * 2.0 ** -22)
+    z = (scale * (1 - 2.0 ** -10) - near * 2 * torch.rand(B * (L + 1), V, generator=g).double()).float()
+    z[:, ::5] = -math.inf
+    z[:, 1::7] = -scale
+    z[2::3] = (-scale + near * torch.rand(V, generator=g).double()).float()
+    z[0, 2100:] = -math.inf
+    z = z.to(dev)
+    u = torch.rand(B, L + 1, generator=g).to(dev)
+    x = torch.zeros(B, L, device=dev, dtype=I64)
+    _check_draft(z, None, x, u, temperature=temperature)
+    _check_tree(z, x.new_zeros(B, L + 1), torch.tensor([-1, 0, 0, 2, 3], device=dev, dtype=torch.int32), u, temperature=temperature)
+
+
 def test_equal_logits(dev):
     """Flat rows: every border is a multiple of 1 / V, and u on a border belongs to the token behind it."""
     V = 4096

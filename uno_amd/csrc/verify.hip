@@ -3,14 +3,16 @@
 // A token is drawn by the inverse distribution function: the lowest index at which the running sum of the weights
 // exp((z - max z) / T) exceeds u times their sum. Of a vocabulary's 150 thousand borders between tokens some lie within an fp32
 // exponential's error (1e-7) of any u: with such weights about one token in 300 would be another one than the logits say, and
-// depend on the order of the sums. The weights and all sums are therefore fp64, with errors around 1e-15, and the vector units form
-// them about as fast as HBM delivers the logits (64 fused multiply-adds per clock and CU, some 20 to a weight).
+// depend on the order of the sums. The weights and all sums are therefore fp64, the weights to 4e-14.
 //
-// The logits are read once, in chunks of CHUNK columns, one wave each: a chunk's largest logit, the sum of its weights relative to
-// that, and the column of the largest. Everything else works on these parts, and on one chunk to a drawn token.
+// The logits are read once, in chunks of CHUNK columns, one wave each, of which little is kept: largest logits and sums of weights.
+// Everything else works on these parts, and on a fourth of a chunk to a drawn token. 16 trees of 64 nodes, 151936 bf16 columns: the
+// parts 99 us (59 at a large copy's rate; 12 fp64 and 3 other vector instructions to a weight, issued three quarters of the time,
+// bound it), the tokens and the paths 9. One row of 32000: 4.2 and 3.7 us, latency of loads and reductions.
 #include "common.h"
 #include "../../include/unok.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace {
@@ -41,21 +43,21 @@ struct Verify {
 };
 
 // 2^x at x = d c, -1022 <= x <= 0, of N numbers side by side: 2^n (1 + r q(r)), r = x - n in [-1/2, 1/2], q the polynomial through
-// (2^r - 1) / r at eight Chebyshev points. Relative error 2.1e-12, of both signs in turn (at 150 thousand columns it moves less than
-// one token in 10^6; another degree, 3.7e-14, takes 5% more time); exactly 1 at 0. n is the low half of x + 1.5 2^52.
+// (2^r - 1) / r at nine Chebyshev points. Relative error 3.7e-14; exactly 1 at 0. n is the low half of x + 1.5 2^52.
 template <int N> __device__ __forceinline__ void exp2_64(double (&d)[N], double c) {
   constexpr double ROUND = 0x1.8p52;
-  constexpr double Q[8] = {0x1.62e42fef9cc69p-1, 0x1.ebfbdff82a734p-3, 0x1.c6b08da70cce3p-5, 0x1.3b2ab70ad2565p-7,
-                           0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13, 0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
+  constexpr double Q[9] = {0x1.62e42fefa39efp-1, 0x1.ebfbdff823cedp-3, 0x1.c6b08d7047e52p-5,
+                           0x1.3b2ab7181b743p-7, 0x1.5d87fe86fe95bp-10, 0x1.4308ac85ad0bbp-13,
+                           0x1.ffcb9515726b1p-17, 0x1.63d13633755aap-20, 0x1.b63880e235143p-24};
   double t[N], r[N], q[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     t[i] = fma(d[i], c, ROUND);
     r[i] = fma(d[i], c, ROUND - t[i]);
-    q[i] = Q[7];
+    q[i] = Q[8];
   }
 #pragma unroll
-  for (int k = 6; k >= 0; --k)
+  for (int k = 7; k >= 0; --k)
 #pragma unroll
     for (int i = 0; i < N; ++i) q[i] = fma(q[i], r[i], Q[k]);
 #pragma unroll
@@ -154,9 +156,9 @@ __device__ __forceinline__ double wave_scan64(double v) {                // sum 
 }
 
 // Sums of weights by a table: 2^x = 2^(N / STEPS) (1 + r q(r)), N + r = STEPS x, r in [-1/2, 1/2], q the polynomial through
-// (2^(r / STEPS) - 1) / r at three Chebyshev points (relative error 9e-12, of both signs in turn). The table holds 2^(j / STEPS) with
+// (2^(r / STEPS) - 1) / r at three Chebyshev points (relative error 3.5e-14). The table holds 2^(j / STEPS) with
 // j / STEPS taken from the exponent, so that N joins it there whole.
-constexpr int STEP_BITS = 6, STEPS = 1 << STEP_BITS;
+constexpr int STEP_BITS = 8, STEPS = 1 << STEP_BITS;
 struct Steps {
   uint64_t v[STEPS];
   constexpr Steps() : v{} {
@@ -173,7 +175,7 @@ __device__ const Steps steps_of_two{};
 // s plus the weights of N logits (`least` in place of those below it); c in steps, k = 1.5 2^52 less the reference's whole step.
 template <int N> __device__ __forceinline__ double add_weights(const float* z, float least, double c, double k, const double* table,
                                                            double s) {
-  constexpr double Q[3] = {0x1.62e42fefa39efp-7, 0x1.ebfc1b10317efp-15, 0x1.c6b0ae350b0b5p-23};
+  constexpr double Q[3] = {0x1.62e42fefa39efp-9, 0x1.ebfbe3a9ac80cp-19, 0x1.c6b08f7c96000p-29};
   double t[N], r[N], w[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -244,11 +246,12 @@ template <typename T> __device__ __forceinline__ void chunk_part(const T* row, i
       arg = wave_min(first);
     } else {
       // (beside the chunk's largest, whose weight is 1, what lies below the lowest weight need not be exactly 0)
-      const double cs = c * STEPS, whole = rint((double)m * cs), low = (double)m + LOWEST / c;
+      const double cs = c * STEPS, whole = rint((double)m * cs);
+      const float least = (float)((double)m + LOWEST / c);
+      const double x = ((double)least - (double)m) * c;  // (LOWEST, unless its logit is no fp32 number's neighbour)
       double s[4] = {0.0, 0.0, 0.0, 0.0};
-      if (fabs(whole) < 0x1p50 && low > -3e38) {
+      if (fabs(whole) < 0x1p50 && x >= LOWEST - 10.0 && x <= LOWEST + 10.0) {
         const double k = 0x1.8p52 - whole;
-        const float least = (float)low;
 #pragma unroll
         for (int i = 0; i < N; i += 4) s[i * 4 / N] = add_weights<4>(z + i, least, cs, k, table, s[i * 4 / N]);
         if (edge) s[0] = add_weights<1>(&zh, least, cs, k, table, s[0]);
@@ -256,7 +259,7 @@ template <typename T> __device__ __forceinline__ void chunk_part(const T* row, i
         double f[1] = {-fma((double)m, cs, -whole)};     // (these are relative to the whole step next to m)
         exp2_64<1>(f, 1.0 / STEPS);
         sum = four_all(s, add64) * f[0];
-      } else {                                           // temperatures so low or high that steps or `low` leave their formats
+      } else {                                           // logits far from 0 by the temperature's measure, or temperatures far off
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
           const float x[4] = {z[i], z[i + 1], z[i + 2], z[i + 3]};
@@ -759,6 +762,20 @@ template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_
 int64_t pieces_of(int V) { return ((int64_t)V + PIECE - 1) / PIECE; }
 int64_t chunks_of(int V) { return ((int64_t)V + CHUNK - 1) / CHUNK; }
 
+struct Span { const void* p; int64_t bytes; };
+
+// What is written, the workspace among it, shares no memory with anything else: workgroups end at different times.
+int verify_apart(const char* what, std::initializer_list<Span> read, std::initializer_list<Span> written) {
+  auto meet = [](const Span& a, const Span& b) {
+    return a.p && b.p && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
+  };
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span& r : read) UNOK_REQUIRE(!meet(*w, r), UNOK_EINVAL, "%s: an output or the workspace overlaps an operand", what);
+    for (const Span* v = written.begin(); v != w; ++v) UNOK_REQUIRE(!meet(*w, *v), UNOK_EINVAL, "%s: outputs or the workspace overlap", what);
+  }
+  return 0;
+}
+
 int verify_sizes_ok(const char* what, int dtype, int B, int T, int V, int64_t rows) {
   UNOK_REQUIRE(dtype == UNOK_BF16 || dtype == UNOK_F32, UNOK_EINVAL, "%s: bad dtype %d", what, dtype);
   UNOK_REQUIRE(B >= 0 && T >= 0 && V > 0 && V <= (1 << 30), UNOK_EINVAL, "%s: B=%d T=%d V=%d", what, B, T, V);
@@ -808,6 +825,11 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
   rc = verify_setup(a, "verify_tree", dtype, B, T, V, z, ldz, rows, tokens, u, temperature, temperatures, counts, token, workspace,
                     ws_bytes, unok_verify_tree_workspace(dtype, B, T, V));
   if (rc) return rc;
+  const int64_t es = dtype == UNOK_BF16 ? 2 : 4, ids = rows * (int64_t)sizeof(int64_t), each = B * (int64_t)sizeof(int64_t);
+  rc = verify_apart("verify_tree",
+                    {{z, ((rows - 1) * ldz + V) * es}, {tokens, ids}, {parents, ((B - 1) * ldp + T) * 4}, {u, rows * 4}, {temperatures, B * 4ll}},
+                    {{nodes, ids}, {counts, each}, {token, each}, {workspace, unok_verify_tree_workspace(dtype, B, T, V)}});
+  if (rc) return rc;
   a.parents = parents; a.ldp = ldp;
   a.nodes = nodes;
   a.fourths = (Fourths*)workspace;
@@ -849,6 +871,12 @@ UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z,
   if (rc) return rc;
   UNOK_REQUIRE(!y || drafts <= 1 || ldy >= V, UNOK_EINVAL, "verify_draft: draft rows of %d logits, %lld apart", V, (long long)ldy);
   UNOK_REQUIRE(((uintptr_t)y & (dtype == UNOK_BF16 ? 1 : 3)) == 0, UNOK_EALIGN, "verify_draft: logits at a fraction of an element");
+  const int64_t es = dtype == UNOK_BF16 ? 2 : 4, each = B * (int64_t)sizeof(int64_t);
+  rc = verify_apart("verify_draft",
+                    {{z, ((targets - 1) * ldz + V) * es}, {y, drafts ? ((drafts - 1) * ldy + V) * es : 0}, {tokens, drafts * 8}, {counts, each},
+                     {u, targets * 4}, {temperatures, B * 4ll}},
+                    {{accepted, each}, {token, each}, {workspace, unok_verify_draft_workspace(dtype, B, L, V)}});
+  if (rc) return rc;
   a.y = y; a.ldy = ldy;
   a.counts = counts;
   a.parts = (Part*)workspace;
