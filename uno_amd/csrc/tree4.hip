@@ -7,7 +7,7 @@
 // this 257.)
 //
 // Measured: one node of 4 sequences over 65536 rows 44 us (232 MB of codes and scales, 5.3 TB/s: what a large copy reaches); 64 nodes of 16
-// sequences over 16384 rows 257 us (820 TFLOP/s; conversions, weights and their rounding, some 200 vector instructions to 32 keys and 32
+// sequences over 16384 rows 257 us (820 TFLOP/s; conversions, weights and their rounding, some 190 vector instructions to 32 keys and 32
 // rows, bound it: the products alone would take 173); 16 nodes of 8 sequences over 4096 rows 22 us (6 at the copy's rate: 16 tiles to a
 // wave, the rest is the queries, the join and the launch).
 //
@@ -219,11 +219,12 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
       }
     }
   f32x4_t o[QT][NDT];
-  float mref[QT], l[QT];
+  float mref[QT];
+  f32x4_t l[QT];                                         // sums of the weights, as a product with ones (254 us; as 16 additions to a tile 260)
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     mref[i] = -INFINITY;
-    l[i] = 0.f;
+    l[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NDT; ++c) o[i][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -297,11 +298,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
   auto weights = [&](int i, const f32x4_t (&s)[2], float (&p)[8]) {
     const float ref = mref[i] == -INFINITY ? 0.f : -mref[i];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], a.walk_scale, ref));
-      l[i] += p[j];
-    }
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j / 4][j % 4], a.walk_scale, ref));
   };
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, u4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   auto add_pv = [&](int i, const bf16x8_t (&v)[NDT], float (&p)[8]) {
     bf16x8_t pf[PARTS];
 #pragma unroll
@@ -320,9 +319,11 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
       pf[part] = __builtin_bit_cast(bf16x8_t, u);
     }
 #pragma unroll
-    for (int part = PARTS - 1; part >= 0; --part)
+    for (int part = PARTS - 1; part >= 0; --part) {
+      l[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[part], l[i], 0, 0, 0);
 #pragma unroll
       for (int c = 0; c < NDT; ++c) o[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[c], pf[part], o[i][c], 0, 0, 0);
+    }
   };
 
   const uint32_t at = lds_addr(mine);
@@ -343,18 +344,13 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
     for (int j = 0; j < 8; ++j) vf[j] = t.v_scale(j, m);
     scores(t, s);
     values(t, vf, v);
-    // the scores' products run while the codes are converted (held here: the compiler would move V's behind the branch)
+    // the scores' products run while the codes are converted (held here: the compiler would move V's behind the
+    // branch; 16 sequences, 64 nodes over 16384 rows 257 us, 267 without)
 #pragma unroll
     for (int c = 0; c < NDT; ++c) {
       u4 u = __builtin_bit_cast(u4, v[c]);
       asm volatile("" : "+v"(u));
       v[c] = __builtin_bit_cast(bf16x8_t, u);
-    }
-    __builtin_amdgcn_sched_group_barrier(SG_VALU, 6, 0);
-#pragma unroll
-    for (int i = 0; i < 2 * KS * QT * PARTS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(SG_VALU, QT == 1 ? 12 : 6, 0);
     }
     reference(s);
     // and the weighted values' while the next rows' weights are formed
@@ -363,14 +359,6 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
       float p[8];
       weights(i, s[i], p);
       add_pv(i, v, p);
-    }
-    if constexpr (QT > 1) {
-      __builtin_amdgcn_sched_group_barrier(SG_VALU, 28, 0);
-#pragma unroll
-      for (int i = 0; i < NDT * (QT - 1); ++i) {
-        __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(SG_VALU, 32 / NDT, 0);
-      }
     }
     next_tile();
   }
@@ -444,7 +432,10 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
 #pragma unroll
     for (int i = 0; i < QT; ++i) merge_pad[16 * i + m] = parent[i] < -1;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // no load is on its way into what becomes the merge's
-  tree_merge<E, D, QT>(a, range, tile, h, id, o, mref, l, (float*)lds, merge_ml, merge_pad,
+  float sum[QT];                                         // (each lane has its query's whole sum; the merge adds four lanes')
+#pragma unroll
+  for (int i = 0; i < QT; ++i) sum[i] = g == 0 ? l[i][0] : 0.f;
+  tree_merge<E, D, QT>(a, range, tile, h, id, o, mref, sum, (float*)lds, merge_ml, merge_pad,
                        [](int c, int e, int g) { return (4 * g + e) * NDT + c; });
 }
 
