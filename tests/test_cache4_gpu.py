@@ -505,3 +505,49 @@ def test_captured_and_replayed(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
         torch.randn(4096, device=dev).sum().item()
+
+
+def test_two_streams_at_once(dev):
+    """Calls of one cache on several streams, each with its own workspace."""
+    g = torch.Generator(device=dev).manual_seed(23)
+    B, T, nq, nk, D, n = 3, 20, 8, 2, 128, 2000
+    k, v = ((torch.randn(B * n, nk * D, device=dev, generator=g)).to(BF) for _ in range(2))
+    caches = [K.Rows4(torch.zeros(B, nk, n, D // 2, device=dev, dtype=torch.uint8), torch.zeros(B, nk, n, D // 32, device=dev, dtype=torch.uint8))
+              for _ in range(2)]
+    K.cache4_store((k, v), caches, torch.zeros(B, device=dev, dtype=torch.int64))
+    lengths = torch.tensor([1900, 700, 0], device=dev)
+    parents = torch.tensor([-1] + [i // 2 for i in range(T - 1)], device=dev, dtype=torch.int32)
+    q = torch.randn(B * T, nq * D, device=dev, generator=g).to(BF)
+    want, rows = K.tree_attn4(q, *caches, lengths, parents), K.cache4_load(caches, lengths, T)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s in [torch.cuda.Stream() for _ in range(3)]:
+            with torch.cuda.stream(s):
+                got.append((K.tree_attn4(q, *caches, lengths, parents), *K.cache4_load(caches, lengths, T)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, (want, *rows)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,heads", [(12, (8, 2, 128)), (70, (4, 2, 64))])
+def test_a_query_without_numbers_leaves_the_others(dev, dtype, T, heads):
+    """A row of NaN or infinities among the queries: its own output is NaN, every other row keeps its bits."""
+    nq, nk, D = heads
+    g = torch.Generator(device=dev).manual_seed(29)
+    B, n = 2, 300 + T
+    rows = [torch.randn(B * n, nk * D, device=dev, generator=g).to(dtype) for _ in range(2)]
+    caches = [K.Rows4(torch.zeros(B, nk, n, D // 2, device=dev, dtype=torch.uint8), torch.zeros(B, nk, n, D // 32, device=dev, dtype=torch.uint8))
+              for _ in range(2)]
+    K.cache4_store(rows, caches, torch.zeros(B, device=dev, dtype=torch.int64))
+    lengths = torch.tensor([300, 17], device=dev)
+    parents = torch.tensor([-1] + [i // 3 for i in range(T - 1)], device=dev, dtype=torch.int32)
+    q = torch.randn(B * T, nq * D, device=dev, generator=g).to(dtype)
+    want = K.tree_attn4(q, *caches, lengths, parents)
+    for bad in (math.nan, math.inf):
+        p = q.clone()
+        p[3, :D], p[T + 5, D:2 * D] = bad, bad
+        got = K.tree_attn4(p, *caches, lengths, parents)
+        assert got[3, :D].isnan().all() and got[T + 5, D:2 * D].isnan().all()
+        got[3, :D], got[T + 5, D:2 * D] = want[3, :D], want[T + 5, D:2 * D]
+        assert torch.equal(got, want)

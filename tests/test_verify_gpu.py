@@ -418,3 +418,57 @@ def test_captured_and_replayed(dev):
         want = [*_draft(z, y, x.cpu(), u.cpu(), counts, temps), *_tree(z, tokens.cpu(), parents.cpu(), u.cpu(), temps)]
         assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
         torch.randn(4096, device=dev).sum().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,skip", [(1, 3), (9, 1), (511, 0), (513, 3), (1100, 5), (2047, 7), (2050, 1), (2560, 2), (5003, 1)])
+def test_every_token_of_flat_rows(dev, dtype, V, skip):
+    """Rows of equal logits at any alignment: u in the middle of token j's share draws j, from p and from what a refused token leaves."""
+    B = min(V, 1300)
+    z = torch.full((B, V + 9), 2.0, device=dev).to(dtype)[:, skip:skip + V]
+    j = (torch.arange(B, device=dev) * V) // B
+    u = ((j + 0.5) / V).float()[:, None]
+    parents = torch.full((B, 1), -1, device=dev, dtype=torch.int32)
+    assert torch.equal(K.verify_tree(z, torch.zeros(B, 1, device=dev, dtype=I64), parents, u)[2], j)
+    assert torch.equal(K.verify_draft(z, None, torch.zeros(B, 0, device=dev, dtype=I64), u)[1], j)
+    if V == 1:
+        return
+    x = (j * 7 + 3) % V                                  # refused (u = 1 > p), then token i of the V - 1 others
+    i = (torch.arange(B, device=dev) * (V - 1)) // B
+    both = torch.stack([torch.ones(B, device=dev), (i + 0.5) / (V - 1)], 1).float()
+    z2 = torch.full((2 * B, V + 9), 2.0, device=dev).to(dtype)[:, skip:skip + V]
+    accepted, token = K.verify_draft(z2, None, x[:, None], both)
+    assert not accepted.any() and torch.equal(token, i + (i >= x))
+    y = torch.where(torch.arange(V, device=dev) == x[:, None], 2.0, -math.inf).to(dtype)   # the same by a drafter that was certain
+    accepted, token = K.verify_draft(z2, y, x[:, None], both)
+    assert not accepted.any() and torch.equal(token, i + (i >= x))
+
+
+def test_two_streams_at_once(dev):
+    z, y, x, u = _drafted(dev, 4, 15, 40000, BF, 3)
+    parents = torch.arange(-1, 15, device=dev, dtype=torch.int32)
+    nodes = torch.cat([x.new_zeros(4, 1), x], 1)
+    want = (*K.verify_draft(z, y, x, u), *K.verify_tree(z, nodes, parents, u))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((*K.verify_draft(z, y, x, u), *K.verify_tree(z, nodes, parents, u)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_outputs_depend_on_the_operands_alone(dev):
+    """A sequence's tokens do not change with the sequences beside it, nor with the number of rows."""
+    z, y, x, u = _drafted(dev, 6, 20, 3000, F32, 5)
+    accepted, token = K.verify_draft(z, y, x, u)
+    parents = torch.arange(-1, 20, device=dev, dtype=torch.int32)
+    nodes = torch.cat([x.new_zeros(6, 1), x], 1)
+    tree = K.verify_tree(z, nodes, parents, u)
+    for b in range(6):
+        own = slice(b * 21, (b + 1) * 21)
+        one = K.verify_draft(z[own], y[b * 20:(b + 1) * 20], x[b:b + 1], u[b:b + 1])
+        assert one[0] == accepted[b] and one[1] == token[b]
+        assert all(torch.equal(a[0], t[b]) for a, t in zip(K.verify_tree(z[own], nodes[b:b + 1], parents, u[b:b + 1]), tree))

@@ -8,7 +8,7 @@
 //
 // Measured: one node of 4 sequences over 65536 rows 44 us (232 MB of codes and scales, 5.3 TB/s: what a large copy reaches); 64 nodes of 16
 // sequences over 16384 rows 257 us (820 TFLOP/s; conversions, weights and their rounding, some 190 vector instructions to 32 keys and 32
-// rows, bound it: the products alone would take 173); 16 nodes of 8 sequences over 4096 rows 22 us (6 at the copy's rate: 16 tiles to a
+// rows, bound it: the products alone would take 173); 16 nodes of 8 sequences over 4096 rows 22 us (6 at the copy's rate: eight tiles to a
 // wave, the rest is the queries, the join and the launch).
 //
 // fp32 queries: a query is the sum of three bf16 numbers (each what the ones before it leave, 8 of its 24 bits), and so is a weight;
