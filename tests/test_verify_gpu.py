@@ -472,3 +472,10 @@ def test_outputs_depend_on_the_operands_alone(dev):
         one = K.verify_draft(z[own], y[b * 20:(b + 1) * 20], x[b:b + 1], u[b:b + 1])
         assert one[0] == accepted[b] and one[1] == token[b]
         assert all(torch.equal(a[0], t[b]) for a, t in zip(K.verify_tree(z[own], nodes[b:b + 1], parents, u[b:b + 1]), tree))
+
+
+def test_single_nodes_that_are_padding(dev):
+    z, _, x, u = _drafted(dev, 4, 1, 700, BF, 31)
+    parents = torch.tensor([[-1], [-2], [-1], [-5]], device=dev, dtype=torch.int32)
+    nodes, counts, _ = _check_tree(z[:4], x, parents, u[:, :1].contiguous())
+    assert counts.tolist() == [1, 0, 1, 0] and nodes.tolist() == [[0], [-1], [0], [-1]]

@@ -36,7 +36,8 @@ template <int D> __device__ __forceinline__ Buffer4 buffer4(const void* codes, c
 
 // Tiles of 32 keys: codes and scales go from memory straight into LDS, NST - 1 tiles ahead, each wave's into its own part, so that
 // nothing but the wave's own counter of loads is waited for. (Two tiles in registers, one of them on its way: 16 sequences, 64 nodes over
-// 16384 rows 309 us, three spill: 518.) A stage: K's codes, V's codes, a dword to a key for its scales of K, and of V. A lane (m, g), m < 16, g < 4, reads
+// 16384 rows 309 us, three spill: 518.) A stage: K's codes, V's codes, a dword to a key for its scales of K, and of V. A lane (m, g),
+// m < 16, g < 4, reads
 //   K (S^T = K Q^T, first operand: 16 keys x 8 dims a lane): the dims of a product may come in any order that Q takes too; lane group g
 //     has dims D/4 g .. of key m and of key 16 + m: one read each, of one scale;
 //   V (O^T = V^T P^T, first operand: one dim x 8 keys): lane m has dims D/16 m .. of keys 4 g .. + 3 and 16 + 4 g .. + 3, which are

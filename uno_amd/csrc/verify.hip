@@ -747,7 +747,8 @@ template <typename T> __global__ __launch_bounds__(64 * WAVES) void verify_next_
   list.each([&](int i, const double2& s) { if ((all ? s.y : s.x) > 0.0) some = i; });
   double base = 0.0;
   bool over;
-  const int at = pick(base, over, t, wave_scan64(all ? p : l), all ? p : l, some, [&](auto f) { list.each([&](int i, const double2& s) { f(i, all ? s.y : s.x); }); });
+  const int at = pick(base, over, t, wave_scan64(all ? p : l), all ? p : l, some,
+                      [&](auto f) { list.each([&](int i, const double2& s) { f(i, all ? s.y : s.x); }); });
   int token = -1;
   if (at >= 0)
     token = pick_column<PIECE / 64, 4>(at * PIECE, min(at * PIECE + PIECE, a.V), base, t, [&](int j) { return row.get(j); },
@@ -853,8 +854,8 @@ UNOK_EXPORT int unok_verify_tree(int dtype, int B, int T, int V, const void* z, 
 
 UNOK_EXPORT int64_t unok_verify_draft_workspace(int dtype, int B, int L, int V) {
   if (verify_sizes_ok("verify_draft", dtype, B, L, V, (int64_t)B * (2 * L + 1))) return -1;
-  return ((int64_t)B * (chunks_of(V) * ((2 * L + 1) * (int64_t)sizeof(Part) + (L + 1) * (int64_t)sizeof(Fourths)) + pieces_of(V) * (int64_t)sizeof(double2) +
-                        4) + 15) / 16 * 16;
+  const int64_t chunks = chunks_of(V) * ((2 * L + 1) * (int64_t)sizeof(Part) + (L + 1) * (int64_t)sizeof(Fourths));
+  return (B * (chunks + pieces_of(V) * (int64_t)sizeof(double2) + 4) + 15) / 16 * 16;
 }
 
 UNOK_EXPORT int unok_verify_draft(int dtype, int B, int L, int V, const void* z, int64_t ldz, const void* y, int64_t ldy,
