@@ -19,19 +19,26 @@
 
 namespace {
 
-// Rows of K and V of one (sequence, K/V head) pair, loaded through buffers that end behind the last row: what lies past it reads as
-// zeros, and a lane's place in a tile is one offset for all tiles.
-struct Buffer4 {
-  __amdgpu_buffer_rsrc_t codes, scales;
+// A range's rows of K or V of one (sequence, K/V head) pair, wave-uniform addresses.
+struct Rows4 {
+  uintptr_t codes, scales;
 };
-template <int D> __device__ __forceinline__ Buffer4 buffer4(const void* codes, const uint8_t* scales, int64_t row, int rows) {
-  auto make = [&](const uint8_t* p, int bytes) {
-    const uintptr_t at = (uintptr_t)(p + row * bytes);
-    const uintptr_t u = ((uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
-    return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, __builtin_amdgcn_readfirstlane(rows) * bytes, 0x00020000);
+template <int D> __device__ __forceinline__ Rows4 rows4(const void* codes, const uint8_t* scales, int64_t row) {
+  auto uniform = [](uintptr_t at) {
+    return ((uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
   };
-  return {make((const uint8_t*)codes, D / 2), make(scales, D / GROUP4)};
+  return {uniform((uintptr_t)codes + row * (D / 2)), uniform((uintptr_t)scales + row * (D / GROUP4))};
+}
+// The rows from `key` on, of `rows` in all, as a buffer that ends behind the last: what lies past it reads as zeros, and of a tile past it
+// nothing is loaded. A tile's place is in its buffer's base, so that a lane's offset alone is held against the buffer's size. (In the loads'
+// scalar offset it would pass that size for tiles past the end, where the size less the scalar offset, which a raw buffer's range check
+// uses, is below zero.)
+__host__ __device__ constexpr int rows_left(int key, int rows) { return key < rows ? rows - key : 0; }
+static_assert(rows_left(0, 130) == 130 && rows_left(128, 130) == 2 && rows_left(130, 130) == 0 && rows_left(512, 130) == 0,
+              "no row past the last is in a buffer");
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer4(uintptr_t first, int key, int rows, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(first + (int64_t)key * bytes), (short)0, rows_left(key, rows) * bytes, 0x00020000);
 }
 
 // Tiles of 32 keys: codes and scales go from memory straight into LDS, NST - 1 tiles ahead, each wave's into its own part, so that
@@ -54,25 +61,27 @@ template <int D> struct Tile4 {
   uint32_t ks[2], v[8];
   u4 vs[2];
 
-  // The wave's loads of the tile at `key` into a stage; lane offsets as `places` gives them.
+  // The wave's loads of the tile at `key`, of `rows` rows in all, into a stage; lane offsets as `places` gives them.
   static __device__ __forceinline__ int2 places(int lane) {
     const int place = lane * 16 / CR, q = place % 16, row = place / 16 * 16 + 4 * (q % 4) + q / 4;
     return make_int2(lane * 16, row * CR + lane * 16 % CR);
   }
-  static __device__ __forceinline__ void issue(const Buffer4& kb, const Buffer4& vb, int key, int2 at, int lane, char* stage) {
+  static __device__ __forceinline__ void issue(const Rows4& k, const Rows4& v, int key, int rows, int2 at, int lane, char* stage) {
     typedef __attribute__((address_space(3))) void* Lds;
+    const __amdgpu_buffer_rsrc_t kc = buffer4(k.codes, key, rows, CR), vc = buffer4(v.codes, key, rows, CR);
+    const __amdgpu_buffer_rsrc_t ks = buffer4(k.scales, key, rows, SR), vs = buffer4(v.scales, key, rows, SR);
 #pragma unroll
     for (int i = 0; i < CODES / 1024; ++i) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.codes, (Lds)(stage + 1024 * i), 16, at.x, key * CR + 1024 * i, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.codes, (Lds)(stage + CODES + 1024 * i), 16, at.y, key * CR + 1024 * i, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kc, (Lds)(stage + 1024 * i), 16, at.x + 1024 * i, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vc, (Lds)(stage + CODES + 1024 * i), 16, at.y + 1024 * i, 0, 0, 0);
     }
     const Lds kx = (Lds)(stage + 2 * CODES), vx = (Lds)(stage + 2 * CODES + SCALES);
     if constexpr (D == 128) {                            // (the size has to be a literal)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.scales, kx, 4, lane * SR, key * SR, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.scales, vx, 4, lane * SR, key * SR, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, kx, 4, lane * SR, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, vx, 4, lane * SR, 0, 0, 0);
     } else {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kb.scales, kx, 2, lane * SR, key * SR, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vb.scales, vx, 2, lane * SR, key * SR, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, kx, 2, lane * SR, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, vx, 2, lane * SR, 0, 0, 0);
     }
   }
   // Reads the stage at LDS address `at` once its loads have arrived (the later tiles' may be on their way; the compiler, which cannot
@@ -179,16 +188,16 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
   const bool tree = hi > n, small = T <= 64;
   const int up = tree && small && lane < T ? a.parents[b * a.ldp + lane] : -2;
 
-  // from the range's first row on: the buffers' offsets are 32-bit
   const int64_t row0 = ((int64_t)b * a.nk + h) * a.max_len + lo;
-  const Buffer4 kb = buffer4<D>(a.k, a.ks, row0, hi - lo), vb = buffer4<D>(a.v, a.vs, row0, hi - lo);
-  const int full = min(hi, n) - lo, all = hi - lo;       // committed rows, which every query sees, and rows, of this range
+  const Rows4 kr = rows4<D>(a.k, a.ks, row0), vr = rows4<D>(a.v, a.vs, row0);
+  // committed rows, which every query sees, and rows, of this range
+  const int full = __builtin_amdgcn_readfirstlane(min(hi, n) - lo), all = __builtin_amdgcn_readfirstlane(hi - lo);
   char* const mine = lds + wid * Tile::NST * Tile::STAGE;
   const int2 place = Tile::places(lane);
   int key = wid * KT, stage = 0;
   if (tree && !small) tree_ancestors(a.parents + b * a.ldp, T, anc, next);
 #pragma unroll
-  for (int i = 0; i < Tile::NST; ++i) Tile::issue(kb, vb, key + 4 * i * KT, place, lane, mine + i * Tile::STAGE);
+  for (int i = 0; i < Tile::NST; ++i) Tile::issue(kr, vr, key + 4 * i * KT, all, place, lane, mine + i * Tile::STAGE);
 
   // what the queries see of the tree, of at most 64 nodes in registers (written to LDS, they would wait for the loads on their way there)
   const int W = (T + 31) / 32;
@@ -329,7 +338,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
 
   const uint32_t at = lds_addr(mine);
   auto next_tile = [&] {                                  // its stage gets the tile NST behind it (zeros past the end)
-    Tile::issue(kb, vb, key + 4 * Tile::NST * KT, place, lane, mine + stage * Tile::STAGE);
+    Tile::issue(kr, vr, key + 4 * Tile::NST * KT, all, place, lane, mine + stage * Tile::STAGE);
     key += 4 * KT;
     stage = stage + 1 < Tile::NST ? stage + 1 : 0;
   };
