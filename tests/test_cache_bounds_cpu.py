@@ -139,3 +139,26 @@ def test_maps_stay_in_the_cache(cache):
     for b in range(B):
         for m in (iv[b, :, 0], iv[b, :, 1] - 1, store[b]):
             assert bool(((m >= b * LEN) & (m < (b + 1) * LEN)).all())
+
+
+def test_caches_of_a_class_of_their_own(cache):
+    """Copies go by the form of the rows, not by the caches' class: a program's own kind of cache copies from a plain one and back."""
+    class Mine(inference.BlockKVCache):
+        pass
+
+    class Mine4(inference.BlockKVCache4):
+        pass
+
+    dec = _decoder()
+    mine = Mine(dec.geo, 1, B, LEN, "cpu", torch.float32)
+    cache.lengths[0] = 9
+    mine.copy_from(cache, [(0, 1)])
+    cache.copy_from(mine, [(1, 1)])
+    assert mine.lengths.tolist() == [0, 9] and cache.lengths.tolist() == [9, 9]
+    four, mine4 = dec.new_cache(B, LEN, bits=4), Mine4(dec.geo, 1, B, LEN, "cpu", torch.float32)
+    four.lengths[1] = 7
+    mine4.copy_from(four, [(1, 0)])
+    assert mine4.lengths.tolist() == [7, 0]
+    for a, b in ((cache, four), (four, cache), (mine, mine4), (mine4, mine), (mine, four), (cache, mine4)):
+        with pytest.raises(RuntimeError, match="do not go into"):
+            a.copy_from(b, [(0, 1)])

@@ -91,7 +91,7 @@ class BlockKVCache:
         layers and their number. ``other`` may be this cache; then no slot is both read and written. No slot is written
         twice. Both hold their rows in the same form. (Reads ``other``'s lengths on the host only if it can hold more rows than
         this cache.)"""
-        if type(other) is not type(self):
+        if isinstance(other, BlockKVCache4) != isinstance(self, BlockKVCache4):
             raise RuntimeError(f"rows of a {type(other).__name__} do not go into a {type(self).__name__}")
         pairs = [(int(a), int(b)) for a, b in pairs]
         if not pairs:
