@@ -551,3 +551,14 @@ def test_a_query_without_numbers_leaves_the_others(dev, dtype, T, heads):
         assert got[3, :D].isnan().all() and got[T + 5, D:2 * D].isnan().all()
         got[3, :D], got[T + 5, D:2 * D] = want[3, :D], want[T + 5, D:2 * D]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_caches_of_no_rows(dev, dtype):
+    """A cache without rows takes none, and all of its rows read as zeros."""
+    B, nk, D, T = 2, 3, 64, 5
+    caches = [_cache(dev, B, nk, 0, D) for _ in "kv"]
+    starts = torch.tensor([0, -2], device=dev)
+    K.cache4_store([torch.ones(B * T, nk * D, device=dev, dtype=dtype)] * 2, caches, starts)
+    for rows in K.cache4_load(caches, starts, T, dtype=dtype):
+        assert rows.shape == (B * T, nk * D) and rows.dtype == dtype and not rows.any()

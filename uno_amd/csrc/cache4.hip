@@ -140,7 +140,7 @@ int move4(const char* what, bool store, int dtype, int ntensors, void* const* ro
   const int64_t es = dtype == UNOK_BF16 ? 2 : 4, n = (int64_t)B * T, width = (int64_t)nk * D;
   const int64_t cbytes = (int64_t)B * nk * max_len * (D / 2), sbytes = (int64_t)B * nk * max_len * (D / GROUP4);
   for (int i = 0; i < ntensors; ++i) {
-    UNOK_REQUIRE(rows[i] && codes[i] && scales[i], UNOK_EINVAL, "%s: null operand", what);
+    UNOK_REQUIRE(rows[i] && ((codes[i] && scales[i]) || max_len == 0), UNOK_EINVAL, "%s: null operand", what);
     UNOK_REQUIRE((((uintptr_t)rows[i] | (uintptr_t)codes[i] | (uintptr_t)scales[i]) & 15) == 0 && ld[i] * es % 16 == 0, UNOK_EALIGN,
                  "%s: rows, codes and scales of tensor %d and the rows' stride must be multiples of 16 bytes", what, i);
     UNOK_REQUIRE(n == 1 || ld[i] >= width, UNOK_EINVAL, "%s: rows of %lld elements, %lld apart", what, (long long)width,
