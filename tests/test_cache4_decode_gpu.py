@@ -347,3 +347,43 @@ def test_refusals(dev):
     with pytest.raises(RuntimeError, match="does not fit"):
         dec.draft_block(dec.new_cache(2, 8, bits=4), torch.zeros(2, 9, device=dev, dtype=torch.int64))
     assert cache.lengths.tolist() == [8, 8]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("name", list(CFGS))
+def test_rows_of_verified_drafts(dev, name, dtype):
+    """What verify_draft keeps of a block in a 4-bit cache: codes and scales of the rows of the last token and the accepted ones, as a pass
+    over the same block stored them, behind rows that stay as they were; and the next pass attends over them."""
+    cfg, params, lora, dec = _build(dev, name, dtype)
+    g = torch.Generator(device=dev).manual_seed(13)
+    B, P, L = 3, 20, 6
+    cache = dec.new_cache(B, 96, bits=4)
+    z = dec.prefill(cache, torch.randint(0, cfg.vocab_size - 1, (B, P), generator=g, device=dev))
+    cache.lengths.copy_(torch.tensor([P, 11, 16]))
+    seed = z[:, -1].float().argmax(1)
+    counts = torch.tensor([L, 3, 0], device=dev)
+    chain = torch.arange(-1, L, device=dev, dtype=torch.int32)
+    tensors = [t for c in cache.k + cache.v for t in c]
+    taken = 0
+    for step in range(4):
+        before = cache.lengths.tolist()
+        block = torch.cat([seed[:, None], torch.zeros(B, L, device=dev, dtype=torch.int64)], 1)
+        for i in range(L):                              # each token the likeliest behind those before it, but some
+            x = dec.tree_block(cache, block, chain)[:, i]
+            block[:, i + 1] = torch.where(x == x.amax(1, keepdim=True), torch.arange(x.shape[1], device=dev), x.shape[1]).amin(1)
+        block[0, 2 + step] = (block[0, 2 + step] + 1) % cfg.vocab_size
+        dec.tree_block(cache, block, chain)
+        want = [t.clone() for t in tensors]
+        accepted, token = dec.verify_draft(cache, block, torch.rand(B, L + 1, generator=g, device=dev), None, counts, 0.0)
+        assert accepted.tolist() == [1 + step, 3, 0]
+        after = cache.lengths.tolist()
+        assert after == [n + 1 + a for n, a in zip(before, accepted.tolist())]
+        for t, w in zip(tensors, want):
+            for b, n in enumerate(after):
+                assert torch.equal(t[b, :, :n], w[b, :, :n])
+        taken += int(accepted.sum())
+        again = dec.tree_block(cache, token[:, None].contiguous(), chain[:1])
+        _check(again, params, lora, cfg, cache, after, token[:, None], torch.full((B, 1), -1, dtype=torch.int32), torch.zeros(B, 1),
+               TOL[dtype])
+        seed = token
+    assert taken == 1 + 2 + 3 + 4 + 4 * 3
