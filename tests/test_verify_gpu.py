@@ -479,3 +479,43 @@ def test_single_nodes_that_are_padding(dev):
     parents = torch.tensor([[-1], [-2], [-1], [-5]], device=dev, dtype=torch.int32)
     nodes, counts, _ = _check_tree(z[:4], x, parents, u[:, :1].contiguous())
     assert counts.tolist() == [1, 0, 1, 0] and nodes.tolist() == [[0], [-1], [0], [-1]]
+
+
+def test_a_tree_s_tokens_are_distributed_as_the_target_says(dev):
+    """60000 trees of a root and one child over six columns: the token drawn at the root, whether the child holds it or not, and the
+    token drawn at the child where it does, have the target's frequencies; counts within six deviations."""
+    B, V, held = 60000, 6, 2
+    g = torch.Generator(device=dev).manual_seed(6)
+    p, r = torch.tensor([0.3, 0.25, 0.2, 0.15, 0.08, 0.02]), torch.tensor([0.05, 0.1, 0.5, 0.3, 0.03, 0.02])
+    z = torch.stack([p.log(), r.log()]).to(dev).repeat(B, 1)
+    tokens = torch.full((B, 2), held, device=dev)
+    parents = torch.tensor([-1, 0], device=dev, dtype=torch.int32)
+    nodes, counts, token = K.verify_tree(z, tokens, parents, torch.rand(B, 2, device=dev, generator=g))
+    down = counts == 2
+    assert bool((counts >= 1).all()) and not nodes[:, 0].any() and torch.equal(nodes[:, 1], torch.where(down, 1, -1))
+    for a, b in ((torch.where(down, held, token), p), (token[down], r)):
+        n = a.numel()
+        off = (torch.bincount(a, minlength=V).cpu().double() - n * b).abs()
+        assert bool((off <= 6 * (n * b * (1 - b)).sqrt()).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [1, 16, 17, 37, 130])
+def test_trees_at_temperatures_of_each_sequence(dev, dtype, T):
+    """Greedy, warm and hot sequences side by side, rows drawn alone and in workgroups of eight; infinity as every finite logit alike."""
+    print(f"[walk temperatures] {dtype} T={T}", flush=True)
+    temps = torch.tensor([0.0, 0.7, 1.0, 3.0, -1.0, math.inf, 0.05])
+    B, V = len(temps), 3001
+    g = torch.Generator().manual_seed(100 + T)
+    z = _logits(dev, B * T, V, dtype, 40 + T, 3)
+    parents = torch.full((B, T), -1, dtype=torch.int32)
+    for t in range(1, T):
+        parents[:, t] = torch.randint(max(0, t - 4), t, (B,), generator=g).int()
+    top = torch.topk(z.float(), 3, dim=1).indices.view(B, T, 3).cpu()
+    pick = torch.randint(0, 3, (B, T), generator=g)
+    tokens = torch.stack([top[b, parents[b].long().clamp(min=0), pick[b]] for b in range(B)]).to(dev)
+    u = torch.rand(B, T, generator=g)
+    got = K.verify_tree(z, tokens, parents.to(dev), u.to(dev), temperature=temps.to(dev))
+    want = _tree(z, tokens.cpu(), parents, u, torch.where(temps.isinf(), 1e30, temps))
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b), (a.tolist(), b.tolist())
