@@ -323,16 +323,17 @@ int unok_tree_depths(int B, int T, const int32_t* parents, int32_t* depths, void
 int unok_tree_prep(int B, int T, int nq, int nk, int D, const void* qkv, int64_t ld, const void* wq, const void* wk,
                    const int64_t* lengths, const int32_t* depth, const float* inv_freq, float eps, void* kc, void* vc,
                    int max_len, void* q, void* stream);
-/* The accepted path of a tree: in each of ntensors cache tensors [B, nk, max_len] rows of row_bytes (a multiple of 16, at most 512),
- * row lengths[b] + nodes[b, i] goes to row lengths[b] + i for i < counts[b]; every row is read before any is
- * written. nodes [B, P], P <= 256; entries outside [0, max_len - lengths[b]) are skipped. `caches` is a host array
- * of device pointers. */
+/* The accepted path of a tree: in each of ntensors cache tensors [B, nk, max_len] rows of row_bytes (2, 4, 8, or a multiple of 16 up to
+ * 512; tensors 16-byte aligned), row lengths[b] + nodes[b, i] goes to row lengths[b] + i for i < counts[b]; every row is read
+ * before any is written. nodes [B, P], P <= 256; entries outside [0, max_len - lengths[b]) are skipped. `caches` is a host
+ * array of device pointers. */
 int unok_cache_keep(int ntensors, void* const* caches, int row_bytes, int B, int nk, int max_len, int P,
                     const int64_t* lengths, const int64_t* nodes, const int64_t* counts, void* stream);
 /* Copies sequences between cache slots: for each of npairs (source slot, destination slot) pairs and every tensor, rows
- * [0, src_lengths[source]) (no more than either cache holds), and dst_lengths[destination] (null: left alone) becomes that number.
- * src and dst are host arrays of ntensors device pointers, pairs a host array. No slot is written twice; source and
- * destination tensors are disjoint, or the same, and then no slot is both read and written. */
+ * [0, src_lengths[source]) (no more than either cache holds) of row_bytes (2, 4, 8 or a multiple of 16; tensors 16-byte aligned),
+ * and dst_lengths[destination] (null: left alone) becomes that number. src and dst are host arrays of ntensors device pointers,
+ * pairs a host array. No slot is written twice; source and destination tensors are disjoint, or the same, and then no slot is both
+ * read and written. */
 int unok_cache_copy(int ntensors, const void* const* src, void* const* dst, int row_bytes, int nk, int src_batch, int src_max,
                     int dst_batch, int dst_max, const int64_t* src_lengths, int64_t* dst_lengths, int npairs,
                     const int* pairs, void* stream);
