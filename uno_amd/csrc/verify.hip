@@ -3,7 +3,9 @@
 // A token is drawn by the inverse distribution function: the lowest index at which the running sum of the weights
 // exp((z - max z) / T) exceeds u times their sum. Of a vocabulary's 150 thousand borders between tokens some lie within an fp32
 // exponential's error (1e-7) of any u: with such weights about one token in 300 would be another one than the logits say, and
-// depend on the order of the sums. The weights and all sums are therefore fp64, the weights to 4e-14.
+// depend on the order of the sums. The weights and all sums are therefore fp64. A weight relative to its row's largest logit is a column's
+// relative to its chunk's times the chunk's, with polynomials of 3.6e-14 and 3.9e-14 (roundings included); the exponent's own roundings, of
+// log2(e) / T and of z - max z where that is not exact, add 2.4e-16 |z - max z| / T. So 8e-14 where weights matter, 2.5e-13 at e^-700.
 //
 // The logits are read once, in chunks of CHUNK columns, one wave each, of which little is kept: largest logits and sums of weights.
 // Everything else works on these parts, and on a fourth of a chunk to a drawn token. 16 trees of 64 nodes, 151936 bf16 columns: the
@@ -43,7 +45,7 @@ struct Verify {
 };
 
 // 2^x at x = d c, -1022 <= x <= 0, of N numbers side by side: 2^n (1 + r q(r)), r = x - n in [-1/2, 1/2], q the polynomial through
-// (2^r - 1) / r at nine Chebyshev points. Relative error 3.7e-14; exactly 1 at 0. n is the low half of x + 1.5 2^52.
+// (2^r - 1) / r at nine Chebyshev points. Relative error 3.7e-14 before roundings; exactly 1 at 0. n is the low half of x + 1.5 2^52.
 template <int N> __device__ __forceinline__ void exp2_64(double (&d)[N], double c) {
   constexpr double ROUND = 0x1.8p52;
   constexpr double Q[9] = {0x1.62e42fefa39efp-1, 0x1.ebfbdff823cedp-3, 0x1.c6b08d7047e52p-5,
@@ -438,12 +440,16 @@ template <typename G, int K> __device__ __forceinline__ Row row_of(const Listed<
 }
 
 // Counts one arrival of `all`; whether it is the last. What the others handed over before theirs is then there: each waited for its
-// stores before it counted. (Release and acquire fences write back and drop whole L2s: 1024 of them took 30 us.) Called by one wave.
+// stores, which go past its caches, before it counted. The last one needs no acquire: what it reads of the others are loads past its own
+// caches (`taken`) alone, issued after the count has come back, since they stand behind a branch on it, and the compiler moves nothing
+// above the empty statement. (Release and acquire fences write back and drop whole L2s: 1024 of them took 30 us.) Called by one wave.
 __device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t all) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   uint32_t n = 0;
   if ((threadIdx.x & 63) == 0) n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return __builtin_amdgcn_readfirstlane(n) + 1 == all;
+  const bool last = __builtin_amdgcn_readfirstlane(n) + 1 == all;
+  asm volatile("" ::: "memory");
+  return last;
 }
 
 // From node 0 on: the token drawn at a node leads to its first child that holds it. One wave; lane l has nodes l, l + 64, ..
