@@ -4,12 +4,18 @@
 // and their scale. Each of a workgroup's four waves walks its own tiles of a range: codes come into its part of LDS, are converted in
 // registers, and serve the wave's 16 QT query rows; no barrier in the walk. (Converted tiles shared through LDS, as the bf16 cache's are,
 // cost LDS reads of numbers four times as large as their codes: 16 sequences, 64 nodes of 32 / 8 heads of 128 over 16384 rows 418 us,
-// this 257.)
+// this 257 at the time.)
 //
-// Measured: one node of 4 sequences over 65536 rows 44 us (232 MB of codes and scales, 5.3 TB/s: what a large copy reaches); 64 nodes of 16
-// sequences over 16384 rows 257 us (820 TFLOP/s; conversions, weights and their rounding, some 190 vector instructions to 32 keys and 32
-// rows, bound it: the products alone would take 173); 16 nodes of 8 sequences over 4096 rows 22 us (6 at the copy's rate: eight tiles to a
-// wave, the rest is the queries, the join and the launch).
+// Measured (32 / 8 heads of 128, sequences from the given number of rows down to half of it): one node of 4 sequences, 65536 rows 45 us (232
+// MB of codes and scales, 5.2 TB/s: what a large copy reaches); 64 nodes of 16 sequences, 16384 rows 241 to 249 us with their merge (210
+// GFLOP, 850 to 880 TFLOP/s; conversions, weights and their rounding, some 190 vector instructions to 32 keys and 32 rows, bound it: the
+// products alone would take 173); 16 nodes of 8 sequences, 4096 rows 21.5 us (6 at the copy's rate: eight tiles to a wave, the rest is the
+// queries, the join and the launch). fp32 queries, 64 nodes of 8 sequences, 8192 rows 170 us (the three products alone 133).
+//
+// bf16 queries: a weight is rounded to bf16 for the product with V, off by at most 2^-8 of itself, and the weights' sum is that of the
+// rounded ones, so that an output is off by the roundings' scatter alone: 2.1e-3 to 2.3e-3 of its size with its own rounding, which alone
+// makes 1.7e-3. Scores, sums and outputs are fp32 until the end. (A second product with what a rounding leaves would add half to the
+// products, which bind long caches; tree.hip measured that.)
 //
 // fp32 queries: a query is the sum of three bf16 numbers (each what the ones before it leave, 8 of its 24 bits), and so is a weight;
 // three products take the place of one, exact but for their sums.
@@ -452,6 +458,11 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 || D == 64 ? 2 : 1) void tree_a
 // Query rows of a workgroup, and one round of workgroups (`share`, two to a CU; fp32 with 128 dims has the registers for one). 32 rows: 64
 // to a wave share a conversion among more products, but leave one wave to a SIMD: 16 sequences, 64 nodes over 16384 rows 273 us (32
 // rows 266), 8 sequences, 16 nodes over 4096 26.2 (22.5).
+// The ranges are those of tree.h, whose figures are of 16/32-bit rows. On these rows (us with the merge, in a graph; ranges of at least one /
+// two / four blocks): one sequence, one node over 1150 rows 10.0 / 9.4 / 9.7, over 2000 10.4 / 9.7 / 10.8, over 4096 14.8 / 11.8 / 11.7; 8
+// sequences, 16 nodes over 500 rows 17.9 / 15.7 / 15.1, over 1000 18.8 / 18.9 / 15.9, from 2000 on alike. Single blocks for sequences of
+// three to eight (with them / without): one node over 1000 rows 8.9 / 9.6, 16 nodes 12.6 / 12.9 (fp32 14.3 / 15.2), fp32 37 nodes of
+// three sequences over 901 11.3 / 12.0; they lose for 16 nodes of four sequences over 500 rows, 13.7 / 13.2.
 TreePlan tree_plan4(int dtype, int B, int T, int nq, int nk, int D, int max_len) {
   const int NR = nq / nk * T;
   TreePlan p;

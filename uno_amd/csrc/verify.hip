@@ -9,8 +9,8 @@
 //
 // The logits are read once, in chunks of CHUNK columns, one wave each, of which little is kept: largest logits and sums of weights.
 // Everything else works on these parts, and on a fourth of a chunk to a drawn token. 16 trees of 64 nodes, 151936 bf16 columns: the
-// parts 99 us (59 at a large copy's rate; 12 fp64 and 3 other vector instructions to a weight, issued three quarters of the time,
-// bound it), the tokens and the paths 9. One row of 32000: 4.2 and 3.7 us, latency of loads and reductions.
+// parts 101 us (59 at a large copy's rate; 12 fp64 and 3 other vector instructions to a weight bound it, issued in 89% of the cycles of
+// busy CUs), the tokens and the paths 10. One row of 32000: 4.3 and 3.6 us, latency of loads and reductions.
 #include "common.h"
 #include "../../include/unok.h"
 
@@ -566,6 +566,10 @@ template <typename T> __device__ __forceinline__ int draw(const T* z, const Veri
 // The token of each node, a wave to a row (-1: padding, or no distribution), ROWS rows of a sequence to a workgroup; the last workgroup
 // of a sequence follows the tree. Workgroups that count their arrival in one place wait for each other: 16 sequences of 64 nodes 18 us
 // where each row has its own, in eights 9.3; 8 sequences of 16 nodes 6.8 and 8.0, since there waves of one CU wait for each other more.
+// Both forms with the parts (us, alone / in eights): 151936 columns, one sequence of 17 nodes 11.4 / 13.0, of 63 15.5 / 17.1, 4 of 16 15.5
+// / 17.3, 4 of 63 35.6 / 34.8, 8 of 16 23.0 / 24.0, 8 of 32 34.9 / 34.8, 8 of 63 59.8 / 57.7, 16 of 16 33.9 / 34.7, 16 of 24 46.7 / 46.0, 16 of 63 120
+// / 114; 32000 columns, 1 of 63 10.8 / 10.9, 4 of 32 12.7 / 12.6, 8 of 16 12.3 / 12.3, 16 of 8 12.1 / 12.2, 16 of 16 16.7 / 15.5. So a rule on
+// the nodes alone is off by up to 2 us for one to four sequences of 17 to 48 nodes, and by 1 for 16 sequences of 16 over small vocabularies.
 constexpr int DRAW_ALONE = 16, DRAW_ROWS = 8;            // up to DRAW_ALONE nodes each has a workgroup
 template <typename T, int ROWS> __global__ __launch_bounds__(64 * ROWS) void verify_draw_kernel(const Verify a, int32_t* drawn) {
   __shared__ int tokens[ROWS];
